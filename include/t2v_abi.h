@@ -27,7 +27,7 @@ typedef void* t2v_stream_t; /* hipStream_t */
 #define T2V_OK 0
 #define T2V_EINVAL (-1)
 #define T2V_ELAUNCH (-2)
-#define T2V_ABI_VERSION 9   /* bumped whenever a struct layout or a signature changes (native.py checks it) */
+#define T2V_ABI_VERSION 10   /* bumped whenever a struct layout or a signature changes (native.py checks it) */
 
 int t2v_abi_version(void);
 const char* t2v_last_error(void);
@@ -285,6 +285,63 @@ typedef struct {
 } T2VAttn;
 int t2v_attn_fwd(const T2VAttn* p, t2v_stream_t stream);
 int t2v_attn_bwd(const T2VAttn* p, t2v_stream_t stream);
+
+/* ---- attention with modified scores (csrc/attn_mod.hip): grouped heads, head dims that are multiples of 8 up to 128, bf16 / fp16 ----
+ *   t_ij = cap * tanh(scale q_i.k_j / cap) (softcap > 0) or scale q_i.k_j,   - slopes[h] |j - i'|,   + bias[h][clip(j - i', -R, R) + R]
+ *   o_i  = sum_j softmax_j(t_ij) v_j over the keys query i may see, zeros where it may see none.
+ * len = kv_len[b] (clamped to 0..Sk) or Sk; i' = i + len - Sq: the queries are the last Sq positions.  Query i sees key j iff
+ * j < len, (not causal or j <= i' or j < prefix), and q_docs[b][i] == kv_docs[b][j] >= 0 (where documents are given).
+ * prefix: [nbatch] or (prefix_per_query) [nbatch, Sq].  bias: [heads, 2 radius + 1], in the operands' type or (bias_f32) fp32; an entry
+ * at or below its type's lowest finite value hides its distance.  Rows that no query may see (key >= len, document < 0) are not read
+ * into any sum: they may hold anything.  Operands as in T2VAttn with head stride D: element (b, s, h, d) at
+ *   ptr + (b / bdiv) * bstride_hi + (b % bdiv) * bstride_lo + s * sstride + h * D + d      (k, v, dk, dv: kv_heads)
+ * lse: fp32 [nbatch, heads, Sq], base-2 log-sum-exp in an order of the library's own: kept for the backward call; NULL: not written.
+ * Backward: the descriptor of the forward with d_o, dq, dk, dv, delta (fp32 [nbatch, heads, Sq] scratch) and dbias (NULL or like
+ * bias) filled in; every row of dq, dk, dv is written.  kv_share: batches b with the same b / kv_share have one K / V (and one
+ * dk / dv, the sum); 1: each has its own.  workspace: t2v_attn_mod_workspace(p, backward) bytes, 256-byte aligned, no
+ * initialisation needed, free for other use when the call's kernels have run. */
+typedef struct T2VAttnMod {
+  int nbatch, heads, kv_heads, Sq, Sk, D, dtype, causal;
+  float scale, softcap;
+  T2VAttnOperand q, k, v, o;
+  float* lse;
+  const int* prefix; int prefix_per_query;
+  const int* kv_len;
+  const int* q_docs; const int* kv_docs;
+  const float* slopes;
+  const void* bias; int bias_f32, radius;
+  T2VAttnOperand d_o, dq, dk, dv;
+  float* delta; void* dbias; int kv_share;
+  void* workspace; long long workspace_bytes;
+} T2VAttnMod;
+long long t2v_attn_mod_workspace(const T2VAttnMod* p, int backward);
+int t2v_attn_mod_fwd(const T2VAttnMod* p, t2v_stream_t stream);
+int t2v_attn_mod_bwd(const T2VAttnMod* p, t2v_stream_t stream);
+
+/* ---- rotary positions with several axes, and the per-head norm of queries and keys in the same pass (csrc/rope.hip) ----
+ *   y = R(pos) (w * xhat + b);  norm 0: xhat = x, w, b unused; 1: RMS norm; 2: layer norm, over the D columns of each head.
+ * Two sides (queries, keys; heads[1] = 0: one side), token matrices [rows, ld] whose row holds heads[i] * D columns; dtype 0 bf16,
+ * 1 fp16, 2 fp32.  The first rot = sum(dims) columns of a head turn: pair p by pos[row, axis(p)] * scale[axis] * freq(p), where the
+ * axes own dims[a] / 2 pairs each, in order, and freq(p) = freqs[p] (fp64 [rot / 2], radians) or theta^(-2 i / d): i and d count
+ * inside the axis (shared = 0) or over all rot columns (shared = 1).  style 0: pair p = columns (2p, 2p + 1); 1: (p, p + rot / 2).
+ * pos: [rows, ldpos], pos_type 0 int32, 1 int64, 2 fp32.  w, b: fp32 [D] or NULL.
+ * Backward: x (norm != 0) and dy in, y = dx out; dw, db: fp32 [D] or NULL each, overwritten; workspace: t2v_qk_rope_bwd_floats()
+ * floats, no initialisation needed.  The row stride in bytes and all pointers must be multiples of 16. */
+typedef struct T2VQkRope {
+  const void* x[2]; long long ldx[2];
+  const void* dy[2]; long long lddy[2];
+  void* y[2]; long long ldy[2];
+  int heads[2];
+  const float* w[2]; const float* b[2];
+  float* dw[2]; float* db[2]; float* workspace;
+  long long rows; int D, dtype, norm; float eps;
+  const void* pos; long long ldpos; int pos_type;
+  int naxes; int dims[4]; double scale[4]; double theta; int shared, style;
+  const double* freqs;
+} T2VQkRope;
+int t2v_qk_rope_fwd(const T2VQkRope* p, t2v_stream_t stream);
+long long t2v_qk_rope_bwd_floats(const T2VQkRope* p);
+int t2v_qk_rope_bwd(const T2VQkRope* p, t2v_stream_t stream);
 
 /* ---- the temporal self-attention unit of TransformerTemporalModel as ONE forward-only launch (ABI v9, csrc/temporal_fused.hip):
  *   out = x + softmax_F((LN(x) Wq^T)(LN(x) Wk^T)^T * scale)(LN(x) Wv^T) Wo^T + bo

@@ -8,10 +8,13 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 LIB = os.path.join(HERE, "libt2v_hip.so")
-SOURCES = ["gemm.hip", "gemm_w8.hip", "norm.hip", "attn.hip", "elementwise.hip", "lora_wgrad.hip", "lora_merge.hip", "temporal_fused.hip"]
+SOURCES = ["gemm.hip", "gemm_w8.hip", "norm.hip", "attn.hip", "elementwise.hip", "lora_wgrad.hip", "lora_merge.hip", "temporal_fused.hip",
+           "rope.hip", "attn_mod.hip"]
 # translation units: (source, object, extra flags).  gemm_w8.hip is compiled three times with -DW8_PART=0/1/2 (plain kernels + entry
 # points / LR = 1 kernels / LR = 2 kernels): its ~60 kernel instantiations took 3 minutes in one hipcc process
-UNITS = [(s, s.replace(".hip", ".o"), []) for s in SOURCES if s != "gemm_w8.hip"] + \
+# NO_PK: the packed fp32 instructions (v_pk_add / mul / fma_f32), which the compiler forms from ordinary float code, are kept out
+NO_PK = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+UNITS = [(s, s.replace(".hip", ".o"), NO_PK if s in ("rope.hip", "attn_mod.hip") else []) for s in SOURCES if s != "gemm_w8.hip"] + \
         [("gemm_w8.hip", f"gemm_w8_p{i}.o", [f"-DW8_PART={i}"]) for i in range(3)]
 
 

@@ -1,0 +1,1397 @@
+// attn_mod.hip — attention with modified scores for gfx950: forward, backward, and the short-query form split over the keys.
+//
+//   t_ij = cap * tanh(scale q_i . k_j / cap)   (or scale q_i . k_j)   - slope_h |j - i'| + table_h[clip(j - i', -R, R)]
+//   o_i  = sum_j softmax_j(t_ij) v_j   over the keys that query i may see;  zeros where it may see none
+// i' = i + (len - Sq): the queries are the last Sq positions of the len = kv_len[b] keys.  A query sees key j iff j < bound_i and their
+// documents agree; bound_i = len, or min(len, max(i' + 1, prefix_i)) for a causal mask: every mask that depends on positions is ONE
+// integer per query, compared once per score and only in tiles that cross it.
+//
+// Layout.  Lane = query in the forward and dQ kernels (S^T = K Q^T: the row maximum and sum stay in the lane, one exchange between the
+// two halves of a wave), lane = key in the dK / dV kernel.  P^T (dS^T) goes from the accumulator registers into the next product
+// as its B operand; the transposed operand comes from the staged LDS tile through ds_read_b64_tr_b16, with the accumulators' row order
+// applied to both.  64-row tiles of the streamed pair (K|V, or Q|dO) are staged once per workgroup, double-buffered; rows of 2 DP
+// bytes, no padding, the 16-byte chunk index XORed with chunk_swizzle(row): row reads and transposed reads both spread over all banks.
+// Grouped heads: the gp query heads that share a K/V head are packed into the row index (row r = query r / gp, head r % gp), so K and V
+// are read once for all of them; with a table each head is a unit of its own (gp = 1: the table of one head lives in LDS).
+// Statistics, the running maximum and sum, lse, delta and all accumulators are fp32; P and dS are rounded to the input type for the
+// matrix cores (one rounding of a factor in [0, 1], and of a gradient, the same size as the output's own rounding).
+#include <type_traits>
+
+#include "common.h"
+
+namespace {
+
+constexpr int TILE = 64;                        // staged rows
+constexpr float LOG2E = 1.44269504088896341f;
+constexpr float LOWEST = -1.0e30f;              // running maximum before the first visible key: finite, below every score
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
+typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
+typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
+
+__device__ __attribute__((aligned(16))) const unsigned zero_chunk[4] = {0, 0, 0, 0};
+
+template <typename T>
+struct El;
+template <>
+struct El<bf16_t> {
+  static __device__ __forceinline__ f32x16 mfma(const bf16x8& a, const bf16x8& b, const f32x16& c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ unsigned pack2(float a, float b) { return pack2bf(a, b); }
+  static __device__ __forceinline__ float up(short v) { return bf2f((unsigned short)v); }
+};
+template <>
+struct El<_Float16> {
+  static __device__ __forceinline__ f32x16 mfma(const bf16x8& a, const bf16x8& b, const f32x16& c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ unsigned pack2(float a, float b) {
+    const t2v_f32x2 v = {a, b};
+    return __builtin_bit_cast(unsigned, __builtin_convertvector(v, f16x2));
+  }
+  static __device__ __forceinline__ float up(short v) { return (float)__builtin_bit_cast(_Float16, v); }
+};
+template <typename T>
+__device__ __forceinline__ bf16x8 pack8(const f32x16& v, int kk) {
+  const u32x4 q = {El<T>::pack2(v[8 * kk], v[8 * kk + 1]), El<T>::pack2(v[8 * kk + 2], v[8 * kk + 3]),
+                   El<T>::pack2(v[8 * kk + 4], v[8 * kk + 5]), El<T>::pack2(v[8 * kk + 6], v[8 * kk + 7])};
+  return __builtin_bit_cast(bf16x8, q);
+}
+
+// accumulator register r of lane half hi holds row crow(r, hi) of the 32 x 32 tile
+__device__ __forceinline__ constexpr int crow(int r, int hi) { return (r & 3) + 8 * (r >> 2) + 4 * hi; }
+__device__ __forceinline__ float xor32(float v) { return __shfl_xor(v, 32); }
+
+template <int DP>
+__device__ __forceinline__ int chunk_swizzle(int row) {
+  return DP == 128 ? ((row & 3) << 2) | ((row >> 2) & 3) : (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
+}
+
+struct QMeta {      // of 64 rows: smallest and largest bound, smallest and largest document >= 0, whether some row has none
+  int bmin, bmax, dmin, dmax, neg;
+};
+struct KMeta {
+  int dmin, dmax, neg;
+};
+
+struct Args {
+  T2VAttnMod p;
+  int gp, nunit, M;                 // heads per unit, units per batch, rows per unit (Sq * gp)
+  unsigned magic;                   // r / gp = r * magic >> 32 (gp > 1)
+  int ntile, splits;                // row (or key) tiles of a unit, splits of the other axis
+  int to_part;                      // dK / dV go to `part` as fp32 (several splits, or several batches that share K / V)
+  const QMeta* qmeta;               // [nbatch][ceil(M / 64)] or NULL
+  const KMeta* kmeta;               // [nbatch][ceil(Sk / 64)] or NULL
+  float* part;                      // partial results of the splits
+  float* part_ml;
+  float* part_bias;                 // [nbatch * ntile][heads][2R + 1]
+};
+
+__device__ __forceinline__ long long op_base(const T2VAttnOperand& o, int b) {
+  return (long long)(b / o.bdiv) * o.bstride_hi + (long long)(b % o.bdiv) * o.bstride_lo;
+}
+__device__ __forceinline__ int div_gp(const Args& a, int r) { return a.gp == 1 ? r : (int)__umulhi((unsigned)r, a.magic); }
+__device__ __forceinline__ int seq_len(const Args& a, int b) {
+  return a.p.kv_len ? max(0, min(a.p.kv_len[b], a.p.Sk)) : a.p.Sk;
+}
+// keys [0, bound) are candidates of query i
+__device__ __forceinline__ int row_bound(const Args& a, int b, int i, int len) {
+  if (!a.p.causal) return len;
+  int m = i + len - a.p.Sq + 1;
+  if (a.p.prefix) m = max(m, a.p.prefix[a.p.prefix_per_query ? (long long)b * a.p.Sq + i : b]);
+  return max(0, min(m, len));
+}
+
+// workgroup id -> (batch, unit): workgroups go round-robin over the eight XCDs, so units that share a K/V head are placed a multiple of
+// nbatch * kv_heads apart, which is the same XCD (and L2) where that is a multiple of eight
+struct Unit {
+  int b, kv, h0;
+};
+__device__ __forceinline__ Unit unit_of(const Args& a, int x) {
+  const int kvb = a.p.nbatch * a.p.kv_heads, gu = x / kvb, y = x - gu * kvb;
+  Unit u;
+  u.b = y / a.p.kv_heads;
+  u.kv = y - u.b * a.p.kv_heads;
+  u.h0 = u.kv * (a.p.heads / a.p.kv_heads) + gu * a.gp;
+  return u;
+}
+
+// ------------------------------------------------------------------------------------------------ staging
+// Two 64-row tiles (A | B) of 2 DP bytes a row, fetched by NT threads into registers one tile ahead and written to the LDS stage after the
+// current tile's mathematics.  Rows that nobody sees are written as zeros: what they hold (inf, NaN) must not meet a zero weight.
+template <int DP, int NT>
+struct Pair {
+  static constexpr int CH = DP / 8, RPP = NT / CH, N = TILE / RPP;      // chunks per row, rows per pass, passes
+  bf16x8 a[N], b[N];
+};
+
+template <int DP>
+struct __attribute__((aligned(16))) Stage {
+  bf16_t a[TILE * DP];
+  bf16_t b[TILE * DP];
+};
+
+template <int DP>
+__device__ __forceinline__ int stage_off(int row, int ch) { return row * DP + ((ch ^ chunk_swizzle<DP>(row)) << 3); }
+
+template <int DP, int NT>
+__device__ __forceinline__ void pair_store(Stage<DP>& st, const Pair<DP, NT>& r, int tid) {
+  typedef Pair<DP, NT> P;
+#pragma unroll
+  for (int i = 0; i < P::N; ++i) {
+    const int o = stage_off<DP>(tid / P::CH + i * P::RPP, tid % P::CH);
+    *(bf16x8*)(st.a + o) = r.a[i];
+    *(bf16x8*)(st.b + o) = r.b[i];
+  }
+}
+
+// fragment of 32 staged rows as an MFMA operand (row = lane & 31, k = the 16 columns of step kd)
+template <int DP>
+__device__ __forceinline__ bf16x8 rowfrag(const bf16_t* s, int blk, int kd, int lane) {
+  const int row = 32 * blk + (lane & 31);
+  return *(const bf16x8*)(s + stage_off<DP>(row, 2 * kd + (lane >> 5)));
+}
+// fragment of the transposed tile: rows = columns [32 fm, 32 fm + 32), k = the 16 staged rows of step kk in the accumulators' order
+template <int DP>
+__device__ __forceinline__ bf16x8 trfrag(const bf16_t* s, int blk, int fm, int kk, int lane) {
+  const int gq = lane >> 4, li = lane & 15;
+  const int row = 32 * blk + 16 * kk + 4 * (gq >> 1) + (li >> 2);
+  const int ch = 4 * fm + 2 * (gq & 1) + ((li & 3) >> 1), in = 4 * (li & 1);
+  const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_bf16x4*)(s + stage_off<DP>(row, ch) + in));
+  const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_bf16x4*)(s + stage_off<DP>(row + 8, ch) + in));
+  return bf16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+}
+
+__device__ __forceinline__ const bf16x8* chunk_ptr(const bf16_t* p, bool ok) { return ok ? (const bf16x8*)p : (const bf16x8*)zero_chunk; }
+
+// ------------------------------------------------------------------------------------------------ scores
+// t (in base-2 exponent units) of one lane's 16 scores.  `d0`: distance j - i' of accumulator row 0 (of the lane's half)
+struct Mod {
+  float c;            // scale * log2e (no cap)
+  float k1, capl;     // cap: 2 log2e scale / cap, cap * log2e
+  bool cap, slope, table;
+  int R;
+};
+__device__ __forceinline__ Mod make_mod(const Args& a) {
+  Mod m;
+  m.cap = a.p.softcap > 0.f;
+  m.slope = a.p.slopes != nullptr;
+  m.table = a.p.bias != nullptr;
+  m.c = a.p.scale * LOG2E;
+  m.k1 = m.cap ? 2.f * LOG2E * a.p.scale / a.p.softcap : 0.f;
+  m.capl = a.p.softcap * LOG2E;
+  m.R = a.p.radius;
+  return m;
+}
+// cap * tanh(x / cap) = cap (1 - 2 / (1 + e^(2 x / cap))): one exp, one reciprocal; exact at +-inf.  Returns it in base-2 units and
+// leaves w = 1 / (1 + e^(..)): the derivative is 4 w (1 - w).
+__device__ __forceinline__ float capped(const Mod& m, float s, float& w) {
+  w = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s * m.k1));
+  return fmaf(w, -2.f * m.capl, m.capl);
+}
+
+// table of head h in base-2 units in LDS; an entry at or below the type's lowest finite value hides its distance (-inf)
+template <typename T>
+__device__ __forceinline__ void load_table(const Args& a, int h, float* tab, int tid, int nt) {
+  const int n = 2 * a.p.radius + 1;
+  for (int i = tid; i < n; i += nt) {
+    const long long at = (long long)h * n + i;
+    float v;
+    if (a.p.bias_f32) {
+      v = ((const float*)a.p.bias)[at];
+      v = v <= -3.4028234e38f ? -INFINITY : v * LOG2E;
+    } else {
+      v = El<T>::up(((const short*)a.p.bias)[at]);
+      v = v <= (std::is_same<T, bf16_t>::value ? -3.3895313e38f : -65504.f) ? -INFINITY : v * LOG2E;
+    }
+    tab[i] = v;
+  }
+}
+
+// next tile >= t (and < end) whose keys / rows may matter; `active(t)` is evaluated for 64 tiles at once, one per lane
+template <typename F>
+__device__ __forceinline__ int next_tile(int t, int end, F active) {
+  const int lane = threadIdx.x & 63;
+  while (t < end) {
+    const int c = t + lane;
+    const unsigned long long m = __ballot(c < end && active(min(c, end - 1)));
+    if (m) return t + __builtin_ctzll(m);
+    t += 64;
+  }
+  return end;
+}
+
+// minimum / maximum over the wave as a scalar
+__device__ __forceinline__ int wave_min_i(int v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o));
+  return __builtin_amdgcn_readfirstlane(v);
+}
+__device__ __forceinline__ int wave_max_i(int v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = max(v, __shfl_xor(v, o));
+  return __builtin_amdgcn_readfirstlane(v);
+}
+
+// What a wave knows about the 32 QB query rows of its lanes (lane & 31 = row of the block)
+template <int QB>
+struct Rows {
+  int r[QB], i[QB], h[QB];          // row in the unit, query, head
+  bool ok[QB];                      // the row exists
+  int bound[QB], pos[QB], doc[QB];  // bound 0: sees nothing
+  float slope[QB];                  // in base-2 units
+  int bmin, bmax, dmin, dmax;       // over the wave
+  bool neg;
+};
+template <int QB>
+__device__ __forceinline__ void load_rows(Rows<QB>& R, const Args& a, const Unit& u, int len, int r0, int lane) {
+  int lo = 0x7fffffff, hi = 0, dlo = 0x7fffffff, dhi = -1, ng = 0;
+#pragma unroll
+  for (int q = 0; q < QB; ++q) {
+    R.r[q] = r0 + 32 * q + (lane & 31);
+    R.ok[q] = R.r[q] < a.M;
+    const int rc = min(R.r[q], a.M - 1);
+    R.i[q] = div_gp(a, rc);
+    R.h[q] = u.h0 + rc - R.i[q] * a.gp;
+    R.bound[q] = R.ok[q] ? row_bound(a, u.b, R.i[q], len) : 0;
+    R.pos[q] = R.i[q] + len - a.p.Sq;
+    R.doc[q] = a.p.q_docs ? a.p.q_docs[(long long)u.b * a.p.Sq + R.i[q]] : 0;
+    if (R.doc[q] < 0) R.bound[q] = 0;
+    R.slope[q] = a.p.slopes ? a.p.slopes[R.h[q]] * LOG2E : 0.f;
+    if (R.ok[q]) lo = min(lo, R.bound[q]);
+    hi = max(hi, R.bound[q]);
+    if (R.bound[q] > 0) {
+      dlo = min(dlo, R.doc[q]);
+      dhi = max(dhi, R.doc[q]);
+    } else if (R.ok[q]) {
+      ng = 1;
+    }
+  }
+  R.bmin = wave_min_i(lo);
+  R.bmax = wave_max_i(hi);
+  R.dmin = wave_min_i(dlo);
+  R.dmax = wave_max_i(dhi);
+  R.neg = wave_max_i(ng) != 0;
+}
+
+// ------------------------------------------------------------------------------------------------ forward
+template <typename T, int DP, int QB, bool MOD>
+__global__ __launch_bounds__(256, (DP == 64 || QB == 1) ? 2 : 1) void attn_mod_fwd_kernel(const Args a) {
+  warm_kernargs<(int)sizeof(Args)>();
+  constexpr int NT = 256, KD = DP / 16, FM = DP / 32;
+  typedef Pair<DP, NT> P;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  Stage<DP>* st = (Stage<DP>*)smem;
+  int* sdoc = (int*)(smem + 2 * sizeof(Stage<DP>));                     // [2][TILE]
+  int* swg = sdoc + 2 * TILE;                                           // [4 waves][4]
+  float* tab = (float*)(swg + 16);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5;
+  const int NU = a.p.nbatch * a.nunit;
+  const int x = blockIdx.x % NU, rest = blockIdx.x / NU;
+  const int sp = rest % a.splits, tile = a.ntile - 1 - rest / a.splits; // the longest rows of a causal mask first
+  const Unit u = unit_of(a, x);
+  const int len = seq_len(a, u.b), D = a.p.D, Sk = a.p.Sk;
+  const bf16_t* Q = (const bf16_t*)a.p.q.ptr + op_base(a.p.q, u.b);
+  const bf16_t* K = (const bf16_t*)a.p.k.ptr + op_base(a.p.k, u.b) + (long long)u.kv * D;
+  const bf16_t* V = (const bf16_t*)a.p.v.ptr + op_base(a.p.v, u.b) + (long long)u.kv * D;
+  const bool docs = a.kmeta && a.p.kv_docs;
+  const int* kdoc = docs ? a.p.kv_docs + (long long)u.b * Sk : nullptr;
+  const Mod mod = make_mod(a);
+
+  Rows<QB> R;
+  load_rows(R, a, u, len, (tile * 4 + wave) * 32 * QB, lane);
+  bf16x8 qf[QB][KD];
+#pragma unroll
+  for (int q = 0; q < QB; ++q) {
+    const bf16_t* qp = Q + (long long)R.i[q] * a.p.q.sstride + (long long)R.h[q] * D;
+#pragma unroll
+    for (int kd = 0; kd < KD; ++kd) qf[q][kd] = *chunk_ptr(qp + 16 * kd + 8 * hi, R.bound[q] > 0 && 16 * kd + 8 * hi < D);
+  }
+  if (MOD && mod.table) load_table<T>(a, u.h0, tab, tid, NT);
+  if (lane == 0) {
+    swg[wave * 4] = R.bmax;
+    swg[wave * 4 + 1] = R.dmin;
+    swg[wave * 4 + 2] = R.dmax;
+  }
+  __syncthreads();
+  int bmax = 0, dmin = 0x7fffffff, dmax = -1;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    bmax = max(bmax, swg[w * 4]);
+    dmin = min(dmin, swg[w * 4 + 1]);
+    dmax = max(dmax, swg[w * 4 + 2]);
+  }
+  bmax = __builtin_amdgcn_readfirstlane(bmax);
+  const int nt = (bmax + TILE - 1) / TILE, per = (nt + a.splits - 1) / a.splits;
+  const int tbeg = min(nt, sp * per), tend = min(nt, tbeg + per);
+  const KMeta* km = docs ? a.kmeta + (long long)u.b * ((Sk + TILE - 1) / TILE) : nullptr;
+  auto next = [&](int t) {
+    return docs ? next_tile(t, tend, [&](int c) { return km[c].dmax >= dmin && km[c].dmin <= dmax; }) : min(t, tend);
+  };
+  P nx;
+  int nd = 0, ndv[P::N];
+  auto fetch = [&](int t) {
+    const int ch = tid % P::CH;
+#pragma unroll
+    for (int i = 0; i < P::N; ++i) {
+      const int row = t * TILE + tid / P::CH + i * P::RPP;
+      const bool ok = row < len && ch * 8 < D;
+      nx.a[i] = *chunk_ptr(K + (long long)row * a.p.k.sstride + ch * 8, ok);
+      nx.b[i] = *chunk_ptr(V + (long long)row * a.p.v.sstride + ch * 8, ok);
+      if (docs) ndv[i] = kdoc[min(row, Sk - 1)];
+    }
+    if (docs && tid < TILE) {
+      const int row = t * TILE + tid;
+      nd = row < len ? kdoc[row] : -1;
+    }
+  };
+  auto store = [&](int sidx) {
+    if (docs) {
+#pragma unroll
+      for (int i = 0; i < P::N; ++i) {
+        const bf16x8 z = {0, 0, 0, 0, 0, 0, 0, 0};
+        nx.a[i] = ndv[i] < 0 ? z : nx.a[i];
+        nx.b[i] = ndv[i] < 0 ? z : nx.b[i];
+      }
+      if (tid < TILE) sdoc[sidx * TILE + tid] = nd;
+    }
+    pair_store(st[sidx], nx, tid);
+  };
+
+  float m[QB], l[QB];
+  f32x16 o[QB][FM];
+#pragma unroll
+  for (int q = 0; q < QB; ++q) {
+    m[q] = LOWEST;
+    l[q] = 0.f;
+#pragma unroll
+    for (int f = 0; f < FM; ++f)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[q][f][r] = 0.f;
+  }
+  int t = next(tbeg), cur = 0;
+  if (t < tend) {
+    fetch(t);
+    store(0);
+  }
+  __syncthreads();
+  while (t < tend) {
+    const int tn = next(t + 1);
+    if (tn < tend) fetch(tn);
+    const int k0 = t * TILE;
+    if (k0 < R.bmax) {
+      const bf16_t* sk = st[cur].a;
+      const bf16_t* sv = st[cur].b;
+      f32x16 s[QB][2];
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+        for (int q = 0; q < QB; ++q)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[q][kb][r] = 0.f;
+#pragma unroll
+        for (int kd = 0; kd < KD; ++kd) {
+          const bf16x8 kf = rowfrag<DP>(sk, kb, kd, lane);
+#pragma unroll
+          for (int q = 0; q < QB; ++q) s[q][kb] = El<T>::mfma(kf, qf[q][kd], s[q][kb]);
+        }
+      }
+      bool partial = k0 + TILE > R.bmin;
+      if (docs) partial |= km[t].neg | (km[t].dmin != km[t].dmax) | (R.dmin != R.dmax) | R.neg | (km[t].dmin != R.dmin);
+      if (MOD) {
+#pragma unroll
+        for (int q = 0; q < QB; ++q)
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb) {
+            f32x16& v = s[q][kb];
+            if (mod.cap) {
+#pragma unroll
+              for (int r = 0; r < 16; ++r) {
+                float w;
+                v[r] = capped(mod, v[r], w);
+              }
+            } else {
+#pragma unroll
+              for (int r = 0; r < 16; ++r) v[r] *= mod.c;
+            }
+            const int d0 = k0 + 32 * kb + 4 * hi - R.pos[q];
+            if (mod.slope) {
+              const float f0 = (float)d0;
+#pragma unroll
+              for (int r = 0; r < 16; ++r) v[r] = fmaf(-R.slope[q], fabsf(f0 + crow(r, 0)), v[r]);
+            }
+            if (mod.table) {
+#pragma unroll
+              for (int r = 0; r < 16; ++r) v[r] += tab[max(-mod.R, min(mod.R, d0 + crow(r, 0))) + mod.R];
+            }
+          }
+      }
+      if (partial) {
+#pragma unroll
+        for (int q = 0; q < QB; ++q)
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb) {
+            const int lim = R.bound[q] - k0 - 32 * kb - 4 * hi;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[q][kb][r] = crow(r, 0) < lim ? s[q][kb][r] : -INFINITY;
+            if (docs) {
+#pragma unroll
+              for (int g = 0; g < 4; ++g) {
+                const int4 dv = *(const int4*)(sdoc + cur * TILE + 32 * kb + 8 * g + 4 * hi);
+                s[q][kb][4 * g] = dv.x == R.doc[q] ? s[q][kb][4 * g] : -INFINITY;
+                s[q][kb][4 * g + 1] = dv.y == R.doc[q] ? s[q][kb][4 * g + 1] : -INFINITY;
+                s[q][kb][4 * g + 2] = dv.z == R.doc[q] ? s[q][kb][4 * g + 2] : -INFINITY;
+                s[q][kb][4 * g + 3] = dv.w == R.doc[q] ? s[q][kb][4 * g + 3] : -INFINITY;
+              }
+            }
+          }
+      }
+      const float c = MOD ? 1.f : mod.c;
+      bf16x8 pb[QB][4];
+#pragma unroll
+      for (int q = 0; q < QB; ++q) {
+        float mx = fmaxf(s[q][0][0], s[q][1][0]);
+#pragma unroll
+        for (int r = 1; r < 16; ++r) mx = fmaxf(fmaxf(mx, s[q][0][r]), s[q][1][r]);
+        mx = fmaxf(mx, xor32(mx));
+        // the running maximum is raised only when some row of the wave grew by more than DEFER exponent units: p <= 2^DEFER instead of
+        // <= 1, the same relative precision, and the common tile skips the rescale of O
+        constexpr float DEFER = 6.f;
+        if (!__all((mx - m[q]) * c <= DEFER)) {
+          const float mn = fmaxf(m[q], mx);
+          const float alpha = __builtin_amdgcn_exp2f((m[q] - mn) * c);
+          m[q] = mn;
+          l[q] *= alpha;
+#pragma unroll
+          for (int f = 0; f < FM; ++f)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[q][f][r] *= alpha;
+        }
+        const float mc = m[q] * c;
+        float rs = 0.f;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const float pv = __builtin_amdgcn_exp2f(MOD ? s[q][kb][r] - mc : fmaf(s[q][kb][r], c, -mc));
+            s[q][kb][r] = pv;
+            rs += pv;
+          }
+          pb[q][2 * kb] = pack8<T>(s[q][kb], 0);
+          pb[q][2 * kb + 1] = pack8<T>(s[q][kb], 1);
+        }
+        l[q] += rs;
+      }
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+          for (int f = 0; f < FM; ++f) {
+            const bf16x8 vf = trfrag<DP>(sv, kb, f, kk, lane);
+#pragma unroll
+            for (int q = 0; q < QB; ++q) o[q][f] = El<T>::mfma(vf, pb[q][2 * kb + kk], o[q][f]);
+          }
+    }
+    if (tn < tend) store(cur ^ 1);
+    __syncthreads();
+    cur ^= 1;
+    t = tn;
+  }
+#pragma unroll
+  for (int q = 0; q < QB; ++q) {
+    const float lt = l[q] + xor32(l[q]);
+    if (!R.ok[q]) continue;
+    const float m2 = MOD ? m[q] : m[q] * mod.c;
+    const long long sidx = ((long long)u.b * a.p.heads + u.h0) * a.p.Sq + R.r[q];
+    if (a.splits > 1) {
+      const long long at = ((long long)sp * NU + ((long long)u.b * a.nunit + u.h0 / a.gp)) * a.M + R.r[q];
+      float* po = a.part + at * D;
+#pragma unroll
+      for (int f = 0; f < FM; ++f)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int col = 32 * f + 8 * g + 4 * hi;
+          if (col < D) *(float4*)(po + col) = float4{o[q][f][4 * g], o[q][f][4 * g + 1], o[q][f][4 * g + 2], o[q][f][4 * g + 3]};
+        }
+      if (hi == 0) *(float2*)(a.part_ml + at * 2) = float2{m2, lt};
+    } else {
+      const float inv = lt > 0.f ? 1.f / lt : 0.f;
+      bf16_t* op = (bf16_t*)a.p.o.ptr + op_base(a.p.o, u.b) + (long long)R.i[q] * a.p.o.sstride + (long long)R.h[q] * D;
+#pragma unroll
+      for (int f = 0; f < FM; ++f)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int col = 32 * f + 8 * g + 4 * hi;
+          if (col < D)
+            *(uint2*)(op + col) = uint2{El<T>::pack2(o[q][f][4 * g] * inv, o[q][f][4 * g + 1] * inv),
+                                        El<T>::pack2(o[q][f][4 * g + 2] * inv, o[q][f][4 * g + 3] * inv)};
+        }
+      // base-2 log-sum-exp; +inf marks a row that saw nothing: every exp2(t - lse) of the backward pass is then 0
+      if (hi == 0 && a.p.lse) a.p.lse[sidx] = lt > 0.f ? m2 + __builtin_amdgcn_logf(lt) : INFINITY;
+    }
+  }
+}
+
+// joins the splits: one group of D / 4 lanes per row
+template <typename T>
+__global__ __launch_bounds__(256) void attn_mod_join_kernel(const Args a) {
+  const int D = a.p.D, lanes = D / 4, gpb = 256 / lanes;
+  const int g = threadIdx.x / lanes, c = threadIdx.x - g * lanes;
+  const long long rows = (long long)a.p.nbatch * a.nunit * a.M;
+  const long long row = (long long)blockIdx.x * gpb + g;
+  if (g >= gpb || row >= rows) return;
+  float m = LOWEST * 4.f;
+  for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.part_ml[((long long)s * rows + row) * 2]);
+  float l = 0.f;
+  float4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int s = 0; s < a.splits; ++s) {
+    const float2 ml = *(const float2*)(a.part_ml + ((long long)s * rows + row) * 2);
+    const float4 v = *(const float4*)(a.part + ((long long)s * rows + row) * D + 4 * c);
+    const float w = __builtin_amdgcn_exp2f(ml.x - m);
+    l = fmaf(w, ml.y, l);
+    acc.x = fmaf(w, v.x, acc.x);
+    acc.y = fmaf(w, v.y, acc.y);
+    acc.z = fmaf(w, v.z, acc.z);
+    acc.w = fmaf(w, v.w, acc.w);
+  }
+  const float inv = l > 0.f ? 1.f / l : 0.f;
+  const long long bu = row / a.M;
+  const int r = (int)(row - bu * a.M), b = (int)(bu / a.nunit), h0 = (int)(bu - (long long)b * a.nunit) * a.gp;
+  const int i = div_gp(a, r), h = h0 + r - i * a.gp;
+  bf16_t* op = (bf16_t*)a.p.o.ptr + op_base(a.p.o, b) + (long long)i * a.p.o.sstride + (long long)h * D + 4 * c;
+  *(uint2*)op = uint2{El<T>::pack2(acc.x * inv, acc.y * inv), El<T>::pack2(acc.z * inv, acc.w * inv)};
+  if (c == 0 && a.p.lse) a.p.lse[((long long)b * a.p.heads + h0) * a.p.Sq + r] = l > 0.f ? m + __builtin_amdgcn_logf(l) : INFINITY;
+}
+
+// bounds and documents of every 64 rows / keys (launched where a mask has documents or one prefix per query): one wave per tile
+__global__ __launch_bounds__(64) void attn_mod_meta_kernel(const Args a, QMeta* qm, KMeta* km, int nq, int nk) {
+  const int lane = threadIdx.x, b = blockIdx.y, t = blockIdx.x, len = seq_len(a, b);
+  if (t < nq) {
+    const int r = t * TILE + lane;
+    int lo = 0x7fffffff, hi = 0, dlo = 0x7fffffff, dhi = -1, ng = 0;
+    if (r < a.M) {
+      const int i = div_gp(a, r), d = a.p.q_docs ? a.p.q_docs[(long long)b * a.p.Sq + i] : 0;
+      const int bd = d < 0 ? 0 : row_bound(a, b, i, len);
+      lo = hi = bd;
+      if (bd > 0) dlo = dhi = d;
+      else ng = 1;
+    }
+    const QMeta q = {wave_min_i(lo), wave_max_i(hi), wave_min_i(dlo), wave_max_i(dhi), wave_max_i(ng)};
+    if (lane == 0) qm[(long long)b * nq + t] = q;
+  } else {
+    const int j = (t - nq) * TILE + lane;
+    int dlo = 0x7fffffff, dhi = -1, ng = 0;
+    if (j < len) {
+      const int d = a.p.kv_docs ? a.p.kv_docs[(long long)b * a.p.Sk + j] : 0;
+      if (d >= 0) dlo = dhi = d;
+      else ng = 1;
+    }
+    const KMeta k = {wave_min_i(dlo), wave_max_i(dhi), wave_max_i(ng)};
+    if (lane == 0) km[(long long)b * nk + t - nq] = k;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ backward: dQ, delta, table gradient
+template <typename T, int DP, int QB, bool MOD>
+__global__ __launch_bounds__(256, (DP == 64 || QB == 1) ? 2 : 1) void attn_mod_dq_kernel(const Args a) {
+  warm_kernargs<(int)sizeof(Args)>();
+  constexpr int NT = 256, KD = DP / 16, FM = DP / 32;
+  typedef Pair<DP, NT> P;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  Stage<DP>* st = (Stage<DP>*)smem;
+  int* sdoc = (int*)(smem + 2 * sizeof(Stage<DP>));
+  int* swg = sdoc + 2 * TILE;
+  float* tab = (float*)(swg + 16);                                      // [2R + 1], then [4 waves][2R + 1] sums
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5;
+  const int NU = a.p.nbatch * a.nunit;
+  const int x = blockIdx.x % NU, tile = a.ntile - 1 - blockIdx.x / NU;
+  const Unit u = unit_of(a, x);
+  const int len = seq_len(a, u.b), D = a.p.D, Sk = a.p.Sk;
+  const bf16_t* K = (const bf16_t*)a.p.k.ptr + op_base(a.p.k, u.b) + (long long)u.kv * D;
+  const bf16_t* V = (const bf16_t*)a.p.v.ptr + op_base(a.p.v, u.b) + (long long)u.kv * D;
+  const bool docs = a.kmeta && a.p.kv_docs;
+  const int* kdoc = docs ? a.p.kv_docs + (long long)u.b * Sk : nullptr;
+  const Mod mod = make_mod(a);
+  const int ntab = 2 * a.p.radius + 1;
+  float* sums = tab + ntab + wave * ntab;
+  const bool dtab = MOD && mod.table && a.p.dbias != nullptr;
+
+  Rows<QB> R;
+  load_rows(R, a, u, len, (tile * 4 + wave) * 32 * QB, lane);
+  bf16x8 qf[QB][KD], gf[QB][KD];
+  float lse[QB], dl[QB];
+#pragma unroll
+  for (int q = 0; q < QB; ++q) {
+    const bf16_t* qp = (const bf16_t*)a.p.q.ptr + op_base(a.p.q, u.b) + (long long)R.i[q] * a.p.q.sstride + (long long)R.h[q] * D;
+    const bf16_t* gp = (const bf16_t*)a.p.d_o.ptr + op_base(a.p.d_o, u.b) + (long long)R.i[q] * a.p.d_o.sstride + (long long)R.h[q] * D;
+    const bf16_t* op = (const bf16_t*)a.p.o.ptr + op_base(a.p.o, u.b) + (long long)R.i[q] * a.p.o.sstride + (long long)R.h[q] * D;
+    float d = 0.f;
+#pragma unroll
+    for (int kd = 0; kd < KD; ++kd) {
+      const bool ok = R.bound[q] > 0 && 16 * kd + 8 * hi < D;
+      qf[q][kd] = *chunk_ptr(qp + 16 * kd + 8 * hi, ok);
+      gf[q][kd] = *chunk_ptr(gp + 16 * kd + 8 * hi, ok);
+      const bf16x8 of = *chunk_ptr(op + 16 * kd + 8 * hi, ok);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) d = fmaf(El<T>::up(of[e]), El<T>::up(gf[q][kd][e]), d);
+    }
+    d += xor32(d);
+    dl[q] = d;
+    const long long sidx = ((long long)u.b * a.p.heads + u.h0) * a.p.Sq + min(R.r[q], a.M - 1);
+    lse[q] = R.ok[q] ? a.p.lse[sidx] : INFINITY;
+    if (R.ok[q] && hi == 0) a.p.delta[sidx] = d;
+  }
+  if (MOD && mod.table) load_table<T>(a, u.h0, tab, tid, NT);
+  if (dtab)
+    for (int i = lane; i < ntab; i += 64) sums[i] = 0.f;
+  if (lane == 0) {
+    swg[wave * 4] = R.bmax;
+    swg[wave * 4 + 1] = R.dmin;
+    swg[wave * 4 + 2] = R.dmax;
+  }
+  __syncthreads();
+  int bmax = 0, dmin = 0x7fffffff, dmax = -1;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    bmax = max(bmax, swg[w * 4]);
+    dmin = min(dmin, swg[w * 4 + 1]);
+    dmax = max(dmax, swg[w * 4 + 2]);
+  }
+  bmax = __builtin_amdgcn_readfirstlane(bmax);
+  const int tend = (bmax + TILE - 1) / TILE;
+  const KMeta* km = docs ? a.kmeta + (long long)u.b * ((Sk + TILE - 1) / TILE) : nullptr;
+  auto next = [&](int t) {
+    return docs ? next_tile(t, tend, [&](int c) { return km[c].dmax >= dmin && km[c].dmin <= dmax; }) : min(t, tend);
+  };
+  P nx;
+  int nd = 0, ndv[P::N];
+  auto fetch = [&](int t) {
+    const int ch = tid % P::CH;
+#pragma unroll
+    for (int i = 0; i < P::N; ++i) {
+      const int row = t * TILE + tid / P::CH + i * P::RPP;
+      const bool ok = row < len && ch * 8 < D;
+      nx.a[i] = *chunk_ptr(K + (long long)row * a.p.k.sstride + ch * 8, ok);
+      nx.b[i] = *chunk_ptr(V + (long long)row * a.p.v.sstride + ch * 8, ok);
+      if (docs) ndv[i] = kdoc[min(row, Sk - 1)];
+    }
+    if (docs && tid < TILE) {
+      const int row = t * TILE + tid;
+      nd = row < len ? kdoc[row] : -1;
+    }
+  };
+  auto store = [&](int sidx) {
+    if (docs) {
+#pragma unroll
+      for (int i = 0; i < P::N; ++i) {
+        const bf16x8 z = {0, 0, 0, 0, 0, 0, 0, 0};
+        nx.a[i] = ndv[i] < 0 ? z : nx.a[i];
+        nx.b[i] = ndv[i] < 0 ? z : nx.b[i];
+      }
+      if (tid < TILE) sdoc[sidx * TILE + tid] = nd;
+    }
+    pair_store(st[sidx], nx, tid);
+  };
+  f32x16 acc[QB][FM];
+#pragma unroll
+  for (int q = 0; q < QB; ++q)
+#pragma unroll
+    for (int f = 0; f < FM; ++f)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[q][f][r] = 0.f;
+  float below = 0.f, above = 0.f;                                       // gradient of the table's two ends, per lane
+  int t = next(0), cur = 0;
+  if (t < tend) {
+    fetch(t);
+    store(0);
+  }
+  __syncthreads();
+  while (t < tend) {
+    const int tn = next(t + 1);
+    if (tn < tend) fetch(tn);
+    const int k0 = t * TILE;
+    if (k0 < R.bmax) {
+      const bf16_t* sk = st[cur].a;
+      const bf16_t* sv = st[cur].b;
+      bool partial = k0 + TILE > R.bmin;
+      if (docs) partial |= km[t].neg | (km[t].dmin != km[t].dmax) | (R.dmin != R.dmax) | R.neg | (km[t].dmin != R.dmin);
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+        f32x16 s[QB], dp[QB];
+#pragma unroll
+        for (int q = 0; q < QB; ++q)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[q][r] = dp[q][r] = 0.f;
+#pragma unroll
+        for (int kd = 0; kd < KD; ++kd) {
+          const bf16x8 kf = rowfrag<DP>(sk, kb, kd, lane), vf = rowfrag<DP>(sv, kb, kd, lane);
+#pragma unroll
+          for (int q = 0; q < QB; ++q) {
+            s[q] = El<T>::mfma(kf, qf[q][kd], s[q]);
+            dp[q] = El<T>::mfma(vf, gf[q][kd], dp[q]);
+          }
+        }
+        bf16x8 db[QB][2];
+#pragma unroll
+        for (int q = 0; q < QB; ++q) {
+          const int d0 = k0 + 32 * kb + 4 * hi - R.pos[q];
+          f32x16 w;                                                     // derivative of the cap
+          if (MOD) {
+            if (mod.cap) {
+#pragma unroll
+              for (int r = 0; r < 16; ++r) {
+                float y;
+                s[q][r] = capped(mod, s[q][r], y);
+                w[r] = 4.f * y * (1.f - y);
+              }
+            } else {
+#pragma unroll
+              for (int r = 0; r < 16; ++r) s[q][r] *= mod.c;
+            }
+            if (mod.slope) {
+              const float f0 = (float)d0;
+#pragma unroll
+              for (int r = 0; r < 16; ++r) s[q][r] = fmaf(-R.slope[q], fabsf(f0 + crow(r, 0)), s[q][r]);
+            }
+            if (mod.table) {
+#pragma unroll
+              for (int r = 0; r < 16; ++r) s[q][r] += tab[max(-mod.R, min(mod.R, d0 + crow(r, 0))) + mod.R];
+            }
+          }
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const float pv = __builtin_amdgcn_exp2f(MOD ? s[q][r] - lse[q] : fmaf(s[q][r], mod.c, -lse[q]));
+            s[q][r] = pv * (dp[q][r] - dl[q]);
+          }
+          if (partial) {
+            const int lim = R.bound[q] - k0 - 32 * kb - 4 * hi;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[q][r] = crow(r, 0) < lim ? s[q][r] : 0.f;
+            if (docs) {
+#pragma unroll
+              for (int g = 0; g < 4; ++g) {
+                const int4 dv = *(const int4*)(sdoc + cur * TILE + 32 * kb + 8 * g + 4 * hi);
+                s[q][4 * g] = dv.x == R.doc[q] ? s[q][4 * g] : 0.f;
+                s[q][4 * g + 1] = dv.y == R.doc[q] ? s[q][4 * g + 1] : 0.f;
+                s[q][4 * g + 2] = dv.z == R.doc[q] ? s[q][4 * g + 2] : 0.f;
+                s[q][4 * g + 3] = dv.w == R.doc[q] ? s[q][4 * g + 3] : 0.f;
+              }
+            }
+          }
+          if (dtab) {
+            // sums over diagonals, in the wave's own table, by LDS additions that complete in program order: a register's 32 lanes of one
+            // half hold 32 different distances, so one half at a time meets no address twice and the order of the additions is fixed
+            // (the wave barriers keep the compiler from joining the two halves); the clipped ends are summed per lane
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const int d = d0 + crow(r, 0);
+              const float v = s[q][r];
+              const bool in = d > -mod.R && d < mod.R;
+              below += d <= -mod.R ? v : 0.f;
+              above += (d >= mod.R && d > -mod.R) ? v : 0.f;
+#pragma unroll
+              for (int half = 0; half < 2; ++half) {
+                if (in && hi == half) __builtin_amdgcn_ds_atomic_fadd_f32((__attribute__((address_space(3))) float*)(sums + d + mod.R), v);
+                __builtin_amdgcn_wave_barrier();
+              }
+            }
+          }
+          if (MOD && mod.cap) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[q][r] *= w[r];
+          }
+          db[q][0] = pack8<T>(s[q], 0);
+          db[q][1] = pack8<T>(s[q], 1);
+        }
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+          for (int f = 0; f < FM; ++f) {
+            const bf16x8 kt = trfrag<DP>(sk, kb, f, kk, lane);
+#pragma unroll
+            for (int q = 0; q < QB; ++q) acc[q][f] = El<T>::mfma(kt, db[q][kk], acc[q][f]);
+          }
+      }
+    }
+    if (tn < tend) store(cur ^ 1);
+    __syncthreads();
+    cur ^= 1;
+    t = tn;
+  }
+#pragma unroll
+  for (int q = 0; q < QB; ++q) {
+    if (!R.ok[q]) continue;
+    bf16_t* op = (bf16_t*)a.p.dq.ptr + op_base(a.p.dq, u.b) + (long long)R.i[q] * a.p.dq.sstride + (long long)R.h[q] * D;
+#pragma unroll
+    for (int f = 0; f < FM; ++f)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int col = 32 * f + 8 * g + 4 * hi;
+        const float c = a.p.scale;
+        if (col < D)
+          *(uint2*)(op + col) = uint2{El<T>::pack2(acc[q][f][4 * g] * c, acc[q][f][4 * g + 1] * c),
+                                      El<T>::pack2(acc[q][f][4 * g + 2] * c, acc[q][f][4 * g + 3] * c)};
+      }
+  }
+  if (dtab) {
+    below = wave_sum(below);
+    above = wave_sum(above);
+    if (lane == 0) {
+      sums[0] += below;
+      sums[ntab - 1] += above;
+    }
+    __syncthreads();
+    float* out = a.part_bias + (((long long)u.b * a.ntile + tile) * a.p.heads + u.h0) * ntab;
+    for (int i = tid; i < ntab; i += NT) {
+      const float* w0 = tab + ntab + i;
+      out[i] = (w0[0] + w0[ntab]) + (w0[2 * ntab] + w0[3 * ntab]);
+    }
+  }
+}
+
+// dtable[h][d] = sum over (batch, row tile), in order; entries that hide their distance get 0 by construction (P = 0 there)
+template <typename T>
+__global__ __launch_bounds__(256) void attn_mod_dbias_kernel(const Args a) {
+  const long long n = (long long)a.p.heads * (2 * a.p.radius + 1), i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  float s = 0.f;
+#pragma unroll 4
+  for (int k = 0; k < a.p.nbatch * a.ntile; ++k) s += a.part_bias[(long long)k * n + i];
+  if (a.p.bias_f32) ((float*)a.p.dbias)[i] = s;
+  else ((unsigned short*)a.p.dbias)[i] = (unsigned short)(El<T>::pack2(s, 0.f) & 0xffffu);
+}
+
+// ------------------------------------------------------------------------------------------------ backward: dK, dV
+struct RowInfo {                    // of one staged query row
+  float lse, delta, slope;
+  int bound, pos, doc;
+};
+template <typename T, int DP, int KB, bool MOD>
+__global__ __launch_bounds__(256, (DP == 64 && KB == 1) ? 2 : 1) void attn_mod_dkdv_kernel(const Args a) {
+  warm_kernargs<(int)sizeof(Args)>();
+  constexpr int NT = 256, KD = DP / 16, FM = DP / 32;
+  typedef Pair<DP, NT> P;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  Stage<DP>* st = (Stage<DP>*)smem;
+  float* sinfo = (float*)(smem + 2 * sizeof(Stage<DP>));                // [2][6][TILE]: lse, delta, slope, bound, pos, doc
+  float* tab = sinfo + 2 * 6 * TILE;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5;
+  const int NKV = a.p.nbatch * a.p.kv_heads;
+  const int y = blockIdx.x % NKV, rest = blockIdx.x / NKV;
+  const int sp = rest % a.splits, ktile = rest / a.splits;              // early keys are seen by the most rows of a causal mask: first
+  const int b = y / a.p.kv_heads, kv = y - b * a.p.kv_heads;
+  const int len = seq_len(a, b), D = a.p.D, Sk = a.p.Sk, G = a.p.heads / a.p.kv_heads, GU = G / a.gp;
+  const bool docs = a.kmeta && a.p.kv_docs;
+  const Mod mod = make_mod(a);
+  const bf16_t* Q = (const bf16_t*)a.p.q.ptr + op_base(a.p.q, b);
+  const bf16_t* dO = (const bf16_t*)a.p.d_o.ptr + op_base(a.p.d_o, b);
+  const int kw0 = (ktile * 4 + wave) * 32 * KB;                         // the wave's first key
+  int key[KB], kd_[KB];
+  bf16x8 kf[KB][KD], vf[KB][KD];
+  int dlo = 0x7fffffff, dhi = -1, ng = 0;
+#pragma unroll
+  for (int j = 0; j < KB; ++j) {
+    key[j] = kw0 + 32 * j + (lane & 31);
+    const int kc = min(key[j], Sk - 1);
+    kd_[j] = docs ? a.p.kv_docs[(long long)b * Sk + kc] : 0;
+    const bool ok = key[j] < len && kd_[j] >= 0;
+    if (ok) {
+      dlo = min(dlo, kd_[j]);
+      dhi = max(dhi, kd_[j]);
+    } else {
+      kd_[j] = -1;
+      ng = 1;
+    }
+    const bf16_t* kp = (const bf16_t*)a.p.k.ptr + op_base(a.p.k, b) + (long long)kc * a.p.k.sstride + (long long)kv * D;
+    const bf16_t* vp = (const bf16_t*)a.p.v.ptr + op_base(a.p.v, b) + (long long)kc * a.p.v.sstride + (long long)kv * D;
+#pragma unroll
+    for (int kd = 0; kd < KD; ++kd) {
+      kf[j][kd] = *chunk_ptr(kp + 16 * kd + 8 * hi, ok && 16 * kd + 8 * hi < D);
+      vf[j][kd] = *chunk_ptr(vp + 16 * kd + 8 * hi, ok && 16 * kd + 8 * hi < D);
+    }
+  }
+  const int wdmin = wave_min_i(dlo), wdmax = wave_max_i(dhi);
+  const bool wneg = wave_max_i(ng) != 0;
+  // over the workgroup's 128 KB keys
+  const int wk0 = ktile * 4 * 32 * KB;
+  int gdmin = 0x7fffffff, gdmax = -1;
+  if (docs) {
+    const KMeta* km = a.kmeta + (long long)b * ((Sk + TILE - 1) / TILE);
+    for (int t = wk0 / TILE; t < min((Sk + TILE - 1) / TILE, (wk0 + 128 * KB) / TILE); ++t) {
+      gdmin = min(gdmin, km[t].dmin);
+      gdmax = max(gdmax, km[t].dmax);
+    }
+  }
+  f32x16 ka[KB][FM], va[KB][FM];
+#pragma unroll
+  for (int j = 0; j < KB; ++j)
+#pragma unroll
+    for (int f = 0; f < FM; ++f)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) ka[j][f][r] = va[j][f][r] = 0.f;
+
+  // row tiles of all units of the K/V head, numbered through; a split takes a run of them
+  const int ntr = (a.M + TILE - 1) / TILE, total = ntr * GU, per = (total + a.splits - 1) / a.splits;
+  const int tbeg = min(total, sp * per), tend = wk0 < len ? min(total, tbeg + per) : tbeg;
+  const QMeta* qm = a.qmeta ? a.qmeta + (long long)b * ntr : nullptr;
+  // largest / smallest bound of row tile t
+  auto tile_bounds = [&](int t, int& lo, int& hi_) {
+    if (qm) {
+      lo = qm[t].bmin;
+      hi_ = qm[t].bmax;
+    } else {      // bounds grow with the query
+      lo = t * TILE + TILE > a.M ? 0 : row_bound(a, b, div_gp(a, t * TILE), len);
+      hi_ = row_bound(a, b, div_gp(a, min(a.M, t * TILE + TILE) - 1), len);
+    }
+  };
+  auto active = [&](int c) {
+    const int t = c % ntr;
+    int lo, hi_;
+    tile_bounds(t, lo, hi_);
+    bool ok = hi_ > wk0;
+    if (docs) ok = ok && qm[t].dmax >= gdmin && qm[t].dmin <= gdmax;
+    return ok;
+  };
+  auto next = [&](int c) { return (a.p.causal || docs) ? next_tile(c, tend, active) : min(c, tend); };
+  P nx;
+  RowInfo ni;
+  int nb[P::N];
+  auto fetch = [&](int c) {
+    const int gu = c / ntr, t = c - gu * ntr, h0 = kv * G + gu * a.gp, ch = tid % P::CH;
+    auto info = [&](int r, int& i, int& h, int& doc) {
+      const int rc = min(r, a.M - 1);
+      i = div_gp(a, rc);
+      h = h0 + rc - i * a.gp;
+      doc = docs ? a.p.q_docs[(long long)b * a.p.Sq + i] : 0;
+      return (r < a.M && doc >= 0) ? row_bound(a, b, i, len) : 0;
+    };
+#pragma unroll
+    for (int n = 0; n < P::N; ++n) {
+      int i, h, doc;
+      nb[n] = info(t * TILE + tid / P::CH + n * P::RPP, i, h, doc);
+      const bool ok = ch * 8 < D;
+      nx.a[n] = *chunk_ptr(Q + (long long)i * a.p.q.sstride + (long long)h * D + ch * 8, ok);
+      nx.b[n] = *chunk_ptr(dO + (long long)i * a.p.d_o.sstride + (long long)h * D + ch * 8, ok);
+    }
+    if (tid < TILE) {
+      int i, h;
+      const int r = t * TILE + tid;
+      ni.bound = info(r, i, h, ni.doc);
+      ni.pos = i + len - a.p.Sq;
+      ni.slope = a.p.slopes ? a.p.slopes[h] * LOG2E : 0.f;
+      const long long sidx = ((long long)b * a.p.heads + h0) * a.p.Sq + min(r, a.M - 1);
+      ni.lse = ni.bound > 0 ? a.p.lse[sidx] : INFINITY;
+      ni.delta = ni.bound > 0 ? a.p.delta[sidx] : 0.f;
+    }
+  };
+  auto store = [&](int sidx) {
+#pragma unroll
+    for (int n = 0; n < P::N; ++n) {
+      const bf16x8 z = {0, 0, 0, 0, 0, 0, 0, 0};
+      nx.a[n] = nb[n] > 0 ? nx.a[n] : z;
+      nx.b[n] = nb[n] > 0 ? nx.b[n] : z;
+    }
+    pair_store(st[sidx], nx, tid);
+    if (tid < TILE) {
+      float* s = sinfo + sidx * 6 * TILE + tid;
+      s[0] = ni.lse;
+      s[TILE] = ni.delta;
+      s[2 * TILE] = ni.slope;
+      s[3 * TILE] = __int_as_float(ni.bound);
+      s[4 * TILE] = __int_as_float(ni.pos);
+      s[5 * TILE] = __int_as_float(ni.doc);
+    }
+  };
+  int c = next(tbeg), cur = 0, gu_tab = -1;
+  if (c < tend) {
+    fetch(c);
+    store(0);
+  }
+  __syncthreads();
+  while (c < tend) {
+    const int cn = next(c + 1);
+    if (cn < tend) fetch(cn);
+    const int gu = c / ntr, t = c - gu * ntr;
+    if (MOD && mod.table && gu != gu_tab) {                             // workgroup-uniform: the next head's table
+      if (gu_tab >= 0) __syncthreads();
+      load_table<T>(a, kv * G + gu, tab, tid, NT);
+      gu_tab = gu;
+      __syncthreads();
+    }
+    int blo, bhi;
+    tile_bounds(t, blo, bhi);
+    if (kw0 < bhi) {
+      const bf16_t* sq = st[cur].a;
+      const bf16_t* sg = st[cur].b;
+      const float* in = sinfo + cur * 6 * TILE;
+      bool partial = kw0 + 32 * KB > blo;
+      if (docs) partial |= wneg | (wdmin != wdmax) | (qm[t].dmin != qm[t].dmax) | (qm[t].neg != 0) | (qm[t].dmin != wdmin);
+#pragma unroll
+      for (int qb = 0; qb < 2; ++qb) {
+        f32x16 s[KB], dp[KB];
+#pragma unroll
+        for (int j = 0; j < KB; ++j)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[j][r] = dp[j][r] = 0.f;
+#pragma unroll
+        for (int kd = 0; kd < KD; ++kd) {
+          const bf16x8 qa = rowfrag<DP>(sq, qb, kd, lane), da = rowfrag<DP>(sg, qb, kd, lane);
+#pragma unroll
+          for (int j = 0; j < KB; ++j) {
+            s[j] = El<T>::mfma(qa, kf[j][kd], s[j]);
+            dp[j] = El<T>::mfma(da, vf[j][kd], dp[j]);
+          }
+        }
+        bf16x8 pb[KB][2], db[KB][2];
+#pragma unroll
+        for (int j = 0; j < KB; ++j) {
+          f32x16 pr;
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const int o = 32 * qb + 8 * g + 4 * hi;
+            const f32x4 L = *(const f32x4*)(in + o), E = *(const f32x4*)(in + TILE + o);
+            f32x4 W = {1.f, 1.f, 1.f, 1.f};
+            if (MOD) {
+              if (mod.cap) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  float w;
+                  s[j][4 * g + e] = capped(mod, s[j][4 * g + e], w);
+                  W[e] = 4.f * w * (1.f - w);
+                }
+              } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[j][4 * g + e] *= mod.c;
+              }
+              if (mod.slope | mod.table) {
+                const int4 pos = *(const int4*)(in + 4 * TILE + o);
+                const int ps[4] = {pos.x, pos.y, pos.z, pos.w};
+                if (mod.slope) {
+                  const f32x4 sl = *(const f32x4*)(in + 2 * TILE + o);
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) s[j][4 * g + e] = fmaf(-sl[e], fabsf((float)(key[j] - ps[e])), s[j][4 * g + e]);
+                }
+                if (mod.table) {
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) s[j][4 * g + e] += tab[max(-mod.R, min(mod.R, key[j] - ps[e])) + mod.R];
+                }
+              }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              pr[4 * g + e] = __builtin_amdgcn_exp2f(MOD ? s[j][4 * g + e] - L[e] : fmaf(s[j][4 * g + e], mod.c, -L[e]));
+            if (partial) {
+              const int4 bd = *(const int4*)(in + 3 * TILE + o);
+              const int bs[4] = {bd.x, bd.y, bd.z, bd.w};
+#pragma unroll
+              for (int e = 0; e < 4; ++e) pr[4 * g + e] = key[j] < bs[e] ? pr[4 * g + e] : 0.f;
+              if (docs) {
+                const int4 dc = *(const int4*)(in + 5 * TILE + o);
+                const int ds[4] = {dc.x, dc.y, dc.z, dc.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) pr[4 * g + e] = kd_[j] == ds[e] ? pr[4 * g + e] : 0.f;
+              }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[j][4 * g + e] = pr[4 * g + e] * (dp[j][4 * g + e] - E[e]) * W[e];
+          }
+          pb[j][0] = pack8<T>(pr, 0);
+          pb[j][1] = pack8<T>(pr, 1);
+          db[j][0] = pack8<T>(s[j], 0);
+          db[j][1] = pack8<T>(s[j], 1);
+        }
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+          for (int f = 0; f < FM; ++f) {
+            const bf16x8 gt = trfrag<DP>(sg, qb, f, kk, lane), qt = trfrag<DP>(sq, qb, f, kk, lane);
+#pragma unroll
+            for (int j = 0; j < KB; ++j) {
+              va[j][f] = El<T>::mfma(gt, pb[j][kk], va[j][f]);
+              ka[j][f] = El<T>::mfma(qt, db[j][kk], ka[j][f]);
+            }
+          }
+      }
+    }
+    if (cn < tend) store(cur ^ 1);
+    __syncthreads();
+    cur ^= 1;
+    c = cn;
+  }
+#pragma unroll
+  for (int j = 0; j < KB; ++j) {
+    if (key[j] >= Sk) continue;
+    if (a.to_part) {
+      const long long n = (long long)NKV * Sk * D, at = (((long long)b * a.p.kv_heads + kv) * Sk + key[j]) * D;
+      float* pk = a.part + (long long)sp * 2 * n + at;
+#pragma unroll
+      for (int f = 0; f < FM; ++f)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int col = 32 * f + 8 * g + 4 * hi;
+          if (col < D) {
+            *(float4*)(pk + col) = float4{ka[j][f][4 * g], ka[j][f][4 * g + 1], ka[j][f][4 * g + 2], ka[j][f][4 * g + 3]};
+            *(float4*)(pk + n + col) = float4{va[j][f][4 * g], va[j][f][4 * g + 1], va[j][f][4 * g + 2], va[j][f][4 * g + 3]};
+          }
+        }
+    } else {
+      bf16_t* kp = (bf16_t*)a.p.dk.ptr + op_base(a.p.dk, b) + (long long)key[j] * a.p.dk.sstride + (long long)kv * D;
+      bf16_t* vp = (bf16_t*)a.p.dv.ptr + op_base(a.p.dv, b) + (long long)key[j] * a.p.dv.sstride + (long long)kv * D;
+      const float sc = a.p.scale;
+#pragma unroll
+      for (int f = 0; f < FM; ++f)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int col = 32 * f + 8 * g + 4 * hi;
+          if (col < D) {
+            *(uint2*)(kp + col) = uint2{El<T>::pack2(ka[j][f][4 * g] * sc, ka[j][f][4 * g + 1] * sc),
+                                        El<T>::pack2(ka[j][f][4 * g + 2] * sc, ka[j][f][4 * g + 3] * sc)};
+            *(uint2*)(vp + col) = uint2{El<T>::pack2(va[j][f][4 * g], va[j][f][4 * g + 1]), El<T>::pack2(va[j][f][4 * g + 2], va[j][f][4 * g + 3])};
+          }
+        }
+    }
+  }
+}
+
+// dK, dV = sum of the partial sums of the splits and of the batches that share a K / V head, in order
+template <typename T>
+__global__ __launch_bounds__(256) void attn_mod_dkdv_join_kernel(const Args a) {
+  const int D = a.p.D, lanes = D / 4, share = a.p.kv_share;
+  const int nbk = (a.p.nbatch + share - 1) / share;
+  const long long per = (long long)a.p.kv_heads * a.p.Sk * D, n = per * a.p.nbatch;        // of a batch, of a split
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i * 4 >= per * nbk) return;
+  const long long row = i / lanes;
+  const int c = (int)(i - row * lanes) * 4;
+  const long long bk = row / a.p.Sk;
+  const int key = (int)(row - bk * a.p.Sk), b0 = (int)(bk / a.p.kv_heads) * share, kv = (int)(bk % a.p.kv_heads);
+  float4 k = {0.f, 0.f, 0.f, 0.f}, v = {0.f, 0.f, 0.f, 0.f};
+  for (int b = b0; b < min(b0 + share, a.p.nbatch); ++b) {
+    const float* p0 = a.part + b * per + ((long long)kv * a.p.Sk + key) * D + c;
+#pragma unroll 4
+    for (int s = 0; s < a.splits; ++s) {
+      const float4 x = *(const float4*)(p0 + s * 2 * n), y = *(const float4*)(p0 + s * 2 * n + n);
+      k.x += x.x;
+      k.y += x.y;
+      k.z += x.z;
+      k.w += x.w;
+      v.x += y.x;
+      v.y += y.y;
+      v.z += y.z;
+      v.w += y.w;
+    }
+  }
+  bf16_t* kp = (bf16_t*)a.p.dk.ptr + op_base(a.p.dk, b0) + (long long)key * a.p.dk.sstride + (long long)kv * D + c;
+  bf16_t* vp = (bf16_t*)a.p.dv.ptr + op_base(a.p.dv, b0) + (long long)key * a.p.dv.sstride + (long long)kv * D + c;
+  const float sc = a.p.scale;
+  *(uint2*)kp = uint2{El<T>::pack2(k.x * sc, k.y * sc), El<T>::pack2(k.z * sc, k.w * sc)};
+  *(uint2*)vp = uint2{El<T>::pack2(v.x, v.y), El<T>::pack2(v.z, v.w)};
+}
+
+// ------------------------------------------------------------------------------------------------ host
+struct Layout {
+  Args a;
+  int qb, dp;
+  int fwd_tiles, fwd_splits, dq_tiles, kv_tiles, kv_splits;
+  bool meta;
+  long long o_qmeta, o_kmeta, o_part, o_ml, o_bias, bytes;
+};
+
+long long align256(long long n) { return (n + 255) & ~255ll; }
+
+int check_mod(const char* fn, const T2VAttnMod* p, bool bwd) {
+  T2V_CHECK_ARG(p && p->nbatch > 0 && p->heads > 0 && p->kv_heads > 0 && p->Sq > 0 && p->Sk > 0, "%s: bad dims", fn);
+  T2V_CHECK_ARG(p->heads % p->kv_heads == 0, "%s: %d heads cannot share %d key / value heads evenly", fn, p->heads, p->kv_heads);
+  T2V_CHECK_ARG(p->D >= 8 && p->D <= 128 && p->D % 8 == 0, "%s: the head dim must be a multiple of 8 up to 128 (got %d)", fn, p->D);
+  T2V_CHECK_ARG(p->dtype == 0 || p->dtype == 1, "%s: bf16 (0) or fp16 (1) operands are wanted", fn);
+  T2V_CHECK_ARG(p->softcap >= 0.f && p->softcap < 1e30f && p->scale == p->scale, "%s: bad softcap / scale", fn);
+  T2V_CHECK_ARG((p->q_docs == nullptr) == (p->kv_docs == nullptr), "%s: documents of queries and keys come together", fn);
+  T2V_CHECK_ARG(!p->prefix || p->causal, "%s: a prefix opens a causal mask: set causal", fn);
+  T2V_CHECK_ARG(!p->bias || (p->radius >= 0 && p->radius <= 1024), "%s: the table's radius must be 0..1024 (got %d)", fn, p->radius);
+  T2V_CHECK_ARG((long long)p->Sq * p->heads < (1ll << 26) && p->Sk < (1 << 26), "%s: too many rows (Sq * heads and Sk below 2^26)", fn);
+  T2V_CHECK_ARG((long long)p->nbatch * p->heads < (1 << 20), "%s: nbatch * heads below 2^20 is wanted", fn);
+  const T2VAttnOperand* ops[] = {&p->q, &p->k, &p->v, &p->o, &p->d_o, &p->dq, &p->dk, &p->dv};
+  const char* names[] = {"q", "k", "v", "o", "d_o", "dq", "dk", "dv"};
+  for (int i = 0; i < (bwd ? 8 : 4); ++i) {
+    const T2VAttnOperand& o = *ops[i];
+    T2V_CHECK_ARG(o.ptr && o.bdiv > 0 && ((uintptr_t)o.ptr & 15) == 0 && o.sstride % 8 == 0 && o.bstride_hi % 8 == 0 && o.bstride_lo % 8 == 0,
+                  "%s: operand %s: 16-byte aligned rows are wanted (ptr %p, row stride %lld)", fn, names[i], o.ptr, o.sstride);
+  }
+  T2V_CHECK_ARG(!bwd || (p->lse && p->delta), "%s: lse and delta are required", fn);
+  T2V_CHECK_ARG(!bwd || p->kv_share >= 1, "%s: kv_share is the number of batches that share a K / V (1: none do)", fn);
+  return T2V_OK;
+}
+
+Layout make_layout(const T2VAttnMod* p, bool bwd) {
+  Layout L{};
+  Args& a = L.a;
+  a.p = *p;
+  const int G = p->heads / p->kv_heads;
+  a.gp = p->bias ? 1 : G;
+  a.nunit = p->heads / a.gp;
+  a.M = p->Sq * a.gp;
+  a.magic = a.gp > 1 ? (unsigned)(((1ull << 32) + a.gp - 1) / a.gp) : 0;
+  L.dp = p->D <= 64 ? 64 : 128;
+  const long long NU = (long long)p->nbatch * a.nunit;
+  L.qb = 1;
+  const int rows = 128 * L.qb;
+  L.fwd_tiles = (a.M + rows - 1) / rows;
+  L.fwd_splits = 1;
+  if (!bwd) {
+    // few workgroups and a long key axis: split the keys until ~512 workgroups exist, at least four 64-key tiles each
+    const long long wgs = NU * L.fwd_tiles;
+    const int kt = (p->Sk + TILE - 1) / TILE;
+    if (wgs < 256) {
+      int s = (int)(512 / wgs);
+      s = s < kt / 4 ? s : kt / 4;
+      s = s > 64 ? 64 : s;
+      L.fwd_splits = s > 1 ? s : 1;
+    }
+  }
+  L.dq_tiles = (a.M + 127) / 128;
+  L.kv_tiles = (p->Sk + 127) / 128;
+  L.kv_splits = 1;
+  if (bwd) {
+    const long long wgs = (long long)p->nbatch * p->kv_heads * L.kv_tiles, tiles = (long long)((a.M + TILE - 1) / TILE) * (G / a.gp);
+    if (wgs < 256) {
+      long long s = 512 / wgs;
+      s = s < tiles / 4 ? s : tiles / 4;
+      s = s > 16 ? 16 : s;
+      L.kv_splits = s > 1 ? (int)s : 1;
+    }
+  }
+  L.meta = p->q_docs || (p->prefix && p->prefix_per_query);
+  long long at = 0;
+  if (L.meta) {
+    L.o_qmeta = at;
+    at = align256(at + (long long)sizeof(QMeta) * p->nbatch * ((a.M + TILE - 1) / TILE));
+    L.o_kmeta = at;
+    at = align256(at + (long long)sizeof(KMeta) * p->nbatch * ((p->Sk + TILE - 1) / TILE));
+  }
+  if (!bwd && L.fwd_splits > 1) {
+    L.o_part = at;
+    at = align256(at + 4ll * L.fwd_splits * NU * a.M * p->D);
+    L.o_ml = at;
+    at = align256(at + 8ll * L.fwd_splits * NU * a.M);
+  }
+  if (bwd && (L.kv_splits > 1 || p->kv_share > 1)) {
+    L.o_part = at;
+    at = align256(at + 8ll * L.kv_splits * p->nbatch * p->kv_heads * p->Sk * p->D);
+  }
+  if (bwd && p->dbias) {
+    L.o_bias = at;
+    at = align256(at + 4ll * p->nbatch * L.dq_tiles * p->heads * (2 * p->radius + 1));
+  }
+  L.bytes = at;
+  char* w = (char*)p->workspace;
+  if (L.meta) {
+    a.qmeta = (const QMeta*)(w + L.o_qmeta);
+    a.kmeta = (const KMeta*)(w + L.o_kmeta);
+  }
+  a.part = (float*)(w + L.o_part);
+  a.part_ml = (float*)(w + L.o_ml);
+  a.part_bias = (float*)(w + L.o_bias);
+  return L;
+}
+
+size_t smem_bytes(const Layout& L, int tables, bool kv) {
+  return 2 * 2 * (size_t)TILE * L.dp * 2 + (kv ? 2 * 6 * TILE * 4 : 2 * TILE * 4 + 64) + (L.a.p.bias ? tables * 4 * (2 * (size_t)L.a.p.radius + 1) : 0);
+}
+template <typename K>
+int launch(int which, K kern, long long grid, size_t smem, hipStream_t st, const Args& a) {
+  if (smem > 64 * 1024) {
+    const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != hipSuccess) {
+      t2v_set_error("t2v_attn_mod: %zu bytes of shared memory: %s", smem, hipGetErrorString(e));
+      return T2V_ELAUNCH;
+    }
+  }
+  t2v_launch_timed(which, kern, dim3((unsigned)grid), dim3(256), (unsigned)smem, st, a);
+  return T2V_OK;
+}
+bool modded(const T2VAttnMod* p) { return p->softcap > 0.f || p->slopes || p->bias || !(p->scale > 0.f); }
+
+template <typename T, int DP>
+int run_fwd(Layout& L, hipStream_t st) {
+  Args& a = L.a;
+  a.ntile = L.fwd_tiles;
+  a.splits = L.fwd_splits;
+  const long long grid = (long long)a.p.nbatch * a.nunit * L.fwd_tiles * L.fwd_splits;
+  const size_t sm = smem_bytes(L, 1, false);
+  const int which = L.fwd_splits > 1 ? 1 : 3;
+  const int e = modded(&a.p) ? launch(which, attn_mod_fwd_kernel<T, DP, 1, true>, grid, sm, st, a)
+                             : launch(which, attn_mod_fwd_kernel<T, DP, 1, false>, grid, sm, st, a);
+  if (e) return e;
+  T2V_CHECK_LAUNCH();
+  if (L.fwd_splits > 1) {
+    const int gpb = 256 / (a.p.D / 4);
+    const long long rows = (long long)a.p.nbatch * a.nunit * a.M;
+    T2V_LAUNCH_LAST(attn_mod_join_kernel<T>, dim3((unsigned)((rows + gpb - 1) / gpb)), dim3(256), 0, st, a);
+    T2V_CHECK_LAUNCH();
+  }
+  return T2V_OK;
+}
+template <typename T, int DP>
+int run_bwd(Layout& L, hipStream_t st) {
+  Args& a = L.a;
+  const bool mod = modded(&a.p);
+  a.ntile = L.dq_tiles;
+  a.splits = 1;
+  const size_t sm = smem_bytes(L, a.p.dbias ? 5 : 1, false);
+  const long long gq = (long long)a.p.nbatch * a.nunit * L.dq_tiles;
+  int e = mod ? launch(1, attn_mod_dq_kernel<T, DP, 1, true>, gq, sm, st, a) : launch(1, attn_mod_dq_kernel<T, DP, 1, false>, gq, sm, st, a);
+  if (e) return e;
+  T2V_CHECK_LAUNCH();
+  if (a.p.dbias) {
+    const long long n = (long long)a.p.heads * (2 * a.p.radius + 1);
+    hipLaunchKernelGGL(attn_mod_dbias_kernel<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, a);
+    T2V_CHECK_LAUNCH();
+  }
+  a.ntile = L.kv_tiles;
+  a.splits = L.kv_splits;
+  const long long gk = (long long)a.p.nbatch * a.p.kv_heads * L.kv_tiles * L.kv_splits;
+  const size_t smk = smem_bytes(L, 1, true);
+  a.to_part = L.kv_splits > 1 || a.p.kv_share > 1;
+  const int which = a.to_part ? 0 : 2;
+  e = mod ? launch(which, attn_mod_dkdv_kernel<T, DP, 1, true>, gk, smk, st, a) : launch(which, attn_mod_dkdv_kernel<T, DP, 1, false>, gk, smk, st, a);
+  if (e) return e;
+  T2V_CHECK_LAUNCH();
+  if (a.to_part) {
+    const long long n = (long long)((a.p.nbatch + a.p.kv_share - 1) / a.p.kv_share) * a.p.kv_heads * a.p.Sk * a.p.D / 4;
+    T2V_LAUNCH_LAST(attn_mod_dkdv_join_kernel<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, a);
+    T2V_CHECK_LAUNCH();
+  }
+  return T2V_OK;
+}
+int run(const char* fn, const T2VAttnMod* p, bool bwd, hipStream_t st) {
+  if (int e = check_mod(fn, p, bwd)) return e;
+  Layout L = make_layout(p, bwd);
+  T2V_CHECK_ARG(L.bytes == 0 || (p->workspace && ((uintptr_t)p->workspace & 255) == 0 && p->workspace_bytes >= L.bytes),
+                "%s: a 256-byte aligned workspace of %lld bytes is wanted (got %p, %lld)", fn, L.bytes, p->workspace, p->workspace_bytes);
+  const long long worst = (long long)p->nbatch * (p->heads > p->kv_heads ? p->heads : p->kv_heads) *
+                          (L.fwd_tiles * (long long)L.fwd_splits > L.kv_tiles * (long long)L.kv_splits ? L.fwd_tiles * (long long)L.fwd_splits
+                                                                                                         : L.kv_tiles * (long long)L.kv_splits);
+  T2V_CHECK_ARG(worst < (1ll << 31), "%s: too many workgroups", fn);
+  if (L.meta) {
+    const int nq = (L.a.M + TILE - 1) / TILE, nk = (p->Sk + TILE - 1) / TILE;
+    T2V_CHECK_ARG(p->nbatch <= 65535, "%s: at most 65535 batches with documents or one prefix per query", fn);
+    hipLaunchKernelGGL(attn_mod_meta_kernel, dim3(nq + nk, p->nbatch), dim3(64), 0, st, L.a, (QMeta*)L.a.qmeta, (KMeta*)L.a.kmeta, nq, nk);
+    T2V_CHECK_LAUNCH();
+  }
+  if (p->dtype == 0) {
+    if (L.dp == 64) return bwd ? run_bwd<bf16_t, 64>(L, st) : run_fwd<bf16_t, 64>(L, st);
+    return bwd ? run_bwd<bf16_t, 128>(L, st) : run_fwd<bf16_t, 128>(L, st);
+  }
+  if (L.dp == 64) return bwd ? run_bwd<_Float16, 64>(L, st) : run_fwd<_Float16, 64>(L, st);
+  return bwd ? run_bwd<_Float16, 128>(L, st) : run_fwd<_Float16, 128>(L, st);
+}
+}  // namespace
+
+extern "C" long long t2v_attn_mod_workspace(const T2VAttnMod* p, int backward) {
+  if (check_mod("t2v_attn_mod_workspace", p, false)) return -1;
+  return make_layout(p, backward != 0).bytes;
+}
+extern "C" int t2v_attn_mod_fwd(const T2VAttnMod* p, t2v_stream_t stream) { return run("t2v_attn_mod_fwd", p, false, (hipStream_t)stream); }
+extern "C" int t2v_attn_mod_bwd(const T2VAttnMod* p, t2v_stream_t stream) { return run("t2v_attn_mod_bwd", p, true, (hipStream_t)stream); }

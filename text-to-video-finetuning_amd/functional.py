@@ -1795,3 +1795,7 @@ def planar_f32_to_tokens(x, width=8):
     y = torch.zeros(n * rows, width, dtype=BF16, device=x.device)
     nv.call("t2v_f32_planar_to_bf16_cl", x.data_ptr(), y.data_ptr(), width, n, Cc, rows, nv.stream())
     return y
+
+
+# --------------------------------------------------------------------------- transformer blocks over video / text tokens
+from .token_ops import RopeAxes, attention_mod, qk_norm_rope, rope  # noqa: E402,F401

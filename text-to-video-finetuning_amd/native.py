@@ -110,7 +110,29 @@ class TemporalFused(C.Structure):
     ]
 
 
-ABI_VERSION = 9          # include/t2v_abi.h T2V_ABI_VERSION
+class QkRope(C.Structure):
+    _fields_ = [
+        ("x", c_void_p * 2), ("ldx", c_ll * 2), ("dy", c_void_p * 2), ("lddy", c_ll * 2), ("y", c_void_p * 2), ("ldy", c_ll * 2),
+        ("heads", c_int * 2), ("w", c_void_p * 2), ("b", c_void_p * 2), ("dw", c_void_p * 2), ("db", c_void_p * 2),
+        ("workspace", c_void_p), ("rows", c_ll), ("D", c_int), ("dtype", c_int), ("norm", c_int), ("eps", c_float),
+        ("pos", c_void_p), ("ldpos", c_ll), ("pos_type", c_int), ("naxes", c_int), ("dims", c_int * 4),
+        ("scale", C.c_double * 4), ("theta", C.c_double), ("shared", c_int), ("style", c_int), ("freqs", c_void_p),
+    ]
+
+
+class AttnMod(C.Structure):
+    _fields_ = [
+        ("nbatch", c_int), ("heads", c_int), ("kv_heads", c_int), ("Sq", c_int), ("Sk", c_int), ("D", c_int), ("dtype", c_int),
+        ("causal", c_int), ("scale", c_float), ("softcap", c_float),
+        ("q", AttnOperand), ("k", AttnOperand), ("v", AttnOperand), ("o", AttnOperand),
+        ("lse", c_void_p), ("prefix", c_void_p), ("prefix_per_query", c_int), ("kv_len", c_void_p),
+        ("q_docs", c_void_p), ("kv_docs", c_void_p), ("slopes", c_void_p), ("bias", c_void_p), ("bias_f32", c_int),
+        ("radius", c_int), ("d_o", AttnOperand), ("dq", AttnOperand), ("dk", AttnOperand), ("dv", AttnOperand),
+        ("delta", c_void_p), ("dbias", c_void_p), ("kv_share", c_int), ("workspace", c_void_p), ("workspace_bytes", c_ll),
+    ]
+
+
+ABI_VERSION = 10          # include/t2v_abi.h T2V_ABI_VERSION
 A_DENSE, A_CONV = 0, 1
 OUT_BF16, OUT_F32, OUT_F32_ATOMIC = 0, 1, 2
 ACT_NONE, ACT_SILU = 0, 1
@@ -154,6 +176,12 @@ SYMBOLS = {
     "t2v_rowgroup_splits": ([c_int, c_int, c_int], c_int),
     "t2v_attn_fwd": ([C.POINTER(Attn), c_void_p], c_int),
     "t2v_attn_bwd": ([C.POINTER(Attn), c_void_p], c_int),
+    "t2v_qk_rope_fwd": ([C.POINTER(QkRope), c_void_p], c_int),
+    "t2v_qk_rope_bwd_floats": ([C.POINTER(QkRope)], c_ll),
+    "t2v_qk_rope_bwd": ([C.POINTER(QkRope), c_void_p], c_int),
+    "t2v_attn_mod_workspace": ([C.POINTER(AttnMod), c_int], c_ll),
+    "t2v_attn_mod_fwd": ([C.POINTER(AttnMod), c_void_p], c_int),
+    "t2v_attn_mod_bwd": ([C.POINTER(AttnMod), c_void_p], c_int),
     "t2v_softmax_rows": ([c_void_p, c_ll, c_void_p, c_ll, c_ll, c_int, c_void_p], c_int),
     "t2v_dropout_mask": ([c_void_p, c_ll, c_void_p, c_ll, c_ll, c_int, c_float, c_ull, c_void_p], c_int),
     "t2v_lowrank_update": ([c_void_p, c_ll, c_void_p, c_ll, c_void_p, c_ll, c_ll, c_int, c_int, c_float, c_void_p], c_int),

@@ -1,0 +1,435 @@
+"""Operators of transformer blocks over video and text tokens: rotary positions with several axes, the per-head norm of queries
+and keys with the rotation in the same pass, and attention with capped scores, distance biases, document and prefix masks.
+
+They work on the token matrices of `functional` ([rows, heads * dim], unit inner stride, any row stride that keeps rows 16-byte
+aligned) and are re-exported there.  Every one launches hand-written HIP kernels (csrc/rope.hip, csrc/attn_mod.hip) on the current
+stream of its operands' device, forward and backward; nothing falls back to torch math, and a call the kernels do not take raises.
+"""
+import ctypes as C
+import functools
+import math
+from dataclasses import dataclass
+
+import torch
+
+from . import native as nv
+
+_TYPE = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_POS = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
+_NORM = {"rms": 1, "layer": 2}
+
+
+# --------------------------------------------------------------------------- helpers
+def _fail(text):
+    raise RuntimeError("t2v_amd: " + text)
+
+
+def _tokens(t, name, types=(torch.bfloat16, torch.float16, torch.float32)):
+    if t.dim() != 2 or t.dtype not in types or (t.shape[1] > 1 and t.stride(1) != 1):
+        _fail(f"{name} must be a 2-D token matrix with unit inner stride in {[str(x)[6:] for x in types]}, got {tuple(t.shape)} {t.dtype} "
+              f"strides {t.stride()}")
+    if not t.is_cuda:
+        nv.require_cuda(t)
+    return t
+
+
+def _ld(t):
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _upstream(dy):
+    """A gradient as autograd hands it over (it may be expanded, transposed or a narrow view): rows the kernels can read."""
+    if dy.stride(1) != 1 or dy.data_ptr() % 16 or (_ld(dy) * dy.element_size()) % 16 or _ld(dy) < dy.shape[1]:
+        return dy.contiguous()
+    return dy
+
+
+def _vector(t, n, dev, name):
+    """fp32 copy / view of a per-column parameter."""
+    if t is None:
+        return None
+    if tuple(t.shape) != (n,) or t.device != dev or not t.is_floating_point():
+        _fail(f"{name} must be a floating vector of {n} elements on {dev}, got {tuple(t.shape)} {t.dtype} on {t.device}")
+    t = t.detach()
+    return t if t.dtype == torch.float32 and t.is_contiguous() else t.float().contiguous()
+
+
+class _on:
+    """The operands' device as the current one (kernels launch on the current stream of the current device)."""
+    __slots__ = ("guard",)
+
+    def __init__(self, dev):
+        self.guard = None if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+# --------------------------------------------------------------------------- rotary positions
+@dataclass(frozen=True)
+class RopeAxes:
+    """Which columns of a head turn, by which coordinate, how fast.
+
+    dims: columns per axis, in order (time, height, width, ...; even numbers, at most four axes, their sum a multiple of 8 and at
+    most the head dim; columns behind them pass through).  An axis of d columns owns d / 2 pairs; pair i turns by
+    pos[axis] * scale[axis] * theta^(-2 i / d), or, with `shared`, by the frequency its number among ALL pairs gives
+    (theta^(-2 p / sum(dims)): one ladder, the axes take turns along it).
+    style: "interleaved" pairs columns (2p, 2p + 1), "half" pairs (p, p + sum(dims) / 2)."""
+    dims: tuple
+    theta: float = 10000.0
+    style: str = "interleaved"
+    shared: bool = False
+    scale: tuple = None
+
+
+@functools.lru_cache(maxsize=256)
+def _rope_template(axes, D, heads, kv_heads, dtype, norm, eps):
+    """The fixed fields of the descriptor, as bytes (by value: nothing of a call's tensors is kept)."""
+    d = nv.QkRope()
+    d.heads[0], d.heads[1] = heads, kv_heads
+    d.D, d.dtype, d.norm, d.eps = D, _TYPE[dtype], _NORM[norm] if norm else 0, eps
+    if axes is not None:
+        dims = tuple(int(n) for n in axes.dims)
+        if not 1 <= len(dims) <= 4 or any(n <= 0 or n % 2 for n in dims) or sum(dims) % 8 or sum(dims) > D:
+            _fail(f"RopeAxes.dims {axes.dims}: one to four even numbers whose sum is a multiple of 8 and at most the head dim {D}")
+        if axes.style not in ("interleaved", "half"):
+            _fail(f"RopeAxes.style {axes.style!r}: 'interleaved' or 'half'")
+        if not (axes.theta > 0 and math.isfinite(axes.theta)):
+            _fail(f"RopeAxes.theta {axes.theta}: a positive number is wanted")
+        scale = (1.0,) * len(dims) if axes.scale is None else tuple(float(s) for s in axes.scale)
+        if len(scale) != len(dims) or not all(math.isfinite(s) for s in scale):
+            _fail(f"RopeAxes.scale {axes.scale}: one finite number per axis")
+        d.naxes, d.theta, d.shared, d.style = len(dims), axes.theta, int(axes.shared), int(axes.style == "half")
+        for n, (k, s) in enumerate(zip(dims, scale)):
+            d.dims[n], d.scale[n] = k, s
+    return bytes(d)
+
+
+def _rope_desc(axes, D, heads, kv_heads, dtype, norm, eps, rows, pos, freqs, dev):
+    d = nv.QkRope.from_buffer_copy(_rope_template(axes, D, heads, kv_heads, dtype, norm, eps))
+    d.rows = rows
+    if axes is not None:
+        if pos is None or pos.dim() != 2 or pos.shape[0] != rows or pos.shape[1] < d.naxes or pos.dtype not in _POS or pos.device != dev:
+            _fail(f"pos must be an int32, int64 or fp32 [{rows}, {d.naxes}] tensor on {dev}, got "
+                  f"{None if pos is None else (tuple(pos.shape), pos.dtype, pos.device)}")
+        if not pos.is_contiguous():
+            if pos.stride(1) != 1 or pos.stride(0) < pos.shape[1]:
+                _fail(f"pos must have unit inner stride and rows that do not overlap, got strides {pos.stride()}")
+        d.pos, d.ldpos, d.pos_type = pos.data_ptr(), pos.stride(0) if rows > 1 else pos.shape[1], _POS[pos.dtype]
+        if freqs is not None:
+            rot = sum(axes.dims)
+            if tuple(freqs.shape) != (rot // 2,) or freqs.dtype != torch.float64 or freqs.device != dev or not freqs.is_contiguous():
+                _fail(f"freqs must be a contiguous fp64 tensor of {rot // 2} frequencies on {dev}")
+            d.freqs = freqs.data_ptr()
+    elif pos is not None or freqs is not None:
+        _fail("positions need RopeAxes that say what they turn")
+    return d
+
+
+def _head_dim(x, heads, name):
+    heads = int(heads)
+    if heads <= 0 or x.shape[1] % heads:
+        _fail(f"{name} has {x.shape[1]} columns: not a multiple of {heads} heads")
+    return x.shape[1] // heads
+
+
+def _rope_fwd(xs, heads, pos, axes, freqs, norm, eps, ws, bs):
+    x0 = xs[0]
+    d = _rope_desc(axes, _head_dim(x0, heads[0], "q"), heads[0], heads[1], x0.dtype, norm, eps, x0.shape[0], pos, freqs, x0.device)
+    ys = []
+    for i, x in enumerate(xs):
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        d.x[i], d.ldx[i], d.y[i], d.ldy[i] = x.data_ptr(), _ld(x), y.data_ptr(), x.shape[1]
+        if norm:
+            d.w[i], d.b[i] = nv.ptr(ws[i]), nv.ptr(bs[i])
+        ys.append(y)
+    if x0.shape[0]:
+        with _on(x0.device):
+            nv.call("t2v_qk_rope_fwd", C.byref(d), nv.stream())
+    return tuple(ys)
+
+
+def _rope_bwd(xs, dys, heads, pos, axes, freqs, norm, eps, ws, bs, want):
+    """want: ((dw, db) wanted, ...) per side.  Returns dxs, dws, dbs (fp32)."""
+    dy0 = dys[0]
+    dev, rows, D = dy0.device, dy0.shape[0], _head_dim(dy0, heads[0], "dy")
+    d = _rope_desc(axes, D, heads[0], heads[1], dy0.dtype, norm, eps, rows, pos, freqs, dev)
+    dxs, dws, dbs = [], [None, None], [None, None]
+    for i, dy in enumerate(dys):
+        dx = torch.empty(dy.shape, dtype=dy.dtype, device=dev)
+        d.dy[i], d.lddy[i], d.y[i], d.ldy[i] = dy.data_ptr(), _ld(dy), dx.data_ptr(), dx.shape[1]
+        if norm:
+            d.x[i], d.ldx[i], d.w[i], d.b[i] = xs[i].data_ptr(), _ld(xs[i]), nv.ptr(ws[i]), nv.ptr(bs[i])
+            new = torch.empty if rows else torch.zeros
+            if want[i][0]:
+                dws[i] = new(D, dtype=torch.float32, device=dev)
+                d.dw[i] = dws[i].data_ptr()
+            if want[i][1]:
+                dbs[i] = new(D, dtype=torch.float32, device=dev)
+                d.db[i] = dbs[i].data_ptr()
+        dxs.append(dx)
+    if rows:
+        with _on(dev):
+            if any(t is not None for t in dws + dbs):
+                n = nv.lib().t2v_qk_rope_bwd_floats(C.byref(d))
+                if n < 0:
+                    nv.check(int(n), "t2v_qk_rope_bwd_floats")
+                work = torch.empty(int(n), dtype=torch.float32, device=dev)
+                d.workspace = work.data_ptr()
+            nv.call("t2v_qk_rope_bwd", C.byref(d), nv.stream())
+    return dxs, dws, dbs
+
+
+class _Rope(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, pos, freqs, heads, axes):
+        ctx.meta = (heads, axes)
+        ctx.save_for_backward(pos, freqs)
+        return _rope_fwd((x,), (heads, 0), pos, axes, freqs, None, 0.0, (None,), (None,))[0]
+
+    @staticmethod
+    def backward(ctx, dy):
+        pos, freqs = ctx.saved_tensors
+        heads, axes = ctx.meta
+        dxs, _, _ = _rope_bwd((None,), (_upstream(dy),), (heads, 0), pos, axes, freqs, None, 0.0, (None,), (None,), None)
+        return dxs[0], None, None, None, None
+
+
+def rope(x, heads, pos, axes, freqs=None):
+    """Rotary positions: x [rows, heads * dim] (bf16, fp16 or fp32) with the columns `axes` (RopeAxes) names turned by pos [rows, number
+    of axes] (int32, int64 or fp32).  Angles are formed in 64 bits.  freqs: fp64 [sum(dims) / 2] radians per unit of position, in the place of the
+    ladder theta gives.  Returns a dense matrix of x's shape; differentiable in x."""
+    x = _tokens(x, "x")
+    heads = int(heads)
+    if torch.is_grad_enabled() and x.requires_grad:
+        return _Rope.apply(x, pos, freqs, heads, axes)
+    return _rope_fwd((x,), (heads, 0), pos, axes, freqs, None, 0.0, (None,), (None,))[0]
+
+
+class _QkNormRope(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, qw, kw, qb, kb, pos, freqs, heads, kv_heads, axes, norm, eps):
+        D = q.shape[1] // heads
+        ws = (_vector(qw, D, q.device, "q_weight"), _vector(kw, D, q.device, "k_weight"))
+        bs = (_vector(qb, D, q.device, "q_bias"), _vector(kb, D, q.device, "k_bias"))
+        ctx.meta = (heads, kv_heads, axes, norm, eps, [None if t is None else t.dtype for t in (qw, kw, qb, kb)])
+        ctx.save_for_backward(q, k, qw, kw, pos, freqs)
+        return _rope_fwd((q, k), (heads, kv_heads), pos, axes, freqs, norm, eps, ws, bs)
+
+    @staticmethod
+    def backward(ctx, dq, dk):
+        q, k, qw, kw, pos, freqs = ctx.saved_tensors
+        heads, kv_heads, axes, norm, eps, dt = ctx.meta
+        D = q.shape[1] // heads
+        ws = (_vector(qw, D, q.device, "q_weight"), _vector(kw, D, q.device, "k_weight"))
+        need = ctx.needs_input_grad
+        dxs, dws, dbs = _rope_bwd((q, k), (_upstream(dq), _upstream(dk)), (heads, kv_heads), pos, axes, freqs, norm, eps, ws, (None, None),
+                                  ((need[2], need[4]), (need[3], need[5])))
+        g = [None if t is None else t.to(y) for t, y in zip((dws[0], dws[1], dbs[0], dbs[1]), dt)]
+        return (dxs[0], dxs[1], *g, None, None, None, None, None, None, None)
+
+
+def qk_norm_rope(q, k, heads, kv_heads, pos, axes, q_weight=None, k_weight=None, q_bias=None, k_bias=None, eps=1e-6, norm="rms",
+                 freqs=None):
+    """Queries [rows, heads * dim] and keys [rows, kv_heads * dim] normed per head and turned, in one launch: returns (q', k').
+
+    norm: "rms" (x * rsqrt(mean x^2 + eps)) or "layer" (centred first); q_weight, k_weight, q_bias, k_bias: [dim] vectors shared by the
+    heads, or None.  pos, axes, freqs: as in `rope`; both None: the norm alone.  Differentiable in q, k and the four vectors; the
+    statistics are recomputed in the backward pass from the saved inputs."""
+    q, k = _tokens(q, "q"), _tokens(k, "k")
+    heads, kv_heads = int(heads), int(kv_heads)
+    if norm not in _NORM:
+        _fail(f"norm {norm!r}: 'rms' or 'layer'")
+    if k.dtype != q.dtype or k.device != q.device or k.shape[0] != q.shape[0] or _head_dim(q, heads, "q") != _head_dim(k, kv_heads, "k"):
+        _fail(f"q {tuple(q.shape)} {q.dtype} and k {tuple(k.shape)} {k.dtype} must have the same rows, type, device and head dim")
+    params = (q_weight, k_weight, q_bias, k_bias)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k) + params):
+        return _QkNormRope.apply(q, k, *params, pos, freqs, heads, kv_heads, axes, norm, float(eps))
+    D = q.shape[1] // heads
+    ws = (_vector(q_weight, D, q.device, "q_weight"), _vector(k_weight, D, q.device, "k_weight"))
+    bs = (_vector(q_bias, D, q.device, "q_bias"), _vector(k_bias, D, q.device, "k_bias"))
+    return _rope_fwd((q, k), (heads, kv_heads), pos, axes, freqs, norm, float(eps), ws, bs)
+
+
+# --------------------------------------------------------------------------- attention with modified scores
+@functools.lru_cache(maxsize=1024)
+def _layout_facts(lay, rows):
+    """(inside, own, covered) of a SeqLayout over a matrix of `rows` rows: every row it names exists; no row is named twice; every row is named."""
+    if min(lay.nbatch, lay.S, lay.hi, lay.lo, lay.ss) < 0 or lay.bdiv < 1:
+        return False, False, False
+    if lay.nbatch * lay.S == 0:
+        return True, True, rows == 0
+    sizes = [(-(-lay.nbatch // lay.bdiv), lay.hi), (min(lay.nbatch, lay.bdiv), lay.lo), (lay.S, lay.ss)]
+    last = sum((n - 1) * s for n, s in sizes)
+    own, reach = True, 0
+    for n, s in sorted((p for p in sizes if p[0] > 1), key=lambda p: p[1]):
+        own = own and s > reach
+        reach += (n - 1) * s
+    return last < rows, own, own and lay.nbatch * lay.S == rows
+
+
+def _operand(t, lay):
+    ld = _ld(t)
+    return nv.AttnOperand(t.data_ptr(), lay.hi * ld, lay.lo * ld, lay.ss * ld, lay.bdiv)
+
+
+def _ints(t, shapes, dev, name):
+    if t is None:
+        return None
+    if t.dtype != torch.int32 or tuple(t.shape) not in shapes or t.device != dev or not t.is_contiguous():
+        _fail(f"{name} must be a contiguous int32 tensor of shape {' or '.join(map(str, shapes))} on {dev}, got {tuple(t.shape)} {t.dtype} on {t.device}")
+    return t.data_ptr()
+
+
+def _attn_desc(q, k, v, o, meta, prefix, kv_len, q_docs, kv_docs, slopes, bias):
+    heads, kv_heads, qlay, klay, scale, causal, softcap = meta
+    a = nv.AttnMod()
+    a.nbatch, a.heads, a.kv_heads, a.Sq, a.Sk, a.D = qlay.nbatch, heads, kv_heads, qlay.S, klay.S, q.shape[1] // heads
+    a.dtype, a.causal, a.scale, a.softcap = _TYPE[q.dtype], causal, scale, softcap
+    a.q, a.k, a.v, a.o = _operand(q, qlay), _operand(k, klay), _operand(v, klay), _operand(o, qlay)
+    if prefix is not None:
+        a.prefix, a.prefix_per_query = prefix.data_ptr(), int(prefix.dim() == 2)
+    if kv_len is not None:
+        a.kv_len = kv_len.data_ptr()
+    if q_docs is not None:
+        a.q_docs, a.kv_docs = q_docs.data_ptr(), kv_docs.data_ptr()
+    if slopes is not None:
+        a.slopes = slopes.data_ptr()
+    if bias is not None:
+        a.bias, a.bias_f32, a.radius = bias.data_ptr(), int(bias.dtype == torch.float32), bias.shape[1] // 2
+    return a
+
+
+def _workspace(a, backward, dev):
+    n = nv.lib().t2v_attn_mod_workspace(C.byref(a), backward)
+    if n < 0:
+        nv.check(int(n), "t2v_attn_mod_workspace")
+    if n == 0:
+        return None
+    w = torch.empty(int(n), dtype=torch.uint8, device=dev)      # (the caching allocator's blocks are 512-byte aligned)
+    a.workspace, a.workspace_bytes = w.data_ptr(), int(n)
+    return w
+
+
+def _attn_fwd(q, k, v, meta, prefix, kv_len, q_docs, kv_docs, slopes, bias, keep):
+    heads, _, qlay, klay = meta[:4]
+    dev = q.device
+    if qlay.nbatch * qlay.S == 0 or klay.S == 0:        # nothing is asked, or there is nothing to see
+        o = torch.zeros(q.shape, dtype=q.dtype, device=dev)
+        return o, (torch.full((qlay.nbatch * heads * qlay.S,), math.inf, device=dev) if keep else None)
+    covered = _layout_facts(qlay, q.shape[0])[2]
+    o = (torch.empty if covered else torch.zeros)(q.shape, dtype=q.dtype, device=dev)      # rows that no sequence owns: zeros
+    a = _attn_desc(q, k, v, o, meta, prefix, kv_len, q_docs, kv_docs, slopes, bias)
+    lse = None
+    if keep:
+        lse = torch.empty(qlay.nbatch * heads * qlay.S, dtype=torch.float32, device=dev)
+        a.lse = lse.data_ptr()
+    with _on(dev):
+        work = _workspace(a, 0, dev)
+        nv.call("t2v_attn_mod_fwd", C.byref(a), nv.stream())
+        del work
+    return o, lse
+
+
+class _AttentionMod(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, bias, prefix, kv_len, q_docs, kv_docs, slopes, meta):
+        o, lse = _attn_fwd(q, k, v, meta, prefix, kv_len, q_docs, kv_docs, slopes, bias, True)
+        ctx.meta = meta
+        ctx.save_for_backward(q, k, v, bias, prefix, kv_len, q_docs, kv_docs, slopes, o, lse)
+        return o
+
+    @staticmethod
+    def backward(ctx, do):
+        q, k, v, bias, prefix, kv_len, q_docs, kv_docs, slopes, o, lse = ctx.saved_tensors
+        qlay, klay = ctx.meta[2:4]
+        dev = q.device
+        do = _upstream(do)
+        empty = qlay.nbatch * qlay.S == 0 or klay.S == 0
+        share = klay.bdiv if klay.bdiv > 1 and klay.lo == 0 else 1
+        kfacts = _layout_facts(klay, k.shape[0])
+        kall = kfacts[2] or (share > 1 and klay.nbatch % share == 0 and klay.nbatch // share * klay.S == k.shape[0])
+        new = lambda t, full: (torch.empty if full and not empty else torch.zeros)(t.shape, dtype=t.dtype, device=dev)  # noqa: E731
+        dq, dk, dv = new(q, _layout_facts(qlay, q.shape[0])[2]), new(k, kall), new(v, kall)
+        dbias = new(bias, True) if bias is not None and ctx.needs_input_grad[3] else None
+        if not empty:
+            a = _attn_desc(q, k, v, o, ctx.meta, prefix, kv_len, q_docs, kv_docs, slopes, bias)
+            delta = torch.empty_like(lse)
+            a.lse, a.delta, a.dbias, a.kv_share = lse.data_ptr(), delta.data_ptr(), nv.ptr(dbias), share
+            a.d_o, a.dq, a.dk, a.dv = _operand(do, qlay), _operand(dq, qlay), _operand(dk, klay), _operand(dv, klay)
+            with _on(dev):
+                work = _workspace(a, 1, dev)
+                nv.call("t2v_attn_mod_bwd", C.byref(a), nv.stream())
+                del work
+        return dq, dk, dv, dbias, None, None, None, None, None, None
+
+
+def attention_mod(q, k, v, heads, qlay, klay, kv_heads=None, scale=None, causal=False, prefix=None, kv_len=None, q_docs=None, kv_docs=None,
+                  softcap=0.0, slopes=None, bias=None):
+    """Attention whose scores may be capped, biased by distance and masked by position and document.
+
+    q: [rows_q, heads * dim]; k, v: [rows_kv, kv_heads * dim] token matrices in bf16 or fp16 (dim a multiple of 8 up to 128; heads a
+    multiple of kv_heads, which defaults to heads); qlay, klay: SeqLayout of the sequences.  With t = scale * q.k (scale defaults to
+    dim^-0.5):
+      softcap > 0    t <- softcap * tanh(t / softcap)
+      slopes         fp32 [heads]: t <- t - slopes[h] * |j - i'|                                  (not trained)
+      bias           [heads, 2R + 1] (R <= 1024, the operands' type or fp32): t <- t + bias[h, clip(j - i', -R, R) + R]; trained when it
+                     requires a gradient; an entry at or below its type's lowest finite value hides its distance
+      kv_len         int32 [nbatch]: keys 0 .. kv_len - 1 exist (default: all)
+      causal         keys j <= i';  prefix (int32 [nbatch] or [nbatch, Sq], with causal): and all keys j < prefix
+      q_docs, kv_docs  int32 [nbatch, Sq], [nbatch, Sk]: only keys of the query's document; numbers below 0 mark padding
+    i' = i + kv_len - Sq is the query's place among the keys: the queries are the last positions.  A row that may see nothing is zero.
+    Keys and values that no query may see (behind kv_len, padding) may hold anything; a key or value that is visible to one query of a
+    sequence must be finite, since masked weights of its tile are exact zeros that multiply it.
+    Few query rows over many keys (serving steps, chunks of new tokens) split the keys over workgroups and join them.
+    Returns [rows_q, heads * dim]; rows that no sequence owns are zero.  Differentiable in q, k, v and bias; K / V shared by the bdiv batches
+    of a layout with lo = 0 get the sum of their gradients.  The order of all sums is fixed: repeated runs are bit-equal."""
+    types = (torch.bfloat16, torch.float16)
+    q, k, v = _tokens(q, "q", types), _tokens(k, "k", types), _tokens(v, "v", types)
+    heads = int(heads)
+    kv_heads = heads if kv_heads is None else int(kv_heads)
+    dev, D = q.device, _head_dim(q, heads, "q")
+    if kv_heads <= 0 or heads % kv_heads:
+        _fail(f"{heads} query heads cannot share {kv_heads} key / value heads evenly")
+    if k.shape != v.shape or k.shape[1] != kv_heads * D or not q.dtype == k.dtype == v.dtype or not dev == k.device == v.device:
+        _fail(f"q {tuple(q.shape)} {q.dtype}, k {tuple(k.shape)} {k.dtype}, v {tuple(v.shape)} {v.dtype}: one type, one device, {kv_heads} "
+              f"key / value heads of {D} columns are wanted")
+    if D % 8 or D > 128:
+        _fail(f"attention_mod takes head dims that are multiples of 8 up to 128, got {D}")
+    nb, Sq, Sk = qlay.nbatch, qlay.S, klay.S
+    qf, kf = _layout_facts(qlay, q.shape[0]), _layout_facts(klay, k.shape[0])
+    if nb != klay.nbatch or not qf[0] or not kf[0]:
+        _fail(f"layouts {qlay} over {q.shape[0]} rows and {klay} over {k.shape[0]} rows: as many batches on both sides, rows that exist")
+    if not qf[1]:
+        _fail(f"query layout {qlay} names a row twice")
+    softcap, scale = float(softcap), float(D ** -0.5 if scale is None else scale)
+    if not 0.0 <= softcap < 1e30 or not math.isfinite(scale):
+        _fail(f"softcap {softcap}, scale {scale}: a finite scale and a cap of 0 (none) or more are wanted")
+    if prefix is not None and not causal:
+        _fail("prefix opens a causal mask: pass causal=True with it")
+    if (q_docs is None) != (kv_docs is None):
+        _fail("q_docs and kv_docs come together")
+    _ints(prefix, ((nb,), (nb, Sq)), dev, "prefix")
+    _ints(kv_len, ((nb,),), dev, "kv_len")
+    _ints(q_docs, ((nb, Sq),), dev, "q_docs")
+    _ints(kv_docs, ((nb, Sk),), dev, "kv_docs")
+    if slopes is not None:
+        if slopes.dtype != torch.float32 or tuple(slopes.shape) != (heads,) or slopes.device != dev or not slopes.is_contiguous():
+            _fail(f"slopes must be a contiguous fp32 tensor of {heads} elements on {dev}")
+        if slopes.requires_grad:
+            _fail("slopes are not trained: pass slopes.detach(), or a bias table for a learned distance bias")
+    if bias is not None:
+        if bias.dtype not in (q.dtype, torch.float32) or bias.dim() != 2 or bias.shape[0] != heads or bias.shape[1] % 2 == 0 or \
+                bias.shape[1] > 2049 or bias.device != dev or not bias.is_contiguous():
+            _fail(f"bias must be a contiguous [{heads}, 2R + 1] table with R <= 1024 in {q.dtype} or fp32 on {dev}, got {tuple(bias.shape)} {bias.dtype}")
+    meta = (heads, kv_heads, qlay, klay, scale, int(bool(causal)), softcap)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (bias is not None and bias.requires_grad)):
+        if not kf[1] and not (klay.bdiv > 1 and klay.lo == 0 and klay.hi >= (klay.S - 1) * klay.ss + 1 and klay.ss > 0):
+            _fail(f"key layout {klay} names a row twice: gradients are defined for rows of their own, or shared by the bdiv batches (lo = 0)")
+        return _AttentionMod.apply(q, k, v, bias, prefix, kv_len, q_docs, kv_docs, slopes, meta)
+    return _attn_fwd(q, k, v, meta, prefix, kv_len, q_docs, kv_docs, slopes, bias, False)[0]
