@@ -130,3 +130,25 @@ def test_the_oracle_finds_a_mistake():
     for n, x in (("o", o), ("dq", Q.grad), ("dk", K.grad), ("dv", V.grad)):
         torch.testing.assert_close(good[n][0][0].transpose(0, 1), x.detach(), rtol=1e-9, atol=1e-9)
     torch.testing.assert_close(good["dbias"][0], B.grad, rtol=1e-9, atol=1e-9)
+
+
+def test_packed_descriptors_have_the_fields_where_the_header_has_them():
+    import t2v_amd.token_ops as T
+    nv = _nv()
+    assert T._FWD.size == nv.AttnMod.d_o.offset and T._FWD.size + T._BWD.size == C.sizeof(nv.AttnMod)
+    n = iter(range(1, 100))
+    nx = lambda k: [next(n) for _ in range(k)]  # noqa: E731
+    a = nv.AttnMod.from_buffer_copy(T._FWD.pack(*nx(8), *nx(2), *nx(20), *nx(10)) + T._BWD.pack(*nx(20), *nx(5)))
+    flat = []
+    for name, _ in nv.AttnMod._fields_:
+        v = getattr(a, name)
+        flat += [getattr(v, f) for f, _ in nv.AttnOperand._fields_] if isinstance(v, nv.AttnOperand) else [v]
+    assert flat == list(range(1, 66))
+    assert T._SIDES.size == nv.QkRope.D.offset and nv.QkRope.pos.offset + T._WHERE.size == nv.QkRope.naxes.offset
+    d = T._rope_desc(T.RopeAxes((16, 24), theta=7.0, style="half", shared=True, scale=(2.0, 3.0)), 64, torch.float16, "layer", 0.5, 11,
+                     torch.zeros(11, 2, dtype=torch.int64), torch.zeros(20, dtype=torch.float64), torch.device("cpu"), (3, 4), ((5, 6), (7, 8)),
+                     ((9, 10), (11, 12)), ((13, 14), (15, 16)), (17, 18), (19, 20), (21, 22), (23, 24), 25)
+    assert [list(getattr(d, f)) for f in ("x", "ldx", "dy", "lddy", "y", "ldy", "heads", "w", "b", "dw", "db")] == [
+        [5, 7], [6, 8], [9, 11], [10, 12], [13, 15], [14, 16], [3, 4], [17, 18], [19, 20], [21, 22], [23, 24]]
+    assert (d.workspace, d.rows, d.D, d.dtype, d.norm, d.eps, d.ldpos, d.pos_type, d.naxes, list(d.dims), list(d.scale), d.theta, d.shared, d.style) == \
+        (25, 11, 64, 1, 2, 0.5, 2, 1, 2, [16, 24, 0, 0], [2.0, 3.0, 0.0, 0.0], 7.0, 1, 1) and d.pos and d.freqs

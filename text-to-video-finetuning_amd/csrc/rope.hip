@@ -36,8 +36,8 @@ struct RopeArgs {
   long long ldpos;
   int pos_type;
   int dims[4];
-  double scale[4];
-  double log2theta;
+  double pw[4][7];                       // of each axis: r, r^2, r^4, ... r^64, the ratio of one frequency to the one before it
+  double first[4];                       // frequency of the axis' first pair, in turns per unit of position (scale / 2 pi)
   int shared;
   const double* freqs;
   float eps;
@@ -85,21 +85,32 @@ __device__ __forceinline__ float group_sum(float v) {
   return v;
 }
 
-// the lane's four angular frequencies in turns per unit of position, and the axis of each pair
+// the lane's four frequencies in turns per unit of position, and the axis of each pair.  theta^(-2 i / d) = r^i comes from the bits of i
+// and the host's powers of r in 64 bits: at most ten products (a relative error of 1e-15, at 10^6 turns 1e-9 of a turn) in the place of
+// four 64-bit exponentials, which took longer than the rest of a launch of few rows (5.4 -> 3.6 us at 8 rows).
 __device__ __forceinline__ void lane_freqs(const RopeArgs& p, int c, double (&f)[4], int (&ax)[4]) {
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     const int pr = 4 * c + e;
-    int a = 0, first = 0;
-    for (int n = 0; n < 3; ++n)
-      if (n + 1 < p.naxes && pr >= first + p.dims[n] / 2 && a == n) {
-        first += p.dims[n] / 2;
-        a = n + 1;
+    int a = 0, first = 0, end = p.dims[0] / 2;
+#pragma unroll
+    for (int n = 1; n < 4; ++n)
+      if (n < p.naxes) {
+        const bool on = pr >= end;
+        a = on ? n : a;
+        first = on ? end : first;
+        end += p.dims[n] / 2;
       }
     ax[e] = a;
-    const int i = p.shared ? pr : pr - first, d = p.shared ? p.rot : p.dims[a];
-    double v = p.freqs ? (pr < p.rot / 2 ? p.freqs[pr] : 0.0) : exp2(-p.log2theta * (2.0 * i) / d);
-    f[e] = v * p.scale[a] * 0.15915494309189533577;
+    if (p.freqs) {
+      f[e] = pr < p.rot / 2 ? p.freqs[pr] * p.first[a] : 0.0;
+    } else {
+      const int i = p.shared ? pr : pr - first;
+      double v = p.first[a];
+#pragma unroll
+      for (int n = 0; n < 7; ++n) v *= (i >> n) & 1 ? p.pw[a][n] : 1.0;
+      f[e] = v;
+    }
   }
 }
 __device__ __forceinline__ double load_pos(const RopeArgs& p, long long row, int a) {
@@ -158,7 +169,14 @@ __global__ __launch_bounds__(256) void rope_kernel(const RopeArgs p) {
       for (int e = 0; e < 4; ++e) {
         double t = load_pos(p, r, ax[e]) * f[e];
         t -= rint(t);
-        sincospif(2.f * (float)t, &sn[e], &cs[e]);
+        if (sizeof(T) == 2) {
+          // the hardware's sine of an angle in turns: at most 1.3e-7 off over a turn (measured), far below half a
+          // step of 16 bits (2^-12)
+          sn[e] = __builtin_amdgcn_sinf((float)t);
+          cs[e] = __builtin_amdgcn_cosf((float)t);
+        } else {
+          sincospif(2.f * (float)t, &sn[e], &cs[e]);
+        }
       }
     }
     for (int h = h0; h < h1; h += UNROLL) {
@@ -285,8 +303,10 @@ __global__ __launch_bounds__(1024) void rope_param_reduce_kernel(const float* __
 struct Plan {
   int lph, gx, hb, nq, nk;
 };
-// Heads per block of work: as many as leave ~2048 workgroups (8 per CU) — a block shares the angles and the per-lane set-up; the
-// backward with parameter gradients bounds its workgroups (one partial row each) and lets every group visit several rows.
+// Heads per block of work: as many as leave 1.5 workgroups per CU — a block shares the angles and the per-lane set-up (16384 rows, five heads of
+// 64: 7.8 us with all heads in a block, 13.1 us with one; 6669 rows of five fp32 heads: 8.7 against 17.0).  Workgroups are bounded and
+// visit several rows: 2048 forward (69120 rows, 2 x 20 heads of 64: 161 us, 172 unbounded; 2 x 8 heads of 128: 113 against 128 us), and 1024
+// where each leaves a partial row of parameter gradients (205 us; 308 at 512, where too few loads are in flight).
 Plan rope_plan(const T2VQkRope* p, bool partials) {
   Plan q;
   const int lanes = p->D / 8;
@@ -294,11 +314,12 @@ Plan rope_plan(const T2VQkRope* p, bool partials) {
   const long long bx = (p->rows * q.lph + 255) / 256;
   for (q.hb = 16; q.hb > 1; q.hb /= 2) {
     const long long blocks = bx * ((p->heads[0] + q.hb - 1) / q.hb + (p->heads[1] + q.hb - 1) / q.hb);
-    if (blocks >= 2048) break;
+    if (blocks >= 384) break;
   }
   q.nq = (p->heads[0] + q.hb - 1) / q.hb;
   q.nk = (p->heads[1] + q.hb - 1) / q.hb;
-  const long long cap = partials ? (1024 / (q.nq + q.nk) > 1 ? 1024 / (q.nq + q.nk) : 1) : 1 << 20;
+  const int most = partials ? 1024 : 2048;
+  const long long cap = most / (q.nq + q.nk) > 1 ? most / (q.nq + q.nk) : 1;
   q.gx = (int)(bx < cap ? bx : cap);
   return q;
 }
@@ -343,14 +364,17 @@ RopeArgs rope_args(const T2VQkRope* p, const Plan& q) {
   for (int n = 0; n < p->naxes; ++n) {
     a.rot += p->dims[n];
     a.dims[n] = p->dims[n];
-    a.scale[n] = p->scale[n];
+  }
+  for (int n = 0; n < p->naxes; ++n) {
+    a.first[n] = p->scale[n] * 0.15915494309189533577;
+    const double step = p->freqs ? 0.0 : -2.0 * log2(p->theta) / (p->shared ? a.rot : p->dims[n]);
+    for (int k = 0; k < 7; ++k) a.pw[n][k] = exp2(step * (1 << k));
   }
   a.nq = q.nq;
   a.hb = q.hb;
   a.pos = p->pos;
   a.ldpos = p->ldpos;
   a.pos_type = p->pos_type;
-  a.log2theta = p->theta > 0 ? log2(p->theta) : 0.0;
   a.shared = p->shared;
   a.freqs = p->freqs;
   a.eps = p->eps;

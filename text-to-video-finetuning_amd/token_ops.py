@@ -8,6 +8,7 @@ stream of its operands' device, forward and backward; nothing falls back to torc
 import ctypes as C
 import functools
 import math
+import struct
 from dataclasses import dataclass
 
 import torch
@@ -54,20 +55,19 @@ def _vector(t, n, dev, name):
     return t if t.dtype == torch.float32 and t.is_contiguous() else t.float().contiguous()
 
 
-class _on:
-    """The operands' device as the current one (kernels launch on the current stream of the current device)."""
-    __slots__ = ("guard",)
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
 
-    def __init__(self, dev):
-        self.guard = None if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
 
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _launch(name, desc, dev):
+    """The entry point `name` on the current stream of the operands' device (made the current device where it is not)."""
+    index = dev.index
+    if index == torch.cuda.current_device():
+        rc = getattr(nv.lib(), name)(C.byref(desc), _raw_stream(index))
+    else:
+        with torch.cuda.device(dev):
+            rc = getattr(nv.lib(), name)(C.byref(desc), _raw_stream(index))
+    if rc:
+        nv.check(rc, name)
 
 
 # --------------------------------------------------------------------------- rotary positions
@@ -87,11 +87,15 @@ class RopeAxes:
     scale: tuple = None
 
 
+# T2VQkRope in three pieces, packed in one go (a ctypes structure filled field by field costs several microseconds of a call that takes ten)
+_SIDES = struct.Struct("@12Q2i8QQq")        # x, ldx, dy, lddy, y, ldy (both sides each); heads; w, b, dw, db; workspace; rows
+_WHERE = struct.Struct("@Qqi")              # pos, ldpos, pos_type
+
+
 @functools.lru_cache(maxsize=256)
-def _rope_template(axes, D, heads, kv_heads, dtype, norm, eps):
-    """The fixed fields of the descriptor, as bytes (by value: nothing of a call's tensors is kept)."""
+def _rope_fixed(axes, D, dtype, norm, eps):
+    """(number of axes, bytes in front of the positions, bytes behind them but for `freqs`): fixed by values, nothing of a call's tensors."""
     d = nv.QkRope()
-    d.heads[0], d.heads[1] = heads, kv_heads
     d.D, d.dtype, d.norm, d.eps = D, _TYPE[dtype], _NORM[norm] if norm else 0, eps
     if axes is not None:
         dims = tuple(int(n) for n in axes.dims)
@@ -107,97 +111,107 @@ def _rope_template(axes, D, heads, kv_heads, dtype, norm, eps):
         d.naxes, d.theta, d.shared, d.style = len(dims), axes.theta, int(axes.shared), int(axes.style == "half")
         for n, (k, s) in enumerate(zip(dims, scale)):
             d.dims[n], d.scale[n] = k, s
-    return bytes(d)
+    raw, q = bytes(d), nv.QkRope
+    return d.naxes, raw[q.D.offset:q.pos.offset], raw[q.naxes.offset:q.freqs.offset]
 
 
-def _rope_desc(axes, D, heads, kv_heads, dtype, norm, eps, rows, pos, freqs, dev):
-    d = nv.QkRope.from_buffer_copy(_rope_template(axes, D, heads, kv_heads, dtype, norm, eps))
-    d.rows = rows
+def _rope_desc(axes, D, dtype, norm, eps, rows, pos, freqs, dev, heads, x, dy, y, w, b, dw, db, work):
+    """x, dy, y: two (pointer, row stride); w, b, dw, db: two pointers; 0: not there."""
+    naxes, mid, tail = _rope_fixed(axes, D, dtype, norm, eps)
+    fr = 0
+    where = (0, 0, 0)
     if axes is not None:
-        if pos is None or pos.dim() != 2 or pos.shape[0] != rows or pos.shape[1] < d.naxes or pos.dtype not in _POS or pos.device != dev:
-            _fail(f"pos must be an int32, int64 or fp32 [{rows}, {d.naxes}] tensor on {dev}, got "
+        if pos is None or pos.dim() != 2 or pos.shape[0] != rows or pos.shape[1] < naxes or pos.dtype not in _POS or pos.device != dev:
+            _fail(f"pos must be an int32, int64 or fp32 [{rows}, {naxes}] tensor on {dev}, got "
                   f"{None if pos is None else (tuple(pos.shape), pos.dtype, pos.device)}")
-        if not pos.is_contiguous():
-            if pos.stride(1) != 1 or pos.stride(0) < pos.shape[1]:
-                _fail(f"pos must have unit inner stride and rows that do not overlap, got strides {pos.stride()}")
-        d.pos, d.ldpos, d.pos_type = pos.data_ptr(), pos.stride(0) if rows > 1 else pos.shape[1], _POS[pos.dtype]
+        ld = pos.stride(0) if rows > 1 else pos.shape[1]
+        if (pos.shape[1] > 1 and pos.stride(1) != 1) or ld < naxes:
+            _fail(f"pos must have unit inner stride and rows that do not overlap, got strides {pos.stride()}")
+        where = (pos.data_ptr(), ld, _POS[pos.dtype])
         if freqs is not None:
             rot = sum(axes.dims)
             if tuple(freqs.shape) != (rot // 2,) or freqs.dtype != torch.float64 or freqs.device != dev or not freqs.is_contiguous():
                 _fail(f"freqs must be a contiguous fp64 tensor of {rot // 2} frequencies on {dev}")
-            d.freqs = freqs.data_ptr()
+            fr = freqs.data_ptr()
     elif pos is not None or freqs is not None:
         _fail("positions need RopeAxes that say what they turn")
-    return d
+    (x0, lx0), (x1, lx1) = x
+    (g0, lg0), (g1, lg1) = dy
+    (y0, ly0), (y1, ly1) = y
+    sides = _SIDES.pack(x0, x1, lx0, lx1, g0, g1, lg0, lg1, y0, y1, ly0, ly1, *heads, *w, *b, *dw, *db, work, rows)
+    return nv.QkRope.from_buffer_copy(sides + mid + _WHERE.pack(*where) + tail + fr.to_bytes(8, "little"))
+
+
+_NO = ((0, 0), (0, 0))
+_ZZ = (0, 0)
 
 
 def _head_dim(x, heads, name):
-    heads = int(heads)
     if heads <= 0 or x.shape[1] % heads:
         _fail(f"{name} has {x.shape[1]} columns: not a multiple of {heads} heads")
     return x.shape[1] // heads
 
 
+def _ptrs(ts):
+    """(pointer, row stride) of one or two matrices."""
+    a = (ts[0].data_ptr(), _ld(ts[0]))
+    return (a, (ts[1].data_ptr(), _ld(ts[1]))) if len(ts) > 1 else (a, (0, 0))
+
+
+def _vptrs(ts):
+    return tuple(0 if t is None else t.data_ptr() for t in ts) if ts is not None else _ZZ
+
+
 def _rope_fwd(xs, heads, pos, axes, freqs, norm, eps, ws, bs):
     x0 = xs[0]
-    d = _rope_desc(axes, _head_dim(x0, heads[0], "q"), heads[0], heads[1], x0.dtype, norm, eps, x0.shape[0], pos, freqs, x0.device)
-    ys = []
-    for i, x in enumerate(xs):
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        d.x[i], d.ldx[i], d.y[i], d.ldy[i] = x.data_ptr(), _ld(x), y.data_ptr(), x.shape[1]
-        if norm:
-            d.w[i], d.b[i] = nv.ptr(ws[i]), nv.ptr(bs[i])
-        ys.append(y)
-    if x0.shape[0]:
-        with _on(x0.device):
-            nv.call("t2v_qk_rope_fwd", C.byref(d), nv.stream())
-    return tuple(ys)
+    dev, rows = x0.device, x0.shape[0]
+    ys = tuple([torch.empty(x.shape, dtype=x.dtype, device=dev) for x in xs])
+    d = _rope_desc(axes, _head_dim(x0, heads[0], "q"), x0.dtype, norm, eps, rows, pos, freqs, dev, heads, _ptrs(xs), _NO, _ptrs(ys),
+                   _vptrs(ws), _vptrs(bs), _ZZ, _ZZ, 0)
+    if rows:
+        _launch("t2v_qk_rope_fwd", d, dev)
+    return ys
 
 
-def _rope_bwd(xs, dys, heads, pos, axes, freqs, norm, eps, ws, bs, want):
-    """want: ((dw, db) wanted, ...) per side.  Returns dxs, dws, dbs (fp32)."""
+def _rope_bwd(xs, dys, heads, pos, axes, freqs, norm, eps, ws, want):
+    """want: per side (dw, db) wanted.  Returns dxs and the parameter gradients (fp32)."""
     dy0 = dys[0]
     dev, rows, D = dy0.device, dy0.shape[0], _head_dim(dy0, heads[0], "dy")
-    d = _rope_desc(axes, D, heads[0], heads[1], dy0.dtype, norm, eps, rows, pos, freqs, dev)
-    dxs, dws, dbs = [], [None, None], [None, None]
-    for i, dy in enumerate(dys):
-        dx = torch.empty(dy.shape, dtype=dy.dtype, device=dev)
-        d.dy[i], d.lddy[i], d.y[i], d.ldy[i] = dy.data_ptr(), _ld(dy), dx.data_ptr(), dx.shape[1]
-        if norm:
-            d.x[i], d.ldx[i], d.w[i], d.b[i] = xs[i].data_ptr(), _ld(xs[i]), nv.ptr(ws[i]), nv.ptr(bs[i])
-            new = torch.empty if rows else torch.zeros
+    dxs = [torch.empty(dy.shape, dtype=dy.dtype, device=dev) for dy in dys]
+    dws, dbs = [None, None], [None, None]
+    if norm:
+        new = torch.empty if rows else torch.zeros
+        for i in range(2):
             if want[i][0]:
                 dws[i] = new(D, dtype=torch.float32, device=dev)
-                d.dw[i] = dws[i].data_ptr()
             if want[i][1]:
                 dbs[i] = new(D, dtype=torch.float32, device=dev)
-                d.db[i] = dbs[i].data_ptr()
-        dxs.append(dx)
+    d = _rope_desc(axes, D, dy0.dtype, norm, eps, rows, pos, freqs, dev, heads, _ptrs(xs) if norm else _NO, _ptrs(dys), _ptrs(dxs),
+                   _vptrs(ws), _ZZ, _vptrs(dws), _vptrs(dbs), 0)
     if rows:
-        with _on(dev):
-            if any(t is not None for t in dws + dbs):
-                n = nv.lib().t2v_qk_rope_bwd_floats(C.byref(d))
-                if n < 0:
-                    nv.check(int(n), "t2v_qk_rope_bwd_floats")
-                work = torch.empty(int(n), dtype=torch.float32, device=dev)
-                d.workspace = work.data_ptr()
-            nv.call("t2v_qk_rope_bwd", C.byref(d), nv.stream())
+        if norm and (want[0][0] or want[0][1] or want[1][0] or want[1][1]):
+            n = nv.lib().t2v_qk_rope_bwd_floats(C.byref(d))
+            if n < 0:
+                nv.check(int(n), "t2v_qk_rope_bwd_floats")
+            work = torch.empty(int(n), dtype=torch.float32, device=dev)
+            d.workspace = work.data_ptr()
+        _launch("t2v_qk_rope_bwd", d, dev)
     return dxs, dws, dbs
 
 
+# (The differentiable tensors are the Functions' arguments, the rest travels in one tuple: apply() spends about a microsecond per argument.)
 class _Rope(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, pos, freqs, heads, axes):
-        ctx.meta = (heads, axes)
+    def forward(ctx, x, rest):
+        heads, pos, axes, freqs = rest
+        ctx.heads, ctx.axes = heads, axes
         ctx.save_for_backward(pos, freqs)
-        return _rope_fwd((x,), (heads, 0), pos, axes, freqs, None, 0.0, (None,), (None,))[0]
+        return _rope_fwd((x,), (heads, 0), pos, axes, freqs, None, 0.0, None, None)[0]
 
     @staticmethod
     def backward(ctx, dy):
         pos, freqs = ctx.saved_tensors
-        heads, axes = ctx.meta
-        dxs, _, _ = _rope_bwd((None,), (_upstream(dy),), (heads, 0), pos, axes, freqs, None, 0.0, (None,), (None,), None)
-        return dxs[0], None, None, None, None
+        return _rope_bwd(None, (_upstream(dy),), (ctx.heads, 0), pos, ctx.axes, freqs, None, 0.0, None, None)[0][0], None
 
 
 def rope(x, heads, pos, axes, freqs=None):
@@ -207,31 +221,29 @@ def rope(x, heads, pos, axes, freqs=None):
     x = _tokens(x, "x")
     heads = int(heads)
     if torch.is_grad_enabled() and x.requires_grad:
-        return _Rope.apply(x, pos, freqs, heads, axes)
-    return _rope_fwd((x,), (heads, 0), pos, axes, freqs, None, 0.0, (None,), (None,))[0]
+        return _Rope.apply(x, (heads, pos, axes, freqs))
+    return _rope_fwd((x,), (heads, 0), pos, axes, freqs, None, 0.0, None, None)[0]
 
 
 class _QkNormRope(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, qw, kw, qb, kb, pos, freqs, heads, kv_heads, axes, norm, eps):
-        D = q.shape[1] // heads
-        ws = (_vector(qw, D, q.device, "q_weight"), _vector(kw, D, q.device, "k_weight"))
-        bs = (_vector(qb, D, q.device, "q_bias"), _vector(kb, D, q.device, "k_bias"))
-        ctx.meta = (heads, kv_heads, axes, norm, eps, [None if t is None else t.dtype for t in (qw, kw, qb, kb)])
+    def forward(ctx, q, k, qw, kw, qb, kb, rest):
+        heads, pos, axes, freqs, norm, eps, ws, bs = rest
+        ctx.meta = (heads, axes, norm, eps)
+        ctx.types = [None if t is None else t.dtype for t in (qw, kw, qb, kb)]
         ctx.save_for_backward(q, k, qw, kw, pos, freqs)
-        return _rope_fwd((q, k), (heads, kv_heads), pos, axes, freqs, norm, eps, ws, bs)
+        return _rope_fwd((q, k), heads, pos, axes, freqs, norm, eps, ws, bs)
 
     @staticmethod
     def backward(ctx, dq, dk):
         q, k, qw, kw, pos, freqs = ctx.saved_tensors
-        heads, kv_heads, axes, norm, eps, dt = ctx.meta
-        D = q.shape[1] // heads
-        ws = (_vector(qw, D, q.device, "q_weight"), _vector(kw, D, q.device, "k_weight"))
-        need = ctx.needs_input_grad
-        dxs, dws, dbs = _rope_bwd((q, k), (_upstream(dq), _upstream(dk)), (heads, kv_heads), pos, axes, freqs, norm, eps, ws, (None, None),
+        heads, axes, norm, eps = ctx.meta
+        D, dev, need = q.shape[1] // heads[0], q.device, ctx.needs_input_grad
+        ws = (_vector(qw, D, dev, "q_weight"), _vector(kw, D, dev, "k_weight"))
+        dxs, dws, dbs = _rope_bwd((q, k), (_upstream(dq), _upstream(dk)), heads, pos, axes, freqs, norm, eps, ws,
                                   ((need[2], need[4]), (need[3], need[5])))
-        g = [None if t is None else t.to(y) for t, y in zip((dws[0], dws[1], dbs[0], dbs[1]), dt)]
-        return (dxs[0], dxs[1], *g, None, None, None, None, None, None, None)
+        g = [None if t is None else t.to(y) for t, y in zip(dws + dbs, ctx.types)]
+        return (dxs[0], dxs[1], *g, None)
 
 
 def qk_norm_rope(q, k, heads, kv_heads, pos, axes, q_weight=None, k_weight=None, q_bias=None, k_bias=None, eps=1e-6, norm="rms",
@@ -247,12 +259,12 @@ def qk_norm_rope(q, k, heads, kv_heads, pos, axes, q_weight=None, k_weight=None,
         _fail(f"norm {norm!r}: 'rms' or 'layer'")
     if k.dtype != q.dtype or k.device != q.device or k.shape[0] != q.shape[0] or _head_dim(q, heads, "q") != _head_dim(k, kv_heads, "k"):
         _fail(f"q {tuple(q.shape)} {q.dtype} and k {tuple(k.shape)} {k.dtype} must have the same rows, type, device and head dim")
+    D, dev = q.shape[1] // heads, q.device
     params = (q_weight, k_weight, q_bias, k_bias)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k) + params):
-        return _QkNormRope.apply(q, k, *params, pos, freqs, heads, kv_heads, axes, norm, float(eps))
-    D = q.shape[1] // heads
-    ws = (_vector(q_weight, D, q.device, "q_weight"), _vector(k_weight, D, q.device, "k_weight"))
-    bs = (_vector(q_bias, D, q.device, "q_bias"), _vector(k_bias, D, q.device, "k_bias"))
+    ws = (_vector(q_weight, D, dev, "q_weight"), _vector(k_weight, D, dev, "k_weight"))
+    bs = (_vector(q_bias, D, dev, "q_bias"), _vector(k_bias, D, dev, "k_bias"))
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or any([t is not None and t.requires_grad for t in params])):
+        return _QkNormRope.apply(q, k, *params, ((heads, kv_heads), pos, axes, freqs, norm, float(eps), ws, bs))
     return _rope_fwd((q, k), (heads, kv_heads), pos, axes, freqs, norm, float(eps), ws, bs)
 
 
@@ -273,9 +285,10 @@ def _layout_facts(lay, rows):
     return last < rows, own, own and lay.nbatch * lay.S == rows
 
 
-def _operand(t, lay):
+def _op(t, lay):
+    """The five fields of a T2VAttnOperand."""
     ld = _ld(t)
-    return nv.AttnOperand(t.data_ptr(), lay.hi * ld, lay.lo * ld, lay.ss * ld, lay.bdiv)
+    return t.data_ptr(), lay.hi * ld, lay.lo * ld, lay.ss * ld, lay.bdiv
 
 
 def _ints(t, shapes, dev, name):
@@ -286,23 +299,21 @@ def _ints(t, shapes, dev, name):
     return t.data_ptr()
 
 
-def _attn_desc(q, k, v, o, meta, prefix, kv_len, q_docs, kv_docs, slopes, bias):
+# T2VAttnMod field by field, packed in one go (see _SIDES); _FWD ends where the fields of the backward pass begin
+_OP = "Qqqqi4x"
+_FWD = struct.Struct("@8i2f" + 4 * _OP + "QQi4xQQQQQii")
+_BWD = struct.Struct("@" + 4 * _OP + "QQi4xQq")
+_NO_BWD = bytes(_BWD.size)
+
+
+def _attn_desc(q, k, v, o, meta, lse, prefix, kv_len, q_docs, kv_docs, slopes, bias, bwd=None):
     heads, kv_heads, qlay, klay, scale, causal, softcap = meta
-    a = nv.AttnMod()
-    a.nbatch, a.heads, a.kv_heads, a.Sq, a.Sk, a.D = qlay.nbatch, heads, kv_heads, qlay.S, klay.S, q.shape[1] // heads
-    a.dtype, a.causal, a.scale, a.softcap = _TYPE[q.dtype], causal, scale, softcap
-    a.q, a.k, a.v, a.o = _operand(q, qlay), _operand(k, klay), _operand(v, klay), _operand(o, qlay)
-    if prefix is not None:
-        a.prefix, a.prefix_per_query = prefix.data_ptr(), int(prefix.dim() == 2)
-    if kv_len is not None:
-        a.kv_len = kv_len.data_ptr()
-    if q_docs is not None:
-        a.q_docs, a.kv_docs = q_docs.data_ptr(), kv_docs.data_ptr()
-    if slopes is not None:
-        a.slopes = slopes.data_ptr()
-    if bias is not None:
-        a.bias, a.bias_f32, a.radius = bias.data_ptr(), int(bias.dtype == torch.float32), bias.shape[1] // 2
-    return a
+    ptr = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
+    fwd = _FWD.pack(qlay.nbatch, heads, kv_heads, qlay.S, klay.S, q.shape[1] // heads, _TYPE[q.dtype], causal, scale, softcap,
+                    *_op(q, qlay), *_op(k, klay), *_op(v, klay), *_op(o, qlay), ptr(lse), ptr(prefix), 0 if prefix is None else prefix.dim() - 1,
+                    ptr(kv_len), ptr(q_docs), ptr(kv_docs), ptr(slopes), ptr(bias), 0 if bias is None else bias.dtype == torch.float32,
+                    0 if bias is None else bias.shape[1] // 2)
+    return nv.AttnMod.from_buffer_copy(fwd + (_NO_BWD if bwd is None else _BWD.pack(*bwd, 0, 0)))
 
 
 def _workspace(a, backward, dev):
@@ -324,21 +335,17 @@ def _attn_fwd(q, k, v, meta, prefix, kv_len, q_docs, kv_docs, slopes, bias, keep
         return o, (torch.full((qlay.nbatch * heads * qlay.S,), math.inf, device=dev) if keep else None)
     covered = _layout_facts(qlay, q.shape[0])[2]
     o = (torch.empty if covered else torch.zeros)(q.shape, dtype=q.dtype, device=dev)      # rows that no sequence owns: zeros
-    a = _attn_desc(q, k, v, o, meta, prefix, kv_len, q_docs, kv_docs, slopes, bias)
-    lse = None
-    if keep:
-        lse = torch.empty(qlay.nbatch * heads * qlay.S, dtype=torch.float32, device=dev)
-        a.lse = lse.data_ptr()
-    with _on(dev):
-        work = _workspace(a, 0, dev)
-        nv.call("t2v_attn_mod_fwd", C.byref(a), nv.stream())
-        del work
+    lse = torch.empty(qlay.nbatch * heads * qlay.S, dtype=torch.float32, device=dev) if keep else None
+    a = _attn_desc(q, k, v, o, meta, lse, prefix, kv_len, q_docs, kv_docs, slopes, bias)
+    work = _workspace(a, 0, dev)      # noqa: F841 (kept until the launch is issued)
+    _launch("t2v_attn_mod_fwd", a, dev)
     return o, lse
 
 
 class _AttentionMod(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, bias, prefix, kv_len, q_docs, kv_docs, slopes, meta):
+    def forward(ctx, q, k, v, bias, rest):
+        meta, prefix, kv_len, q_docs, kv_docs, slopes = rest
         o, lse = _attn_fwd(q, k, v, meta, prefix, kv_len, q_docs, kv_docs, slopes, bias, True)
         ctx.meta = meta
         ctx.save_for_backward(q, k, v, bias, prefix, kv_len, q_docs, kv_docs, slopes, o, lse)
@@ -358,15 +365,13 @@ class _AttentionMod(torch.autograd.Function):
         dq, dk, dv = new(q, _layout_facts(qlay, q.shape[0])[2]), new(k, kall), new(v, kall)
         dbias = new(bias, True) if bias is not None and ctx.needs_input_grad[3] else None
         if not empty:
-            a = _attn_desc(q, k, v, o, ctx.meta, prefix, kv_len, q_docs, kv_docs, slopes, bias)
             delta = torch.empty_like(lse)
-            a.lse, a.delta, a.dbias, a.kv_share = lse.data_ptr(), delta.data_ptr(), nv.ptr(dbias), share
-            a.d_o, a.dq, a.dk, a.dv = _operand(do, qlay), _operand(dq, qlay), _operand(dk, klay), _operand(dv, klay)
-            with _on(dev):
-                work = _workspace(a, 1, dev)
-                nv.call("t2v_attn_mod_bwd", C.byref(a), nv.stream())
-                del work
-        return dq, dk, dv, dbias, None, None, None, None, None, None
+            a = _attn_desc(q, k, v, o, ctx.meta, lse, prefix, kv_len, q_docs, kv_docs, slopes, bias,
+                           (*_op(do, qlay), *_op(dq, qlay), *_op(dk, klay), *_op(dv, klay), delta.data_ptr(),
+                            0 if dbias is None else dbias.data_ptr(), share))
+            work = _workspace(a, 1, dev)      # noqa: F841 (kept until the launches are issued)
+            _launch("t2v_attn_mod_bwd", a, dev)
+        return dq, dk, dv, dbias, None
 
 
 def attention_mod(q, k, v, heads, qlay, klay, kv_heads=None, scale=None, causal=False, prefix=None, kv_len=None, q_docs=None, kv_docs=None,
@@ -431,5 +436,5 @@ def attention_mod(q, k, v, heads, qlay, klay, kv_heads=None, scale=None, causal=
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (bias is not None and bias.requires_grad)):
         if not kf[1] and not (klay.bdiv > 1 and klay.lo == 0 and klay.hi >= (klay.S - 1) * klay.ss + 1 and klay.ss > 0):
             _fail(f"key layout {klay} names a row twice: gradients are defined for rows of their own, or shared by the bdiv batches (lo = 0)")
-        return _AttentionMod.apply(q, k, v, bias, prefix, kv_len, q_docs, kv_docs, slopes, meta)
+        return _AttentionMod.apply(q, k, v, bias, (meta, prefix, kv_len, q_docs, kv_docs, slopes))
     return _attn_fwd(q, k, v, meta, prefix, kv_len, q_docs, kv_docs, slopes, bias, False)[0]
