@@ -9,8 +9,8 @@
 // Layout.  Lane = query in the forward and dQ kernels (S^T = K Q^T: the row maximum and sum stay in the lane, one exchange between the
 // two halves of a wave), lane = key in the dK / dV kernel.  P^T (dS^T) goes from the accumulator registers into the next product
 // as its B operand; the transposed operand comes from the staged LDS tile through ds_read_b64_tr_b16, with the accumulators' row order
-// applied to both.  64-row tiles of the streamed pair (K|V, or Q|dO) are staged once per workgroup, double-buffered; rows of 2 DP
-// bytes, no padding, the 16-byte chunk index XORed with chunk_swizzle(row): row reads and transposed reads both spread over all banks.
+// applied to both.  64-row tiles of the streamed pair (K|V, or Q|dO) are staged once per workgroup, double-buffered; see
+// Stage for how their rows lie.
 // Grouped heads: the gp query heads that share a K/V head are packed into the row index (row r = query r / gp, head r % gp), so K and V
 // are read once for all of them; with a table each head is a unit of its own (gp = 1: the table of one head lives in LDS).
 // Statistics, the running maximum and sum, lse, delta and all accumulators are fp32; P and dS are rounded to the input type for the
@@ -62,11 +62,6 @@ __device__ __forceinline__ bf16x8 pack8(const f32x16& v, int kk) {
 __device__ __forceinline__ constexpr int crow(int r, int hi) { return (r & 3) + 8 * (r >> 2) + 4 * hi; }
 __device__ __forceinline__ float xor32(float v) { return __shfl_xor(v, 32); }
 
-template <int DP>
-__device__ __forceinline__ int chunk_swizzle(int row) {
-  return DP == 128 ? ((row & 3) << 2) | ((row >> 2) & 3) : (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
-}
-
 struct QMeta {      // of 64 rows: smallest and largest bound, smallest and largest document >= 0, whether some row has none
   int bmin, bmax, dmin, dmax, neg;
 };
@@ -91,15 +86,27 @@ __device__ __forceinline__ long long op_base(const T2VAttnOperand& o, int b) {
   return (long long)(b / o.bdiv) * o.bstride_hi + (long long)(b % o.bdiv) * o.bstride_lo;
 }
 __device__ __forceinline__ int div_gp(const Args& a, int r) { return a.gp == 1 ? r : (int)__umulhi((unsigned)r, a.magic); }
-__device__ __forceinline__ int seq_len(const Args& a, int b) {
-  return a.p.kv_len ? max(0, min(a.p.kv_len[b], a.p.Sk)) : a.p.Sk;
+// what a workgroup knows of its sequence
+struct Seq {
+  int b, len, off, prefix;          // off = len - Sq: the first query's place among the keys; prefix of the whole sequence
+  const int* per_query;             // or one per query
+  bool causal;
+};
+__device__ __forceinline__ Seq load_seq(const Args& a, int b) {
+  Seq s;
+  s.b = b;
+  s.len = a.p.kv_len ? max(0, min(a.p.kv_len[b], a.p.Sk)) : a.p.Sk;
+  s.off = s.len - a.p.Sq;
+  s.causal = a.p.causal != 0;
+  s.per_query = s.causal && a.p.prefix && a.p.prefix_per_query ? a.p.prefix + (long long)b * a.p.Sq : nullptr;
+  s.prefix = s.causal && a.p.prefix && !a.p.prefix_per_query ? a.p.prefix[b] : 0;
+  return s;
 }
 // keys [0, bound) are candidates of query i
-__device__ __forceinline__ int row_bound(const Args& a, int b, int i, int len) {
-  if (!a.p.causal) return len;
-  int m = i + len - a.p.Sq + 1;
-  if (a.p.prefix) m = max(m, a.p.prefix[a.p.prefix_per_query ? (long long)b * a.p.Sq + i : b]);
-  return max(0, min(m, len));
+__device__ __forceinline__ int row_bound(const Seq& s, int i) {
+  if (!s.causal) return s.len;
+  const int pf = s.per_query ? s.per_query[i] : s.prefix;
+  return max(0, min(max(i + s.off + 1, pf), s.len));
 }
 
 // workgroup id -> (batch, unit): workgroups go round-robin over the eight XCDs, so units that share a K/V head are placed a multiple of
@@ -117,48 +124,76 @@ __device__ __forceinline__ Unit unit_of(const Args& a, int x) {
 }
 
 // ------------------------------------------------------------------------------------------------ staging
-// Two 64-row tiles (A | B) of 2 DP bytes a row, fetched by NT threads into registers one tile ahead and written to the LDS stage after the
-// current tile's mathematics.  Rows that nobody sees are written as zeros: what they hold (inf, NaN) must not meet a zero weight.
-template <int DP, int NT>
-struct Pair {
-  static constexpr int CH = DP / 8, RPP = NT / CH, N = TILE / RPP;      // chunks per row, rows per pass, passes
-  bf16x8 a[N], b[N];
-};
-
+// Two 64-row tiles (A | B) of 2 DP bytes a row, double-buffered.  They go from memory to LDS without passing registers: 16 bytes per lane,
+// and a wave's instruction fills 1 KB of consecutive LDS addresses, a GROUP.  A group holds the rows of a 32-row block (DP = 128; of the
+// tile: DP = 64) with one row & 7, and groups lie 1056 bytes apart: eight lanes that read eight consecutive rows (ds_read_b128), and the
+// eight rows of a transposed read, start 32 bytes apart modulo the banks.  Every fragment is a lane's constant address plus an
+// immediate: an XOR swizzle needed a register per fragment and stage (136 spills in dQ), row padding cannot be had with these loads.
+constexpr int GROUP = 512 + 16;                 // elements
 template <int DP>
 struct __attribute__((aligned(16))) Stage {
-  bf16_t a[TILE * DP];
-  bf16_t b[TILE * DP];
+  bf16_t a[TILE * DP / 512 * GROUP];
+  bf16_t b[TILE * DP / 512 * GROUP];
 };
-
 template <int DP>
-__device__ __forceinline__ int stage_off(int row, int ch) { return row * DP + ((ch ^ chunk_swizzle<DP>(row)) << 3); }
+__device__ __forceinline__ constexpr int row_off(int row) {
+  return DP == 128 ? ((row >> 5) * 8 + (row & 7)) * GROUP + ((row >> 3) & 3) * 128 : (row & 7) * GROUP + (row >> 3) * 64;
+}
 
-template <int DP, int NT>
-__device__ __forceinline__ void pair_store(Stage<DP>& st, const Pair<DP, NT>& r, int tid) {
-  typedef Pair<DP, NT> P;
-#pragma unroll
-  for (int i = 0; i < P::N; ++i) {
-    const int o = stage_off<DP>(tid / P::CH + i * P::RPP, tid % P::CH);
-    *(bf16x8*)(st.a + o) = r.a[i];
-    *(bf16x8*)(st.b + o) = r.b[i];
+// What a lane loads: instruction i of a wave fills group 4 i + wave.  Columns behind the head dim come from a chunk of zeros (row stride 0).
+template <int DP>
+struct Lane {
+  static constexpr int NI = TILE * DP / 512 / 4;                        // instructions per wave
+  int wave, sub, ch;
+  bool ok;
+  __device__ __forceinline__ Lane(int w, int lane, int D) {
+    wave = w;
+    sub = 8 * (lane / (DP / 8));
+    ch = lane % (DP / 8);
+    ok = ch * 8 < D;
+  }
+  __device__ __forceinline__ int row_of(int i) const {
+    const int g = 4 * i + wave;
+    return (DP == 128 ? 32 * (g >> 3) + (g & 7) : g) + sub;
+  }
+  __device__ __forceinline__ int group(int i) const { return (4 * i + wave) * GROUP; }
+};
+__device__ __forceinline__ void copy16(const void* src, void* lds) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src, (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
+}
+// (the builtin and not inline asm: the compiler then knows that nothing is in flight behind it, and does not wait again, for the next tile's
+// copies, at the first use of what was loaded in front of the loop)
+__device__ __forceinline__ void copies_done() { __builtin_amdgcn_s_waitcnt(0x0f70); }      // vmcnt(0)
+// zero the staged rows for which `dead(row)`: rows that nobody sees may hold inf / NaN, which must not meet a zero weight
+template <int DP, typename F>
+__device__ __forceinline__ void clear_rows(Stage<DP>& st, int tid, F dead) {
+  const bf16x8 z = {0, 0, 0, 0, 0, 0, 0, 0};
+  for (int i = tid; i < TILE * DP / 8; i += 256) {
+    const int row = i / (DP / 8), o = row_off<DP>(row) + (i % (DP / 8)) * 8;
+    if (dead(row)) {
+      *(bf16x8*)(st.a + o) = z;
+      *(bf16x8*)(st.b + o) = z;
+    }
   }
 }
 
-// fragment of 32 staged rows as an MFMA operand (row = lane & 31, k = the 16 columns of step kd)
+// lane's part of the address of a row fragment (32 staged rows as an MFMA operand: row = lane & 31, k = the 16 columns of step kd) and of a
+// transposed fragment (rows = columns [32 fm, 32 fm + 32), k = the 16 staged rows of step kk in the accumulators' order)
 template <int DP>
-__device__ __forceinline__ bf16x8 rowfrag(const bf16_t* s, int blk, int kd, int lane) {
-  const int row = 32 * blk + (lane & 31);
-  return *(const bf16x8*)(s + stage_off<DP>(row, 2 * kd + (lane >> 5)));
-}
-// fragment of the transposed tile: rows = columns [32 fm, 32 fm + 32), k = the 16 staged rows of step kk in the accumulators' order
+__device__ __forceinline__ int lane_row(int lane) { return row_off<DP>(lane & 31) + 8 * (lane >> 5); }
 template <int DP>
-__device__ __forceinline__ bf16x8 trfrag(const bf16_t* s, int blk, int fm, int kk, int lane) {
+__device__ __forceinline__ int lane_tr(int lane) {
   const int gq = lane >> 4, li = lane & 15;
-  const int row = 32 * blk + 16 * kk + 4 * (gq >> 1) + (li >> 2);
-  const int ch = 4 * fm + 2 * (gq & 1) + ((li & 3) >> 1), in = 4 * (li & 1);
-  const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_bf16x4*)(s + stage_off<DP>(row, ch) + in));
-  const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_bf16x4*)(s + stage_off<DP>(row + 8, ch) + in));
+  return row_off<DP>(4 * (gq >> 1) + (li >> 2)) + 16 * (gq & 1) + 4 * (li & 3);
+}
+template <int DP>
+__device__ __forceinline__ bf16x8 rowfrag(const bf16_t* s, int blk, int kd) {
+  return *(const bf16x8*)(s + row_off<DP>(32 * blk) + 16 * kd);
+}
+template <int DP>
+__device__ __forceinline__ bf16x8 trfrag(const bf16_t* s, int blk, int fm, int kk) {
+  const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_bf16x4*)(s + row_off<DP>(32 * blk + 16 * kk) + 32 * fm));
+  const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_bf16x4*)(s + row_off<DP>(32 * blk + 16 * kk + 8) + 32 * fm));
   return bf16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
 }
 
@@ -208,17 +243,25 @@ __device__ __forceinline__ void load_table(const Args& a, int h, float* tab, int
   }
 }
 
-// next tile >= t (and < end) whose keys / rows may matter; `active(t)` is evaluated for 64 tiles at once, one per lane
+// The tiles in [t, end) that may matter, in order: `active` is evaluated for 64 tiles at once, one per lane, and kept as a mask; without
+// `filter` every tile counts.  All waves of a workgroup walk the same tiles.
+struct TileIter {
+  unsigned long long m;
+  int base, end;
+  bool filter;
+};
 template <typename F>
-__device__ __forceinline__ int next_tile(int t, int end, F active) {
-  const int lane = threadIdx.x & 63;
-  while (t < end) {
-    const int c = t + lane;
-    const unsigned long long m = __ballot(c < end && active(min(c, end - 1)));
-    if (m) return t + __builtin_ctzll(m);
-    t += 64;
+__device__ __forceinline__ int tile_next(TileIter& it, F active) {
+  if (!it.filter) return it.base < it.end ? it.base++ : it.end;
+  while (it.m == 0) {
+    if (it.base >= it.end) return it.end;
+    const int c = it.base + (int)(threadIdx.x & 63);
+    it.m = __ballot(c < it.end && active(min(c, it.end - 1)));
+    it.base += 64;
   }
-  return end;
+  const int t = it.base - 64 + __builtin_ctzll(it.m);
+  it.m &= it.m - 1;
+  return t;
 }
 
 // minimum / maximum over the wave as a scalar
@@ -240,11 +283,11 @@ struct Rows {
   bool ok[QB];                      // the row exists
   int bound[QB], pos[QB], doc[QB];  // bound 0: sees nothing
   float slope[QB];                  // in base-2 units
-  int bmin, bmax, dmin, dmax;       // over the wave
+  int bmin, bmax, dmin, dmax, pmin; // over the wave
   bool neg;
 };
 template <int QB>
-__device__ __forceinline__ void load_rows(Rows<QB>& R, const Args& a, const Unit& u, int len, int r0, int lane) {
+__device__ __forceinline__ void load_rows(Rows<QB>& R, const Args& a, const Unit& u, const Seq& sq, int r0, int lane) {
   int lo = 0x7fffffff, hi = 0, dlo = 0x7fffffff, dhi = -1, ng = 0;
 #pragma unroll
   for (int q = 0; q < QB; ++q) {
@@ -253,8 +296,8 @@ __device__ __forceinline__ void load_rows(Rows<QB>& R, const Args& a, const Unit
     const int rc = min(R.r[q], a.M - 1);
     R.i[q] = div_gp(a, rc);
     R.h[q] = u.h0 + rc - R.i[q] * a.gp;
-    R.bound[q] = R.ok[q] ? row_bound(a, u.b, R.i[q], len) : 0;
-    R.pos[q] = R.i[q] + len - a.p.Sq;
+    R.bound[q] = R.ok[q] ? row_bound(sq, R.i[q]) : 0;
+    R.pos[q] = R.i[q] + sq.off;
     R.doc[q] = a.p.q_docs ? a.p.q_docs[(long long)u.b * a.p.Sq + R.i[q]] : 0;
     if (R.doc[q] < 0) R.bound[q] = 0;
     R.slope[q] = a.p.slopes ? a.p.slopes[R.h[q]] * LOG2E : 0.f;
@@ -268,6 +311,7 @@ __device__ __forceinline__ void load_rows(Rows<QB>& R, const Args& a, const Unit
     }
   }
   R.bmin = wave_min_i(lo);
+  R.pmin = __builtin_amdgcn_readfirstlane(div_gp(a, min(r0, a.M - 1)) + sq.off);      // rows are in the queries' order
   R.bmax = wave_max_i(hi);
   R.dmin = wave_min_i(dlo);
   R.dmax = wave_max_i(dhi);
@@ -275,11 +319,11 @@ __device__ __forceinline__ void load_rows(Rows<QB>& R, const Args& a, const Unit
 }
 
 // ------------------------------------------------------------------------------------------------ forward
-template <typename T, int DP, int QB, bool MOD>
-__global__ __launch_bounds__(256, (DP == 64 || QB == 1) ? 2 : 1) void attn_mod_fwd_kernel(const Args a) {
+// MOD: bit 0 cap, bit 1 distance bias (slopes / table), compile-time so that a tile is straight-line code
+template <typename T, int DP, int QB, int MOD>
+__global__ __launch_bounds__(256, (DP * QB <= 128) ? 2 : 1) void attn_mod_fwd_kernel(const Args a) {
   warm_kernargs<(int)sizeof(Args)>();
   constexpr int NT = 256, KD = DP / 16, FM = DP / 32;
-  typedef Pair<DP, NT> P;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   Stage<DP>* st = (Stage<DP>*)smem;
   int* sdoc = (int*)(smem + 2 * sizeof(Stage<DP>));                     // [2][TILE]
@@ -290,16 +334,15 @@ __global__ __launch_bounds__(256, (DP == 64 || QB == 1) ? 2 : 1) void attn_mod_f
   const int x = blockIdx.x % NU, rest = blockIdx.x / NU;
   const int sp = rest % a.splits, tile = a.ntile - 1 - rest / a.splits; // the longest rows of a causal mask first
   const Unit u = unit_of(a, x);
-  const int len = seq_len(a, u.b), D = a.p.D, Sk = a.p.Sk;
+  const Seq seq = load_seq(a, u.b);
+  const int len = seq.len, D = a.p.D, Sk = a.p.Sk;
   const bf16_t* Q = (const bf16_t*)a.p.q.ptr + op_base(a.p.q, u.b);
-  const bf16_t* K = (const bf16_t*)a.p.k.ptr + op_base(a.p.k, u.b) + (long long)u.kv * D;
-  const bf16_t* V = (const bf16_t*)a.p.v.ptr + op_base(a.p.v, u.b) + (long long)u.kv * D;
   const bool docs = a.kmeta && a.p.kv_docs;
   const int* kdoc = docs ? a.p.kv_docs + (long long)u.b * Sk : nullptr;
   const Mod mod = make_mod(a);
 
   Rows<QB> R;
-  load_rows(R, a, u, len, (tile * 4 + wave) * 32 * QB, lane);
+  load_rows(R, a, u, seq, (tile * 4 + wave) * 32 * QB, lane);
   bf16x8 qf[QB][KD];
 #pragma unroll
   for (int q = 0; q < QB; ++q) {
@@ -307,7 +350,7 @@ __global__ __launch_bounds__(256, (DP == 64 || QB == 1) ? 2 : 1) void attn_mod_f
 #pragma unroll
     for (int kd = 0; kd < KD; ++kd) qf[q][kd] = *chunk_ptr(qp + 16 * kd + 8 * hi, R.bound[q] > 0 && 16 * kd + 8 * hi < D);
   }
-  if (MOD && mod.table) load_table<T>(a, u.h0, tab, tid, NT);
+  if ((MOD & 2) && mod.table) load_table<T>(a, u.h0, tab, tid, NT);
   if (lane == 0) {
     swg[wave * 4] = R.bmax;
     swg[wave * 4 + 1] = R.dmin;
@@ -325,37 +368,34 @@ __global__ __launch_bounds__(256, (DP == 64 || QB == 1) ? 2 : 1) void attn_mod_f
   const int nt = (bmax + TILE - 1) / TILE, per = (nt + a.splits - 1) / a.splits;
   const int tbeg = min(nt, sp * per), tend = min(nt, tbeg + per);
   const KMeta* km = docs ? a.kmeta + (long long)u.b * ((Sk + TILE - 1) / TILE) : nullptr;
-  auto next = [&](int t) {
-    return docs ? next_tile(t, tend, [&](int c) { return km[c].dmax >= dmin && km[c].dmin <= dmax; }) : min(t, tend);
-  };
-  P nx;
-  int nd = 0, ndv[P::N];
-  auto fetch = [&](int t) {
-    const int ch = tid % P::CH;
+  auto active = [&](int c) { return km[c].dmax >= dmin && km[c].dmin <= dmax; };
+  TileIter it = {0ull, tbeg, tend, docs};
+  const Lane<DP> ln(wave, lane, D);
+  const int lrow = lane_row<DP>(lane), ltr = lane_tr<DP>(lane);
+  const bf16_t* kp = ln.ok ? (const bf16_t*)a.p.k.ptr + op_base(a.p.k, u.b) + (long long)u.kv * D + ln.ch * 8 : (const bf16_t*)zero_chunk;
+  const bf16_t* vp = ln.ok ? (const bf16_t*)a.p.v.ptr + op_base(a.p.v, u.b) + (long long)u.kv * D + ln.ch * 8 : (const bf16_t*)zero_chunk;
+  const unsigned ks = ln.ok ? (unsigned)a.p.k.sstride : 0u, vs = ln.ok ? (unsigned)a.p.v.sstride : 0u;
+  int nd = 0;
+  auto fetch = [&](int t, int sidx) {                                   // rows behind the last key repeat it (masked by the bounds)
 #pragma unroll
-    for (int i = 0; i < P::N; ++i) {
-      const int row = t * TILE + tid / P::CH + i * P::RPP;
-      const bool ok = row < len && ch * 8 < D;
-      nx.a[i] = *chunk_ptr(K + (long long)row * a.p.k.sstride + ch * 8, ok);
-      nx.b[i] = *chunk_ptr(V + (long long)row * a.p.v.sstride + ch * 8, ok);
-      if (docs) ndv[i] = kdoc[min(row, Sk - 1)];
+    for (int i = 0; i < Lane<DP>::NI; ++i) {
+      const unsigned row = (unsigned)min(t * TILE + ln.row_of(i), len - 1);
+      copy16(kp + (unsigned long long)row * ks, st[sidx].a + ln.group(i));
+      copy16(vp + (unsigned long long)row * vs, st[sidx].b + ln.group(i));
     }
     if (docs && tid < TILE) {
       const int row = t * TILE + tid;
       nd = row < len ? kdoc[row] : -1;
     }
   };
-  auto store = [&](int sidx) {
-    if (docs) {
-#pragma unroll
-      for (int i = 0; i < P::N; ++i) {
-        const bf16x8 z = {0, 0, 0, 0, 0, 0, 0, 0};
-        nx.a[i] = ndv[i] < 0 ? z : nx.a[i];
-        nx.b[i] = ndv[i] < 0 ? z : nx.b[i];
-      }
-      if (tid < TILE) sdoc[sidx * TILE + tid] = nd;
+  auto landed = [&](int sidx, int neg) {                                // the tile fetched into stage sidx is there for all waves
+    if (docs && tid < TILE) sdoc[sidx * TILE + tid] = nd;
+    copies_done();
+    __syncthreads();
+    if (neg) {
+      clear_rows(st[sidx], tid, [&](int r) { return sdoc[sidx * TILE + r] < 0; });
+      __syncthreads();
     }
-    pair_store(st[sidx], nx, tid);
   };
 
   float m[QB], l[QB];
@@ -369,132 +409,162 @@ __global__ __launch_bounds__(256, (DP == 64 || QB == 1) ? 2 : 1) void attn_mod_f
 #pragma unroll
       for (int r = 0; r < 16; ++r) o[q][f][r] = 0.f;
   }
-  int t = next(tbeg), cur = 0;
+  int t = tile_next(it, active), cur = 0;
+  KMeta kn = {0, 0, 0};                                                 // of the tile at hand (documents)
   if (t < tend) {
-    fetch(t);
-    store(0);
+    if (docs) kn = km[t];
+    fetch(t, 0);
+    landed(0, kn.neg);
   }
-  __syncthreads();
-  while (t < tend) {
-    const int tn = next(t + 1);
-    if (tn < tend) fetch(tn);
+  auto math = [&](bool partial, int t) {
     const int k0 = t * TILE;
-    if (k0 < R.bmax) {
-      const bf16_t* sk = st[cur].a;
-      const bf16_t* sv = st[cur].b;
-      f32x16 s[QB][2];
+    const bf16_t* sk = st[cur].a;
+    const bf16_t* sv = st[cur].b;
+    f32x16 s[QB][2];
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb) {
+    for (int kb = 0; kb < 2; ++kb) {
 #pragma unroll
-        for (int q = 0; q < QB; ++q)
+      for (int q = 0; q < QB; ++q)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s[q][kb][r] = 0.f;
+        for (int r = 0; r < 16; ++r) s[q][kb][r] = 0.f;
+      bf16x8 kf[KD];
 #pragma unroll
-        for (int kd = 0; kd < KD; ++kd) {
-          const bf16x8 kf = rowfrag<DP>(sk, kb, kd, lane);
+      for (int kd = 0; kd < KD; ++kd) kf[kd] = rowfrag<DP>(sk + lrow, kb, kd);
 #pragma unroll
-          for (int q = 0; q < QB; ++q) s[q][kb] = El<T>::mfma(kf, qf[q][kd], s[q][kb]);
-        }
-      }
-      bool partial = k0 + TILE > R.bmin;
-      if (docs) partial |= km[t].neg | (km[t].dmin != km[t].dmax) | (R.dmin != R.dmax) | R.neg | (km[t].dmin != R.dmin);
-      if (MOD) {
+      for (int kd = 0; kd < KD; ++kd)
 #pragma unroll
-        for (int q = 0; q < QB; ++q)
+        for (int q = 0; q < QB; ++q) s[q][kb] = El<T>::mfma(kf[kd], qf[q][kd], s[q][kb]);
+    }
+    const float c = MOD ? 1.f : mod.c;
+    bf16x8 pb[QB][4];
 #pragma unroll
-          for (int kb = 0; kb < 2; ++kb) {
-            f32x16& v = s[q][kb];
-            if (mod.cap) {
+    for (int q = 0; q < QB; ++q) {
+      float off[2] = {0.f, 0.f};                                        // score = s + off[kb]
+      if (MOD & 1) {
 #pragma unroll
-              for (int r = 0; r < 16; ++r) {
-                float w;
-                v[r] = capped(mod, v[r], w);
-              }
-            } else {
+        for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-              for (int r = 0; r < 16; ++r) v[r] *= mod.c;
-            }
-            const int d0 = k0 + 32 * kb + 4 * hi - R.pos[q];
-            if (mod.slope) {
-              const float f0 = (float)d0;
-#pragma unroll
-              for (int r = 0; r < 16; ++r) v[r] = fmaf(-R.slope[q], fabsf(f0 + crow(r, 0)), v[r]);
-            }
-            if (mod.table) {
-#pragma unroll
-              for (int r = 0; r < 16; ++r) v[r] += tab[max(-mod.R, min(mod.R, d0 + crow(r, 0))) + mod.R];
-            }
+          for (int r = 0; r < 16; ++r) {
+            float w;
+            s[q][kb][r] = capped(mod, s[q][kb][r], w);
           }
+      }
+      if (MOD & 2) {
+        const int d0 = k0 + 4 * hi - R.pos[q];
+        const float cc = (MOD & 1) ? 1.f : mod.c;
+        if (mod.slope) {
+          if (k0 + TILE - 1 <= R.pmin) {                                // every key at or before every query: |d| = -d, linear in the row
+            const float sl = R.slope[q];
+            off[0] = sl * (float)d0;
+            off[1] = sl * (float)(d0 + 32);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const float b = sl * (float)crow(r, 0);
+              s[q][0][r] = fmaf(s[q][0][r], cc, b);
+              s[q][1][r] = fmaf(s[q][1][r], cc, b);
+            }
+          } else {
+            const float f0 = (float)d0;
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+              for (int r = 0; r < 16; ++r)
+                s[q][kb][r] = fmaf(-R.slope[q], fabsf(f0 + (32 * kb + crow(r, 0))), s[q][kb][r] * cc);
+          }
+        } else if (!(MOD & 1)) {
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[q][kb][r] *= cc;
+        }
+        if (mod.table) {
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[q][kb][r] += tab[max(-mod.R, min(mod.R, d0 + 32 * kb + crow(r, 0))) + mod.R];
+        }
       }
       if (partial) {
 #pragma unroll
-        for (int q = 0; q < QB; ++q)
+        for (int kb = 0; kb < 2; ++kb) {
+          const int lim = R.bound[q] - k0 - 32 * kb - 4 * hi;
 #pragma unroll
-          for (int kb = 0; kb < 2; ++kb) {
-            const int lim = R.bound[q] - k0 - 32 * kb - 4 * hi;
+          for (int r = 0; r < 16; ++r) s[q][kb][r] = crow(r, 0) < lim ? s[q][kb][r] : -INFINITY;
+          if (docs) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[q][kb][r] = crow(r, 0) < lim ? s[q][kb][r] : -INFINITY;
-            if (docs) {
-#pragma unroll
-              for (int g = 0; g < 4; ++g) {
-                const int4 dv = *(const int4*)(sdoc + cur * TILE + 32 * kb + 8 * g + 4 * hi);
-                s[q][kb][4 * g] = dv.x == R.doc[q] ? s[q][kb][4 * g] : -INFINITY;
-                s[q][kb][4 * g + 1] = dv.y == R.doc[q] ? s[q][kb][4 * g + 1] : -INFINITY;
-                s[q][kb][4 * g + 2] = dv.z == R.doc[q] ? s[q][kb][4 * g + 2] : -INFINITY;
-                s[q][kb][4 * g + 3] = dv.w == R.doc[q] ? s[q][kb][4 * g + 3] : -INFINITY;
-              }
+            for (int g = 0; g < 4; ++g) {
+              const int4 dv = *(const int4*)(sdoc + cur * TILE + 32 * kb + 8 * g + 4 * hi);
+              s[q][kb][4 * g] = dv.x == R.doc[q] ? s[q][kb][4 * g] : -INFINITY;
+              s[q][kb][4 * g + 1] = dv.y == R.doc[q] ? s[q][kb][4 * g + 1] : -INFINITY;
+              s[q][kb][4 * g + 2] = dv.z == R.doc[q] ? s[q][kb][4 * g + 2] : -INFINITY;
+              s[q][kb][4 * g + 3] = dv.w == R.doc[q] ? s[q][kb][4 * g + 3] : -INFINITY;
             }
           }
-      }
-      const float c = MOD ? 1.f : mod.c;
-      bf16x8 pb[QB][4];
-#pragma unroll
-      for (int q = 0; q < QB; ++q) {
-        float mx = fmaxf(s[q][0][0], s[q][1][0]);
-#pragma unroll
-        for (int r = 1; r < 16; ++r) mx = fmaxf(fmaxf(mx, s[q][0][r]), s[q][1][r]);
-        mx = fmaxf(mx, xor32(mx));
-        // the running maximum is raised only when some row of the wave grew by more than DEFER exponent units: p <= 2^DEFER instead of
-        // <= 1, the same relative precision, and the common tile skips the rescale of O
-        constexpr float DEFER = 6.f;
-        if (!__all((mx - m[q]) * c <= DEFER)) {
-          const float mn = fmaxf(m[q], mx);
-          const float alpha = __builtin_amdgcn_exp2f((m[q] - mn) * c);
-          m[q] = mn;
-          l[q] *= alpha;
-#pragma unroll
-          for (int f = 0; f < FM; ++f)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) o[q][f][r] *= alpha;
         }
-        const float mc = m[q] * c;
-        float rs = 0.f;
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const float pv = __builtin_amdgcn_exp2f(MOD ? s[q][kb][r] - mc : fmaf(s[q][kb][r], c, -mc));
-            s[q][kb][r] = pv;
-            rs += pv;
-          }
-          pb[q][2 * kb] = pack8<T>(s[q][kb], 0);
-          pb[q][2 * kb + 1] = pack8<T>(s[q][kb], 1);
-        }
-        l[q] += rs;
       }
+      float mx0 = s[q][0][0], mx1 = s[q][1][0];
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
+      for (int r = 1; r < 16; ++r) {
+        mx0 = fmaxf(mx0, s[q][0][r]);
+        mx1 = fmaxf(mx1, s[q][1][r]);
+      }
+      float mx = fmaxf(mx0 + off[0], mx1 + off[1]);
+      mx = fmaxf(mx, xor32(mx));
+      // the running maximum is raised only when some row of the wave grew by more than DEFER exponent units: p <= 2^DEFER instead of
+      // <= 1, the same relative precision, and the common tile skips the rescale of O
+      constexpr float DEFER = 6.f;
+      if (!__all((mx - m[q]) * c <= DEFER)) {
+        const float mn = fmaxf(m[q], mx);
+        const float alpha = __builtin_amdgcn_exp2f((m[q] - mn) * c);
+        m[q] = mn;
+        l[q] *= alpha;
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk)
+        for (int f = 0; f < FM; ++f)
 #pragma unroll
-          for (int f = 0; f < FM; ++f) {
-            const bf16x8 vf = trfrag<DP>(sv, kb, f, kk, lane);
+          for (int r = 0; r < 16; ++r) o[q][f][r] *= alpha;
+      }
+      float rs[2] = {0.f, 0.f};
 #pragma unroll
-            for (int q = 0; q < QB; ++q) o[q][f] = El<T>::mfma(vf, pb[q][2 * kb + kk], o[q][f]);
-          }
+      for (int kb = 0; kb < 2; ++kb) {
+        const float mc = MOD ? m[q] - off[kb] : m[q] * c;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float pv = __builtin_amdgcn_exp2f(MOD ? s[q][kb][r] - mc : fmaf(s[q][kb][r], c, -mc));
+          s[q][kb][r] = pv;
+          rs[r & 1] += pv;
+        }
+        pb[q][2 * kb] = pack8<T>(s[q][kb], 0);
+        pb[q][2 * kb + 1] = pack8<T>(s[q][kb], 1);
+      }
+      l[q] += rs[0] + rs[1];
     }
-    if (tn < tend) store(cur ^ 1);
-    __syncthreads();
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk) {
+        bf16x8 vf[FM];
+#pragma unroll
+        for (int f = 0; f < FM; ++f) vf[f] = trfrag<DP>(sv + ltr, kb, f, kk);
+#pragma unroll
+        for (int f = 0; f < FM; ++f)
+#pragma unroll
+          for (int q = 0; q < QB; ++q) o[q][f] = El<T>::mfma(vf[f], pb[q][2 * kb + kk], o[q][f]);
+      }
+  };
+  while (t < tend) {
+    const int tn = tile_next(it, active);
+    const KMeta kt = kn;
+    if (tn < tend) {
+      fetch(tn, cur ^ 1);
+      if (docs) kn = km[tn];
+    }
+    const int k0 = t * TILE;
+    if (k0 < R.bmax) {
+      bool partial = k0 + TILE > R.bmin;
+      if (docs) partial |= (kt.neg != 0) | (kt.dmin != kt.dmax) | (R.dmin != R.dmax) | R.neg | (kt.dmin != R.dmin);
+      math(partial, t);
+    }
+    if (tn < tend) landed(cur ^ 1, docs ? kn.neg : 0);
     cur ^= 1;
     t = tn;
   }
@@ -567,13 +637,15 @@ __global__ __launch_bounds__(256) void attn_mod_join_kernel(const Args a) {
 
 // bounds and documents of every 64 rows / keys (launched where a mask has documents or one prefix per query): one wave per tile
 __global__ __launch_bounds__(64) void attn_mod_meta_kernel(const Args a, QMeta* qm, KMeta* km, int nq, int nk) {
-  const int lane = threadIdx.x, b = blockIdx.y, t = blockIdx.x, len = seq_len(a, b);
+  const int lane = threadIdx.x, b = blockIdx.y, t = blockIdx.x;
+  const Seq seq = load_seq(a, b);
+  const int len = seq.len;
   if (t < nq) {
     const int r = t * TILE + lane;
     int lo = 0x7fffffff, hi = 0, dlo = 0x7fffffff, dhi = -1, ng = 0;
     if (r < a.M) {
       const int i = div_gp(a, r), d = a.p.q_docs ? a.p.q_docs[(long long)b * a.p.Sq + i] : 0;
-      const int bd = d < 0 ? 0 : row_bound(a, b, i, len);
+      const int bd = d < 0 ? 0 : row_bound(seq, i);
       lo = hi = bd;
       if (bd > 0) dlo = dhi = d;
       else ng = 1;
@@ -594,11 +666,10 @@ __global__ __launch_bounds__(64) void attn_mod_meta_kernel(const Args a, QMeta* 
 }
 
 // ------------------------------------------------------------------------------------------------ backward: dQ, delta, table gradient
-template <typename T, int DP, int QB, bool MOD>
-__global__ __launch_bounds__(256, (DP == 64 || QB == 1) ? 2 : 1) void attn_mod_dq_kernel(const Args a) {
+template <typename T, int DP, int QB, int MOD>
+__global__ __launch_bounds__(256, (DP * QB <= 128) ? 2 : 1) void attn_mod_dq_kernel(const Args a) {
   warm_kernargs<(int)sizeof(Args)>();
   constexpr int NT = 256, KD = DP / 16, FM = DP / 32;
-  typedef Pair<DP, NT> P;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   Stage<DP>* st = (Stage<DP>*)smem;
   int* sdoc = (int*)(smem + 2 * sizeof(Stage<DP>));
@@ -608,18 +679,17 @@ __global__ __launch_bounds__(256, (DP == 64 || QB == 1) ? 2 : 1) void attn_mod_d
   const int NU = a.p.nbatch * a.nunit;
   const int x = blockIdx.x % NU, tile = a.ntile - 1 - blockIdx.x / NU;
   const Unit u = unit_of(a, x);
-  const int len = seq_len(a, u.b), D = a.p.D, Sk = a.p.Sk;
-  const bf16_t* K = (const bf16_t*)a.p.k.ptr + op_base(a.p.k, u.b) + (long long)u.kv * D;
-  const bf16_t* V = (const bf16_t*)a.p.v.ptr + op_base(a.p.v, u.b) + (long long)u.kv * D;
+  const Seq seq = load_seq(a, u.b);
+  const int len = seq.len, D = a.p.D, Sk = a.p.Sk;
   const bool docs = a.kmeta && a.p.kv_docs;
   const int* kdoc = docs ? a.p.kv_docs + (long long)u.b * Sk : nullptr;
   const Mod mod = make_mod(a);
   const int ntab = 2 * a.p.radius + 1;
   float* sums = tab + ntab + wave * ntab;
-  const bool dtab = MOD && mod.table && a.p.dbias != nullptr;
+  const bool dtab = (MOD & 2) && mod.table && a.p.dbias != nullptr;
 
   Rows<QB> R;
-  load_rows(R, a, u, len, (tile * 4 + wave) * 32 * QB, lane);
+  load_rows(R, a, u, seq, (tile * 4 + wave) * 32 * QB, lane);
   bf16x8 qf[QB][KD], gf[QB][KD];
   float lse[QB], dl[QB];
 #pragma unroll
@@ -643,7 +713,7 @@ __global__ __launch_bounds__(256, (DP == 64 || QB == 1) ? 2 : 1) void attn_mod_d
     lse[q] = R.ok[q] ? a.p.lse[sidx] : INFINITY;
     if (R.ok[q] && hi == 0) a.p.delta[sidx] = d;
   }
-  if (MOD && mod.table) load_table<T>(a, u.h0, tab, tid, NT);
+  if ((MOD & 2) && mod.table) load_table<T>(a, u.h0, tab, tid, NT);
   if (dtab)
     for (int i = lane; i < ntab; i += 64) sums[i] = 0.f;
   if (lane == 0) {
@@ -662,37 +732,34 @@ __global__ __launch_bounds__(256, (DP == 64 || QB == 1) ? 2 : 1) void attn_mod_d
   bmax = __builtin_amdgcn_readfirstlane(bmax);
   const int tend = (bmax + TILE - 1) / TILE;
   const KMeta* km = docs ? a.kmeta + (long long)u.b * ((Sk + TILE - 1) / TILE) : nullptr;
-  auto next = [&](int t) {
-    return docs ? next_tile(t, tend, [&](int c) { return km[c].dmax >= dmin && km[c].dmin <= dmax; }) : min(t, tend);
-  };
-  P nx;
-  int nd = 0, ndv[P::N];
-  auto fetch = [&](int t) {
-    const int ch = tid % P::CH;
+  auto active = [&](int c) { return km[c].dmax >= dmin && km[c].dmin <= dmax; };
+  TileIter it = {0ull, 0, tend, docs};
+  const Lane<DP> ln(wave, lane, D);
+  const int lrow = lane_row<DP>(lane), ltr = lane_tr<DP>(lane);
+  const bf16_t* kp = ln.ok ? (const bf16_t*)a.p.k.ptr + op_base(a.p.k, u.b) + (long long)u.kv * D + ln.ch * 8 : (const bf16_t*)zero_chunk;
+  const bf16_t* vp = ln.ok ? (const bf16_t*)a.p.v.ptr + op_base(a.p.v, u.b) + (long long)u.kv * D + ln.ch * 8 : (const bf16_t*)zero_chunk;
+  const unsigned ks = ln.ok ? (unsigned)a.p.k.sstride : 0u, vs = ln.ok ? (unsigned)a.p.v.sstride : 0u;
+  int nd = 0;
+  auto fetch = [&](int t, int sidx) {                                   // rows behind the last key repeat it (masked by the bounds)
 #pragma unroll
-    for (int i = 0; i < P::N; ++i) {
-      const int row = t * TILE + tid / P::CH + i * P::RPP;
-      const bool ok = row < len && ch * 8 < D;
-      nx.a[i] = *chunk_ptr(K + (long long)row * a.p.k.sstride + ch * 8, ok);
-      nx.b[i] = *chunk_ptr(V + (long long)row * a.p.v.sstride + ch * 8, ok);
-      if (docs) ndv[i] = kdoc[min(row, Sk - 1)];
+    for (int i = 0; i < Lane<DP>::NI; ++i) {
+      const unsigned row = (unsigned)min(t * TILE + ln.row_of(i), len - 1);
+      copy16(kp + (unsigned long long)row * ks, st[sidx].a + ln.group(i));
+      copy16(vp + (unsigned long long)row * vs, st[sidx].b + ln.group(i));
     }
     if (docs && tid < TILE) {
       const int row = t * TILE + tid;
       nd = row < len ? kdoc[row] : -1;
     }
   };
-  auto store = [&](int sidx) {
-    if (docs) {
-#pragma unroll
-      for (int i = 0; i < P::N; ++i) {
-        const bf16x8 z = {0, 0, 0, 0, 0, 0, 0, 0};
-        nx.a[i] = ndv[i] < 0 ? z : nx.a[i];
-        nx.b[i] = ndv[i] < 0 ? z : nx.b[i];
-      }
-      if (tid < TILE) sdoc[sidx * TILE + tid] = nd;
+  auto landed = [&](int sidx, int neg) {                                // the tile fetched into stage sidx is there for all waves
+    if (docs && tid < TILE) sdoc[sidx * TILE + tid] = nd;
+    copies_done();
+    __syncthreads();
+    if (neg) {
+      clear_rows(st[sidx], tid, [&](int r) { return sdoc[sidx * TILE + r] < 0; });
+      __syncthreads();
     }
-    pair_store(st[sidx], nx, tid);
   };
   f32x16 acc[QB][FM];
 #pragma unroll
@@ -702,121 +769,129 @@ __global__ __launch_bounds__(256, (DP == 64 || QB == 1) ? 2 : 1) void attn_mod_d
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[q][f][r] = 0.f;
   float below = 0.f, above = 0.f;                                       // gradient of the table's two ends, per lane
-  int t = next(0), cur = 0;
+  int t = tile_next(it, active), cur = 0;
+  KMeta kn = {0, 0, 0};                                                 // of the tile at hand (documents)
   if (t < tend) {
-    fetch(t);
-    store(0);
+    if (docs) kn = km[t];
+    fetch(t, 0);
+    landed(0, kn.neg);
   }
-  __syncthreads();
-  while (t < tend) {
-    const int tn = next(t + 1);
-    if (tn < tend) fetch(tn);
+  auto math = [&](bool partial, int t) {
     const int k0 = t * TILE;
-    if (k0 < R.bmax) {
-      const bf16_t* sk = st[cur].a;
-      const bf16_t* sv = st[cur].b;
-      bool partial = k0 + TILE > R.bmin;
-      if (docs) partial |= km[t].neg | (km[t].dmin != km[t].dmax) | (R.dmin != R.dmax) | R.neg | (km[t].dmin != R.dmin);
+    const bf16_t* sk = st[cur].a;
+    const bf16_t* sv = st[cur].b;
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb) {
-        f32x16 s[QB], dp[QB];
+    for (int kb = 0; kb < 2; ++kb) {
+      f32x16 s[QB], dp[QB];
 #pragma unroll
-        for (int q = 0; q < QB; ++q)
+      for (int q = 0; q < QB; ++q)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s[q][r] = dp[q][r] = 0.f;
+        for (int r = 0; r < 16; ++r) s[q][r] = dp[q][r] = 0.f;
 #pragma unroll
-        for (int kd = 0; kd < KD; ++kd) {
-          const bf16x8 kf = rowfrag<DP>(sk, kb, kd, lane), vf = rowfrag<DP>(sv, kb, kd, lane);
-#pragma unroll
-          for (int q = 0; q < QB; ++q) {
-            s[q] = El<T>::mfma(kf, qf[q][kd], s[q]);
-            dp[q] = El<T>::mfma(vf, gf[q][kd], dp[q]);
-          }
-        }
-        bf16x8 db[QB][2];
+      for (int kd = 0; kd < KD; ++kd) {
+        const bf16x8 kf = rowfrag<DP>(sk + lrow, kb, kd), vf = rowfrag<DP>(sv + lrow, kb, kd);
 #pragma unroll
         for (int q = 0; q < QB; ++q) {
-          const int d0 = k0 + 32 * kb + 4 * hi - R.pos[q];
-          f32x16 w;                                                     // derivative of the cap
-          if (MOD) {
-            if (mod.cap) {
+          s[q] = El<T>::mfma(kf, qf[q][kd], s[q]);
+          dp[q] = El<T>::mfma(vf, gf[q][kd], dp[q]);
+        }
+      }
+      bf16x8 db[QB][2];
 #pragma unroll
-              for (int r = 0; r < 16; ++r) {
-                float y;
-                s[q][r] = capped(mod, s[q][r], y);
-                w[r] = 4.f * y * (1.f - y);
-              }
-            } else {
-#pragma unroll
-              for (int r = 0; r < 16; ++r) s[q][r] *= mod.c;
-            }
-            if (mod.slope) {
-              const float f0 = (float)d0;
-#pragma unroll
-              for (int r = 0; r < 16; ++r) s[q][r] = fmaf(-R.slope[q], fabsf(f0 + crow(r, 0)), s[q][r]);
-            }
-            if (mod.table) {
-#pragma unroll
-              for (int r = 0; r < 16; ++r) s[q][r] += tab[max(-mod.R, min(mod.R, d0 + crow(r, 0))) + mod.R];
-            }
-          }
+      for (int q = 0; q < QB; ++q) {
+        const int d0 = k0 + 32 * kb + 4 * hi - R.pos[q];
+        f32x16 w;                                                       // derivative of the cap
+        if (MOD & 1) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
-            const float pv = __builtin_amdgcn_exp2f(MOD ? s[q][r] - lse[q] : fmaf(s[q][r], mod.c, -lse[q]));
-            s[q][r] = pv * (dp[q][r] - dl[q]);
+            float y;
+            s[q][r] = capped(mod, s[q][r], y);
+            w[r] = 4.f * y * (1.f - y);
           }
-          if (partial) {
-            const int lim = R.bound[q] - k0 - 32 * kb - 4 * hi;
+        } else if (MOD & 2) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[q][r] = crow(r, 0) < lim ? s[q][r] : 0.f;
-            if (docs) {
+          for (int r = 0; r < 16; ++r) s[q][r] *= mod.c;
+        }
+        if (MOD & 2) {
+          if (mod.slope) {
+            const float f0 = (float)d0;
 #pragma unroll
-              for (int g = 0; g < 4; ++g) {
-                const int4 dv = *(const int4*)(sdoc + cur * TILE + 32 * kb + 8 * g + 4 * hi);
-                s[q][4 * g] = dv.x == R.doc[q] ? s[q][4 * g] : 0.f;
-                s[q][4 * g + 1] = dv.y == R.doc[q] ? s[q][4 * g + 1] : 0.f;
-                s[q][4 * g + 2] = dv.z == R.doc[q] ? s[q][4 * g + 2] : 0.f;
-                s[q][4 * g + 3] = dv.w == R.doc[q] ? s[q][4 * g + 3] : 0.f;
-              }
-            }
+            for (int r = 0; r < 16; ++r) s[q][r] = fmaf(-R.slope[q], fabsf(f0 + crow(r, 0)), s[q][r]);
           }
-          if (dtab) {
-            // sums over diagonals, in the wave's own table, by LDS additions that complete in program order: a register's 32 lanes of one
-            // half hold 32 different distances, so one half at a time meets no address twice and the order of the additions is fixed
-            // (the wave barriers keep the compiler from joining the two halves); the clipped ends are summed per lane
+          if (mod.table) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              const int d = d0 + crow(r, 0);
-              const float v = s[q][r];
-              const bool in = d > -mod.R && d < mod.R;
-              below += d <= -mod.R ? v : 0.f;
-              above += (d >= mod.R && d > -mod.R) ? v : 0.f;
-#pragma unroll
-              for (int half = 0; half < 2; ++half) {
-                if (in && hi == half) __builtin_amdgcn_ds_atomic_fadd_f32((__attribute__((address_space(3))) float*)(sums + d + mod.R), v);
-                __builtin_amdgcn_wave_barrier();
-              }
-            }
+            for (int r = 0; r < 16; ++r) s[q][r] += tab[max(-mod.R, min(mod.R, d0 + crow(r, 0))) + mod.R];
           }
-          if (MOD && mod.cap) {
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[q][r] *= w[r];
-          }
-          db[q][0] = pack8<T>(s[q], 0);
-          db[q][1] = pack8<T>(s[q], 1);
         }
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk)
+        for (int r = 0; r < 16; ++r) {
+          const float pv = __builtin_amdgcn_exp2f(MOD ? s[q][r] - lse[q] : fmaf(s[q][r], mod.c, -lse[q]));
+          s[q][r] = pv * (dp[q][r] - dl[q]);
+        }
+        if (partial) {
+          const int lim = R.bound[q] - k0 - 32 * kb - 4 * hi;
 #pragma unroll
-          for (int f = 0; f < FM; ++f) {
-            const bf16x8 kt = trfrag<DP>(sk, kb, f, kk, lane);
+          for (int r = 0; r < 16; ++r) s[q][r] = crow(r, 0) < lim ? s[q][r] : 0.f;
+          if (docs) {
 #pragma unroll
-            for (int q = 0; q < QB; ++q) acc[q][f] = El<T>::mfma(kt, db[q][kk], acc[q][f]);
+            for (int g = 0; g < 4; ++g) {
+              const int4 dv = *(const int4*)(sdoc + cur * TILE + 32 * kb + 8 * g + 4 * hi);
+              s[q][4 * g] = dv.x == R.doc[q] ? s[q][4 * g] : 0.f;
+              s[q][4 * g + 1] = dv.y == R.doc[q] ? s[q][4 * g + 1] : 0.f;
+              s[q][4 * g + 2] = dv.z == R.doc[q] ? s[q][4 * g + 2] : 0.f;
+              s[q][4 * g + 3] = dv.w == R.doc[q] ? s[q][4 * g + 3] : 0.f;
+            }
           }
+        }
+        if ((MOD & 2) && dtab) {
+          // sums over diagonals, in the wave's own table, by LDS additions that complete in program order: a register's 32 lanes of one
+          // half hold 32 different distances, so one half at a time meets no address twice and the order of the additions is fixed
+          // (the wave barriers keep the compiler from joining the two halves); the clipped ends are summed per lane
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int d = d0 + crow(r, 0);
+            const float v = s[q][r];
+            const bool in = d > -mod.R && d < mod.R;
+            below += d <= -mod.R ? v : 0.f;
+            above += (d >= mod.R && d > -mod.R) ? v : 0.f;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              if (in && hi == half) __builtin_amdgcn_ds_atomic_fadd_f32((__attribute__((address_space(3))) float*)(sums + d + mod.R), v);
+              __builtin_amdgcn_wave_barrier();
+            }
+          }
+        }
+        if (MOD & 1) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[q][r] *= w[r];
+        }
+        db[q][0] = pack8<T>(s[q], 0);
+        db[q][1] = pack8<T>(s[q], 1);
       }
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+        for (int f = 0; f < FM; ++f) {
+          const bf16x8 kT = trfrag<DP>(sk + ltr, kb, f, kk);
+#pragma unroll
+          for (int q = 0; q < QB; ++q) acc[q][f] = El<T>::mfma(kT, db[q][kk], acc[q][f]);
+        }
     }
-    if (tn < tend) store(cur ^ 1);
-    __syncthreads();
+  };
+  while (t < tend) {
+    const int tn = tile_next(it, active);
+    const KMeta kt = kn;
+    if (tn < tend) {
+      fetch(tn, cur ^ 1);
+      if (docs) kn = km[tn];
+    }
+    const int k0 = t * TILE;
+    if (k0 < R.bmax) {
+      bool partial = k0 + TILE > R.bmin;
+      if (docs) partial |= (kt.neg != 0) | (kt.dmin != kt.dmax) | (R.dmin != R.dmax) | R.neg | (kt.dmin != R.dmin);
+      math(partial, t);
+    }
+    if (tn < tend) landed(cur ^ 1, docs ? kn.neg : 0);
     cur ^= 1;
     t = tn;
   }
@@ -868,11 +943,10 @@ struct RowInfo {                    // of one staged query row
   float lse, delta, slope;
   int bound, pos, doc;
 };
-template <typename T, int DP, int KB, bool MOD>
+template <typename T, int DP, int KB, int MOD>
 __global__ __launch_bounds__(256, (DP == 64 && KB == 1) ? 2 : 1) void attn_mod_dkdv_kernel(const Args a) {
   warm_kernargs<(int)sizeof(Args)>();
   constexpr int NT = 256, KD = DP / 16, FM = DP / 32;
-  typedef Pair<DP, NT> P;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   Stage<DP>* st = (Stage<DP>*)smem;
   float* sinfo = (float*)(smem + 2 * sizeof(Stage<DP>));                // [2][6][TILE]: lse, delta, slope, bound, pos, doc
@@ -882,7 +956,8 @@ __global__ __launch_bounds__(256, (DP == 64 && KB == 1) ? 2 : 1) void attn_mod_d
   const int y = blockIdx.x % NKV, rest = blockIdx.x / NKV;
   const int sp = rest % a.splits, ktile = rest / a.splits;              // early keys are seen by the most rows of a causal mask: first
   const int b = y / a.p.kv_heads, kv = y - b * a.p.kv_heads;
-  const int len = seq_len(a, b), D = a.p.D, Sk = a.p.Sk, G = a.p.heads / a.p.kv_heads, GU = G / a.gp;
+  const Seq seq = load_seq(a, b);
+  const int len = seq.len, D = a.p.D, Sk = a.p.Sk, G = a.p.heads / a.p.kv_heads, GU = G / a.gp;
   const bool docs = a.kmeta && a.p.kv_docs;
   const Mod mod = make_mod(a);
   const bf16_t* Q = (const bf16_t*)a.p.q.ptr + op_base(a.p.q, b);
@@ -936,187 +1011,185 @@ __global__ __launch_bounds__(256, (DP == 64 && KB == 1) ? 2 : 1) void attn_mod_d
   const int ntr = (a.M + TILE - 1) / TILE, total = ntr * GU, per = (total + a.splits - 1) / a.splits;
   const int tbeg = min(total, sp * per), tend = wk0 < len ? min(total, tbeg + per) : tbeg;
   const QMeta* qm = a.qmeta ? a.qmeta + (long long)b * ntr : nullptr;
-  // largest / smallest bound of row tile t
-  auto tile_bounds = [&](int t, int& lo, int& hi_) {
-    if (qm) {
-      lo = qm[t].bmin;
-      hi_ = qm[t].bmax;
-    } else {      // bounds grow with the query
-      lo = t * TILE + TILE > a.M ? 0 : row_bound(a, b, div_gp(a, t * TILE), len);
-      hi_ = row_bound(a, b, div_gp(a, min(a.M, t * TILE + TILE) - 1), len);
-    }
+  // Row tile t: bounds and documents of its rows.  Without the meta table bounds grow with the query, and the rows that see key wk0 or a
+  // later one are the last of a unit: tiles [first, ntr).
+  auto tile_meta = [&](int t) {
+    if (qm) return qm[t];
+    return QMeta{t * TILE + TILE > a.M ? 0 : row_bound(seq, div_gp(a, t * TILE)), row_bound(seq, div_gp(a, min(a.M, t * TILE + TILE) - 1)), 0, 0, 0};
   };
+  const int first = qm || !seq.causal || seq.prefix > wk0 ? 0 : max(0, wk0 - seq.off) * a.gp / TILE;
   auto active = [&](int c) {
     const int t = c % ntr;
-    int lo, hi_;
-    tile_bounds(t, lo, hi_);
-    bool ok = hi_ > wk0;
-    if (docs) ok = ok && qm[t].dmax >= gdmin && qm[t].dmin <= gdmax;
-    return ok;
+    if (!qm) return t >= first;
+    const QMeta m = qm[t];
+    return m.bmax > wk0 && (!docs || (m.dmax >= gdmin && m.dmin <= gdmax));
   };
-  auto next = [&](int c) { return (a.p.causal || docs) ? next_tile(c, tend, active) : min(c, tend); };
-  P nx;
+  TileIter it = {0ull, tbeg, tend, qm || first > 0};
+  const Lane<DP> ln(wave, lane, D);
+  const int lrow = lane_row<DP>(lane), ltr = lane_tr<DP>(lane);
+  const bf16_t* qp = ln.ok ? Q + ln.ch * 8 : (const bf16_t*)zero_chunk;
+  const bf16_t* gp = ln.ok ? dO + ln.ch * 8 : (const bf16_t*)zero_chunk;
+  const unsigned qs = ln.ok ? (unsigned)a.p.q.sstride : 0u, gs = ln.ok ? (unsigned)a.p.d_o.sstride : 0u, hs = ln.ok ? (unsigned)D : 0u;
   RowInfo ni;
-  int nb[P::N];
-  auto fetch = [&](int c) {
-    const int gu = c / ntr, t = c - gu * ntr, h0 = kv * G + gu * a.gp, ch = tid % P::CH;
-    auto info = [&](int r, int& i, int& h, int& doc) {
-      const int rc = min(r, a.M - 1);
-      i = div_gp(a, rc);
-      h = h0 + rc - i * a.gp;
-      doc = docs ? a.p.q_docs[(long long)b * a.p.Sq + i] : 0;
-      return (r < a.M && doc >= 0) ? row_bound(a, b, i, len) : 0;
-    };
+  auto fetch = [&](int c, int sidx) {                                   // rows behind the last repeat it (their weights are masked to 0)
+    const int gu = c / ntr, t = c - gu * ntr, h0 = kv * G + gu * a.gp;
 #pragma unroll
-    for (int n = 0; n < P::N; ++n) {
-      int i, h, doc;
-      nb[n] = info(t * TILE + tid / P::CH + n * P::RPP, i, h, doc);
-      const bool ok = ch * 8 < D;
-      nx.a[n] = *chunk_ptr(Q + (long long)i * a.p.q.sstride + (long long)h * D + ch * 8, ok);
-      nx.b[n] = *chunk_ptr(dO + (long long)i * a.p.d_o.sstride + (long long)h * D + ch * 8, ok);
+    for (int n = 0; n < Lane<DP>::NI; ++n) {
+      const int rc = min(t * TILE + ln.row_of(n), a.M - 1), i = div_gp(a, rc);
+      const unsigned h = (unsigned)(h0 + rc - i * a.gp) * hs;
+      copy16(qp + (unsigned long long)(unsigned)i * qs + h, st[sidx].a + ln.group(n));
+      copy16(gp + (unsigned long long)(unsigned)i * gs + h, st[sidx].b + ln.group(n));
     }
     if (tid < TILE) {
-      int i, h;
-      const int r = t * TILE + tid;
-      ni.bound = info(r, i, h, ni.doc);
-      ni.pos = i + len - a.p.Sq;
-      ni.slope = a.p.slopes ? a.p.slopes[h] * LOG2E : 0.f;
-      const long long sidx = ((long long)b * a.p.heads + h0) * a.p.Sq + min(r, a.M - 1);
-      ni.lse = ni.bound > 0 ? a.p.lse[sidx] : INFINITY;
-      ni.delta = ni.bound > 0 ? a.p.delta[sidx] : 0.f;
+      const int r = t * TILE + tid, rc = min(r, a.M - 1), i = div_gp(a, rc);
+      ni.doc = docs ? a.p.q_docs[(long long)b * a.p.Sq + i] : 0;
+      ni.bound = (r < a.M && ni.doc >= 0) ? row_bound(seq, i) : 0;
+      ni.pos = i + seq.off;
+      ni.slope = (MOD & 2) && a.p.slopes ? a.p.slopes[h0 + rc - i * a.gp] * LOG2E : 0.f;
+      const long long sidx = ((long long)b * a.p.heads + h0) * a.p.Sq + rc;
+      const float l = a.p.lse[sidx], d = a.p.delta[sidx];
+      ni.lse = ni.bound > 0 ? l : INFINITY;
+      ni.delta = ni.bound > 0 ? d : 0.f;
     }
   };
-  auto store = [&](int sidx) {
-#pragma unroll
-    for (int n = 0; n < P::N; ++n) {
-      const bf16x8 z = {0, 0, 0, 0, 0, 0, 0, 0};
-      nx.a[n] = nb[n] > 0 ? nx.a[n] : z;
-      nx.b[n] = nb[n] > 0 ? nx.b[n] : z;
-    }
-    pair_store(st[sidx], nx, tid);
+  auto landed = [&](int sidx, bool dead) {
+    float* in = sinfo + sidx * 6 * TILE;
     if (tid < TILE) {
-      float* s = sinfo + sidx * 6 * TILE + tid;
-      s[0] = ni.lse;
-      s[TILE] = ni.delta;
-      s[2 * TILE] = ni.slope;
-      s[3 * TILE] = __int_as_float(ni.bound);
-      s[4 * TILE] = __int_as_float(ni.pos);
-      s[5 * TILE] = __int_as_float(ni.doc);
+      in[tid] = ni.lse;
+      in[TILE + tid] = ni.delta;
+      in[2 * TILE + tid] = ni.slope;
+      in[3 * TILE + tid] = __int_as_float(ni.bound);
+      in[4 * TILE + tid] = __int_as_float(ni.pos);
+      in[5 * TILE + tid] = __int_as_float(ni.doc);
     }
-  };
-  int c = next(tbeg), cur = 0, gu_tab = -1;
-  if (c < tend) {
-    fetch(c);
-    store(0);
-  }
-  __syncthreads();
-  while (c < tend) {
-    const int cn = next(c + 1);
-    if (cn < tend) fetch(cn);
-    const int gu = c / ntr, t = c - gu * ntr;
-    if (MOD && mod.table && gu != gu_tab) {                             // workgroup-uniform: the next head's table
-      if (gu_tab >= 0) __syncthreads();
-      load_table<T>(a, kv * G + gu, tab, tid, NT);
-      gu_tab = gu;
+    copies_done();
+    __syncthreads();
+    if (dead) {
+      clear_rows(st[sidx], tid, [&](int r) { return __float_as_int(in[3 * TILE + r]) <= 0; });
       __syncthreads();
     }
-    int blo, bhi;
-    tile_bounds(t, blo, bhi);
-    if (kw0 < bhi) {
-      const bf16_t* sq = st[cur].a;
-      const bf16_t* sg = st[cur].b;
-      const float* in = sinfo + cur * 6 * TILE;
-      bool partial = kw0 + 32 * KB > blo;
-      if (docs) partial |= wneg | (wdmin != wdmax) | (qm[t].dmin != qm[t].dmax) | (qm[t].neg != 0) | (qm[t].dmin != wdmin);
+  };
+  int c = tile_next(it, active), cur = 0, gu_tab = -1;
+  QMeta mn = {0, 0, 0, 0, 0};
+  if (c < tend) {
+    mn = tile_meta(c % ntr);
+    fetch(c, 0);
+    landed(0, mn.bmin <= 0);
+  }
+  auto math = [&](bool partial) {
+    const bf16_t* sq = st[cur].a;
+    const bf16_t* sg = st[cur].b;
+    const float* in = sinfo + cur * 6 * TILE;
 #pragma unroll
-      for (int qb = 0; qb < 2; ++qb) {
-        f32x16 s[KB], dp[KB];
+    for (int qb = 0; qb < 2; ++qb) {
+      f32x16 s[KB], dp[KB];
 #pragma unroll
-        for (int j = 0; j < KB; ++j)
+      for (int j = 0; j < KB; ++j)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s[j][r] = dp[j][r] = 0.f;
+        for (int r = 0; r < 16; ++r) s[j][r] = dp[j][r] = 0.f;
 #pragma unroll
-        for (int kd = 0; kd < KD; ++kd) {
-          const bf16x8 qa = rowfrag<DP>(sq, qb, kd, lane), da = rowfrag<DP>(sg, qb, kd, lane);
-#pragma unroll
-          for (int j = 0; j < KB; ++j) {
-            s[j] = El<T>::mfma(qa, kf[j][kd], s[j]);
-            dp[j] = El<T>::mfma(da, vf[j][kd], dp[j]);
-          }
-        }
-        bf16x8 pb[KB][2], db[KB][2];
+      for (int kd = 0; kd < KD; ++kd) {
+        const bf16x8 qa = rowfrag<DP>(sq + lrow, qb, kd), da = rowfrag<DP>(sg + lrow, qb, kd);
 #pragma unroll
         for (int j = 0; j < KB; ++j) {
-          f32x16 pr;
-#pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const int o = 32 * qb + 8 * g + 4 * hi;
-            const f32x4 L = *(const f32x4*)(in + o), E = *(const f32x4*)(in + TILE + o);
-            f32x4 W = {1.f, 1.f, 1.f, 1.f};
-            if (MOD) {
-              if (mod.cap) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  float w;
-                  s[j][4 * g + e] = capped(mod, s[j][4 * g + e], w);
-                  W[e] = 4.f * w * (1.f - w);
-                }
-              } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) s[j][4 * g + e] *= mod.c;
-              }
-              if (mod.slope | mod.table) {
-                const int4 pos = *(const int4*)(in + 4 * TILE + o);
-                const int ps[4] = {pos.x, pos.y, pos.z, pos.w};
-                if (mod.slope) {
-                  const f32x4 sl = *(const f32x4*)(in + 2 * TILE + o);
-#pragma unroll
-                  for (int e = 0; e < 4; ++e) s[j][4 * g + e] = fmaf(-sl[e], fabsf((float)(key[j] - ps[e])), s[j][4 * g + e]);
-                }
-                if (mod.table) {
-#pragma unroll
-                  for (int e = 0; e < 4; ++e) s[j][4 * g + e] += tab[max(-mod.R, min(mod.R, key[j] - ps[e])) + mod.R];
-                }
-              }
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              pr[4 * g + e] = __builtin_amdgcn_exp2f(MOD ? s[j][4 * g + e] - L[e] : fmaf(s[j][4 * g + e], mod.c, -L[e]));
-            if (partial) {
-              const int4 bd = *(const int4*)(in + 3 * TILE + o);
-              const int bs[4] = {bd.x, bd.y, bd.z, bd.w};
-#pragma unroll
-              for (int e = 0; e < 4; ++e) pr[4 * g + e] = key[j] < bs[e] ? pr[4 * g + e] : 0.f;
-              if (docs) {
-                const int4 dc = *(const int4*)(in + 5 * TILE + o);
-                const int ds[4] = {dc.x, dc.y, dc.z, dc.w};
-#pragma unroll
-                for (int e = 0; e < 4; ++e) pr[4 * g + e] = kd_[j] == ds[e] ? pr[4 * g + e] : 0.f;
-              }
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[j][4 * g + e] = pr[4 * g + e] * (dp[j][4 * g + e] - E[e]) * W[e];
-          }
-          pb[j][0] = pack8<T>(pr, 0);
-          pb[j][1] = pack8<T>(pr, 1);
-          db[j][0] = pack8<T>(s[j], 0);
-          db[j][1] = pack8<T>(s[j], 1);
+          s[j] = El<T>::mfma(qa, kf[j][kd], s[j]);
+          dp[j] = El<T>::mfma(da, vf[j][kd], dp[j]);
         }
+      }
+      bf16x8 pb[KB][2], db[KB][2];
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk)
+      for (int j = 0; j < KB; ++j) {
+        f32x16 pr;
 #pragma unroll
-          for (int f = 0; f < FM; ++f) {
-            const bf16x8 gt = trfrag<DP>(sg, qb, f, kk, lane), qt = trfrag<DP>(sq, qb, f, kk, lane);
+        for (int g = 0; g < 4; ++g) {
+          const int o = 32 * qb + 8 * g + 4 * hi;
+          const f32x4 L = *(const f32x4*)(in + o), E = *(const f32x4*)(in + TILE + o);
+          f32x4 W = {1.f, 1.f, 1.f, 1.f};
+          if (MOD & 1) {
 #pragma unroll
-            for (int j = 0; j < KB; ++j) {
-              va[j][f] = El<T>::mfma(gt, pb[j][kk], va[j][f]);
-              ka[j][f] = El<T>::mfma(qt, db[j][kk], ka[j][f]);
+            for (int e = 0; e < 4; ++e) {
+              float w;
+              s[j][4 * g + e] = capped(mod, s[j][4 * g + e], w);
+              W[e] = 4.f * w * (1.f - w);
+            }
+          } else if (MOD & 2) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[j][4 * g + e] *= mod.c;
+          }
+          if (MOD & 2) {
+            const int4 pos = *(const int4*)(in + 4 * TILE + o);
+            const int ps[4] = {pos.x, pos.y, pos.z, pos.w};
+            if (mod.slope) {
+              const f32x4 sl = *(const f32x4*)(in + 2 * TILE + o);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) s[j][4 * g + e] = fmaf(-sl[e], fabsf((float)(key[j] - ps[e])), s[j][4 * g + e]);
+            }
+            if (mod.table) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) s[j][4 * g + e] += tab[max(-mod.R, min(mod.R, key[j] - ps[e])) + mod.R];
             }
           }
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            pr[4 * g + e] = __builtin_amdgcn_exp2f(MOD ? s[j][4 * g + e] - L[e] : fmaf(s[j][4 * g + e], mod.c, -L[e]));
+          if (partial) {
+            const int4 bd = *(const int4*)(in + 3 * TILE + o);
+            const int bs[4] = {bd.x, bd.y, bd.z, bd.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) pr[4 * g + e] = key[j] < bs[e] ? pr[4 * g + e] : 0.f;
+            if (docs) {
+              const int4 dc = *(const int4*)(in + 5 * TILE + o);
+              const int ds[4] = {dc.x, dc.y, dc.z, dc.w};
+#pragma unroll
+              for (int e = 0; e < 4; ++e) pr[4 * g + e] = kd_[j] == ds[e] ? pr[4 * g + e] : 0.f;
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float d = pr[4 * g + e] * (dp[j][4 * g + e] - E[e]);
+            s[j][4 * g + e] = (MOD & 1) ? d * W[e] : d;
+          }
+        }
+        pb[j][0] = pack8<T>(pr, 0);
+        pb[j][1] = pack8<T>(pr, 1);
+        db[j][0] = pack8<T>(s[j], 0);
+        db[j][1] = pack8<T>(s[j], 1);
+      }
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+        for (int f = 0; f < FM; ++f) {
+          const bf16x8 gt = trfrag<DP>(sg + ltr, qb, f, kk), qt = trfrag<DP>(sq + ltr, qb, f, kk);
+#pragma unroll
+          for (int j = 0; j < KB; ++j) {
+            va[j][f] = El<T>::mfma(gt, pb[j][kk], va[j][f]);
+            ka[j][f] = El<T>::mfma(qt, db[j][kk], ka[j][f]);
+          }
+        }
+    }
+  };
+  while (c < tend) {
+    const int cn = tile_next(it, active);
+    const QMeta mt = mn;
+    if (cn < tend) {
+      fetch(cn, cur ^ 1);
+      mn = tile_meta(cn % ntr);
+    }
+    if ((MOD & 2) && mod.table) {                                       // workgroup-uniform: the next head's table
+      const int gu = c / ntr;
+      if (gu != gu_tab) {
+        if (gu_tab >= 0) __syncthreads();
+        load_table<T>(a, kv * G + gu, tab, tid, NT);
+        gu_tab = gu;
+        __syncthreads();
       }
     }
-    if (cn < tend) store(cur ^ 1);
-    __syncthreads();
+    if (kw0 < mt.bmax) {
+      bool partial = kw0 + 32 * KB > mt.bmin;
+      if (docs) partial |= wneg | (wdmin != wdmax) | (mt.dmin != mt.dmax) | (mt.neg != 0) | (mt.dmin != wdmin);
+      math(partial);
+    }
+    if (cn < tend) landed(cur ^ 1, mn.bmin <= 0);
     cur ^= 1;
     c = cn;
   }
@@ -1216,8 +1289,9 @@ int check_mod(const char* fn, const T2VAttnMod* p, bool bwd) {
   const char* names[] = {"q", "k", "v", "o", "d_o", "dq", "dk", "dv"};
   for (int i = 0; i < (bwd ? 8 : 4); ++i) {
     const T2VAttnOperand& o = *ops[i];
-    T2V_CHECK_ARG(o.ptr && o.bdiv > 0 && ((uintptr_t)o.ptr & 15) == 0 && o.sstride % 8 == 0 && o.bstride_hi % 8 == 0 && o.bstride_lo % 8 == 0,
-                  "%s: operand %s: 16-byte aligned rows are wanted (ptr %p, row stride %lld)", fn, names[i], o.ptr, o.sstride);
+    T2V_CHECK_ARG(o.ptr && o.bdiv > 0 && ((uintptr_t)o.ptr & 15) == 0 && o.sstride % 8 == 0 && o.bstride_hi % 8 == 0 && o.bstride_lo % 8 == 0 &&
+                      o.sstride >= 0 && o.sstride < (1ll << 31),
+                  "%s: operand %s: 16-byte aligned rows, less than 2^31 elements apart, are wanted (ptr %p, row stride %lld)", fn, names[i], o.ptr, o.sstride);
   }
   T2V_CHECK_ARG(!bwd || (p->lse && p->delta), "%s: lse and delta are required", fn);
   T2V_CHECK_ARG(!bwd || p->kv_share >= 1, "%s: kv_share is the number of batches that share a K / V (1: none do)", fn);
@@ -1297,7 +1371,7 @@ Layout make_layout(const T2VAttnMod* p, bool bwd) {
 }
 
 size_t smem_bytes(const Layout& L, int tables, bool kv) {
-  return 2 * 2 * (size_t)TILE * L.dp * 2 + (kv ? 2 * 6 * TILE * 4 : 2 * TILE * 4 + 64) + (L.a.p.bias ? tables * 4 * (2 * (size_t)L.a.p.radius + 1) : 0);
+  return 2 * (L.dp == 64 ? sizeof(Stage<64>) : sizeof(Stage<128>)) + (kv ? 2 * 6 * TILE * 4 : 2 * TILE * 4 + 64) + (L.a.p.bias ? tables * 4 * (2 * (size_t)L.a.p.radius + 1) : 0);
 }
 template <typename K>
 int launch(int which, K kern, long long grid, size_t smem, hipStream_t st, const Args& a) {
@@ -1311,7 +1385,8 @@ int launch(int which, K kern, long long grid, size_t smem, hipStream_t st, const
   t2v_launch_timed(which, kern, dim3((unsigned)grid), dim3(256), (unsigned)smem, st, a);
   return T2V_OK;
 }
-bool modded(const T2VAttnMod* p) { return p->softcap > 0.f || p->slopes || p->bias || !(p->scale > 0.f); }
+// bit 0 cap, bit 1 distance bias; a scale that is not positive takes the form that does not fold it into the running maximum
+int mod_bits(const T2VAttnMod* p) { return (p->softcap > 0.f ? 1 : 0) | (p->slopes || p->bias || !(p->scale > 0.f) ? 2 : 0); }
 
 template <typename T, int DP>
 int run_fwd(Layout& L, hipStream_t st) {
@@ -1321,8 +1396,9 @@ int run_fwd(Layout& L, hipStream_t st) {
   const long long grid = (long long)a.p.nbatch * a.nunit * L.fwd_tiles * L.fwd_splits;
   const size_t sm = smem_bytes(L, 1, false);
   const int which = L.fwd_splits > 1 ? 1 : 3;
-  const int e = modded(&a.p) ? launch(which, attn_mod_fwd_kernel<T, DP, 1, true>, grid, sm, st, a)
-                             : launch(which, attn_mod_fwd_kernel<T, DP, 1, false>, grid, sm, st, a);
+  const int mb = mod_bits(&a.p);
+  const int e = mb == 0 ? launch(which, attn_mod_fwd_kernel<T, DP, 1, 0>, grid, sm, st, a) : mb == 1 ? launch(which, attn_mod_fwd_kernel<T, DP, 1, 1>, grid, sm, st, a) :
+                mb == 2 ? launch(which, attn_mod_fwd_kernel<T, DP, 1, 2>, grid, sm, st, a) : launch(which, attn_mod_fwd_kernel<T, DP, 1, 3>, grid, sm, st, a);
   if (e) return e;
   T2V_CHECK_LAUNCH();
   if (L.fwd_splits > 1) {
@@ -1336,12 +1412,13 @@ int run_fwd(Layout& L, hipStream_t st) {
 template <typename T, int DP>
 int run_bwd(Layout& L, hipStream_t st) {
   Args& a = L.a;
-  const bool mod = modded(&a.p);
+  const int mb = mod_bits(&a.p);
   a.ntile = L.dq_tiles;
   a.splits = 1;
   const size_t sm = smem_bytes(L, a.p.dbias ? 5 : 1, false);
   const long long gq = (long long)a.p.nbatch * a.nunit * L.dq_tiles;
-  int e = mod ? launch(1, attn_mod_dq_kernel<T, DP, 1, true>, gq, sm, st, a) : launch(1, attn_mod_dq_kernel<T, DP, 1, false>, gq, sm, st, a);
+  int e = mb == 0 ? launch(1, attn_mod_dq_kernel<T, DP, 1, 0>, gq, sm, st, a) : mb == 1 ? launch(1, attn_mod_dq_kernel<T, DP, 1, 1>, gq, sm, st, a) :
+          mb == 2 ? launch(1, attn_mod_dq_kernel<T, DP, 1, 2>, gq, sm, st, a) : launch(1, attn_mod_dq_kernel<T, DP, 1, 3>, gq, sm, st, a);
   if (e) return e;
   T2V_CHECK_LAUNCH();
   if (a.p.dbias) {
@@ -1355,7 +1432,8 @@ int run_bwd(Layout& L, hipStream_t st) {
   const size_t smk = smem_bytes(L, 1, true);
   a.to_part = L.kv_splits > 1 || a.p.kv_share > 1;
   const int which = a.to_part ? 0 : 2;
-  e = mod ? launch(which, attn_mod_dkdv_kernel<T, DP, 1, true>, gk, smk, st, a) : launch(which, attn_mod_dkdv_kernel<T, DP, 1, false>, gk, smk, st, a);
+  e = mb == 0 ? launch(which, attn_mod_dkdv_kernel<T, DP, 1, 0>, gk, smk, st, a) : mb == 1 ? launch(which, attn_mod_dkdv_kernel<T, DP, 1, 1>, gk, smk, st, a) :
+      mb == 2 ? launch(which, attn_mod_dkdv_kernel<T, DP, 1, 2>, gk, smk, st, a) : launch(which, attn_mod_dkdv_kernel<T, DP, 1, 3>, gk, smk, st, a);
   if (e) return e;
   T2V_CHECK_LAUNCH();
   if (a.to_part) {
