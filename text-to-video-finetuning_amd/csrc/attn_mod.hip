@@ -15,6 +15,7 @@
 // are read once for all of them; with a table each head is a unit of its own (gp = 1: the table of one head lives in LDS).
 // Statistics, the running maximum and sum, lse, delta and all accumulators are fp32; P and dS are rounded to the input type for the
 // matrix cores (one rounding of a factor in [0, 1], and of a gradient, the same size as the output's own rounding).
+#include <stdlib.h>
 #include <type_traits>
 
 #include "common.h"
@@ -68,12 +69,21 @@ struct QMeta {      // of 64 rows: smallest and largest bound, smallest and larg
 struct KMeta {
   int dmin, dmax, neg;
 };
+// (what the compiler cannot see to be the same in all lanes it keeps in vector registers and branches on with exec masks)
+__device__ __forceinline__ QMeta uniform(const QMeta& m) {
+  return QMeta{__builtin_amdgcn_readfirstlane(m.bmin), __builtin_amdgcn_readfirstlane(m.bmax), __builtin_amdgcn_readfirstlane(m.dmin),
+               __builtin_amdgcn_readfirstlane(m.dmax), __builtin_amdgcn_readfirstlane(m.neg)};
+}
+__device__ __forceinline__ KMeta uniform(const KMeta& m) {
+  return KMeta{__builtin_amdgcn_readfirstlane(m.dmin), __builtin_amdgcn_readfirstlane(m.dmax), __builtin_amdgcn_readfirstlane(m.neg)};
+}
 
 struct Args {
   T2VAttnMod p;
   int gp, nunit, M;                 // heads per unit, units per batch, rows per unit (Sq * gp)
   unsigned magic;                   // r / gp = r * magic >> 32 (gp > 1)
   int ntile, splits;                // row (or key) tiles of a unit, splits of the other axis
+  int chunk;                        // row tiles a split of dK / dV takes
   int to_part;                      // dK / dV go to `part` as fp32 (several splits, or several batches that share K / V)
   const QMeta* qmeta;               // [nbatch][ceil(M / 64)] or NULL
   const KMeta* kmeta;               // [nbatch][ceil(Sk / 64)] or NULL
@@ -109,6 +119,11 @@ __device__ __forceinline__ int row_bound(const Seq& s, int i) {
   return max(0, min(max(i + s.off + 1, pf), s.len));
 }
 
+// the first of a unit's row tiles that may see key wk0 or a later one (0 where the meta table tells it tile by tile)
+__device__ __forceinline__ int first_tile(const Args& a, const Seq& s, int wk0) {
+  return a.qmeta || !s.causal || s.prefix > wk0 ? 0 : min((a.M + TILE - 1) / TILE, max(0, wk0 - s.off) * a.gp / TILE);
+}
+
 // workgroup id -> (batch, unit): workgroups go round-robin over the eight XCDs, so units that share a K/V head are placed a multiple of
 // nbatch * kv_heads apart, which is the same XCD (and L2) where that is a multiple of eight
 struct Unit {
@@ -140,10 +155,10 @@ __device__ __forceinline__ constexpr int row_off(int row) {
   return DP == 128 ? ((row >> 5) * 8 + (row & 7)) * GROUP + ((row >> 3) & 3) * 128 : (row & 7) * GROUP + (row >> 3) * 64;
 }
 
-// What a lane loads: instruction i of a wave fills group 4 i + wave.  Columns behind the head dim come from a chunk of zeros (row stride 0).
-template <int DP>
+// What a lane loads: instruction i of a wave fills group NW i + wave.  Columns behind the head dim come from a chunk of zeros (row stride 0).
+template <int DP, int NW>
 struct Lane {
-  static constexpr int NI = TILE * DP / 512 / 4;                        // instructions per wave
+  static constexpr int NI = TILE * DP / 512 / NW;                       // instructions per wave
   int wave, sub, ch;
   bool ok;
   __device__ __forceinline__ Lane(int w, int lane, int D) {
@@ -153,10 +168,10 @@ struct Lane {
     ok = ch * 8 < D;
   }
   __device__ __forceinline__ int row_of(int i) const {
-    const int g = 4 * i + wave;
+    const int g = NW * i + wave;
     return (DP == 128 ? 32 * (g >> 3) + (g & 7) : g) + sub;
   }
-  __device__ __forceinline__ int group(int i) const { return (4 * i + wave) * GROUP; }
+  __device__ __forceinline__ int group(int i) const { return (NW * i + wave) * GROUP; }
 };
 __device__ __forceinline__ void copy16(const void* src, void* lds) {
   __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src, (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
@@ -165,10 +180,10 @@ __device__ __forceinline__ void copy16(const void* src, void* lds) {
 // copies, at the first use of what was loaded in front of the loop)
 __device__ __forceinline__ void copies_done() { __builtin_amdgcn_s_waitcnt(0x0f70); }      // vmcnt(0)
 // zero the staged rows for which `dead(row)`: rows that nobody sees may hold inf / NaN, which must not meet a zero weight
-template <int DP, typename F>
+template <int DP, int NT, typename F>
 __device__ __forceinline__ void clear_rows(Stage<DP>& st, int tid, F dead) {
   const bf16x8 z = {0, 0, 0, 0, 0, 0, 0, 0};
-  for (int i = tid; i < TILE * DP / 8; i += 256) {
+  for (int i = tid; i < TILE * DP / 8; i += NT) {
     const int row = i / (DP / 8), o = row_off<DP>(row) + (i % (DP / 8)) * 8;
     if (dead(row)) {
       *(bf16x8*)(st.a + o) = z;
@@ -370,7 +385,7 @@ __global__ __launch_bounds__(256, (DP * QB <= 128) ? 2 : 1) void attn_mod_fwd_ke
   const KMeta* km = docs ? a.kmeta + (long long)u.b * ((Sk + TILE - 1) / TILE) : nullptr;
   auto active = [&](int c) { return km[c].dmax >= dmin && km[c].dmin <= dmax; };
   TileIter it = {0ull, tbeg, tend, docs};
-  const Lane<DP> ln(wave, lane, D);
+  const Lane<DP, 4> ln(wave, lane, D);
   const int lrow = lane_row<DP>(lane), ltr = lane_tr<DP>(lane);
   const bf16_t* kp = ln.ok ? (const bf16_t*)a.p.k.ptr + op_base(a.p.k, u.b) + (long long)u.kv * D + ln.ch * 8 : (const bf16_t*)zero_chunk;
   const bf16_t* vp = ln.ok ? (const bf16_t*)a.p.v.ptr + op_base(a.p.v, u.b) + (long long)u.kv * D + ln.ch * 8 : (const bf16_t*)zero_chunk;
@@ -378,7 +393,7 @@ __global__ __launch_bounds__(256, (DP * QB <= 128) ? 2 : 1) void attn_mod_fwd_ke
   int nd = 0;
   auto fetch = [&](int t, int sidx) {                                   // rows behind the last key repeat it (masked by the bounds)
 #pragma unroll
-    for (int i = 0; i < Lane<DP>::NI; ++i) {
+    for (int i = 0; i < Lane<DP, 4>::NI; ++i) {
       const unsigned row = (unsigned)min(t * TILE + ln.row_of(i), len - 1);
       copy16(kp + (unsigned long long)row * ks, st[sidx].a + ln.group(i));
       copy16(vp + (unsigned long long)row * vs, st[sidx].b + ln.group(i));
@@ -393,7 +408,7 @@ __global__ __launch_bounds__(256, (DP * QB <= 128) ? 2 : 1) void attn_mod_fwd_ke
     copies_done();
     __syncthreads();
     if (neg) {
-      clear_rows(st[sidx], tid, [&](int r) { return sdoc[sidx * TILE + r] < 0; });
+      clear_rows<DP, NT>(st[sidx], tid, [&](int r) { return sdoc[sidx * TILE + r] < 0; });
       __syncthreads();
     }
   };
@@ -412,7 +427,7 @@ __global__ __launch_bounds__(256, (DP * QB <= 128) ? 2 : 1) void attn_mod_fwd_ke
   int t = tile_next(it, active), cur = 0;
   KMeta kn = {0, 0, 0};                                                 // of the tile at hand (documents)
   if (t < tend) {
-    if (docs) kn = km[t];
+    if (docs) kn = uniform(km[t]);
     fetch(t, 0);
     landed(0, kn.neg);
   }
@@ -556,13 +571,13 @@ __global__ __launch_bounds__(256, (DP * QB <= 128) ? 2 : 1) void attn_mod_fwd_ke
     const KMeta kt = kn;
     if (tn < tend) {
       fetch(tn, cur ^ 1);
-      if (docs) kn = km[tn];
+      if (docs) kn = uniform(km[tn]);
     }
     const int k0 = t * TILE;
     if (k0 < R.bmax) {
       bool partial = k0 + TILE > R.bmin;
       if (docs) partial |= (kt.neg != 0) | (kt.dmin != kt.dmax) | (R.dmin != R.dmax) | R.neg | (kt.dmin != R.dmin);
-      math(partial, t);
+      math(__builtin_amdgcn_readfirstlane(partial), t);
     }
     if (tn < tend) landed(cur ^ 1, docs ? kn.neg : 0);
     cur ^= 1;
@@ -734,7 +749,7 @@ __global__ __launch_bounds__(256, (DP * QB <= 128) ? 2 : 1) void attn_mod_dq_ker
   const KMeta* km = docs ? a.kmeta + (long long)u.b * ((Sk + TILE - 1) / TILE) : nullptr;
   auto active = [&](int c) { return km[c].dmax >= dmin && km[c].dmin <= dmax; };
   TileIter it = {0ull, 0, tend, docs};
-  const Lane<DP> ln(wave, lane, D);
+  const Lane<DP, 4> ln(wave, lane, D);
   const int lrow = lane_row<DP>(lane), ltr = lane_tr<DP>(lane);
   const bf16_t* kp = ln.ok ? (const bf16_t*)a.p.k.ptr + op_base(a.p.k, u.b) + (long long)u.kv * D + ln.ch * 8 : (const bf16_t*)zero_chunk;
   const bf16_t* vp = ln.ok ? (const bf16_t*)a.p.v.ptr + op_base(a.p.v, u.b) + (long long)u.kv * D + ln.ch * 8 : (const bf16_t*)zero_chunk;
@@ -742,7 +757,7 @@ __global__ __launch_bounds__(256, (DP * QB <= 128) ? 2 : 1) void attn_mod_dq_ker
   int nd = 0;
   auto fetch = [&](int t, int sidx) {                                   // rows behind the last key repeat it (masked by the bounds)
 #pragma unroll
-    for (int i = 0; i < Lane<DP>::NI; ++i) {
+    for (int i = 0; i < Lane<DP, 4>::NI; ++i) {
       const unsigned row = (unsigned)min(t * TILE + ln.row_of(i), len - 1);
       copy16(kp + (unsigned long long)row * ks, st[sidx].a + ln.group(i));
       copy16(vp + (unsigned long long)row * vs, st[sidx].b + ln.group(i));
@@ -757,7 +772,7 @@ __global__ __launch_bounds__(256, (DP * QB <= 128) ? 2 : 1) void attn_mod_dq_ker
     copies_done();
     __syncthreads();
     if (neg) {
-      clear_rows(st[sidx], tid, [&](int r) { return sdoc[sidx * TILE + r] < 0; });
+      clear_rows<DP, NT>(st[sidx], tid, [&](int r) { return sdoc[sidx * TILE + r] < 0; });
       __syncthreads();
     }
   };
@@ -772,7 +787,7 @@ __global__ __launch_bounds__(256, (DP * QB <= 128) ? 2 : 1) void attn_mod_dq_ker
   int t = tile_next(it, active), cur = 0;
   KMeta kn = {0, 0, 0};                                                 // of the tile at hand (documents)
   if (t < tend) {
-    if (docs) kn = km[t];
+    if (docs) kn = uniform(km[t]);
     fetch(t, 0);
     landed(0, kn.neg);
   }
@@ -883,13 +898,13 @@ __global__ __launch_bounds__(256, (DP * QB <= 128) ? 2 : 1) void attn_mod_dq_ker
     const KMeta kt = kn;
     if (tn < tend) {
       fetch(tn, cur ^ 1);
-      if (docs) kn = km[tn];
+      if (docs) kn = uniform(km[tn]);
     }
     const int k0 = t * TILE;
     if (k0 < R.bmax) {
       bool partial = k0 + TILE > R.bmin;
       if (docs) partial |= (kt.neg != 0) | (kt.dmin != kt.dmax) | (R.dmin != R.dmax) | R.neg | (kt.dmin != R.dmin);
-      math(partial, t);
+      math(__builtin_amdgcn_readfirstlane(partial), t);
     }
     if (tn < tend) landed(cur ^ 1, docs ? kn.neg : 0);
     cur ^= 1;
@@ -943,10 +958,16 @@ struct RowInfo {                    // of one staged query row
   float lse, delta, slope;
   int bound, pos, doc;
 };
-template <typename T, int DP, int KB, int MOD>
-__global__ __launch_bounds__(256, (DP == 64 && KB == 1) ? 2 : 1) void attn_mod_dkdv_kernel(const Args a) {
+// A wave owns 32 keys and streams the rows that see them.  K, V, dK and dV of 32 keys of 128 columns are 192 registers: with the score and
+// gradient tiles a wave would need more than half of a SIMD's file, and one wave per SIMD has nothing to run under its exponentials
+// (measured 301 us at 2 x 2011 rows, 16 / 4 heads; this form: see the table).  So at DP = 128 the workgroup is eight waves, its V rows
+// stay in LDS (read once per block: LDS then delivers 156 bytes per clock at full matrix rate, against its 128), and two waves share a SIMD.
+template <typename T, int DP, int MOD>
+__global__ __launch_bounds__(DP == 128 ? 512 : 256, 2) void attn_mod_dkdv_kernel(const Args a) {
   warm_kernargs<(int)sizeof(Args)>();
-  constexpr int NT = 256, KD = DP / 16, FM = DP / 32;
+  constexpr int NW = DP == 128 ? 8 : 4, NT = 64 * NW, KD = DP / 16, FM = DP / 32, KEYS = 32 * NW;
+  constexpr bool VLDS = DP == 128;
+  constexpr int HALF = TILE * DP / 512 * GROUP;                         // elements of 64 staged rows
   extern __shared__ __attribute__((aligned(16))) char smem[];
   Stage<DP>* st = (Stage<DP>*)smem;
   float* sinfo = (float*)(smem + 2 * sizeof(Stage<DP>));                // [2][6][TILE]: lse, delta, slope, bound, pos, doc
@@ -962,79 +983,77 @@ __global__ __launch_bounds__(256, (DP == 64 && KB == 1) ? 2 : 1) void attn_mod_d
   const Mod mod = make_mod(a);
   const bf16_t* Q = (const bf16_t*)a.p.q.ptr + op_base(a.p.q, b);
   const bf16_t* dO = (const bf16_t*)a.p.d_o.ptr + op_base(a.p.d_o, b);
-  const int kw0 = (ktile * 4 + wave) * 32 * KB;                         // the wave's first key
-  int key[KB], kd_[KB];
-  bf16x8 kf[KB][KD], vf[KB][KD];
-  int dlo = 0x7fffffff, dhi = -1, ng = 0;
+  bf16_t* sV = (bf16_t*)(tab + (a.p.bias ? (2 * a.p.radius + 1 + 3) / 4 * 4 : 0)) + (wave >> 1) * HALF;      // VLDS: the wave's 64-key tile
+  const int wk0 = ktile * KEYS, kw0 = wk0 + wave * 32;                  // the first key of the workgroup, of the wave
+  const int key = kw0 + (lane & 31);
+  // does the key exist, and may some query see it
+  auto key_doc = [&](int j) { return j < len ? (docs ? a.p.kv_docs[(long long)b * Sk + j] : 0) : -1; };
+  const int kd_ = key_doc(key);
+  const bool kok = kd_ >= 0;
+  const bf16_t* K = (const bf16_t*)a.p.k.ptr + op_base(a.p.k, b) + (long long)kv * D;
+  const bf16_t* V = (const bf16_t*)a.p.v.ptr + op_base(a.p.v, b) + (long long)kv * D;
+  bf16x8 kf[KD], vf[VLDS ? 1 : KD];
 #pragma unroll
-  for (int j = 0; j < KB; ++j) {
-    key[j] = kw0 + 32 * j + (lane & 31);
-    const int kc = min(key[j], Sk - 1);
-    kd_[j] = docs ? a.p.kv_docs[(long long)b * Sk + kc] : 0;
-    const bool ok = key[j] < len && kd_[j] >= 0;
-    if (ok) {
-      dlo = min(dlo, kd_[j]);
-      dhi = max(dhi, kd_[j]);
-    } else {
-      kd_[j] = -1;
-      ng = 1;
-    }
-    const bf16_t* kp = (const bf16_t*)a.p.k.ptr + op_base(a.p.k, b) + (long long)kc * a.p.k.sstride + (long long)kv * D;
-    const bf16_t* vp = (const bf16_t*)a.p.v.ptr + op_base(a.p.v, b) + (long long)kc * a.p.v.sstride + (long long)kv * D;
+  for (int kd = 0; kd < KD; ++kd) {
+    const bool ok = kok && 16 * kd + 8 * hi < D;
+    kf[kd] = *chunk_ptr(K + (long long)key * a.p.k.sstride + 16 * kd + 8 * hi, ok);
+    if constexpr (!VLDS) vf[kd] = *chunk_ptr(V + (long long)key * a.p.v.sstride + 16 * kd + 8 * hi, ok);
+  }
+  const int lrow = lane_row<DP>(lane), ltr = lane_tr<DP>(lane);
+  if constexpr (VLDS) {                                                 // each wave loads, and reads, its own 32 rows
 #pragma unroll
-    for (int kd = 0; kd < KD; ++kd) {
-      kf[j][kd] = *chunk_ptr(kp + 16 * kd + 8 * hi, ok && 16 * kd + 8 * hi < D);
-      vf[j][kd] = *chunk_ptr(vp + 16 * kd + 8 * hi, ok && 16 * kd + 8 * hi < D);
+    for (int g = 0; g < 8; ++g) {
+      const int j = kw0 + g + 8 * (lane >> 4), ch = lane & 15;
+      copy16(chunk_ptr(V + (long long)j * a.p.v.sstride + ch * 8, key_doc(j) >= 0 && ch * 8 < D), sV + ((wave & 1) * 8 + g) * GROUP);
     }
   }
+  auto vfrag = [&](int kd) {
+    if constexpr (VLDS) return rowfrag<DP>(sV + lrow + row_off<DP>(32 * (wave & 1)), 0, kd);
+    else return vf[kd];
+  };
+  int dlo = kok ? kd_ : 0x7fffffff, dhi = kd_, ng = !kok;
   const int wdmin = wave_min_i(dlo), wdmax = wave_max_i(dhi);
   const bool wneg = wave_max_i(ng) != 0;
-  // over the workgroup's 128 KB keys
-  const int wk0 = ktile * 4 * 32 * KB;
+  // over the workgroup's keys
   int gdmin = 0x7fffffff, gdmax = -1;
   if (docs) {
     const KMeta* km = a.kmeta + (long long)b * ((Sk + TILE - 1) / TILE);
-    for (int t = wk0 / TILE; t < min((Sk + TILE - 1) / TILE, (wk0 + 128 * KB) / TILE); ++t) {
+    for (int t = wk0 / TILE; t < min((Sk + TILE - 1) / TILE, (wk0 + KEYS) / TILE); ++t) {
       gdmin = min(gdmin, km[t].dmin);
       gdmax = max(gdmax, km[t].dmax);
     }
   }
-  f32x16 ka[KB][FM], va[KB][FM];
+  f32x16 ka[FM], va[FM];
 #pragma unroll
-  for (int j = 0; j < KB; ++j)
+  for (int f = 0; f < FM; ++f)
 #pragma unroll
-    for (int f = 0; f < FM; ++f)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) ka[j][f][r] = va[j][f][r] = 0.f;
+    for (int r = 0; r < 16; ++r) ka[f][r] = va[f][r] = 0.f;
 
-  // row tiles of all units of the K/V head, numbered through; a split takes a run of them
-  const int ntr = (a.M + TILE - 1) / TILE, total = ntr * GU, per = (total + a.splits - 1) / a.splits;
-  const int tbeg = min(total, sp * per), tend = wk0 < len ? min(total, tbeg + per) : tbeg;
+  // The row tiles that matter, of all units of the K / V head, are numbered through and a split takes `chunk` of them.  With the meta table
+  // those are all tiles, filtered on the way; without it bounds grow with the query, and only the last tiles of a unit see key wk0 or a later one.
+  const int ntr = (a.M + TILE - 1) / TILE;
   const QMeta* qm = a.qmeta ? a.qmeta + (long long)b * ntr : nullptr;
-  // Row tile t: bounds and documents of its rows.  Without the meta table bounds grow with the query, and the rows that see key wk0 or a
-  // later one are the last of a unit: tiles [first, ntr).
+  const int first = first_tile(a, seq, wk0), run = ntr - first, total = wk0 < len ? run * GU : 0;
+  const int tbeg = sp * a.chunk, tend = min(total, tbeg + a.chunk);
+  if (sp > 0 && tbeg >= total) return;                                  // workgroup-uniform; the join knows how many splits there are
   auto tile_meta = [&](int t) {
-    if (qm) return qm[t];
-    return QMeta{t * TILE + TILE > a.M ? 0 : row_bound(seq, div_gp(a, t * TILE)), row_bound(seq, div_gp(a, min(a.M, t * TILE + TILE) - 1)), 0, 0, 0};
+    if (qm) return uniform(qm[t]);
+    return uniform(QMeta{t * TILE + TILE > a.M ? 0 : row_bound(seq, div_gp(a, t * TILE)), row_bound(seq, div_gp(a, min(a.M, t * TILE + TILE) - 1)), 0, 0, 0});
   };
-  const int first = qm || !seq.causal || seq.prefix > wk0 ? 0 : max(0, wk0 - seq.off) * a.gp / TILE;
   auto active = [&](int c) {
-    const int t = c % ntr;
-    if (!qm) return t >= first;
-    const QMeta m = qm[t];
+    const QMeta m = qm[c % ntr];
     return m.bmax > wk0 && (!docs || (m.dmax >= gdmin && m.dmin <= gdmax));
   };
-  TileIter it = {0ull, tbeg, tend, qm || first > 0};
-  const Lane<DP> ln(wave, lane, D);
-  const int lrow = lane_row<DP>(lane), ltr = lane_tr<DP>(lane);
+  TileIter it = {0ull, tbeg, tend, qm != nullptr};
+  const Lane<DP, NW> ln(wave, lane, D);
   const bf16_t* qp = ln.ok ? Q + ln.ch * 8 : (const bf16_t*)zero_chunk;
   const bf16_t* gp = ln.ok ? dO + ln.ch * 8 : (const bf16_t*)zero_chunk;
   const unsigned qs = ln.ok ? (unsigned)a.p.q.sstride : 0u, gs = ln.ok ? (unsigned)a.p.d_o.sstride : 0u, hs = ln.ok ? (unsigned)D : 0u;
   RowInfo ni;
   auto fetch = [&](int c, int sidx) {                                   // rows behind the last repeat it (their weights are masked to 0)
-    const int gu = c / ntr, t = c - gu * ntr, h0 = kv * G + gu * a.gp;
+    const int gu = c / run, t = first + c - gu * run, h0 = kv * G + gu * a.gp;
 #pragma unroll
-    for (int n = 0; n < Lane<DP>::NI; ++n) {
+    for (int n = 0; n < Lane<DP, NW>::NI; ++n) {
       const int rc = min(t * TILE + ln.row_of(n), a.M - 1), i = div_gp(a, rc);
       const unsigned h = (unsigned)(h0 + rc - i * a.gp) * hs;
       copy16(qp + (unsigned long long)(unsigned)i * qs + h, st[sidx].a + ln.group(n));
@@ -1065,14 +1084,14 @@ __global__ __launch_bounds__(256, (DP == 64 && KB == 1) ? 2 : 1) void attn_mod_d
     copies_done();
     __syncthreads();
     if (dead) {
-      clear_rows(st[sidx], tid, [&](int r) { return __float_as_int(in[3 * TILE + r]) <= 0; });
+      clear_rows<DP, NT>(st[sidx], tid, [&](int r) { return __float_as_int(in[3 * TILE + r]) <= 0; });
       __syncthreads();
     }
   };
   int c = tile_next(it, active), cur = 0, gu_tab = -1;
   QMeta mn = {0, 0, 0, 0, 0};
   if (c < tend) {
-    mn = tile_meta(c % ntr);
+    mn = tile_meta(first + c % run);
     fetch(c, 0);
     landed(0, mn.bmin <= 0);
   }
@@ -1082,24 +1101,16 @@ __global__ __launch_bounds__(256, (DP == 64 && KB == 1) ? 2 : 1) void attn_mod_d
     const float* in = sinfo + cur * 6 * TILE;
 #pragma unroll
     for (int qb = 0; qb < 2; ++qb) {
-      f32x16 s[KB], dp[KB];
+      f32x16 s, dp, pr;
 #pragma unroll
-      for (int j = 0; j < KB; ++j)
+      for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.f;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[j][r] = dp[j][r] = 0.f;
+      for (int kd = 0; kd < KD; ++kd) s = El<T>::mfma(rowfrag<DP>(sq + lrow, qb, kd), kf[kd], s);
 #pragma unroll
-      for (int kd = 0; kd < KD; ++kd) {
-        const bf16x8 qa = rowfrag<DP>(sq + lrow, qb, kd), da = rowfrag<DP>(sg + lrow, qb, kd);
-#pragma unroll
-        for (int j = 0; j < KB; ++j) {
-          s[j] = El<T>::mfma(qa, kf[j][kd], s[j]);
-          dp[j] = El<T>::mfma(da, vf[j][kd], dp[j]);
-        }
-      }
-      bf16x8 pb[KB][2], db[KB][2];
-#pragma unroll
-      for (int j = 0; j < KB; ++j) {
-        f32x16 pr;
+      for (int kd = 0; kd < KD; ++kd) dp = El<T>::mfma(rowfrag<DP>(sg + lrow, qb, kd), vfrag(kd), dp);
+      bf16x8 pb[2], db[2];
+      __builtin_amdgcn_sched_barrier(0);
+      {
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           const int o = 32 * qb + 8 * g + 4 * hi;
@@ -1109,12 +1120,12 @@ __global__ __launch_bounds__(256, (DP == 64 && KB == 1) ? 2 : 1) void attn_mod_d
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               float w;
-              s[j][4 * g + e] = capped(mod, s[j][4 * g + e], w);
+              s[4 * g + e] = capped(mod, s[4 * g + e], w);
               W[e] = 4.f * w * (1.f - w);
             }
           } else if (MOD & 2) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[j][4 * g + e] *= mod.c;
+            for (int e = 0; e < 4; ++e) s[4 * g + e] *= mod.c;
           }
           if (MOD & 2) {
             const int4 pos = *(const int4*)(in + 4 * TILE + o);
@@ -1122,50 +1133,52 @@ __global__ __launch_bounds__(256, (DP == 64 && KB == 1) ? 2 : 1) void attn_mod_d
             if (mod.slope) {
               const f32x4 sl = *(const f32x4*)(in + 2 * TILE + o);
 #pragma unroll
-              for (int e = 0; e < 4; ++e) s[j][4 * g + e] = fmaf(-sl[e], fabsf((float)(key[j] - ps[e])), s[j][4 * g + e]);
+              for (int e = 0; e < 4; ++e) s[4 * g + e] = fmaf(-sl[e], fabsf((float)(key - ps[e])), s[4 * g + e]);
             }
             if (mod.table) {
 #pragma unroll
-              for (int e = 0; e < 4; ++e) s[j][4 * g + e] += tab[max(-mod.R, min(mod.R, key[j] - ps[e])) + mod.R];
-            }
-          }
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            pr[4 * g + e] = __builtin_amdgcn_exp2f(MOD ? s[j][4 * g + e] - L[e] : fmaf(s[j][4 * g + e], mod.c, -L[e]));
-          if (partial) {
-            const int4 bd = *(const int4*)(in + 3 * TILE + o);
-            const int bs[4] = {bd.x, bd.y, bd.z, bd.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) pr[4 * g + e] = key[j] < bs[e] ? pr[4 * g + e] : 0.f;
-            if (docs) {
-              const int4 dc = *(const int4*)(in + 5 * TILE + o);
-              const int ds[4] = {dc.x, dc.y, dc.z, dc.w};
-#pragma unroll
-              for (int e = 0; e < 4; ++e) pr[4 * g + e] = kd_[j] == ds[e] ? pr[4 * g + e] : 0.f;
+              for (int e = 0; e < 4; ++e) s[4 * g + e] += tab[max(-mod.R, min(mod.R, key - ps[e])) + mod.R];
             }
           }
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float d = pr[4 * g + e] * (dp[j][4 * g + e] - E[e]);
-            s[j][4 * g + e] = (MOD & 1) ? d * W[e] : d;
+            pr[4 * g + e] = __builtin_amdgcn_exp2f(MOD ? s[4 * g + e] - L[e] : fmaf(s[4 * g + e], mod.c, -L[e]));
+            const float d = pr[4 * g + e] * (dp[4 * g + e] - E[e]);
+            s[4 * g + e] = (MOD & 1) ? d * W[e] : d;
           }
         }
-        pb[j][0] = pack8<T>(pr, 0);
-        pb[j][1] = pack8<T>(pr, 1);
-        db[j][0] = pack8<T>(s[j], 0);
-        db[j][1] = pack8<T>(s[j], 1);
+        if (partial) {
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const int o = 32 * qb + 8 * g + 4 * hi;
+            const int4 bd = *(const int4*)(in + 3 * TILE + o);
+            const int bs[4] = {bd.x, bd.y, bd.z, bd.w};
+            int4 dc = {0, 0, 0, 0};
+            if (docs) dc = *(const int4*)(in + 5 * TILE + o);
+            const int ds[4] = {dc.x, dc.y, dc.z, dc.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const bool live = (key < bs[e]) & (!docs | (kd_ == ds[e]));
+              pr[4 * g + e] = live ? pr[4 * g + e] : 0.f;
+              s[4 * g + e] = live ? s[4 * g + e] : 0.f;
+            }
+          }
+        }
+        pb[0] = pack8<T>(pr, 0);
+        pb[1] = pack8<T>(pr, 1);
+        db[0] = pack8<T>(s, 0);
+        db[1] = pack8<T>(s, 1);
       }
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
         for (int f = 0; f < FM; ++f) {
           const bf16x8 gt = trfrag<DP>(sg + ltr, qb, f, kk), qt = trfrag<DP>(sq + ltr, qb, f, kk);
-#pragma unroll
-          for (int j = 0; j < KB; ++j) {
-            va[j][f] = El<T>::mfma(gt, pb[j][kk], va[j][f]);
-            ka[j][f] = El<T>::mfma(qt, db[j][kk], ka[j][f]);
-          }
+          va[f] = El<T>::mfma(gt, pb[kk], va[f]);
+          ka[f] = El<T>::mfma(qt, db[kk], ka[f]);
         }
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
   while (c < tend) {
@@ -1173,10 +1186,10 @@ __global__ __launch_bounds__(256, (DP == 64 && KB == 1) ? 2 : 1) void attn_mod_d
     const QMeta mt = mn;
     if (cn < tend) {
       fetch(cn, cur ^ 1);
-      mn = tile_meta(cn % ntr);
+      mn = tile_meta(first + cn % run);
     }
     if ((MOD & 2) && mod.table) {                                       // workgroup-uniform: the next head's table
-      const int gu = c / ntr;
+      const int gu = c / run;
       if (gu != gu_tab) {
         if (gu_tab >= 0) __syncthreads();
         load_table<T>(a, kv * G + gu, tab, tid, NT);
@@ -1185,46 +1198,42 @@ __global__ __launch_bounds__(256, (DP == 64 && KB == 1) ? 2 : 1) void attn_mod_d
       }
     }
     if (kw0 < mt.bmax) {
-      bool partial = kw0 + 32 * KB > mt.bmin;
+      bool partial = kw0 + 32 > mt.bmin;
       if (docs) partial |= wneg | (wdmin != wdmax) | (mt.dmin != mt.dmax) | (mt.neg != 0) | (mt.dmin != wdmin);
-      math(partial);
+      math(__builtin_amdgcn_readfirstlane(partial));
     }
     if (cn < tend) landed(cur ^ 1, mn.bmin <= 0);
     cur ^= 1;
     c = cn;
   }
+  if (key >= Sk) return;
+  if (a.to_part) {
+    const long long n = (long long)NKV * Sk * D, at = (((long long)b * a.p.kv_heads + kv) * Sk + key) * D;
+    float* pk = a.part + (long long)sp * 2 * n + at;
 #pragma unroll
-  for (int j = 0; j < KB; ++j) {
-    if (key[j] >= Sk) continue;
-    if (a.to_part) {
-      const long long n = (long long)NKV * Sk * D, at = (((long long)b * a.p.kv_heads + kv) * Sk + key[j]) * D;
-      float* pk = a.part + (long long)sp * 2 * n + at;
+    for (int f = 0; f < FM; ++f)
 #pragma unroll
-      for (int f = 0; f < FM; ++f)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const int col = 32 * f + 8 * g + 4 * hi;
-          if (col < D) {
-            *(float4*)(pk + col) = float4{ka[j][f][4 * g], ka[j][f][4 * g + 1], ka[j][f][4 * g + 2], ka[j][f][4 * g + 3]};
-            *(float4*)(pk + n + col) = float4{va[j][f][4 * g], va[j][f][4 * g + 1], va[j][f][4 * g + 2], va[j][f][4 * g + 3]};
-          }
+      for (int g = 0; g < 4; ++g) {
+        const int col = 32 * f + 8 * g + 4 * hi;
+        if (col < D) {
+          *(float4*)(pk + col) = float4{ka[f][4 * g], ka[f][4 * g + 1], ka[f][4 * g + 2], ka[f][4 * g + 3]};
+          *(float4*)(pk + n + col) = float4{va[f][4 * g], va[f][4 * g + 1], va[f][4 * g + 2], va[f][4 * g + 3]};
         }
-    } else {
-      bf16_t* kp = (bf16_t*)a.p.dk.ptr + op_base(a.p.dk, b) + (long long)key[j] * a.p.dk.sstride + (long long)kv * D;
-      bf16_t* vp = (bf16_t*)a.p.dv.ptr + op_base(a.p.dv, b) + (long long)key[j] * a.p.dv.sstride + (long long)kv * D;
-      const float sc = a.p.scale;
+      }
+  } else {
+    bf16_t* kp = (bf16_t*)a.p.dk.ptr + op_base(a.p.dk, b) + (long long)key * a.p.dk.sstride + (long long)kv * D;
+    bf16_t* vp = (bf16_t*)a.p.dv.ptr + op_base(a.p.dv, b) + (long long)key * a.p.dv.sstride + (long long)kv * D;
+    const float sc = a.p.scale;
 #pragma unroll
-      for (int f = 0; f < FM; ++f)
+    for (int f = 0; f < FM; ++f)
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const int col = 32 * f + 8 * g + 4 * hi;
-          if (col < D) {
-            *(uint2*)(kp + col) = uint2{El<T>::pack2(ka[j][f][4 * g] * sc, ka[j][f][4 * g + 1] * sc),
-                                        El<T>::pack2(ka[j][f][4 * g + 2] * sc, ka[j][f][4 * g + 3] * sc)};
-            *(uint2*)(vp + col) = uint2{El<T>::pack2(va[j][f][4 * g], va[j][f][4 * g + 1]), El<T>::pack2(va[j][f][4 * g + 2], va[j][f][4 * g + 3])};
-          }
+      for (int g = 0; g < 4; ++g) {
+        const int col = 32 * f + 8 * g + 4 * hi;
+        if (col < D) {
+          *(uint2*)(kp + col) = uint2{El<T>::pack2(ka[f][4 * g] * sc, ka[f][4 * g + 1] * sc), El<T>::pack2(ka[f][4 * g + 2] * sc, ka[f][4 * g + 3] * sc)};
+          *(uint2*)(vp + col) = uint2{El<T>::pack2(va[f][4 * g], va[f][4 * g + 1]), El<T>::pack2(va[f][4 * g + 2], va[f][4 * g + 3])};
         }
-    }
+      }
   }
 }
 
@@ -1242,9 +1251,12 @@ __global__ __launch_bounds__(256) void attn_mod_dkdv_join_kernel(const Args a) {
   const int key = (int)(row - bk * a.p.Sk), b0 = (int)(bk / a.p.kv_heads) * share, kv = (int)(bk % a.p.kv_heads);
   float4 k = {0.f, 0.f, 0.f, 0.f}, v = {0.f, 0.f, 0.f, 0.f};
   for (int b = b0; b < min(b0 + share, a.p.nbatch); ++b) {
+    const Seq seq = load_seq(a, b);
+    const int keys = a.p.D <= 64 ? 128 : 256, wk0 = key / keys * keys, run = (a.M + TILE - 1) / TILE - first_tile(a, seq, wk0);
+    const int used = wk0 < seq.len ? max(1, (run * (a.p.heads / a.p.kv_heads / a.gp) + a.chunk - 1) / a.chunk) : 1;      // splits that wrote
     const float* p0 = a.part + b * per + ((long long)kv * a.p.Sk + key) * D + c;
 #pragma unroll 4
-    for (int s = 0; s < a.splits; ++s) {
+    for (int s = 0; s < used; ++s) {
       const float4 x = *(const float4*)(p0 + s * 2 * n), y = *(const float4*)(p0 + s * 2 * n + n);
       k.x += x.x;
       k.y += x.y;
@@ -1325,15 +1337,21 @@ Layout make_layout(const T2VAttnMod* p, bool bwd) {
     }
   }
   L.dq_tiles = (a.M + 127) / 128;
-  L.kv_tiles = (p->Sk + 127) / 128;
+  const int keys = L.dp == 64 ? 128 : 256;      // of a dK / dV workgroup
+  L.kv_tiles = (p->Sk + keys - 1) / keys;
   L.kv_splits = 1;
+  a.chunk = 1 << 30;
   if (bwd) {
+    // few K / V heads and keys: the row tiles are split so that about KV_WGS workgroups of equal work exist (half of all pairs under a causal mask)
     const long long wgs = (long long)p->nbatch * p->kv_heads * L.kv_tiles, tiles = (long long)((a.M + TILE - 1) / TILE) * (G / a.gp);
-    if (wgs < 256) {
-      long long s = 512 / wgs;
-      s = s < tiles / 4 ? s : tiles / 4;
-      s = s > 16 ? 16 : s;
-      L.kv_splits = s > 1 ? (int)s : 1;
+    static const int KV_WGS = getenv("KVW") ? atoi(getenv("KVW")) : 384;
+    const long long work = wgs * tiles / (p->causal && !p->q_docs && p->Sq > 1 ? 2 : 1);
+    if (wgs < 256 && tiles > 4) {
+      long long c = (work + KV_WGS - 1) / KV_WGS;
+      c = c < 4 ? 4 : c;
+      if (tiles > 16 * c) c = (tiles + 15) / 16;
+      a.chunk = (int)(c < tiles ? c : tiles);
+      L.kv_splits = (int)((tiles + a.chunk - 1) / a.chunk);
     }
   }
   L.meta = p->q_docs || (p->prefix && p->prefix_per_query);
@@ -1371,10 +1389,14 @@ Layout make_layout(const T2VAttnMod* p, bool bwd) {
 }
 
 size_t smem_bytes(const Layout& L, int tables, bool kv) {
-  return 2 * (L.dp == 64 ? sizeof(Stage<64>) : sizeof(Stage<128>)) + (kv ? 2 * 6 * TILE * 4 : 2 * TILE * 4 + 64) + (L.a.p.bias ? tables * 4 * (2 * (size_t)L.a.p.radius + 1) : 0);
+  if (kv) {
+    const size_t tab = L.a.p.bias ? 4 * ((2 * (size_t)L.a.p.radius + 1 + 3) / 4 * 4) : 0;
+    return (L.dp == 64 ? 2 * sizeof(Stage<64>) : 2 * sizeof(Stage<128>) + 4 * sizeof(Stage<128>) / 2) + 2 * 6 * TILE * 4 + tab;
+  }
+  return 2 * (L.dp == 64 ? sizeof(Stage<64>) : sizeof(Stage<128>)) + 2 * TILE * 4 + 64 + (L.a.p.bias ? tables * 4 * (2 * (size_t)L.a.p.radius + 1) : 0);
 }
 template <typename K>
-int launch(int which, K kern, long long grid, size_t smem, hipStream_t st, const Args& a) {
+int launch(int which, K kern, long long grid, size_t smem, hipStream_t st, const Args& a, int threads = 256) {
   if (smem > 64 * 1024) {
     const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != hipSuccess) {
@@ -1382,7 +1404,7 @@ int launch(int which, K kern, long long grid, size_t smem, hipStream_t st, const
       return T2V_ELAUNCH;
     }
   }
-  t2v_launch_timed(which, kern, dim3((unsigned)grid), dim3(256), (unsigned)smem, st, a);
+  t2v_launch_timed(which, kern, dim3((unsigned)grid), dim3(threads), (unsigned)smem, st, a);
   return T2V_OK;
 }
 // bit 0 cap, bit 1 distance bias; a scale that is not positive takes the form that does not fold it into the running maximum
@@ -1432,8 +1454,8 @@ int run_bwd(Layout& L, hipStream_t st) {
   const size_t smk = smem_bytes(L, 1, true);
   a.to_part = L.kv_splits > 1 || a.p.kv_share > 1;
   const int which = a.to_part ? 0 : 2;
-  e = mb == 0 ? launch(which, attn_mod_dkdv_kernel<T, DP, 1, 0>, gk, smk, st, a) : mb == 1 ? launch(which, attn_mod_dkdv_kernel<T, DP, 1, 1>, gk, smk, st, a) :
-      mb == 2 ? launch(which, attn_mod_dkdv_kernel<T, DP, 1, 2>, gk, smk, st, a) : launch(which, attn_mod_dkdv_kernel<T, DP, 1, 3>, gk, smk, st, a);
+  e = mb == 0 ? launch(which, attn_mod_dkdv_kernel<T, DP, 0>, gk, smk, st, a, DP == 128 ? 512 : 256) : mb == 1 ? launch(which, attn_mod_dkdv_kernel<T, DP, 1>, gk, smk, st, a, DP == 128 ? 512 : 256) :
+      mb == 2 ? launch(which, attn_mod_dkdv_kernel<T, DP, 2>, gk, smk, st, a, DP == 128 ? 512 : 256) : launch(which, attn_mod_dkdv_kernel<T, DP, 3>, gk, smk, st, a, DP == 128 ? 512 : 256);
   if (e) return e;
   T2V_CHECK_LAUNCH();
   if (a.to_part) {
