@@ -15,7 +15,6 @@
 // are read once for all of them; with a table each head is a unit of its own (gp = 1: the table of one head lives in LDS).
 // Statistics, the running maximum and sum, lse, delta and all accumulators are fp32; P and dS are rounded to the input type for the
 // matrix cores (one rounding of a factor in [0, 1], and of a gradient, the same size as the output's own rounding).
-#include <stdlib.h>
 #include <type_traits>
 
 #include "common.h"
@@ -83,7 +82,10 @@ struct Args {
   int gp, nunit, M;                 // heads per unit, units per batch, rows per unit (Sq * gp)
   unsigned magic;                   // r / gp = r * magic >> 32 (gp > 1)
   int ntile, splits;                // row (or key) tiles of a unit, splits of the other axis
-  int chunk;                        // row tiles a split of dK / dV takes
+  int chunk, wgs;                   // dK / dV: row tiles a split is meant to take, workgroups of a K / V head (see kv_runs)
+  int fold;                         // order of the row tiles (see row_tile)
+  const int* qorder;                // [nbatch * row tiles], [nbatch * key tiles]: (batch, tile) pairs by falling work, or NULL
+  const int* korder;
   int to_part;                      // dK / dV go to `part` as fp32 (several splits, or several batches that share K / V)
   const QMeta* qmeta;               // [nbatch][ceil(M / 64)] or NULL
   const KMeta* kmeta;               // [nbatch][ceil(Sk / 64)] or NULL
@@ -124,10 +126,27 @@ __device__ __forceinline__ int first_tile(const Args& a, const Seq& s, int wk0) 
   return a.qmeta || !s.causal || s.prefix > wk0 ? 0 : min((a.M + TILE - 1) / TILE, max(0, wk0 - s.off) * a.gp / TILE);
 }
 
+// dK / dV: how many workgroups share the rows of key tile k.  It is fixed by sizes alone (a causal mask, no prefix, whole lengths), so that the
+// grid has no workgroup without work where those hold: 43 % of idle ones put the busy ones unevenly on the shader engines, and the
+// launch took two rounds where one was enough (193 -> 128 us).  What the mask really leaves is divided evenly among them.
+__host__ __device__ __forceinline__ int kv_runs(const Args& a, int k, int keys, int tiles) {
+  if (a.chunk >= tiles) return 1;
+  const long long first = a.p.causal && !a.qmeta ? ((long long)k * keys - (a.p.Sk - a.p.Sq)) * a.gp / TILE : 0;
+  const int run = tiles - (int)(first > 0 ? first : 0) * (a.p.heads / a.p.kv_heads / a.gp);
+  return run > a.chunk ? (run + a.chunk - 1) / a.chunk : 1;
+}
+// forward, dQ: the row tile of rank r.  Under a causal mask the last tiles are the longest: they come first (they then end first come, first
+// served), or (fold) the long half falls and the short half rises, where all workgroups are resident at once, two per CU: the second
+// workgroup of a CU is then short where the first is long.
+__device__ __forceinline__ int row_tile(const Args& a, int r) {
+  const int half = (a.ntile + 1) / 2;
+  return a.fold && r >= half ? r - half : a.ntile - 1 - r;
+}
+
 // workgroup id -> (batch, unit): workgroups go round-robin over the eight XCDs, so units that share a K/V head are placed a multiple of
 // nbatch * kv_heads apart, which is the same XCD (and L2) where that is a multiple of eight
 struct Unit {
-  int b, kv, h0;
+  int b, kv, h0, x;                 // x: number of the unit, as unit_of counts them
 };
 __device__ __forceinline__ Unit unit_of(const Args& a, int x) {
   const int kvb = a.p.nbatch * a.p.kv_heads, gu = x / kvb, y = x - gu * kvb;
@@ -135,7 +154,19 @@ __device__ __forceinline__ Unit unit_of(const Args& a, int x) {
   u.b = y / a.p.kv_heads;
   u.kv = y - u.b * a.p.kv_heads;
   u.h0 = u.kv * (a.p.heads / a.p.kv_heads) + gu * a.gp;
+  u.x = x;
   return u;
+}
+// the unit and row tile of workgroup `id` (of one split)
+__device__ __forceinline__ Unit work_of(const Args& a, int id, int& tile) {
+  if (a.qorder) {
+    const int e = a.qorder[id / a.nunit], v = id % a.nunit, b = e / a.ntile, gus = a.nunit / a.p.kv_heads;
+    tile = e - b * a.ntile;
+    return unit_of(a, (v % gus) * a.p.nbatch * a.p.kv_heads + b * a.p.kv_heads + v / gus);
+  }
+  const int NU = a.p.nbatch * a.nunit;
+  tile = row_tile(a, id / NU);
+  return unit_of(a, id % NU);
 }
 
 // ------------------------------------------------------------------------------------------------ staging
@@ -210,6 +241,31 @@ __device__ __forceinline__ bf16x8 trfrag(const bf16_t* s, int blk, int fm, int k
   const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_bf16x4*)(s + row_off<DP>(32 * blk + 16 * kk) + 32 * fm));
   const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_bf16x4*)(s + row_off<DP>(32 * blk + 16 * kk + 8) + 32 * fm));
   return bf16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+}
+
+// 32 FM columns of the lane's row from the accumulators, times mul, 16 bytes per store: the halves of a wave hold columns 4 hi .. 4 hi + 3 of
+// every eight and exchange them first (v_permlane32_swap), so that the lower half stores eight columns and the upper the next eight
+template <typename T, int FM>
+__device__ __forceinline__ void store_row(bf16_t* row, const f32x16 (&v)[FM], float mul, int hi, int D, bool ok) {
+#pragma unroll
+  for (int f = 0; f < FM; ++f)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = 8 * h;
+      const auto x = __builtin_amdgcn_permlane32_swap(El<T>::pack2(v[f][r] * mul, v[f][r + 1] * mul), El<T>::pack2(v[f][r + 4] * mul, v[f][r + 5] * mul), false, false);
+      const auto y = __builtin_amdgcn_permlane32_swap(El<T>::pack2(v[f][r + 2] * mul, v[f][r + 3] * mul), El<T>::pack2(v[f][r + 6] * mul, v[f][r + 7] * mul), false, false);
+      const int col = 32 * f + 16 * h + 8 * hi;
+      if (ok && col < D) *(u32x4*)(row + col) = u32x4{x[0], y[0], x[1], y[1]};
+    }
+}
+// the accumulators as they are, a wave's registers one after the other (1 KB per instruction): partial sums of the splits
+template <int FM>
+__device__ __forceinline__ void store_part(float* wave_part, const f32x16 (&v)[FM], int lane, bool ok) {
+#pragma unroll
+  for (int f = 0; f < FM; ++f)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      if (ok) *(float4*)(wave_part + ((f * 4 + g) * 64 + lane) * 4) = float4{v[f][4 * g], v[f][4 * g + 1], v[f][4 * g + 2], v[f][4 * g + 3]};
 }
 
 __device__ __forceinline__ const bf16x8* chunk_ptr(const bf16_t* p, bool ok) { return ok ? (const bf16x8*)p : (const bf16x8*)zero_chunk; }
@@ -346,9 +402,9 @@ __global__ __launch_bounds__(256, (DP * QB <= 128) ? 2 : 1) void attn_mod_fwd_ke
   float* tab = (float*)(swg + 16);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5;
   const int NU = a.p.nbatch * a.nunit;
-  const int x = blockIdx.x % NU, rest = blockIdx.x / NU;
-  const int sp = rest % a.splits, tile = a.ntile - 1 - rest / a.splits; // the longest rows of a causal mask first
-  const Unit u = unit_of(a, x);
+  const int sp = blockIdx.x / NU % a.splits;
+  int tile;
+  const Unit u = work_of(a, blockIdx.x / (NU * a.splits) * NU + blockIdx.x % NU, tile);
   const Seq seq = load_seq(a, u.b);
   const int len = seq.len, D = a.p.D, Sk = a.p.Sk;
   const bf16_t* Q = (const bf16_t*)a.p.q.ptr + op_base(a.p.q, u.b);
@@ -586,68 +642,61 @@ __global__ __launch_bounds__(256, (DP * QB <= 128) ? 2 : 1) void attn_mod_fwd_ke
 #pragma unroll
   for (int q = 0; q < QB; ++q) {
     const float lt = l[q] + xor32(l[q]);
-    if (!R.ok[q]) continue;
     const float m2 = MOD ? m[q] : m[q] * mod.c;
-    const long long sidx = ((long long)u.b * a.p.heads + u.h0) * a.p.Sq + R.r[q];
     if (a.splits > 1) {
-      const long long at = ((long long)sp * NU + ((long long)u.b * a.nunit + u.h0 / a.gp)) * a.M + R.r[q];
-      float* po = a.part + at * D;
-#pragma unroll
-      for (int f = 0; f < FM; ++f)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const int col = 32 * f + 8 * g + 4 * hi;
-          if (col < D) *(float4*)(po + col) = float4{o[q][f][4 * g], o[q][f][4 * g + 1], o[q][f][4 * g + 2], o[q][f][4 * g + 3]};
-        }
-      if (hi == 0) *(float2*)(a.part_ml + at * 2) = float2{m2, lt};
+      const long long block = (((long long)sp * NU + u.x) * a.ntile + tile) * 4 * QB + wave * QB + q;       // of 32 rows
+      store_part<FM>(a.part + block * (32 * DP), o[q], lane, R.ok[q]);
+      if (R.ok[q] && hi == 0) *(float2*)(a.part_ml + (block * 32 + lane) * 2) = float2{m2, lt};
     } else {
-      const float inv = lt > 0.f ? 1.f / lt : 0.f;
       bf16_t* op = (bf16_t*)a.p.o.ptr + op_base(a.p.o, u.b) + (long long)R.i[q] * a.p.o.sstride + (long long)R.h[q] * D;
-#pragma unroll
-      for (int f = 0; f < FM; ++f)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const int col = 32 * f + 8 * g + 4 * hi;
-          if (col < D)
-            *(uint2*)(op + col) = uint2{El<T>::pack2(o[q][f][4 * g] * inv, o[q][f][4 * g + 1] * inv),
-                                        El<T>::pack2(o[q][f][4 * g + 2] * inv, o[q][f][4 * g + 3] * inv)};
-        }
+      store_row<T, FM>(op, o[q], lt > 0.f ? 1.f / lt : 0.f, hi, D, R.ok[q]);
       // base-2 log-sum-exp; +inf marks a row that saw nothing: every exp2(t - lse) of the backward pass is then 0
-      if (hi == 0 && a.p.lse) a.p.lse[sidx] = lt > 0.f ? m2 + __builtin_amdgcn_logf(lt) : INFINITY;
+      if (R.ok[q] && hi == 0 && a.p.lse)
+        a.p.lse[((long long)u.b * a.p.heads + u.h0) * a.p.Sq + R.r[q]] = lt > 0.f ? m2 + __builtin_amdgcn_logf(lt) : INFINITY;
     }
   }
 }
 
-// joins the splits: one group of D / 4 lanes per row
-template <typename T>
-__global__ __launch_bounds__(256) void attn_mod_join_kernel(const Args a) {
-  const int D = a.p.D, lanes = D / 4, gpb = 256 / lanes;
-  const int g = threadIdx.x / lanes, c = threadIdx.x - g * lanes;
-  const long long rows = (long long)a.p.nbatch * a.nunit * a.M;
-  const long long row = (long long)blockIdx.x * gpb + g;
-  if (g >= gpb || row >= rows) return;
+// joins the splits: one wave per 32 rows and 32 columns, laid out like the accumulators
+template <typename T, int DP>
+__global__ __launch_bounds__(64) void attn_mod_join_kernel(const Args a) {
+  constexpr int FM = DP / 32;
+  const int lane = threadIdx.x, hi = lane >> 5, D = a.p.D;
+  const int f = blockIdx.x % FM;
+  const long long block = blockIdx.x / FM;                              // over (unit x, tile, 32 rows)
+  const int NU = a.p.nbatch * a.nunit, per = a.ntile * 4, x = (int)(block / per);
+  const int r = (int)(block - (long long)x * per) * 32 + (lane & 31);
+  const bool ok = r < a.M;
+  const long long stride = (long long)NU * per;                         // blocks of a split
+  if (__all(!ok)) return;
+  const long long at = block * 32 + (lane & 31);
+  // (lanes behind the last row read their part of the padded buffer, whatever it holds, and store nothing: a branch around the loads would
+  //  put a wait behind each)
   float m = LOWEST * 4.f;
-  for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.part_ml[((long long)s * rows + row) * 2]);
+#pragma unroll 8
+  for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.part_ml[(s * stride * 32 + at) * 2]);
   float l = 0.f;
-  float4 acc = {0.f, 0.f, 0.f, 0.f};
+  f32x16 acc[1];
+#pragma unroll
+  for (int e = 0; e < 16; ++e) acc[0][e] = 0.f;
 #pragma unroll 4
   for (int s = 0; s < a.splits; ++s) {
-    const float2 ml = *(const float2*)(a.part_ml + ((long long)s * rows + row) * 2);
-    const float4 v = *(const float4*)(a.part + ((long long)s * rows + row) * D + 4 * c);
+    const float2 ml = *(const float2*)(a.part_ml + (s * stride * 32 + at) * 2);
+    const float* p = a.part + (s * stride + block) * (32 * DP) + (f * 256 + lane) * 4;
     const float w = __builtin_amdgcn_exp2f(ml.x - m);
     l = fmaf(w, ml.y, l);
-    acc.x = fmaf(w, v.x, acc.x);
-    acc.y = fmaf(w, v.y, acc.y);
-    acc.z = fmaf(w, v.z, acc.z);
-    acc.w = fmaf(w, v.w, acc.w);
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const f32x4 v = *(const f32x4*)(p + g * 256);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[0][4 * g + e] = fmaf(w, v[e], acc[0][4 * g + e]);
+    }
   }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
-  const long long bu = row / a.M;
-  const int r = (int)(row - bu * a.M), b = (int)(bu / a.nunit), h0 = (int)(bu - (long long)b * a.nunit) * a.gp;
-  const int i = div_gp(a, r), h = h0 + r - i * a.gp;
-  bf16_t* op = (bf16_t*)a.p.o.ptr + op_base(a.p.o, b) + (long long)i * a.p.o.sstride + (long long)h * D + 4 * c;
-  *(uint2*)op = uint2{El<T>::pack2(acc.x * inv, acc.y * inv), El<T>::pack2(acc.z * inv, acc.w * inv)};
-  if (c == 0 && a.p.lse) a.p.lse[((long long)b * a.p.heads + h0) * a.p.Sq + r] = l > 0.f ? m + __builtin_amdgcn_logf(l) : INFINITY;
+  const Unit u = unit_of(a, x);
+  const int i = div_gp(a, min(r, a.M - 1)), h = u.h0 + min(r, a.M - 1) - i * a.gp;
+  bf16_t* op = (bf16_t*)a.p.o.ptr + op_base(a.p.o, u.b) + (long long)i * a.p.o.sstride + (long long)h * D + 32 * f;
+  store_row<T, 1>(op, acc, l > 0.f ? 1.f / l : 0.f, hi, D - 32 * f, ok);
+  if (ok && f == 0 && hi == 0 && a.p.lse) a.p.lse[((long long)u.b * a.p.heads + u.h0) * a.p.Sq + r] = l > 0.f ? m + __builtin_amdgcn_logf(l) : INFINITY;
 }
 
 // bounds and documents of every 64 rows / keys (launched where a mask has documents or one prefix per query): one wave per tile
@@ -691,9 +740,8 @@ __global__ __launch_bounds__(256, (DP * QB <= 128) ? 2 : 1) void attn_mod_dq_ker
   int* swg = sdoc + 2 * TILE;
   float* tab = (float*)(swg + 16);                                      // [2R + 1], then [4 waves][2R + 1] sums
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5;
-  const int NU = a.p.nbatch * a.nunit;
-  const int x = blockIdx.x % NU, tile = a.ntile - 1 - blockIdx.x / NU;
-  const Unit u = unit_of(a, x);
+  int tile;
+  const Unit u = work_of(a, blockIdx.x, tile);
   const Seq seq = load_seq(a, u.b);
   const int len = seq.len, D = a.p.D, Sk = a.p.Sk;
   const bool docs = a.kmeta && a.p.kv_docs;
@@ -912,18 +960,8 @@ __global__ __launch_bounds__(256, (DP * QB <= 128) ? 2 : 1) void attn_mod_dq_ker
   }
 #pragma unroll
   for (int q = 0; q < QB; ++q) {
-    if (!R.ok[q]) continue;
     bf16_t* op = (bf16_t*)a.p.dq.ptr + op_base(a.p.dq, u.b) + (long long)R.i[q] * a.p.dq.sstride + (long long)R.h[q] * D;
-#pragma unroll
-    for (int f = 0; f < FM; ++f)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int col = 32 * f + 8 * g + 4 * hi;
-        const float c = a.p.scale;
-        if (col < D)
-          *(uint2*)(op + col) = uint2{El<T>::pack2(acc[q][f][4 * g] * c, acc[q][f][4 * g + 1] * c),
-                                      El<T>::pack2(acc[q][f][4 * g + 2] * c, acc[q][f][4 * g + 3] * c)};
-      }
+    store_row<T, FM>(op, acc[q], a.p.scale, hi, D, R.ok[q]);
   }
   if (dtab) {
     below = wave_sum(below);
@@ -973,12 +1011,20 @@ __global__ __launch_bounds__(DP == 128 ? 512 : 256, 2) void attn_mod_dkdv_kernel
   float* sinfo = (float*)(smem + 2 * sizeof(Stage<DP>));                // [2][6][TILE]: lse, delta, slope, bound, pos, doc
   float* tab = sinfo + 2 * 6 * TILE;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5;
-  const int NKV = a.p.nbatch * a.p.kv_heads;
-  const int y = blockIdx.x % NKV, rest = blockIdx.x / NKV;
-  const int sp = rest % a.splits, ktile = rest / a.splits;              // early keys are seen by the most rows of a causal mask: first
+  const int NKV = a.p.nbatch * a.p.kv_heads, G = a.p.heads / a.p.kv_heads, GU = G / a.gp, ntr = (a.M + TILE - 1) / TILE;
+  int y = blockIdx.x % NKV, ktile = blockIdx.x / NKV, sp = 0, runs = 1; // early keys are seen by the most rows of a causal mask: first
+  const int w = ktile;
+  if (a.korder) {
+    const int e = a.korder[blockIdx.x / a.p.kv_heads];
+    ktile = e % a.ntile;
+    y = e / a.ntile * a.p.kv_heads + blockIdx.x % a.p.kv_heads;
+  } else if (a.to_part) {
+    sp = ktile;
+    for (ktile = 0; sp >= (runs = kv_runs(a, ktile, KEYS, ntr * GU)); ++ktile) sp -= runs;
+  }
   const int b = y / a.p.kv_heads, kv = y - b * a.p.kv_heads;
   const Seq seq = load_seq(a, b);
-  const int len = seq.len, D = a.p.D, Sk = a.p.Sk, G = a.p.heads / a.p.kv_heads, GU = G / a.gp;
+  const int len = seq.len, D = a.p.D, Sk = a.p.Sk;
   const bool docs = a.kmeta && a.p.kv_docs;
   const Mod mod = make_mod(a);
   const bf16_t* Q = (const bf16_t*)a.p.q.ptr + op_base(a.p.q, b);
@@ -1029,13 +1075,11 @@ __global__ __launch_bounds__(DP == 128 ? 512 : 256, 2) void attn_mod_dkdv_kernel
 #pragma unroll
     for (int r = 0; r < 16; ++r) ka[f][r] = va[f][r] = 0.f;
 
-  // The row tiles that matter, of all units of the K / V head, are numbered through and a split takes `chunk` of them.  With the meta table
+  // The row tiles that matter, of all units of the K / V head, are numbered through and divided among the `runs` workgroups.  With the meta table
   // those are all tiles, filtered on the way; without it bounds grow with the query, and only the last tiles of a unit see key wk0 or a later one.
-  const int ntr = (a.M + TILE - 1) / TILE;
   const QMeta* qm = a.qmeta ? a.qmeta + (long long)b * ntr : nullptr;
   const int first = first_tile(a, seq, wk0), run = ntr - first, total = wk0 < len ? run * GU : 0;
-  const int tbeg = sp * a.chunk, tend = min(total, tbeg + a.chunk);
-  if (sp > 0 && tbeg >= total) return;                                  // workgroup-uniform; the join knows how many splits there are
+  const int per = (total + runs - 1) / runs, tbeg = min(total, sp * per), tend = min(total, tbeg + per);
   auto tile_meta = [&](int t) {
     if (qm) return uniform(qm[t]);
     return uniform(QMeta{t * TILE + TILE > a.M ? 0 : row_bound(seq, div_gp(a, t * TILE)), row_bound(seq, div_gp(a, min(a.M, t * TILE + TILE) - 1)), 0, 0, 0});
@@ -1206,81 +1250,54 @@ __global__ __launch_bounds__(DP == 128 ? 512 : 256, 2) void attn_mod_dkdv_kernel
     cur ^= 1;
     c = cn;
   }
-  if (key >= Sk) return;
   if (a.to_part) {
-    const long long n = (long long)NKV * Sk * D, at = (((long long)b * a.p.kv_heads + kv) * Sk + key) * D;
-    float* pk = a.part + (long long)sp * 2 * n + at;
-#pragma unroll
-    for (int f = 0; f < FM; ++f)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int col = 32 * f + 8 * g + 4 * hi;
-        if (col < D) {
-          *(float4*)(pk + col) = float4{ka[f][4 * g], ka[f][4 * g + 1], ka[f][4 * g + 2], ka[f][4 * g + 3]};
-          *(float4*)(pk + n + col) = float4{va[f][4 * g], va[f][4 * g + 1], va[f][4 * g + 2], va[f][4 * g + 3]};
-        }
-      }
+    const long long block = ((long long)y * a.wgs + w) * NW + wave;       // of 32 keys
+    store_part<FM>(a.part + block * (64 * DP), ka, lane, true);
+    store_part<FM>(a.part + block * (64 * DP) + 32 * DP, va, lane, true);
   } else {
-    bf16_t* kp = (bf16_t*)a.p.dk.ptr + op_base(a.p.dk, b) + (long long)key * a.p.dk.sstride + (long long)kv * D;
-    bf16_t* vp = (bf16_t*)a.p.dv.ptr + op_base(a.p.dv, b) + (long long)key * a.p.dv.sstride + (long long)kv * D;
-    const float sc = a.p.scale;
-#pragma unroll
-    for (int f = 0; f < FM; ++f)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int col = 32 * f + 8 * g + 4 * hi;
-        if (col < D) {
-          *(uint2*)(kp + col) = uint2{El<T>::pack2(ka[f][4 * g] * sc, ka[f][4 * g + 1] * sc), El<T>::pack2(ka[f][4 * g + 2] * sc, ka[f][4 * g + 3] * sc)};
-          *(uint2*)(vp + col) = uint2{El<T>::pack2(va[f][4 * g], va[f][4 * g + 1]), El<T>::pack2(va[f][4 * g + 2], va[f][4 * g + 3])};
-        }
-      }
+    store_row<T, FM>((bf16_t*)a.p.dk.ptr + op_base(a.p.dk, b) + (long long)key * a.p.dk.sstride + (long long)kv * D, ka, a.p.scale, hi, D, key < Sk);
+    store_row<T, FM>((bf16_t*)a.p.dv.ptr + op_base(a.p.dv, b) + (long long)key * a.p.dv.sstride + (long long)kv * D, va, 1.f, hi, D, key < Sk);
   }
 }
 
-// dK, dV = sum of the partial sums of the splits and of the batches that share a K / V head, in order
-template <typename T>
-__global__ __launch_bounds__(256) void attn_mod_dkdv_join_kernel(const Args a) {
-  const int D = a.p.D, lanes = D / 4, share = a.p.kv_share;
-  const int nbk = (a.p.nbatch + share - 1) / share;
-  const long long per = (long long)a.p.kv_heads * a.p.Sk * D, n = per * a.p.nbatch;        // of a batch, of a split
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (i * 4 >= per * nbk) return;
-  const long long row = i / lanes;
-  const int c = (int)(i - row * lanes) * 4;
-  const long long bk = row / a.p.Sk;
-  const int key = (int)(row - bk * a.p.Sk), b0 = (int)(bk / a.p.kv_heads) * share, kv = (int)(bk % a.p.kv_heads);
-  float4 k = {0.f, 0.f, 0.f, 0.f}, v = {0.f, 0.f, 0.f, 0.f};
+// dK, dV = sum of the partial sums of the splits and of the batches that share a K / V head, in order: one wave per 32 keys, 32 columns and side
+template <typename T, int DP>
+__global__ __launch_bounds__(64) void attn_mod_dkdv_join_kernel(const Args a) {
+  constexpr int FM = DP / 32, NW = DP == 128 ? 8 : 4, KEYS = 32 * NW;
+  const int lane = threadIdx.x, hi = lane >> 5, D = a.p.D, share = a.p.kv_share, KV = a.p.kv_heads;
+  const int f = blockIdx.x % FM, side = blockIdx.x / FM % 2;
+  const int blk = blockIdx.x / (2 * FM), wave = blk % NW, ktile = blk / NW % a.ntile, yk = blk / NW / a.ntile;
+  const int b0 = yk / KV * share, kv = yk % KV;
+  const int key = ktile * KEYS + wave * 32 + (lane & 31);
+  const int tiles = (a.M + TILE - 1) / TILE * (a.p.heads / KV / a.gp), runs = kv_runs(a, ktile, KEYS, tiles);
+  int w0 = 0;
+  for (int k = 0; k < ktile; ++k) w0 += kv_runs(a, k, KEYS, tiles);
+  f32x16 acc[1];
+#pragma unroll
+  for (int e = 0; e < 16; ++e) acc[0][e] = 0.f;
   for (int b = b0; b < min(b0 + share, a.p.nbatch); ++b) {
-    const Seq seq = load_seq(a, b);
-    const int keys = a.p.D <= 64 ? 128 : 256, wk0 = key / keys * keys, run = (a.M + TILE - 1) / TILE - first_tile(a, seq, wk0);
-    const int used = wk0 < seq.len ? max(1, (run * (a.p.heads / a.p.kv_heads / a.gp) + a.chunk - 1) / a.chunk) : 1;      // splits that wrote
-    const float* p0 = a.part + b * per + ((long long)kv * a.p.Sk + key) * D + c;
 #pragma unroll 4
-    for (int s = 0; s < used; ++s) {
-      const float4 x = *(const float4*)(p0 + s * 2 * n), y = *(const float4*)(p0 + s * 2 * n + n);
-      k.x += x.x;
-      k.y += x.y;
-      k.z += x.z;
-      k.w += x.w;
-      v.x += y.x;
-      v.y += y.y;
-      v.z += y.z;
-      v.w += y.w;
+    for (int s = 0; s < runs; ++s) {
+      const float* p = a.part + (((long long)(b * KV + kv) * a.wgs + w0 + s) * NW + wave) * (64 * DP) + side * 32 * DP + (f * 256 + lane) * 4;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 v = *(const f32x4*)(p + g * 256);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[0][4 * g + e] += v[e];
+      }
     }
   }
-  bf16_t* kp = (bf16_t*)a.p.dk.ptr + op_base(a.p.dk, b0) + (long long)key * a.p.dk.sstride + (long long)kv * D + c;
-  bf16_t* vp = (bf16_t*)a.p.dv.ptr + op_base(a.p.dv, b0) + (long long)key * a.p.dv.sstride + (long long)kv * D + c;
-  const float sc = a.p.scale;
-  *(uint2*)kp = uint2{El<T>::pack2(k.x * sc, k.y * sc), El<T>::pack2(k.z * sc, k.w * sc)};
-  *(uint2*)vp = uint2{El<T>::pack2(v.x, v.y), El<T>::pack2(v.z, v.w)};
+  const T2VAttnOperand& o = side ? a.p.dv : a.p.dk;
+  bf16_t* op = (bf16_t*)o.ptr + op_base(o, b0) + (long long)key * o.sstride + (long long)kv * D + 32 * f;
+  store_row<T, 1>(op, acc, side ? 1.f : a.p.scale, hi, D - 32 * f, key < a.p.Sk);
 }
 
 // ------------------------------------------------------------------------------------------------ host
 struct Layout {
   Args a;
   int qb, dp;
-  int fwd_tiles, fwd_splits, dq_tiles, kv_tiles, kv_splits;
-  bool meta;
+  int fwd_tiles, fwd_splits, dq_tiles, kv_tiles;
+  bool kv_split, meta;
   long long o_qmeta, o_kmeta, o_part, o_ml, o_bias, bytes;
 };
 
@@ -1339,22 +1356,37 @@ Layout make_layout(const T2VAttnMod* p, bool bwd) {
   L.dq_tiles = (a.M + 127) / 128;
   const int keys = L.dp == 64 ? 128 : 256;      // of a dK / dV workgroup
   L.kv_tiles = (p->Sk + keys - 1) / keys;
-  L.kv_splits = 1;
+  L.meta = p->q_docs || (p->prefix && p->prefix_per_query);
   a.chunk = 1 << 30;
   if (bwd) {
-    // few K / V heads and keys: the row tiles are split so that about KV_WGS workgroups of equal work exist (half of all pairs under a causal mask)
-    const long long wgs = (long long)p->nbatch * p->kv_heads * L.kv_tiles, tiles = (long long)((a.M + TILE - 1) / TILE) * (G / a.gp);
-    static const int KV_WGS = getenv("KVW") ? atoi(getenv("KVW")) : 384;
-    const long long work = wgs * tiles / (p->causal && !p->q_docs && p->Sq > 1 ? 2 : 1);
-    if (wgs < 256 && tiles > 4) {
-      long long c = (work + KV_WGS - 1) / KV_WGS;
-      c = c < 4 ? 4 : c;
-      if (tiles > 16 * c) c = (tiles + 15) / 16;
-      a.chunk = (int)(c < tiles ? c : tiles);
-      L.kv_splits = (int)((tiles + a.chunk - 1) / a.chunk);
+    // Few K / V heads and keys: the row tiles are split.  A split costs what about four row tiles do (its prologue, and 256 KB of partial sums
+    // written and read), and one workgroup runs per CU (two at DP = 64): the run length is the one with the least rounds * (length + 4).
+    const long long tiles = (long long)((a.M + TILE - 1) / TILE) * (G / a.gp), heads = (long long)p->nbatch * p->kv_heads;
+    const int slots = L.dp == 64 ? 512 : 256;
+    a.qmeta = L.meta ? (const QMeta*)1 : nullptr;                          // (kv_runs asks whether it is there)
+    // (with documents most tiles are passed over: only very few workgroups are worth a split)
+    if (heads * L.kv_tiles < (L.meta ? slots / 4 : 2 * slots) && tiles > 4 && tiles < (1 << 24)) {
+      double best = 1e30;
+      int chunk = (int)tiles;
+      for (long long c = tiles; c >= 4 && c * 16 >= tiles; c = c > 64 ? c * 15 / 16 : c - 1) {
+        long long wgs = 0;
+        a.chunk = (int)c;
+        for (int k = 0; k < L.kv_tiles; ++k) wgs += kv_runs(a, k, keys, (int)tiles);
+        const double cost = (double)((heads * wgs + slots - 1) / slots) * (double)(c + (c < tiles ? 4 : 0));
+        if (cost < best) {
+          best = cost;
+          chunk = (int)c;
+        }
+      }
+      a.chunk = chunk;
+      L.kv_split = chunk < tiles;
+    }
+    a.wgs = L.kv_tiles;
+    if (L.kv_split) {
+      a.wgs = 0;
+      for (int k = 0; k < L.kv_tiles; ++k) a.wgs += kv_runs(a, k, keys, (int)tiles);
     }
   }
-  L.meta = p->q_docs || (p->prefix && p->prefix_per_query);
   long long at = 0;
   if (L.meta) {
     L.o_qmeta = at;
@@ -1364,13 +1396,13 @@ Layout make_layout(const T2VAttnMod* p, bool bwd) {
   }
   if (!bwd && L.fwd_splits > 1) {
     L.o_part = at;
-    at = align256(at + 4ll * L.fwd_splits * NU * a.M * p->D);
+    at = align256(at + 4ll * L.fwd_splits * NU * L.fwd_tiles * 128 * L.dp);
     L.o_ml = at;
-    at = align256(at + 8ll * L.fwd_splits * NU * a.M);
+    at = align256(at + 8ll * L.fwd_splits * NU * L.fwd_tiles * 128);
   }
-  if (bwd && (L.kv_splits > 1 || p->kv_share > 1)) {
+  if (bwd && (L.kv_split || p->kv_share > 1)) {
     L.o_part = at;
-    at = align256(at + 8ll * L.kv_splits * p->nbatch * p->kv_heads * p->Sk * p->D);
+    at = align256(at + 8ll * p->nbatch * p->kv_heads * a.wgs * keys * L.dp);
   }
   if (bwd && p->dbias) {
     L.o_bias = at;
@@ -1410,11 +1442,18 @@ int launch(int which, K kern, long long grid, size_t smem, hipStream_t st, const
 // bit 0 cap, bit 1 distance bias; a scale that is not positive takes the form that does not fold it into the running maximum
 int mod_bits(const T2VAttnMod* p) { return (p->softcap > 0.f ? 1 : 0) | (p->slopes || p->bias || !(p->scale > 0.f) ? 2 : 0); }
 
+// all workgroups resident, two on some CUs
+int fold(const Layout& L, long long tiles) {
+  const long long wgs = (long long)L.a.p.nbatch * L.a.nunit * tiles;
+  return L.a.p.causal && wgs > 256 && wgs <= 512;
+}
+
 template <typename T, int DP>
 int run_fwd(Layout& L, hipStream_t st) {
   Args& a = L.a;
   a.ntile = L.fwd_tiles;
   a.splits = L.fwd_splits;
+  a.fold = fold(L, L.fwd_tiles * L.fwd_splits);
   const long long grid = (long long)a.p.nbatch * a.nunit * L.fwd_tiles * L.fwd_splits;
   const size_t sm = smem_bytes(L, 1, false);
   const int which = L.fwd_splits > 1 ? 1 : 3;
@@ -1424,9 +1463,8 @@ int run_fwd(Layout& L, hipStream_t st) {
   if (e) return e;
   T2V_CHECK_LAUNCH();
   if (L.fwd_splits > 1) {
-    const int gpb = 256 / (a.p.D / 4);
-    const long long rows = (long long)a.p.nbatch * a.nunit * a.M;
-    T2V_LAUNCH_LAST(attn_mod_join_kernel<T>, dim3((unsigned)((rows + gpb - 1) / gpb)), dim3(256), 0, st, a);
+    const long long blocks = (long long)a.p.nbatch * a.nunit * a.ntile * 4 * (DP / 32);
+    T2V_LAUNCH_LAST((attn_mod_join_kernel<T, DP>), dim3((unsigned)blocks), dim3(64), 0, st, a);
     T2V_CHECK_LAUNCH();
   }
   return T2V_OK;
@@ -1437,6 +1475,7 @@ int run_bwd(Layout& L, hipStream_t st) {
   const int mb = mod_bits(&a.p);
   a.ntile = L.dq_tiles;
   a.splits = 1;
+  a.fold = fold(L, L.dq_tiles);
   const size_t sm = smem_bytes(L, a.p.dbias ? 5 : 1, false);
   const long long gq = (long long)a.p.nbatch * a.nunit * L.dq_tiles;
   int e = mb == 0 ? launch(1, attn_mod_dq_kernel<T, DP, 1, 0>, gq, sm, st, a) : mb == 1 ? launch(1, attn_mod_dq_kernel<T, DP, 1, 1>, gq, sm, st, a) :
@@ -1449,18 +1488,17 @@ int run_bwd(Layout& L, hipStream_t st) {
     T2V_CHECK_LAUNCH();
   }
   a.ntile = L.kv_tiles;
-  a.splits = L.kv_splits;
-  const long long gk = (long long)a.p.nbatch * a.p.kv_heads * L.kv_tiles * L.kv_splits;
+  const long long gk = (long long)a.p.nbatch * a.p.kv_heads * a.wgs;
   const size_t smk = smem_bytes(L, 1, true);
-  a.to_part = L.kv_splits > 1 || a.p.kv_share > 1;
+  a.to_part = L.kv_split || a.p.kv_share > 1;
   const int which = a.to_part ? 0 : 2;
   e = mb == 0 ? launch(which, attn_mod_dkdv_kernel<T, DP, 0>, gk, smk, st, a, DP == 128 ? 512 : 256) : mb == 1 ? launch(which, attn_mod_dkdv_kernel<T, DP, 1>, gk, smk, st, a, DP == 128 ? 512 : 256) :
       mb == 2 ? launch(which, attn_mod_dkdv_kernel<T, DP, 2>, gk, smk, st, a, DP == 128 ? 512 : 256) : launch(which, attn_mod_dkdv_kernel<T, DP, 3>, gk, smk, st, a, DP == 128 ? 512 : 256);
   if (e) return e;
   T2V_CHECK_LAUNCH();
   if (a.to_part) {
-    const long long n = (long long)((a.p.nbatch + a.p.kv_share - 1) / a.p.kv_share) * a.p.kv_heads * a.p.Sk * a.p.D / 4;
-    T2V_LAUNCH_LAST(attn_mod_dkdv_join_kernel<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, a);
+    const long long blocks = (long long)((a.p.nbatch + a.p.kv_share - 1) / a.p.kv_share) * a.p.kv_heads * a.ntile * (DP == 128 ? 8 : 4) * 2 * (DP / 32);
+    T2V_LAUNCH_LAST((attn_mod_dkdv_join_kernel<T, DP>), dim3((unsigned)blocks), dim3(64), 0, st, a);
     T2V_CHECK_LAUNCH();
   }
   return T2V_OK;
@@ -1470,9 +1508,7 @@ int run(const char* fn, const T2VAttnMod* p, bool bwd, hipStream_t st) {
   Layout L = make_layout(p, bwd);
   T2V_CHECK_ARG(L.bytes == 0 || (p->workspace && ((uintptr_t)p->workspace & 255) == 0 && p->workspace_bytes >= L.bytes),
                 "%s: a 256-byte aligned workspace of %lld bytes is wanted (got %p, %lld)", fn, L.bytes, p->workspace, p->workspace_bytes);
-  const long long worst = (long long)p->nbatch * (p->heads > p->kv_heads ? p->heads : p->kv_heads) *
-                          (L.fwd_tiles * (long long)L.fwd_splits > L.kv_tiles * (long long)L.kv_splits ? L.fwd_tiles * (long long)L.fwd_splits
-                                                                                                         : L.kv_tiles * (long long)L.kv_splits);
+  const long long worst = (long long)p->nbatch * p->heads * ((long long)L.fwd_tiles * L.fwd_splits * 4 * (L.dp / 32) + (bwd ? (long long)L.a.wgs * 64 : 0));
   T2V_CHECK_ARG(worst < (1ll << 31), "%s: too many workgroups", fn);
   if (L.meta) {
     const int nq = (L.a.M + TILE - 1) / TILE, nk = (p->Sk + TILE - 1) / TILE;
