@@ -60,7 +60,15 @@ __device__ __forceinline__ bf16x8 pack8(const f32x16& v, int kk) {
 
 // accumulator register r of lane half hi holds row crow(r, hi) of the 32 x 32 tile
 __device__ __forceinline__ constexpr int crow(int r, int hi) { return (r & 3) + 8 * (r >> 2) + 4 * hi; }
-__device__ __forceinline__ float xor32(float v) { return __shfl_xor(v, 32); }
+// maximum / sum of the two halves' values of a lane pair (l, l + 32), in both (v_permlane32_swap: no trip through LDS)
+__device__ __forceinline__ float half_max(float v) {
+  const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+}
+__device__ __forceinline__ float half_sum(float v) {
+  const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(x[0]) + __uint_as_float(x[1]);
+}
 
 struct QMeta {      // of 64 rows: smallest and largest bound, smallest and largest document >= 0, whether some row has none
   int bmin, bmax, dmin, dmax, neg;
@@ -211,13 +219,13 @@ __device__ __forceinline__ void copy16(const void* src, void* lds) {
 // copies, at the first use of what was loaded in front of the loop)
 __device__ __forceinline__ void copies_done() { __builtin_amdgcn_s_waitcnt(0x0f70); }      // vmcnt(0)
 // zero the staged rows for which `dead(row)`: rows that nobody sees may hold inf / NaN, which must not meet a zero weight
-template <int DP, int NT, typename F>
+template <int DP, int NT, bool BOTH, typename F>
 __device__ __forceinline__ void clear_rows(Stage<DP>& st, int tid, F dead) {
   const bf16x8 z = {0, 0, 0, 0, 0, 0, 0, 0};
   for (int i = tid; i < TILE * DP / 8; i += NT) {
     const int row = i / (DP / 8), o = row_off<DP>(row) + (i % (DP / 8)) * 8;
     if (dead(row)) {
-      *(bf16x8*)(st.a + o) = z;
+      if (BOTH) *(bf16x8*)(st.a + o) = z;
       *(bf16x8*)(st.b + o) = z;
     }
   }
@@ -392,7 +400,7 @@ __device__ __forceinline__ void load_rows(Rows<QB>& R, const Args& a, const Unit
 // ------------------------------------------------------------------------------------------------ forward
 // MOD: bit 0 cap, bit 1 distance bias (slopes / table), compile-time so that a tile is straight-line code
 template <typename T, int DP, int QB, int MOD>
-__global__ __launch_bounds__(256, (DP * QB <= 128) ? 2 : 1) void attn_mod_fwd_kernel(const Args a) {
+__global__ __launch_bounds__(256, DP == 64 && MOD < 2 ? 3 : DP * QB <= 128 ? 2 : 1) void attn_mod_fwd_kernel(const Args a) {
   warm_kernargs<(int)sizeof(Args)>();
   constexpr int NT = 256, KD = DP / 16, FM = DP / 32;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -446,31 +454,35 @@ __global__ __launch_bounds__(256, (DP * QB <= 128) ? 2 : 1) void attn_mod_fwd_ke
   const bf16_t* kp = ln.ok ? (const bf16_t*)a.p.k.ptr + op_base(a.p.k, u.b) + (long long)u.kv * D + ln.ch * 8 : (const bf16_t*)zero_chunk;
   const bf16_t* vp = ln.ok ? (const bf16_t*)a.p.v.ptr + op_base(a.p.v, u.b) + (long long)u.kv * D + ln.ch * 8 : (const bf16_t*)zero_chunk;
   const unsigned ks = ln.ok ? (unsigned)a.p.k.sstride : 0u, vs = ln.ok ? (unsigned)a.p.v.sstride : 0u;
+  // Iteration n works on tile n: its scores were formed in iteration n - 1, so that the matrix products of tile n + 1's scores run under the
+  // exponentials of tile n in the same wave.  K is fetched two tiles ahead and V one: stage halves n & 1 hold K(n + 2) and V(n).
   int nd = 0;
-  auto fetch = [&](int t, int sidx) {                                   // rows behind the last key repeat it (masked by the bounds)
+  auto fetch_k = [&](int t, int sidx) {                                 // rows behind the last key repeat it (masked by the bounds)
 #pragma unroll
-    for (int i = 0; i < Lane<DP, 4>::NI; ++i) {
-      const unsigned row = (unsigned)min(t * TILE + ln.row_of(i), len - 1);
-      copy16(kp + (unsigned long long)row * ks, st[sidx].a + ln.group(i));
-      copy16(vp + (unsigned long long)row * vs, st[sidx].b + ln.group(i));
-    }
+    for (int i = 0; i < Lane<DP, 4>::NI; ++i)
+      copy16(kp + (unsigned long long)(unsigned)min(t * TILE + ln.row_of(i), len - 1) * ks, st[sidx].a + ln.group(i));
+  };
+  auto fetch_v = [&](int t, int sidx) {
+#pragma unroll
+    for (int i = 0; i < Lane<DP, 4>::NI; ++i)
+      copy16(vp + (unsigned long long)(unsigned)min(t * TILE + ln.row_of(i), len - 1) * vs, st[sidx].b + ln.group(i));
     if (docs && tid < TILE) {
       const int row = t * TILE + tid;
       nd = row < len ? kdoc[row] : -1;
     }
   };
-  auto landed = [&](int sidx, int neg) {                                // the tile fetched into stage sidx is there for all waves
+  auto landed = [&](int sidx, int neg) {                                // what was fetched is there for all waves; V (and documents) in stage sidx
     if (docs && tid < TILE) sdoc[sidx * TILE + tid] = nd;
     copies_done();
     __syncthreads();
-    if (neg) {
-      clear_rows<DP, NT>(st[sidx], tid, [&](int r) { return sdoc[sidx * TILE + r] < 0; });
+    if (neg) {                                                          // (K may hold what it likes there: its scores are masked by selects)
+      clear_rows<DP, NT, false>(st[sidx], tid, [&](int r) { return sdoc[sidx * TILE + r] < 0; });
       __syncthreads();
     }
   };
 
   float m[QB], l[QB];
-  f32x16 o[QB][FM];
+  f32x16 o[QB][FM], s[QB][2];
 #pragma unroll
   for (int q = 0; q < QB; ++q) {
     m[q] = LOWEST;
@@ -480,168 +492,183 @@ __global__ __launch_bounds__(256, (DP * QB <= 128) ? 2 : 1) void attn_mod_fwd_ke
 #pragma unroll
       for (int r = 0; r < 16; ++r) o[q][f][r] = 0.f;
   }
-  int t = tile_next(it, active), cur = 0;
-  KMeta kn = {0, 0, 0};                                                 // of the tile at hand (documents)
-  if (t < tend) {
-    if (docs) kn = uniform(km[t]);
-    fetch(t, 0);
-    landed(0, kn.neg);
-  }
-  auto math = [&](bool partial, int t) {
-    const int k0 = t * TILE;
-    const bf16_t* sk = st[cur].a;
-    const bf16_t* sv = st[cur].b;
-    f32x16 s[QB][2];
+  auto scores = [&](f32x16 (&x)[QB][2], const bf16_t* sk) {             // K Q^T of a tile
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
 #pragma unroll
       for (int q = 0; q < QB; ++q)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[q][kb][r] = 0.f;
-      bf16x8 kf[KD];
+        for (int r = 0; r < 16; ++r) x[q][kb][r] = 0.f;
 #pragma unroll
-      for (int kd = 0; kd < KD; ++kd) kf[kd] = rowfrag<DP>(sk + lrow, kb, kd);
+      for (int kd = 0; kd < KD; ++kd) {
+        const bf16x8 kf = rowfrag<DP>(sk + lrow, kb, kd);
 #pragma unroll
-      for (int kd = 0; kd < KD; ++kd)
-#pragma unroll
-        for (int q = 0; q < QB; ++q) s[q][kb] = El<T>::mfma(kf[kd], qf[q][kd], s[q][kb]);
-    }
-    const float c = MOD ? 1.f : mod.c;
-    bf16x8 pb[QB][4];
-#pragma unroll
-    for (int q = 0; q < QB; ++q) {
-      float off[2] = {0.f, 0.f};                                        // score = s + off[kb]
-      if (MOD & 1) {
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            float w;
-            s[q][kb][r] = capped(mod, s[q][kb][r], w);
-          }
+        for (int q = 0; q < QB; ++q) x[q][kb] = El<T>::mfma(kf, qf[q][kd], x[q][kb]);
       }
-      if (MOD & 2) {
-        const int d0 = k0 + 4 * hi - R.pos[q];
-        const float cc = (MOD & 1) ? 1.f : mod.c;
-        if (mod.slope) {
-          if (k0 + TILE - 1 <= R.pmin) {                                // every key at or before every query: |d| = -d, linear in the row
-            const float sl = R.slope[q];
-            off[0] = sl * (float)d0;
-            off[1] = sl * (float)(d0 + 32);
+    }
+  };
+  int t = tile_next(it, active), t1 = tend, cur = 0;
+  KMeta kn = {0, 0, 0}, k1 = {0, 0, 0};                                 // of the tile at hand and the next (documents)
+  if (t < tend) {
+    t1 = tile_next(it, active);
+    if (docs) kn = uniform(km[t]);
+    fetch_k(t, 0);
+    fetch_v(t, 0);
+    if (t1 < tend) fetch_k(t1, 1);
+    landed(0, kn.neg);
+    scores(s, st[0].a);
+    __syncthreads();                                                    // all waves have read K of stage 0
+  }
+  while (t < tend) {
+    const int t2 = t1 < tend ? tile_next(it, active) : tend;
+    if (t2 < tend) fetch_k(t2, cur);
+    if (t1 < tend) {
+      fetch_v(t1, cur ^ 1);
+      if (docs) k1 = uniform(km[t1]);
+    }
+    const int k0 = t * TILE;
+    if (k0 < R.bmax) {                                                  // (tiles rise: a wave that is through stays so)
+      bool part = k0 + TILE > R.bmin;
+      if (docs) part |= (kn.neg != 0) | (kn.dmin != kn.dmax) | (R.dmin != R.dmax) | R.neg | (kn.dmin != R.dmin);
+      const bool partial = __builtin_amdgcn_readfirstlane(part);
+      const bf16_t* sv = st[cur].b;
+      f32x16 n[QB][2];
+      const float c = MOD ? 1.f : mod.c;
+      float off[QB][2];                                                 // score = s + off[kb]
+      if (MOD & 1) {                                                    // the cap's exponentials run beside the next tile's scores
+        scores(n, st[cur ^ 1].a);
+#pragma unroll
+        for (int q = 0; q < QB; ++q)
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-              const float b = sl * (float)crow(r, 0);
-              s[q][0][r] = fmaf(s[q][0][r], cc, b);
-              s[q][1][r] = fmaf(s[q][1][r], cc, b);
+              float w;
+              s[q][kb][r] = capped(mod, s[q][kb][r], w);
             }
-          } else {
-            const float f0 = (float)d0;
+      }
+#pragma unroll
+      for (int q = 0; q < QB; ++q) {
+        off[q][0] = off[q][1] = 0.f;
+        if (MOD & 2) {
+          const int d0 = k0 + 4 * hi - R.pos[q];
+          const float cc = (MOD & 1) ? 1.f : mod.c;
+          if (mod.slope) {
+            if (k0 + TILE - 1 <= R.pmin) {                              // every key at or before every query: |d| = -d, linear in the row
+              const float sl = R.slope[q];
+              off[q][0] = sl * (float)d0;
+              off[q][1] = sl * (float)(d0 + 32);
+#pragma unroll
+              for (int r = 0; r < 16; ++r) {
+                const float b = sl * (float)crow(r, 0);
+                s[q][0][r] = fmaf(s[q][0][r], cc, b);
+                s[q][1][r] = fmaf(s[q][1][r], cc, b);
+              }
+            } else {
+              const float f0 = (float)d0;
+#pragma unroll
+              for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                  s[q][kb][r] = fmaf(-R.slope[q], fabsf(f0 + (32 * kb + crow(r, 0))), s[q][kb][r] * cc);
+            }
+          } else if (!(MOD & 1)) {
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-              for (int r = 0; r < 16; ++r)
-                s[q][kb][r] = fmaf(-R.slope[q], fabsf(f0 + (32 * kb + crow(r, 0))), s[q][kb][r] * cc);
+              for (int r = 0; r < 16; ++r) s[q][kb][r] *= cc;
           }
-        } else if (!(MOD & 1)) {
+          if (mod.table) {
 #pragma unroll
-          for (int kb = 0; kb < 2; ++kb)
+            for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[q][kb][r] *= cc;
+              for (int r = 0; r < 16; ++r) s[q][kb][r] += tab[max(-mod.R, min(mod.R, d0 + 32 * kb + crow(r, 0))) + mod.R];
+          }
         }
-        if (mod.table) {
+        if (partial) {
 #pragma unroll
-          for (int kb = 0; kb < 2; ++kb)
+          for (int kb = 0; kb < 2; ++kb) {
+            const int lim = R.bound[q] - k0 - 32 * kb - 4 * hi;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[q][kb][r] += tab[max(-mod.R, min(mod.R, d0 + 32 * kb + crow(r, 0))) + mod.R];
-        }
-      }
-      if (partial) {
+            for (int r = 0; r < 16; ++r) s[q][kb][r] = crow(r, 0) < lim ? s[q][kb][r] : -INFINITY;
+            if (docs) {
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-          const int lim = R.bound[q] - k0 - 32 * kb - 4 * hi;
-#pragma unroll
-          for (int r = 0; r < 16; ++r) s[q][kb][r] = crow(r, 0) < lim ? s[q][kb][r] : -INFINITY;
-          if (docs) {
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-              const int4 dv = *(const int4*)(sdoc + cur * TILE + 32 * kb + 8 * g + 4 * hi);
-              s[q][kb][4 * g] = dv.x == R.doc[q] ? s[q][kb][4 * g] : -INFINITY;
-              s[q][kb][4 * g + 1] = dv.y == R.doc[q] ? s[q][kb][4 * g + 1] : -INFINITY;
-              s[q][kb][4 * g + 2] = dv.z == R.doc[q] ? s[q][kb][4 * g + 2] : -INFINITY;
-              s[q][kb][4 * g + 3] = dv.w == R.doc[q] ? s[q][kb][4 * g + 3] : -INFINITY;
+              for (int g = 0; g < 4; ++g) {
+                const int4 dv = *(const int4*)(sdoc + cur * TILE + 32 * kb + 8 * g + 4 * hi);
+                s[q][kb][4 * g] = dv.x == R.doc[q] ? s[q][kb][4 * g] : -INFINITY;
+                s[q][kb][4 * g + 1] = dv.y == R.doc[q] ? s[q][kb][4 * g + 1] : -INFINITY;
+                s[q][kb][4 * g + 2] = dv.z == R.doc[q] ? s[q][kb][4 * g + 2] : -INFINITY;
+                s[q][kb][4 * g + 3] = dv.w == R.doc[q] ? s[q][kb][4 * g + 3] : -INFINITY;
+              }
             }
           }
         }
-      }
-      float mx0 = s[q][0][0], mx1 = s[q][1][0];
+        float mx0 = s[q][0][0], mx1 = s[q][1][0];
 #pragma unroll
-      for (int r = 1; r < 16; ++r) {
-        mx0 = fmaxf(mx0, s[q][0][r]);
-        mx1 = fmaxf(mx1, s[q][1][r]);
-      }
-      float mx = fmaxf(mx0 + off[0], mx1 + off[1]);
-      mx = fmaxf(mx, xor32(mx));
-      // the running maximum is raised only when some row of the wave grew by more than DEFER exponent units: p <= 2^DEFER instead of
-      // <= 1, the same relative precision, and the common tile skips the rescale of O
-      constexpr float DEFER = 6.f;
-      if (!__all((mx - m[q]) * c <= DEFER)) {
-        const float mn = fmaxf(m[q], mx);
-        const float alpha = __builtin_amdgcn_exp2f((m[q] - mn) * c);
-        m[q] = mn;
-        l[q] *= alpha;
-#pragma unroll
-        for (int f = 0; f < FM; ++f)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) o[q][f][r] *= alpha;
-      }
-      float rs[2] = {0.f, 0.f};
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb) {
-        const float mc = MOD ? m[q] - off[kb] : m[q] * c;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const float pv = __builtin_amdgcn_exp2f(MOD ? s[q][kb][r] - mc : fmaf(s[q][kb][r], c, -mc));
-          s[q][kb][r] = pv;
-          rs[r & 1] += pv;
+        for (int r = 1; r < 16; ++r) {
+          mx0 = fmaxf(mx0, s[q][0][r]);
+          mx1 = fmaxf(mx1, s[q][1][r]);
         }
-        pb[q][2 * kb] = pack8<T>(s[q][kb], 0);
-        pb[q][2 * kb + 1] = pack8<T>(s[q][kb], 1);
+        const float mx = half_max(fmaxf(mx0 + off[q][0], mx1 + off[q][1]));
+        // the running maximum is raised only when some row of the wave grew by more than DEFER exponent units: p <= 2^DEFER instead of
+        // <= 1, the same relative precision, and the common tile skips the rescale of O
+        constexpr float DEFER = 6.f;
+        if (!__all((mx - m[q]) * c <= DEFER)) {
+          const float mn = fmaxf(m[q], mx);
+          const float alpha = __builtin_amdgcn_exp2f((m[q] - mn) * c);
+          m[q] = mn;
+          l[q] *= alpha;
+#pragma unroll
+          for (int f = 0; f < FM; ++f)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[q][f][r] *= alpha;
+        }
       }
-      l[q] += rs[0] + rs[1];
-    }
+      // one straight block: the next tile's scores, this tile's exponentials, P V  (behind the last tile the scores are of stale rows, unused)
+      if (!(MOD & 1)) scores(n, st[cur ^ 1].a);
+      bf16x8 pb[QB][4];
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
+      for (int q = 0; q < QB; ++q) {
+        float rs[2] = {0.f, 0.f};
 #pragma unroll
-      for (int kk = 0; kk < 2; ++kk) {
-        bf16x8 vf[FM];
+        for (int kb = 0; kb < 2; ++kb) {
+          const float mc = MOD ? m[q] - off[q][kb] : m[q] * c;
 #pragma unroll
-        for (int f = 0; f < FM; ++f) vf[f] = trfrag<DP>(sv + ltr, kb, f, kk);
-#pragma unroll
-        for (int f = 0; f < FM; ++f)
-#pragma unroll
-          for (int q = 0; q < QB; ++q) o[q][f] = El<T>::mfma(vf[f], pb[q][2 * kb + kk], o[q][f]);
+          for (int r = 0; r < 16; ++r) {
+            const float pv = __builtin_amdgcn_exp2f(MOD ? s[q][kb][r] - mc : fmaf(s[q][kb][r], c, -mc));
+            s[q][kb][r] = pv;
+            rs[r & 1] += pv;
+          }
+          pb[q][2 * kb] = pack8<T>(s[q][kb], 0);
+          pb[q][2 * kb + 1] = pack8<T>(s[q][kb], 1);
+        }
+        l[q] += rs[0] + rs[1];
       }
-  };
-  while (t < tend) {
-    const int tn = tile_next(it, active);
-    const KMeta kt = kn;
-    if (tn < tend) {
-      fetch(tn, cur ^ 1);
-      if (docs) kn = uniform(km[tn]);
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+          for (int f = 0; f < FM; ++f) {
+            const bf16x8 vf = trfrag<DP>(sv + ltr, kb, f, kk);
+#pragma unroll
+            for (int q = 0; q < QB; ++q) o[q][f] = El<T>::mfma(vf, pb[q][2 * kb + kk], o[q][f]);
+          }
+#pragma unroll
+      for (int q = 0; q < QB; ++q) {
+        s[q][0] = n[q][0];
+        s[q][1] = n[q][1];
+      }
     }
-    const int k0 = t * TILE;
-    if (k0 < R.bmax) {
-      bool partial = k0 + TILE > R.bmin;
-      if (docs) partial |= (kt.neg != 0) | (kt.dmin != kt.dmax) | (R.dmin != R.dmax) | R.neg | (kt.dmin != R.dmin);
-      math(__builtin_amdgcn_readfirstlane(partial), t);
-    }
-    if (tn < tend) landed(cur ^ 1, docs ? kn.neg : 0);
+    if (t1 < tend) landed(cur ^ 1, docs ? k1.neg : 0);
     cur ^= 1;
-    t = tn;
+    t = t1;
+    t1 = t2;
+    kn = k1;
   }
 #pragma unroll
   for (int q = 0; q < QB; ++q) {
-    const float lt = l[q] + xor32(l[q]);
+    const float lt = half_sum(l[q]);
     const float m2 = MOD ? m[q] : m[q] * mod.c;
     if (a.splits > 1) {
       const long long block = (((long long)sp * NU + u.x) * a.ntile + tile) * 4 * QB + wave * QB + q;       // of 32 rows
@@ -770,7 +797,7 @@ __global__ __launch_bounds__(256, (DP * QB <= 128) ? 2 : 1) void attn_mod_dq_ker
 #pragma unroll
       for (int e = 0; e < 8; ++e) d = fmaf(El<T>::up(of[e]), El<T>::up(gf[q][kd][e]), d);
     }
-    d += xor32(d);
+    d = half_sum(d);
     dl[q] = d;
     const long long sidx = ((long long)u.b * a.p.heads + u.h0) * a.p.Sq + min(R.r[q], a.M - 1);
     lse[q] = R.ok[q] ? a.p.lse[sidx] : INFINITY;
@@ -820,7 +847,7 @@ __global__ __launch_bounds__(256, (DP * QB <= 128) ? 2 : 1) void attn_mod_dq_ker
     copies_done();
     __syncthreads();
     if (neg) {
-      clear_rows<DP, NT>(st[sidx], tid, [&](int r) { return sdoc[sidx * TILE + r] < 0; });
+      clear_rows<DP, NT, true>(st[sidx], tid, [&](int r) { return sdoc[sidx * TILE + r] < 0; });
       __syncthreads();
     }
   };
@@ -1128,7 +1155,7 @@ __global__ __launch_bounds__(DP == 128 ? 512 : 256, 2) void attn_mod_dkdv_kernel
     copies_done();
     __syncthreads();
     if (dead) {
-      clear_rows<DP, NT>(st[sidx], tid, [&](int r) { return __float_as_int(in[3 * TILE + r]) <= 0; });
+      clear_rows<DP, NT, true>(st[sidx], tid, [&](int r) { return __float_as_int(in[3 * TILE + r]) <= 0; });
       __syncthreads();
     }
   };
