@@ -299,7 +299,9 @@ int t2v_attn_bwd(const T2VAttn* p, t2v_stream_t stream);
  * Backward: the descriptor of the forward with d_o, dq, dk, dv, delta (fp32 [nbatch, heads, Sq] scratch) and dbias (NULL or like
  * bias) filled in; every row of dq, dk, dv is written.  kv_share: batches b with the same b / kv_share have one K / V (and one
  * dk / dv, the sum); 1: each has its own.  workspace: t2v_attn_mod_workspace(p, backward) bytes, 256-byte aligned, no
- * initialisation needed, free for other use when the call's kernels have run. */
+ * initialisation needed, free for other use when the call's kernels have run.  meta: t2v_attn_mod_meta_bytes(p) bytes (0 without documents
+ * and prefixes per query), 256-byte aligned: what the call derives from them, tile by tile; a caller that keeps it from the forward call to
+ * the backward call of the SAME masks sets meta_ready there. */
 typedef struct T2VAttnMod {
   int nbatch, heads, kv_heads, Sq, Sk, D, dtype, causal;
   float scale, softcap;
@@ -313,7 +315,9 @@ typedef struct T2VAttnMod {
   T2VAttnOperand d_o, dq, dk, dv;
   float* delta; void* dbias; int kv_share;
   void* workspace; long long workspace_bytes;
+  void* meta; long long meta_bytes; int meta_ready;
 } T2VAttnMod;
+long long t2v_attn_mod_meta_bytes(const T2VAttnMod* p);
 long long t2v_attn_mod_workspace(const T2VAttnMod* p, int backward);
 int t2v_attn_mod_fwd(const T2VAttnMod* p, t2v_stream_t stream);
 int t2v_attn_mod_bwd(const T2VAttnMod* p, t2v_stream_t stream);

@@ -55,6 +55,11 @@ def test_attention_operands_and_workspaces_that_are_refused():
         assert l.t2v_attn_mod_fwd(C.byref(a), None) == -1 and b"operand" in l.t2v_last_error()
     assert l.t2v_attn_mod_bwd(C.byref(_mod()), None) == -1           # no gradients named
     a = _mod(q_docs=256, kv_docs=256)
+    need = l.t2v_attn_mod_meta_bytes(C.byref(a))
+    assert need > 0 and l.t2v_attn_mod_fwd(C.byref(a), None) == -1 and b"meta" in l.t2v_last_error()
+    a.meta, a.meta_bytes = 1 << 20, need - 1
+    assert l.t2v_attn_mod_fwd(C.byref(a), None) == -1
+    a = _mod(nbatch=1, Sq=1, Sk=4096)                                # few rows, many keys: the keys are split
     need = l.t2v_attn_mod_workspace(C.byref(a), 0)
     assert need > 0 and l.t2v_attn_mod_fwd(C.byref(a), None) == -1 and b"workspace" in l.t2v_last_error()
     a.workspace, a.workspace_bytes = 1 << 20, need - 1
@@ -138,12 +143,12 @@ def test_packed_descriptors_have_the_fields_where_the_header_has_them():
     assert T._FWD.size == nv.AttnMod.d_o.offset and T._FWD.size + T._BWD.size == C.sizeof(nv.AttnMod)
     n = iter(range(1, 100))
     nx = lambda k: [next(n) for _ in range(k)]  # noqa: E731
-    a = nv.AttnMod.from_buffer_copy(T._FWD.pack(*nx(8), *nx(2), *nx(20), *nx(10)) + T._BWD.pack(*nx(20), *nx(5)))
+    a = nv.AttnMod.from_buffer_copy(T._FWD.pack(*nx(8), *nx(2), *nx(20), *nx(10)) + T._BWD.pack(*nx(20), *nx(8)))
     flat = []
     for name, _ in nv.AttnMod._fields_:
         v = getattr(a, name)
         flat += [getattr(v, f) for f, _ in nv.AttnOperand._fields_] if isinstance(v, nv.AttnOperand) else [v]
-    assert flat == list(range(1, 66))
+    assert flat == list(range(1, 69))
     assert T._SIDES.size == nv.QkRope.D.offset and nv.QkRope.pos.offset + T._WHERE.size == nv.QkRope.naxes.offset
     d = T._rope_desc(T.RopeAxes((16, 24), theta=7.0, style="half", shared=True, scale=(2.0, 3.0)), 64, torch.float16, "layer", 0.5, 11,
                      torch.zeros(11, 2, dtype=torch.int64), torch.zeros(20, dtype=torch.float64), torch.device("cpu"), (3, 4), ((5, 6), (7, 8)),

@@ -76,13 +76,15 @@ struct QMeta {      // of 64 rows: smallest and largest bound, smallest and larg
 struct KMeta {
   int dmin, dmax, neg;
 };
-// (what the compiler cannot see to be the same in all lanes it keeps in vector registers and branches on with exec masks)
-__device__ __forceinline__ QMeta uniform(const QMeta& m) {
-  return QMeta{__builtin_amdgcn_readfirstlane(m.bmin), __builtin_amdgcn_readfirstlane(m.bmax), __builtin_amdgcn_readfirstlane(m.dmin),
-               __builtin_amdgcn_readfirstlane(m.dmax), __builtin_amdgcn_readfirstlane(m.neg)};
-}
-__device__ __forceinline__ KMeta uniform(const KMeta& m) {
-  return KMeta{__builtin_amdgcn_readfirstlane(m.dmin), __builtin_amdgcn_readfirstlane(m.dmax), __builtin_amdgcn_readfirstlane(m.neg)};
+// A tile's entry through the scalar cache: the index is the same in all lanes, and a vector load that is waited for would wait for the next
+// tile's copies too, which were issued in front of it (the counter is in order)
+template <typename M>
+__device__ __forceinline__ M tile_entry(const M* table, int t) {
+  const __attribute__((address_space(4))) int* p = (const __attribute__((address_space(4))) int*)(table + __builtin_amdgcn_readfirstlane(t));
+  M m;
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(M) / 4); ++i) ((int*)&m)[i] = p[i];
+  return m;
 }
 
 struct Args {
@@ -123,11 +125,10 @@ __device__ __forceinline__ Seq load_seq(const Args& a, int b) {
   return s;
 }
 // keys [0, bound) are candidates of query i
-__device__ __forceinline__ int row_bound(const Seq& s, int i) {
-  if (!s.causal) return s.len;
-  const int pf = s.per_query ? s.per_query[i] : s.prefix;
-  return max(0, min(max(i + s.off + 1, pf), s.len));
+__device__ __forceinline__ int bound_of(const Seq& s, int i, int prefix) {
+  return s.causal ? max(0, min(max(i + s.off + 1, prefix), s.len)) : s.len;
 }
+__device__ __forceinline__ int row_bound(const Seq& s, int i) { return bound_of(s, i, s.per_query ? s.per_query[i] : s.prefix); }
 
 // the first of a unit's row tiles that may see key wk0 or a later one (0 where the meta table tells it tile by tile)
 __device__ __forceinline__ int first_tile(const Args& a, const Seq& s, int wk0) {
@@ -466,13 +467,10 @@ __global__ __launch_bounds__(256, DP == 64 && MOD < 2 ? 3 : DP * QB <= 128 ? 2 :
 #pragma unroll
     for (int i = 0; i < Lane<DP, 4>::NI; ++i)
       copy16(vp + (unsigned long long)(unsigned)min(t * TILE + ln.row_of(i), len - 1) * vs, st[sidx].b + ln.group(i));
-    if (docs && tid < TILE) {
-      const int row = t * TILE + tid;
-      nd = row < len ? kdoc[row] : -1;
-    }
+    if (docs && tid < TILE) nd = kdoc[min(t * TILE + tid, len - 1)];
   };
-  auto landed = [&](int sidx, int neg) {                                // what was fetched is there for all waves; V (and documents) in stage sidx
-    if (docs && tid < TILE) sdoc[sidx * TILE + tid] = nd;
+  auto landed = [&](int t, int sidx, int neg) {                         // what was fetched is there for all waves; V (and documents) in stage sidx
+    if (docs && tid < TILE) sdoc[sidx * TILE + tid] = t * TILE + tid < len ? nd : -1;
     copies_done();
     __syncthreads();
     if (neg) {                                                          // (K may hold what it likes there: its scores are masked by selects)
@@ -511,11 +509,11 @@ __global__ __launch_bounds__(256, DP == 64 && MOD < 2 ? 3 : DP * QB <= 128 ? 2 :
   KMeta kn = {0, 0, 0}, k1 = {0, 0, 0};                                 // of the tile at hand and the next (documents)
   if (t < tend) {
     t1 = tile_next(it, active);
-    if (docs) kn = uniform(km[t]);
+    if (docs) kn = tile_entry(km, t);
     fetch_k(t, 0);
     fetch_v(t, 0);
     if (t1 < tend) fetch_k(t1, 1);
-    landed(0, kn.neg);
+    landed(t, 0, kn.neg);
     scores(s, st[0].a);
     __syncthreads();                                                    // all waves have read K of stage 0
   }
@@ -524,7 +522,7 @@ __global__ __launch_bounds__(256, DP == 64 && MOD < 2 ? 3 : DP * QB <= 128 ? 2 :
     if (t2 < tend) fetch_k(t2, cur);
     if (t1 < tend) {
       fetch_v(t1, cur ^ 1);
-      if (docs) k1 = uniform(km[t1]);
+      if (docs) k1 = tile_entry(km, t1);
     }
     const int k0 = t * TILE;
     if (k0 < R.bmax) {                                                  // (tiles rise: a wave that is through stays so)
@@ -660,7 +658,7 @@ __global__ __launch_bounds__(256, DP == 64 && MOD < 2 ? 3 : DP * QB <= 128 ? 2 :
         s[q][1] = n[q][1];
       }
     }
-    if (t1 < tend) landed(cur ^ 1, docs ? k1.neg : 0);
+    if (t1 < tend) landed(t1, cur ^ 1, docs ? k1.neg : 0);
     cur ^= 1;
     t = t1;
     t1 = t2;
@@ -756,6 +754,54 @@ __global__ __launch_bounds__(64) void attn_mod_meta_kernel(const Args a, QMeta* 
   }
 }
 
+// With documents the work of a row tile (and of a key tile) depends on them, and with about as many workgroups as the card holds at once the
+// launch takes as long as the CU with the longest ones: (batch, tile) pairs are sorted by the tiles they will visit, the longest first, and
+// equal ones stay in order.  Block 0: row tiles of 128; block 1: key tiles.  One wave counts one pair, then a bitonic sort in LDS.
+constexpr int ORDER_MAX = 1024;
+__global__ __launch_bounds__(1024) void attn_mod_order_kernel(const Args a, int* qorder, int* korder, int nq, int nk, int keys) {
+  __shared__ unsigned long long key[ORDER_MAX];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, side = blockIdx.x;
+  const int ntile = side ? nk : nq, n = a.p.nbatch * ntile, per = side ? keys / TILE : 2;
+  const int nqt = (a.M + TILE - 1) / TILE, nkt = (a.p.Sk + TILE - 1) / TILE;
+  int P = 1;
+  while (P < n) P *= 2;
+  for (int i = tid; i < P; i += 1024) key[i] = 0;
+  __syncthreads();
+  for (int e = wave; e < n; e += 16) {
+    const int b = e / ntile, t = e - b * ntile;
+    const QMeta* qm = a.qmeta + (long long)b * nqt;
+    const KMeta* km = a.kmeta + (long long)b * nkt;
+    int lo = 0x7fffffff, hi = -1, bmax = 0, count = 0;
+    for (int i = t * per; i < min((t + 1) * per, side ? nkt : nqt); ++i) {
+      lo = min(lo, side ? km[i].dmin : qm[i].dmin);
+      hi = max(hi, side ? km[i].dmax : qm[i].dmax);
+      if (!side) bmax = max(bmax, qm[i].bmax);
+    }
+    const int end = side ? nqt : (bmax + TILE - 1) / TILE;
+    for (int c0 = 0; c0 < end; c0 += 64) {
+      const int c = min(c0 + lane, end - 1);
+      const bool on = side ? (qm[c].bmax > t * keys && qm[c].dmax >= lo && qm[c].dmin <= hi) : (km[c].dmax >= lo && km[c].dmin <= hi);
+      count += __popcll(__ballot(on && c0 + lane < end));
+    }
+    if (lane == 0) key[e] = ((unsigned long long)(count + 1) << 32) | (unsigned)(~e);
+  }
+  __syncthreads();
+  for (int k = 2; k <= P; k *= 2)
+    for (int j = k / 2; j > 0; j /= 2) {
+      const int i = tid, l = i ^ j;
+      if (i < P && l > i) {
+        const unsigned long long x = key[i], y = key[l];
+        if ((x < y) == ((i & k) == 0)) {
+          key[i] = y;
+          key[l] = x;
+        }
+      }
+      __syncthreads();
+    }
+  int* out = side ? korder : qorder;
+  for (int i = tid; i < n; i += 1024) out[i] = (int)~(unsigned)key[i];
+}
+
 // ------------------------------------------------------------------------------------------------ backward: dQ, delta, table gradient
 template <typename T, int DP, int QB, int MOD>
 __global__ __launch_bounds__(256, (DP * QB <= 128) ? 2 : 1) void attn_mod_dq_kernel(const Args a) {
@@ -837,13 +883,10 @@ __global__ __launch_bounds__(256, (DP * QB <= 128) ? 2 : 1) void attn_mod_dq_ker
       copy16(kp + (unsigned long long)row * ks, st[sidx].a + ln.group(i));
       copy16(vp + (unsigned long long)row * vs, st[sidx].b + ln.group(i));
     }
-    if (docs && tid < TILE) {
-      const int row = t * TILE + tid;
-      nd = row < len ? kdoc[row] : -1;
-    }
+    if (docs && tid < TILE) nd = kdoc[min(t * TILE + tid, len - 1)];
   };
-  auto landed = [&](int sidx, int neg) {                                // the tile fetched into stage sidx is there for all waves
-    if (docs && tid < TILE) sdoc[sidx * TILE + tid] = nd;
+  auto landed = [&](int t, int sidx, int neg) {                         // tile t, fetched into stage sidx, is there for all waves
+    if (docs && tid < TILE) sdoc[sidx * TILE + tid] = t * TILE + tid < len ? nd : -1;
     copies_done();
     __syncthreads();
     if (neg) {
@@ -862,9 +905,9 @@ __global__ __launch_bounds__(256, (DP * QB <= 128) ? 2 : 1) void attn_mod_dq_ker
   int t = tile_next(it, active), cur = 0;
   KMeta kn = {0, 0, 0};                                                 // of the tile at hand (documents)
   if (t < tend) {
-    if (docs) kn = uniform(km[t]);
+    if (docs) kn = tile_entry(km, t);
     fetch(t, 0);
-    landed(0, kn.neg);
+    landed(t, 0, kn.neg);
   }
   auto math = [&](bool partial, int t) {
     const int k0 = t * TILE;
@@ -973,7 +1016,7 @@ __global__ __launch_bounds__(256, (DP * QB <= 128) ? 2 : 1) void attn_mod_dq_ker
     const KMeta kt = kn;
     if (tn < tend) {
       fetch(tn, cur ^ 1);
-      if (docs) kn = uniform(km[tn]);
+      if (docs) kn = tile_entry(km, tn);
     }
     const int k0 = t * TILE;
     if (k0 < R.bmax) {
@@ -981,7 +1024,7 @@ __global__ __launch_bounds__(256, (DP * QB <= 128) ? 2 : 1) void attn_mod_dq_ker
       if (docs) partial |= (kt.neg != 0) | (kt.dmin != kt.dmax) | (R.dmin != R.dmax) | R.neg | (kt.dmin != R.dmin);
       math(__builtin_amdgcn_readfirstlane(partial), t);
     }
-    if (tn < tend) landed(cur ^ 1, docs ? kn.neg : 0);
+    if (tn < tend) landed(tn, cur ^ 1, docs ? kn.neg : 0);
     cur ^= 1;
     t = tn;
   }
@@ -1019,9 +1062,9 @@ __global__ __launch_bounds__(256) void attn_mod_dbias_kernel(const Args a) {
 }
 
 // ------------------------------------------------------------------------------------------------ backward: dK, dV
-struct RowInfo {                    // of one staged query row
+struct RowInfo {                    // of one query row, as loaded
   float lse, delta, slope;
-  int bound, pos, doc;
+  int doc, prefix;
 };
 // A wave owns 32 keys and streams the rows that see them.  K, V, dK and dV of 32 keys of 128 columns are 192 registers: with the score and
 // gradient tiles a wave would need more than half of a SIMD's file, and one wave per SIMD has nothing to run under its exponentials
@@ -1108,8 +1151,8 @@ __global__ __launch_bounds__(DP == 128 ? 512 : 256, 2) void attn_mod_dkdv_kernel
   const int first = first_tile(a, seq, wk0), run = ntr - first, total = wk0 < len ? run * GU : 0;
   const int per = (total + runs - 1) / runs, tbeg = min(total, sp * per), tend = min(total, tbeg + per);
   auto tile_meta = [&](int t) {
-    if (qm) return uniform(qm[t]);
-    return uniform(QMeta{t * TILE + TILE > a.M ? 0 : row_bound(seq, div_gp(a, t * TILE)), row_bound(seq, div_gp(a, min(a.M, t * TILE + TILE) - 1)), 0, 0, 0});
+    if (qm) return tile_entry(qm, t);
+    return QMeta{t * TILE + TILE > a.M ? 0 : row_bound(seq, div_gp(a, t * TILE)), row_bound(seq, div_gp(a, min(a.M, t * TILE + TILE) - 1)), 0, 0, 0};
   };
   auto active = [&](int c) {
     const QMeta m = qm[c % ntr];
@@ -1120,7 +1163,7 @@ __global__ __launch_bounds__(DP == 128 ? 512 : 256, 2) void attn_mod_dkdv_kernel
   const bf16_t* qp = ln.ok ? Q + ln.ch * 8 : (const bf16_t*)zero_chunk;
   const bf16_t* gp = ln.ok ? dO + ln.ch * 8 : (const bf16_t*)zero_chunk;
   const unsigned qs = ln.ok ? (unsigned)a.p.q.sstride : 0u, gs = ln.ok ? (unsigned)a.p.d_o.sstride : 0u, hs = ln.ok ? (unsigned)D : 0u;
-  RowInfo ni;
+  RowInfo ni = {0.f, 0.f, 0.f, 0, 0};
   auto fetch = [&](int c, int sidx) {                                   // rows behind the last repeat it (their weights are masked to 0)
     const int gu = c / run, t = first + c - gu * run, h0 = kv * G + gu * a.gp;
 #pragma unroll
@@ -1130,26 +1173,26 @@ __global__ __launch_bounds__(DP == 128 ? 512 : 256, 2) void attn_mod_dkdv_kernel
       copy16(qp + (unsigned long long)(unsigned)i * qs + h, st[sidx].a + ln.group(n));
       copy16(gp + (unsigned long long)(unsigned)i * gs + h, st[sidx].b + ln.group(n));
     }
-    if (tid < TILE) {
-      const int r = t * TILE + tid, rc = min(r, a.M - 1), i = div_gp(a, rc);
-      ni.doc = docs ? a.p.q_docs[(long long)b * a.p.Sq + i] : 0;
-      ni.bound = (r < a.M && ni.doc >= 0) ? row_bound(seq, i) : 0;
-      ni.pos = i + seq.off;
-      ni.slope = (MOD & 2) && a.p.slopes ? a.p.slopes[h0 + rc - i * a.gp] * LOG2E : 0.f;
-      const long long sidx = ((long long)b * a.p.heads + h0) * a.p.Sq + rc;
-      const float l = a.p.lse[sidx], d = a.p.delta[sidx];
-      ni.lse = ni.bound > 0 ? l : INFINITY;
-      ni.delta = ni.bound > 0 ? d : 0.f;
+    if (tid < TILE) {                                                   // (raw values only: what is computed from them waits for them)
+      const int rc = min(t * TILE + tid, a.M - 1), i = div_gp(a, rc);
+      const long long at = ((long long)b * a.p.heads + h0) * a.p.Sq + rc;
+      ni.lse = a.p.lse[at];
+      ni.delta = a.p.delta[at];
+      if (docs) ni.doc = a.p.q_docs[(long long)b * a.p.Sq + i];
+      if ((MOD & 2) && a.p.slopes) ni.slope = a.p.slopes[h0 + rc - i * a.gp];
+      if (seq.per_query) ni.prefix = seq.per_query[i];
     }
   };
-  auto landed = [&](int sidx, bool dead) {
+  auto landed = [&](int c, int sidx, bool dead) {
     float* in = sinfo + sidx * 6 * TILE;
     if (tid < TILE) {
-      in[tid] = ni.lse;
-      in[TILE + tid] = ni.delta;
-      in[2 * TILE + tid] = ni.slope;
-      in[3 * TILE + tid] = __int_as_float(ni.bound);
-      in[4 * TILE + tid] = __int_as_float(ni.pos);
+      const int r = (first + c % run) * TILE + tid, i = div_gp(a, min(r, a.M - 1));
+      const int bound = (r < a.M && ni.doc >= 0) ? bound_of(seq, i, seq.per_query ? ni.prefix : seq.prefix) : 0;
+      in[tid] = bound > 0 ? ni.lse : INFINITY;
+      in[TILE + tid] = bound > 0 ? ni.delta : 0.f;
+      in[2 * TILE + tid] = ni.slope * LOG2E;
+      in[3 * TILE + tid] = __int_as_float(bound);
+      in[4 * TILE + tid] = __int_as_float(i + seq.off);
       in[5 * TILE + tid] = __int_as_float(ni.doc);
     }
     copies_done();
@@ -1164,7 +1207,7 @@ __global__ __launch_bounds__(DP == 128 ? 512 : 256, 2) void attn_mod_dkdv_kernel
   if (c < tend) {
     mn = tile_meta(first + c % run);
     fetch(c, 0);
-    landed(0, mn.bmin <= 0);
+    landed(c, 0, mn.bmin <= 0);
   }
   auto math = [&](bool partial) {
     const bf16_t* sq = st[cur].a;
@@ -1273,7 +1316,7 @@ __global__ __launch_bounds__(DP == 128 ? 512 : 256, 2) void attn_mod_dkdv_kernel
       if (docs) partial |= wneg | (wdmin != wdmax) | (mt.dmin != mt.dmax) | (mt.neg != 0) | (mt.dmin != wdmin);
       math(__builtin_amdgcn_readfirstlane(partial));
     }
-    if (cn < tend) landed(cur ^ 1, mn.bmin <= 0);
+    if (cn < tend) landed(cn, cur ^ 1, mn.bmin <= 0);
     cur ^= 1;
     c = cn;
   }
@@ -1325,7 +1368,8 @@ struct Layout {
   int qb, dp;
   int fwd_tiles, fwd_splits, dq_tiles, kv_tiles;
   bool kv_split, meta;
-  long long o_qmeta, o_kmeta, o_part, o_ml, o_bias, bytes;
+  long long o_qmeta, o_kmeta, o_qorder, o_korder, meta_bytes, o_part, o_ml, o_bias, bytes;
+  bool order;
 };
 
 long long align256(long long n) { return (n + 255) & ~255ll; }
@@ -1420,7 +1464,19 @@ Layout make_layout(const T2VAttnMod* p, bool bwd) {
     at = align256(at + (long long)sizeof(QMeta) * p->nbatch * ((a.M + TILE - 1) / TILE));
     L.o_kmeta = at;
     at = align256(at + (long long)sizeof(KMeta) * p->nbatch * ((p->Sk + TILE - 1) / TILE));
+    // sorted where a launch is a few workgroups per CU (more than a few are dealt out evenly by their number) and sorting is short
+    const int key_tiles = (p->Sk + (L.dp == 64 ? 127 : 255)) / (L.dp == 64 ? 128 : 256);
+    const long long nq = (long long)p->nbatch * L.dq_tiles, nk = (long long)p->nbatch * key_tiles;
+    L.order = p->q_docs && nq <= ORDER_MAX && nk <= ORDER_MAX && nq * a.nunit > 256 && nq * ((p->Sk + 4095) / 4096) <= 2048;
+    if (L.order) {
+      L.o_qorder = at;
+      at = align256(at + 4 * nq);
+      L.o_korder = at;
+      at = align256(at + 4 * nk);
+    }
   }
+  L.meta_bytes = at;
+  at = 0;
   if (!bwd && L.fwd_splits > 1) {
     L.o_part = at;
     at = align256(at + 4ll * L.fwd_splits * NU * L.fwd_tiles * 128 * L.dp);
@@ -1436,11 +1492,12 @@ Layout make_layout(const T2VAttnMod* p, bool bwd) {
     at = align256(at + 4ll * p->nbatch * L.dq_tiles * p->heads * (2 * p->radius + 1));
   }
   L.bytes = at;
-  char* w = (char*)p->workspace;
-  if (L.meta) {
-    a.qmeta = (const QMeta*)(w + L.o_qmeta);
-    a.kmeta = (const KMeta*)(w + L.o_kmeta);
-  }
+  char* w = (char*)p->meta;
+  a.qmeta = L.meta ? (const QMeta*)(w + L.o_qmeta) : nullptr;
+  a.kmeta = L.meta ? (const KMeta*)(w + L.o_kmeta) : nullptr;
+  a.qorder = L.order ? (const int*)(w + L.o_qorder) : nullptr;
+  a.korder = L.order && !L.kv_split ? (const int*)(w + L.o_korder) : nullptr;
+  w = (char*)p->workspace;
   a.part = (float*)(w + L.o_part);
   a.part_ml = (float*)(w + L.o_ml);
   a.part_bias = (float*)(w + L.o_bias);
@@ -1537,11 +1594,21 @@ int run(const char* fn, const T2VAttnMod* p, bool bwd, hipStream_t st) {
                 "%s: a 256-byte aligned workspace of %lld bytes is wanted (got %p, %lld)", fn, L.bytes, p->workspace, p->workspace_bytes);
   const long long worst = (long long)p->nbatch * p->heads * ((long long)L.fwd_tiles * L.fwd_splits * 4 * (L.dp / 32) + (bwd ? (long long)L.a.wgs * 64 : 0));
   T2V_CHECK_ARG(worst < (1ll << 31), "%s: too many workgroups", fn);
-  if (L.meta) {
+  T2V_CHECK_ARG(!L.meta || (p->meta && ((uintptr_t)p->meta & 255) == 0 && p->meta_bytes >= L.meta_bytes),
+                "%s: documents and prefixes per query want a 256-byte aligned meta buffer of %lld bytes (got %p, %lld)", fn, L.meta_bytes, p->meta,
+                p->meta_bytes);
+  if (L.meta && !p->meta_ready) {
     const int nq = (L.a.M + TILE - 1) / TILE, nk = (p->Sk + TILE - 1) / TILE;
     T2V_CHECK_ARG(p->nbatch <= 65535, "%s: at most 65535 batches with documents or one prefix per query", fn);
     hipLaunchKernelGGL(attn_mod_meta_kernel, dim3(nq + nk, p->nbatch), dim3(64), 0, st, L.a, (QMeta*)L.a.qmeta, (KMeta*)L.a.kmeta, nq, nk);
     T2V_CHECK_LAUNCH();
+    if (L.order) {
+      const int keys = L.dp == 64 ? 128 : 256;
+      char* w = (char*)p->meta;
+      hipLaunchKernelGGL(attn_mod_order_kernel, dim3(2), dim3(1024), 0, st, L.a, (int*)(w + L.o_qorder), (int*)(w + L.o_korder), L.dq_tiles,
+                         (p->Sk + keys - 1) / keys, keys);
+      T2V_CHECK_LAUNCH();
+    }
   }
   if (p->dtype == 0) {
     if (L.dp == 64) return bwd ? run_bwd<bf16_t, 64>(L, st) : run_fwd<bf16_t, 64>(L, st);
@@ -1555,6 +1622,10 @@ int run(const char* fn, const T2VAttnMod* p, bool bwd, hipStream_t st) {
 extern "C" long long t2v_attn_mod_workspace(const T2VAttnMod* p, int backward) {
   if (check_mod("t2v_attn_mod_workspace", p, false)) return -1;
   return make_layout(p, backward != 0).bytes;
+}
+extern "C" long long t2v_attn_mod_meta_bytes(const T2VAttnMod* p) {
+  if (check_mod("t2v_attn_mod_meta_bytes", p, false)) return -1;
+  return make_layout(p, false).meta_bytes;
 }
 extern "C" int t2v_attn_mod_fwd(const T2VAttnMod* p, t2v_stream_t stream) { return run("t2v_attn_mod_fwd", p, false, (hipStream_t)stream); }
 extern "C" int t2v_attn_mod_bwd(const T2VAttnMod* p, t2v_stream_t stream) { return run("t2v_attn_mod_bwd", p, true, (hipStream_t)stream); }

@@ -129,6 +129,7 @@ class AttnMod(C.Structure):
         ("q_docs", c_void_p), ("kv_docs", c_void_p), ("slopes", c_void_p), ("bias", c_void_p), ("bias_f32", c_int),
         ("radius", c_int), ("d_o", AttnOperand), ("dq", AttnOperand), ("dk", AttnOperand), ("dv", AttnOperand),
         ("delta", c_void_p), ("dbias", c_void_p), ("kv_share", c_int), ("workspace", c_void_p), ("workspace_bytes", c_ll),
+        ("meta", c_void_p), ("meta_bytes", c_ll), ("meta_ready", c_int),
     ]
 
 
@@ -180,6 +181,7 @@ SYMBOLS = {
     "t2v_qk_rope_bwd_floats": ([C.POINTER(QkRope)], c_ll),
     "t2v_qk_rope_bwd": ([C.POINTER(QkRope), c_void_p], c_int),
     "t2v_attn_mod_workspace": ([C.POINTER(AttnMod), c_int], c_ll),
+    "t2v_attn_mod_meta_bytes": ([C.POINTER(AttnMod)], c_ll),
     "t2v_attn_mod_fwd": ([C.POINTER(AttnMod), c_void_p], c_int),
     "t2v_attn_mod_bwd": ([C.POINTER(AttnMod), c_void_p], c_int),
     "t2v_softmax_rows": ([c_void_p, c_ll, c_void_p, c_ll, c_ll, c_int, c_void_p], c_int),

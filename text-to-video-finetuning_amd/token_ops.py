@@ -302,7 +302,7 @@ def _ints(t, shapes, dev, name):
 # T2VAttnMod field by field, packed in one go (see _SIDES); _FWD ends where the fields of the backward pass begin
 _OP = "Qqqqi4x"
 _FWD = struct.Struct("@8i2f" + 4 * _OP + "QQi4xQQQQQii")
-_BWD = struct.Struct("@" + 4 * _OP + "QQi4xQq")
+_BWD = struct.Struct("@" + 4 * _OP + "QQi4xQqQqi4x")
 _NO_BWD = bytes(_BWD.size)
 
 
@@ -313,7 +313,7 @@ def _attn_desc(q, k, v, o, meta, lse, prefix, kv_len, q_docs, kv_docs, slopes, b
                     *_op(q, qlay), *_op(k, klay), *_op(v, klay), *_op(o, qlay), ptr(lse), ptr(prefix), 0 if prefix is None else prefix.dim() - 1,
                     ptr(kv_len), ptr(q_docs), ptr(kv_docs), ptr(slopes), ptr(bias), 0 if bias is None else bias.dtype == torch.float32,
                     0 if bias is None else bias.shape[1] // 2)
-    return nv.AttnMod.from_buffer_copy(fwd + (_NO_BWD if bwd is None else _BWD.pack(*bwd, 0, 0)))
+    return nv.AttnMod.from_buffer_copy(fwd + (_NO_BWD if bwd is None else _BWD.pack(*bwd, 0, 0, 0, 0, 0)))
 
 
 def _workspace(a, backward, dev):
@@ -327,33 +327,46 @@ def _workspace(a, backward, dev):
     return w
 
 
+def _meta(a, dev):
+    """The buffer for what a call derives from documents and prefixes per query, tile by tile (None where there are none)."""
+    if not a.q_docs and not (a.prefix and a.prefix_per_query):
+        return None
+    n = nv.lib().t2v_attn_mod_meta_bytes(C.byref(a))
+    if n < 0:
+        nv.check(int(n), "t2v_attn_mod_meta_bytes")
+    m = torch.empty(int(n), dtype=torch.uint8, device=dev)
+    a.meta, a.meta_bytes = m.data_ptr(), int(n)
+    return m
+
+
 def _attn_fwd(q, k, v, meta, prefix, kv_len, q_docs, kv_docs, slopes, bias, keep):
     heads, _, qlay, klay = meta[:4]
     dev = q.device
     if qlay.nbatch * qlay.S == 0 or klay.S == 0:        # nothing is asked, or there is nothing to see
         o = torch.zeros(q.shape, dtype=q.dtype, device=dev)
-        return o, (torch.full((qlay.nbatch * heads * qlay.S,), math.inf, device=dev) if keep else None)
+        return o, (torch.full((qlay.nbatch * heads * qlay.S,), math.inf, device=dev) if keep else None), None
     covered = _layout_facts(qlay, q.shape[0])[2]
     o = (torch.empty if covered else torch.zeros)(q.shape, dtype=q.dtype, device=dev)      # rows that no sequence owns: zeros
     lse = torch.empty(qlay.nbatch * heads * qlay.S, dtype=torch.float32, device=dev) if keep else None
     a = _attn_desc(q, k, v, o, meta, lse, prefix, kv_len, q_docs, kv_docs, slopes, bias)
+    tiles = _meta(a, dev)
     work = _workspace(a, 0, dev)      # noqa: F841 (kept until the launch is issued)
     _launch("t2v_attn_mod_fwd", a, dev)
-    return o, lse
+    return o, lse, tiles
 
 
 class _AttentionMod(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, bias, rest):
         meta, prefix, kv_len, q_docs, kv_docs, slopes = rest
-        o, lse = _attn_fwd(q, k, v, meta, prefix, kv_len, q_docs, kv_docs, slopes, bias, True)
+        o, lse, tiles = _attn_fwd(q, k, v, meta, prefix, kv_len, q_docs, kv_docs, slopes, bias, True)
         ctx.meta = meta
-        ctx.save_for_backward(q, k, v, bias, prefix, kv_len, q_docs, kv_docs, slopes, o, lse)
+        ctx.save_for_backward(q, k, v, bias, prefix, kv_len, q_docs, kv_docs, slopes, o, lse, tiles)
         return o
 
     @staticmethod
     def backward(ctx, do):
-        q, k, v, bias, prefix, kv_len, q_docs, kv_docs, slopes, o, lse = ctx.saved_tensors
+        q, k, v, bias, prefix, kv_len, q_docs, kv_docs, slopes, o, lse, tiles = ctx.saved_tensors
         qlay, klay = ctx.meta[2:4]
         dev = q.device
         do = _upstream(do)
@@ -369,6 +382,8 @@ class _AttentionMod(torch.autograd.Function):
             a = _attn_desc(q, k, v, o, ctx.meta, lse, prefix, kv_len, q_docs, kv_docs, slopes, bias,
                            (*_op(do, qlay), *_op(dq, qlay), *_op(dk, klay), *_op(dv, klay), delta.data_ptr(),
                             0 if dbias is None else dbias.data_ptr(), share))
+            if tiles is not None:
+                a.meta, a.meta_bytes, a.meta_ready = tiles.data_ptr(), tiles.numel(), 1
             work = _workspace(a, 1, dev)      # noqa: F841 (kept until the launches are issued)
             _launch("t2v_attn_mod_bwd", a, dev)
         return dq, dk, dv, dbias, None
