@@ -207,6 +207,11 @@ ATTN = {  # B, Sq, Sk, H, KV, D, dtype, options
     "documents, table": (1, 160, 160, 2, 2, 64, BF, dict(docs=((80, 70), 10), bias=8, causal=True)),
     "all at once": (2, 130, 200, 4, 2, 88, BF, dict(docs="shuffled", bias=20, softcap=6.0, slopes=True, causal=True, prefix=[30, 199],
                                                      kv_len=[200, 131])),
+    # enough workgroups for the sorted work lists of packed documents (row tiles * heads above 256), with and without a table
+    "many documents": (2, 2070, 2070, 9, 9, 8, BF, dict(docs=((300, 1, 500, 77, 128, 640, 390), 34), softcap=9.0)),
+    "many documents, table": (1, 2070, 2070, 16, 16, 16, BF, dict(docs=((300, 1, 500, 77, 128, 640, 390), 34), bias=12, causal=True)),
+    "many documents of 128": (1, 1100, 1100, 32, 32, 72, HF, dict(docs=((200, 333, 5, 400), 162))),
+    "many documents shuffled": (2, 1100, 1100, 16, 16, 8, BF, dict(docs="shuffled")),
     "long": (1, 1100, 1100, 2, 1, 64, BF, dict(causal=True, softcap=15.0)),
     "long keys": (1, 5, 4000, 4, 2, 128, BF, dict(causal=True, slopes=True)),
     "few keys, many rows": (1, 1500, 30, 2, 2, 64, BF, {}),

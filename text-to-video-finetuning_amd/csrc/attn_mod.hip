@@ -101,7 +101,7 @@ struct Args {
   const KMeta* kmeta;               // [nbatch][ceil(Sk / 64)] or NULL
   float* part;                      // partial results of the splits
   float* part_ml;
-  float* part_bias;                 // [nbatch * ntile][heads][2R + 1]
+  float* part_bias;                 // [nbatch * ntile (* parts)][heads][2R + 1]
 };
 
 __device__ __forceinline__ long long op_base(const T2VAttnOperand& o, int b) {
@@ -166,15 +166,33 @@ __device__ __forceinline__ Unit unit_of(const Args& a, int x) {
   u.x = x;
   return u;
 }
-// the unit and row tile of workgroup `id` (of one split)
-__device__ __forceinline__ Unit work_of(const Args& a, int id, int& tile) {
+// Which rows (keys) of a tile are a workgroup's own: all of them, or those of its entry (see attn_mod_order_kernel)
+struct Part {
+  int first, part;                  // part 0: documents <= first (and none), 1: documents > first, -1: all
+  bool none;                        // an entry without rows
+  __device__ __forceinline__ bool owns(int doc) const { return part < 0 || (doc > first) == (part == 1); }
+};
+template <typename M>
+__device__ __forceinline__ Part part_of(const M* table, int t, int per, int n, int part) {
+  int lo = 0x7fffffff, hi = -1;
+  for (int i = t * per; i < min((t + 1) * per, n); ++i) {
+    const M m = tile_entry(table, i);
+    lo = min(lo, m.dmin);
+    hi = max(hi, m.dmax);
+  }
+  return Part{lo, part, part == 1 && hi <= lo};
+}
+// the unit, row tile and part of workgroup `id` (of one split)
+__device__ __forceinline__ Unit work_of(const Args& a, int id, int& tile, Part& part) {
   if (a.qorder) {
-    const int e = a.qorder[id / a.nunit], v = id % a.nunit, b = e / a.ntile, gus = a.nunit / a.p.kv_heads;
-    tile = e - b * a.ntile;
+    const int e = a.qorder[id / a.nunit], v = id % a.nunit, b = (e >> 1) / a.ntile, gus = a.nunit / a.p.kv_heads, nqt = (a.M + TILE - 1) / TILE;
+    tile = (e >> 1) - b * a.ntile;
+    part = part_of(a.qmeta + (long long)b * nqt, tile, 2, nqt, e & 1);
     return unit_of(a, (v % gus) * a.p.nbatch * a.p.kv_heads + b * a.p.kv_heads + v / gus);
   }
   const int NU = a.p.nbatch * a.nunit;
   tile = row_tile(a, id / NU);
+  part = Part{0, -1, false};
   return unit_of(a, id % NU);
 }
 
@@ -367,7 +385,7 @@ struct Rows {
   bool neg;
 };
 template <int QB>
-__device__ __forceinline__ void load_rows(Rows<QB>& R, const Args& a, const Unit& u, const Seq& sq, int r0, int lane) {
+__device__ __forceinline__ void load_rows(Rows<QB>& R, const Args& a, const Unit& u, const Seq& sq, const Part& part, int r0, int lane) {
   int lo = 0x7fffffff, hi = 0, dlo = 0x7fffffff, dhi = -1, ng = 0;
 #pragma unroll
   for (int q = 0; q < QB; ++q) {
@@ -376,9 +394,10 @@ __device__ __forceinline__ void load_rows(Rows<QB>& R, const Args& a, const Unit
     const int rc = min(R.r[q], a.M - 1);
     R.i[q] = div_gp(a, rc);
     R.h[q] = u.h0 + rc - R.i[q] * a.gp;
+    R.doc[q] = a.p.q_docs ? a.p.q_docs[(long long)u.b * a.p.Sq + R.i[q]] : 0;
+    R.ok[q] = R.ok[q] && part.owns(R.doc[q]);
     R.bound[q] = R.ok[q] ? row_bound(sq, R.i[q]) : 0;
     R.pos[q] = R.i[q] + sq.off;
-    R.doc[q] = a.p.q_docs ? a.p.q_docs[(long long)u.b * a.p.Sq + R.i[q]] : 0;
     if (R.doc[q] < 0) R.bound[q] = 0;
     R.slope[q] = a.p.slopes ? a.p.slopes[R.h[q]] * LOG2E : 0.f;
     if (R.ok[q]) lo = min(lo, R.bound[q]);
@@ -413,7 +432,9 @@ __global__ __launch_bounds__(256, DP == 64 && MOD < 2 ? 3 : DP * QB <= 128 ? 2 :
   const int NU = a.p.nbatch * a.nunit;
   const int sp = blockIdx.x / NU % a.splits;
   int tile;
-  const Unit u = work_of(a, blockIdx.x / (NU * a.splits) * NU + blockIdx.x % NU, tile);
+  Part part;
+  const Unit u = work_of(a, blockIdx.x / (NU * a.splits) * NU + blockIdx.x % NU, tile, part);
+  if (part.none) return;                                                // workgroup-uniform
   const Seq seq = load_seq(a, u.b);
   const int len = seq.len, D = a.p.D, Sk = a.p.Sk;
   const bf16_t* Q = (const bf16_t*)a.p.q.ptr + op_base(a.p.q, u.b);
@@ -422,7 +443,7 @@ __global__ __launch_bounds__(256, DP == 64 && MOD < 2 ? 3 : DP * QB <= 128 ? 2 :
   const Mod mod = make_mod(a);
 
   Rows<QB> R;
-  load_rows(R, a, u, seq, (tile * 4 + wave) * 32 * QB, lane);
+  load_rows(R, a, u, seq, part, (tile * 4 + wave) * 32 * QB, lane);
   bf16x8 qf[QB][KD];
 #pragma unroll
   for (int q = 0; q < QB; ++q) {
@@ -526,9 +547,9 @@ __global__ __launch_bounds__(256, DP == 64 && MOD < 2 ? 3 : DP * QB <= 128 ? 2 :
     }
     const int k0 = t * TILE;
     if (k0 < R.bmax) {                                                  // (tiles rise: a wave that is through stays so)
-      bool part = k0 + TILE > R.bmin;
-      if (docs) part |= (kn.neg != 0) | (kn.dmin != kn.dmax) | (R.dmin != R.dmax) | R.neg | (kn.dmin != R.dmin);
-      const bool partial = __builtin_amdgcn_readfirstlane(part);
+      bool some = k0 + TILE > R.bmin;
+      if (docs) some |= (kn.neg != 0) | (kn.dmin != kn.dmax) | (R.dmin != R.dmax) | R.neg | (kn.dmin != R.dmin);
+      const bool partial = __builtin_amdgcn_readfirstlane(some);
       const bf16_t* sv = st[cur].b;
       f32x16 n[QB][2];
       const float c = MOD ? 1.f : mod.c;
@@ -755,51 +776,48 @@ __global__ __launch_bounds__(64) void attn_mod_meta_kernel(const Args a, QMeta* 
 }
 
 // With documents the work of a row tile (and of a key tile) depends on them, and with about as many workgroups as the card holds at once the
-// launch takes as long as the CU with the longest ones: (batch, tile) pairs are sorted by the tiles they will visit, the longest first, and
-// equal ones stay in order.  Block 0: row tiles of 128; block 1: key tiles.  One wave counts one pair, then a bitonic sort in LDS.
-constexpr int ORDER_MAX = 1024;
+// launch takes as long as its longest workgroup.  A tile across the border of two documents would visit both: it becomes two entries, one
+// for the rows of its first document (and those of none), one for the others.  Entries (batch, tile, part) are sorted by the tiles they
+// will visit, the longest first; equal ones stay in order, and second parts of tiles with one document come last and end at once.
+// Block 0: row tiles of 128; block 1: key tiles.  One thread counts an entry and its rank among the others.
+// (Nine clips of 273 .. 1804 tokens: see the table of the operators; the two short launches are paid once per mask.)
+constexpr int ORDER_MAX = 1024, ORDER_TILES = 4096;
 __global__ __launch_bounds__(1024) void attn_mod_order_kernel(const Args a, int* qorder, int* korder, int nq, int nk, int keys) {
   __shared__ unsigned long long key[ORDER_MAX];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, side = blockIdx.x;
-  const int ntile = side ? nk : nq, n = a.p.nbatch * ntile, per = side ? keys / TILE : 2;
-  const int nqt = (a.M + TILE - 1) / TILE, nkt = (a.p.Sk + TILE - 1) / TILE;
-  int P = 1;
-  while (P < n) P *= 2;
-  for (int i = tid; i < P; i += 1024) key[i] = 0;
-  __syncthreads();
-  for (int e = wave; e < n; e += 16) {
-    const int b = e / ntile, t = e - b * ntile;
-    const QMeta* qm = a.qmeta + (long long)b * nqt;
-    const KMeta* km = a.kmeta + (long long)b * nkt;
-    int lo = 0x7fffffff, hi = -1, bmax = 0, count = 0;
-    for (int i = t * per; i < min((t + 1) * per, side ? nkt : nqt); ++i) {
-      lo = min(lo, side ? km[i].dmin : qm[i].dmin);
-      hi = max(hi, side ? km[i].dmax : qm[i].dmax);
-      if (!side) bmax = max(bmax, qm[i].bmax);
-    }
-    const int end = side ? nqt : (bmax + TILE - 1) / TILE;
-    for (int c0 = 0; c0 < end; c0 += 64) {
-      const int c = min(c0 + lane, end - 1);
-      const bool on = side ? (qm[c].bmax > t * keys && qm[c].dmax >= lo && qm[c].dmin <= hi) : (km[c].dmax >= lo && km[c].dmin <= hi);
-      count += __popcll(__ballot(on && c0 + lane < end));
-    }
-    if (lane == 0) key[e] = ((unsigned long long)(count + 1) << 32) | (unsigned)(~e);
+  __shared__ int slo[ORDER_TILES], shi[ORDER_TILES], sbound[ORDER_TILES];     // of the other side's 64-row tiles
+  const int tid = threadIdx.x, side = blockIdx.x;
+  const int ntile = side ? nk : nq, n = 2 * a.p.nbatch * ntile, per = side ? keys / TILE : 2;
+  const int nqt = (a.M + TILE - 1) / TILE, nkt = (a.p.Sk + TILE - 1) / TILE, nown = side ? nkt : nqt, nother = side ? nqt : nkt;
+  for (int i = tid; i < a.p.nbatch * nother; i += 1024) {
+    slo[i] = side ? a.qmeta[i].dmin : a.kmeta[i].dmin;
+    shi[i] = side ? a.qmeta[i].dmax : a.kmeta[i].dmax;
+    sbound[i] = side ? a.qmeta[i].bmax : 0x7fffffff;
   }
+  const int e = min(tid, n - 1), part = e & 1, b = (e >> 1) / ntile, t = (e >> 1) - b * ntile;
+  int lo = 0x7fffffff, hi = -1, bmax = 0;
+  for (int i = t * per; i < min((t + 1) * per, nown); ++i) {
+    const long long at = (long long)b * nown + i;
+    lo = min(lo, side ? a.kmeta[at].dmin : a.qmeta[at].dmin);
+    hi = max(hi, side ? a.kmeta[at].dmax : a.qmeta[at].dmax);
+    if (!side) bmax = max(bmax, a.qmeta[at].bmax);
+  }
+  if (part) lo = lo == 0x7fffffff ? lo : lo + 1;
+  else hi = min(lo, hi);
+  const int end = lo > hi ? 0 : side ? nqt : (bmax + TILE - 1) / TILE, floor = side ? t * keys : 0;
   __syncthreads();
-  for (int k = 2; k <= P; k *= 2)
-    for (int j = k / 2; j > 0; j /= 2) {
-      const int i = tid, l = i ^ j;
-      if (i < P && l > i) {
-        const unsigned long long x = key[i], y = key[l];
-        if ((x < y) == ((i & k) == 0)) {
-          key[i] = y;
-          key[l] = x;
-        }
-      }
-      __syncthreads();
-    }
-  int* out = side ? korder : qorder;
-  for (int i = tid; i < n; i += 1024) out[i] = (int)~(unsigned)key[i];
+  int count = 0;
+#pragma unroll 4
+  for (int c = 0; c < end; ++c) {
+    const int i = b * nother + c;
+    count += (sbound[i] > floor) & (shi[i] >= lo) & (slo[i] <= hi);
+  }
+  const unsigned long long mine = ((unsigned long long)(2 * count + 2 - part) << 32) | (unsigned)(~e);
+  if (tid < n) key[tid] = mine;
+  __syncthreads();
+  int rank = 0;
+#pragma unroll 8
+  for (int k = 0; k < n; ++k) rank += key[k] > mine;
+  if (tid < n) (side ? korder : qorder)[rank] = tid;
 }
 
 // ------------------------------------------------------------------------------------------------ backward: dQ, delta, table gradient
@@ -814,7 +832,15 @@ __global__ __launch_bounds__(256, (DP * QB <= 128) ? 2 : 1) void attn_mod_dq_ker
   float* tab = (float*)(swg + 16);                                      // [2R + 1], then [4 waves][2R + 1] sums
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5;
   int tile;
-  const Unit u = work_of(a, blockIdx.x, tile);
+  Part part;
+  const Unit u = work_of(a, blockIdx.x, tile, part);
+  float* dtable = a.part_bias;                                          // of this workgroup (its head's 2R + 1 sums)
+  if (a.p.dbias) dtable += ((((long long)u.b * a.ntile + tile) * (a.qorder ? 2 : 1) + max(part.part, 0)) * a.p.heads + u.h0) * (2 * a.p.radius + 1);
+  if (part.none) {                                                      // workgroup-uniform
+    if (a.p.dbias)
+      for (int i = threadIdx.x; i < 2 * a.p.radius + 1; i += 256) dtable[i] = 0.f;
+    return;
+  }
   const Seq seq = load_seq(a, u.b);
   const int len = seq.len, D = a.p.D, Sk = a.p.Sk;
   const bool docs = a.kmeta && a.p.kv_docs;
@@ -825,7 +851,7 @@ __global__ __launch_bounds__(256, (DP * QB <= 128) ? 2 : 1) void attn_mod_dq_ker
   const bool dtab = (MOD & 2) && mod.table && a.p.dbias != nullptr;
 
   Rows<QB> R;
-  load_rows(R, a, u, seq, (tile * 4 + wave) * 32 * QB, lane);
+  load_rows(R, a, u, seq, part, (tile * 4 + wave) * 32 * QB, lane);
   bf16x8 qf[QB][KD], gf[QB][KD];
   float lse[QB], dl[QB];
 #pragma unroll
@@ -1041,10 +1067,9 @@ __global__ __launch_bounds__(256, (DP * QB <= 128) ? 2 : 1) void attn_mod_dq_ker
       sums[ntab - 1] += above;
     }
     __syncthreads();
-    float* out = a.part_bias + (((long long)u.b * a.ntile + tile) * a.p.heads + u.h0) * ntab;
     for (int i = tid; i < ntab; i += NT) {
       const float* w0 = tab + ntab + i;
-      out[i] = (w0[0] + w0[ntab]) + (w0[2 * ntab] + w0[3 * ntab]);
+      dtable[i] = (w0[0] + w0[ntab]) + (w0[2 * ntab] + w0[3 * ntab]);
     }
   }
 }
@@ -1056,7 +1081,7 @@ __global__ __launch_bounds__(256) void attn_mod_dbias_kernel(const Args a) {
   if (i >= n) return;
   float s = 0.f;
 #pragma unroll 4
-  for (int k = 0; k < a.p.nbatch * a.ntile; ++k) s += a.part_bias[(long long)k * n + i];
+  for (int k = 0; k < a.p.nbatch * a.ntile * (a.qorder ? 2 : 1); ++k) s += a.part_bias[(long long)k * n + i];
   if (a.p.bias_f32) ((float*)a.p.dbias)[i] = s;
   else ((unsigned short*)a.p.dbias)[i] = (unsigned short)(El<T>::pack2(s, 0.f) & 0xffffu);
 }
@@ -1082,12 +1107,15 @@ __global__ __launch_bounds__(DP == 128 ? 512 : 256, 2) void attn_mod_dkdv_kernel
   float* tab = sinfo + 2 * 6 * TILE;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5;
   const int NKV = a.p.nbatch * a.p.kv_heads, G = a.p.heads / a.p.kv_heads, GU = G / a.gp, ntr = (a.M + TILE - 1) / TILE;
+  Part part = {0, -1, false};
   int y = blockIdx.x % NKV, ktile = blockIdx.x / NKV, sp = 0, runs = 1; // early keys are seen by the most rows of a causal mask: first
   const int w = ktile;
   if (a.korder) {
-    const int e = a.korder[blockIdx.x / a.p.kv_heads];
-    ktile = e % a.ntile;
-    y = e / a.ntile * a.p.kv_heads + blockIdx.x % a.p.kv_heads;
+    const int e = a.korder[blockIdx.x / a.p.kv_heads], bt = (e >> 1) / a.ntile, nkt = (a.p.Sk + TILE - 1) / TILE;
+    ktile = (e >> 1) - bt * a.ntile;
+    y = bt * a.p.kv_heads + blockIdx.x % a.p.kv_heads;
+    part = part_of(a.kmeta + (long long)bt * nkt, ktile, KEYS / TILE, nkt, e & 1);
+    if (part.none) return;                                              // workgroup-uniform
   } else if (a.to_part) {
     sp = ktile;
     for (ktile = 0; sp >= (runs = kv_runs(a, ktile, KEYS, ntr * GU)); ++ktile) sp -= runs;
@@ -1104,7 +1132,9 @@ __global__ __launch_bounds__(DP == 128 ? 512 : 256, 2) void attn_mod_dkdv_kernel
   const int key = kw0 + (lane & 31);
   // does the key exist, and may some query see it
   auto key_doc = [&](int j) { return j < len ? (docs ? a.p.kv_docs[(long long)b * Sk + j] : 0) : -1; };
-  const int kd_ = key_doc(key);
+  const int kdoc = key_doc(key);
+  const bool own = key < Sk && part.owns(kdoc);                         // its gradients are written here
+  const int kd_ = own ? kdoc : -1;
   const bool kok = kd_ >= 0;
   const bf16_t* K = (const bf16_t*)a.p.k.ptr + op_base(a.p.k, b) + (long long)kv * D;
   const bf16_t* V = (const bf16_t*)a.p.v.ptr + op_base(a.p.v, b) + (long long)kv * D;
@@ -1130,14 +1160,17 @@ __global__ __launch_bounds__(DP == 128 ? 512 : 256, 2) void attn_mod_dkdv_kernel
   int dlo = kok ? kd_ : 0x7fffffff, dhi = kd_, ng = !kok;
   const int wdmin = wave_min_i(dlo), wdmax = wave_max_i(dhi);
   const bool wneg = wave_max_i(ng) != 0;
-  // over the workgroup's keys
+  // over the workgroup's own keys
   int gdmin = 0x7fffffff, gdmax = -1;
   if (docs) {
     const KMeta* km = a.kmeta + (long long)b * ((Sk + TILE - 1) / TILE);
     for (int t = wk0 / TILE; t < min((Sk + TILE - 1) / TILE, (wk0 + KEYS) / TILE); ++t) {
-      gdmin = min(gdmin, km[t].dmin);
-      gdmax = max(gdmax, km[t].dmax);
+      const KMeta m = tile_entry(km, t);
+      gdmin = min(gdmin, m.dmin);
+      gdmax = max(gdmax, m.dmax);
     }
+    if (part.part == 0) gdmax = min(gdmax, part.first);
+    if (part.part == 1) gdmin = part.first + 1;
   }
   f32x16 ka[FM], va[FM];
 #pragma unroll
@@ -1325,8 +1358,8 @@ __global__ __launch_bounds__(DP == 128 ? 512 : 256, 2) void attn_mod_dkdv_kernel
     store_part<FM>(a.part + block * (64 * DP), ka, lane, true);
     store_part<FM>(a.part + block * (64 * DP) + 32 * DP, va, lane, true);
   } else {
-    store_row<T, FM>((bf16_t*)a.p.dk.ptr + op_base(a.p.dk, b) + (long long)key * a.p.dk.sstride + (long long)kv * D, ka, a.p.scale, hi, D, key < Sk);
-    store_row<T, FM>((bf16_t*)a.p.dv.ptr + op_base(a.p.dv, b) + (long long)key * a.p.dv.sstride + (long long)kv * D, va, 1.f, hi, D, key < Sk);
+    store_row<T, FM>((bf16_t*)a.p.dk.ptr + op_base(a.p.dk, b) + (long long)key * a.p.dk.sstride + (long long)kv * D, ka, a.p.scale, hi, D, own);
+    store_row<T, FM>((bf16_t*)a.p.dv.ptr + op_base(a.p.dv, b) + (long long)key * a.p.dv.sstride + (long long)kv * D, va, 1.f, hi, D, own);
   }
 }
 
@@ -1466,8 +1499,9 @@ Layout make_layout(const T2VAttnMod* p, bool bwd) {
     at = align256(at + (long long)sizeof(KMeta) * p->nbatch * ((p->Sk + TILE - 1) / TILE));
     // sorted where a launch is a few workgroups per CU (more than a few are dealt out evenly by their number) and sorting is short
     const int key_tiles = (p->Sk + (L.dp == 64 ? 127 : 255)) / (L.dp == 64 ? 128 : 256);
-    const long long nq = (long long)p->nbatch * L.dq_tiles, nk = (long long)p->nbatch * key_tiles;
-    L.order = p->q_docs && nq <= ORDER_MAX && nk <= ORDER_MAX && nq * a.nunit > 256 && nq * ((p->Sk + 4095) / 4096) <= 2048;
+    const long long nq = 2ll * p->nbatch * L.dq_tiles, nk = 2ll * p->nbatch * key_tiles;
+    L.order = p->q_docs && nq <= ORDER_MAX && nk <= ORDER_MAX && nq * a.nunit > 512 && (long long)p->nbatch * (a.M + TILE) <= ORDER_TILES * TILE &&
+              (long long)p->nbatch * (p->Sk + TILE) <= ORDER_TILES * TILE;
     if (L.order) {
       L.o_qorder = at;
       at = align256(at + 4 * nq);
@@ -1489,14 +1523,14 @@ Layout make_layout(const T2VAttnMod* p, bool bwd) {
   }
   if (bwd && p->dbias) {
     L.o_bias = at;
-    at = align256(at + 4ll * p->nbatch * L.dq_tiles * p->heads * (2 * p->radius + 1));
+    at = align256(at + 4ll * p->nbatch * L.dq_tiles * (L.order ? 2 : 1) * p->heads * (2 * p->radius + 1));
   }
   L.bytes = at;
   char* w = (char*)p->meta;
   a.qmeta = L.meta ? (const QMeta*)(w + L.o_qmeta) : nullptr;
   a.kmeta = L.meta ? (const KMeta*)(w + L.o_kmeta) : nullptr;
   a.qorder = L.order ? (const int*)(w + L.o_qorder) : nullptr;
-  a.korder = L.order && !L.kv_split ? (const int*)(w + L.o_korder) : nullptr;
+  a.korder = L.order && !L.kv_split && p->kv_share <= 1 ? (const int*)(w + L.o_korder) : nullptr;
   w = (char*)p->workspace;
   a.part = (float*)(w + L.o_part);
   a.part_ml = (float*)(w + L.o_ml);
@@ -1538,7 +1572,7 @@ int run_fwd(Layout& L, hipStream_t st) {
   a.ntile = L.fwd_tiles;
   a.splits = L.fwd_splits;
   a.fold = fold(L, L.fwd_tiles * L.fwd_splits);
-  const long long grid = (long long)a.p.nbatch * a.nunit * L.fwd_tiles * L.fwd_splits;
+  const long long grid = (long long)a.p.nbatch * a.nunit * L.fwd_tiles * L.fwd_splits * (a.qorder ? 2 : 1);
   const size_t sm = smem_bytes(L, 1, false);
   const int which = L.fwd_splits > 1 ? 1 : 3;
   const int mb = mod_bits(&a.p);
@@ -1561,7 +1595,7 @@ int run_bwd(Layout& L, hipStream_t st) {
   a.splits = 1;
   a.fold = fold(L, L.dq_tiles);
   const size_t sm = smem_bytes(L, a.p.dbias ? 5 : 1, false);
-  const long long gq = (long long)a.p.nbatch * a.nunit * L.dq_tiles;
+  const long long gq = (long long)a.p.nbatch * a.nunit * L.dq_tiles * (a.qorder ? 2 : 1);
   int e = mb == 0 ? launch(1, attn_mod_dq_kernel<T, DP, 1, 0>, gq, sm, st, a) : mb == 1 ? launch(1, attn_mod_dq_kernel<T, DP, 1, 1>, gq, sm, st, a) :
           mb == 2 ? launch(1, attn_mod_dq_kernel<T, DP, 1, 2>, gq, sm, st, a) : launch(1, attn_mod_dq_kernel<T, DP, 1, 3>, gq, sm, st, a);
   if (e) return e;
@@ -1572,7 +1606,7 @@ int run_bwd(Layout& L, hipStream_t st) {
     T2V_CHECK_LAUNCH();
   }
   a.ntile = L.kv_tiles;
-  const long long gk = (long long)a.p.nbatch * a.p.kv_heads * a.wgs;
+  const long long gk = (long long)a.p.nbatch * a.p.kv_heads * a.wgs * (a.korder ? 2 : 1);
   const size_t smk = smem_bytes(L, 1, true);
   a.to_part = L.kv_split || a.p.kv_share > 1;
   const int which = a.to_part ? 0 : 2;
