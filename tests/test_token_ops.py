@@ -137,23 +137,41 @@ def test_the_oracle_finds_a_mistake():
     torch.testing.assert_close(good["dbias"][0], B.grad, rtol=1e-9, atol=1e-9)
 
 
-def test_packed_descriptors_have_the_fields_where_the_header_has_them():
+def test_flat_descriptors_have_the_pointers_where_the_header_has_them():
     import t2v_amd.token_ops as T
     nv = _nv()
-    assert T._FWD.size == nv.AttnMod.d_o.offset and T._FWD.size + T._BWD.size == C.sizeof(nv.AttnMod)
-    n = iter(range(1, 100))
-    nx = lambda k: [next(n) for _ in range(k)]  # noqa: E731
-    a = nv.AttnMod.from_buffer_copy(T._FWD.pack(*nx(8), *nx(2), *nx(20), *nx(10)) + T._BWD.pack(*nx(20), *nx(8)))
-    flat = []
-    for name, _ in nv.AttnMod._fields_:
-        v = getattr(a, name)
-        flat += [getattr(v, f) for f, _ in nv.AttnOperand._fields_] if isinstance(v, nv.AttnOperand) else [v]
-    assert flat == list(range(1, 69))
-    assert T._SIDES.size == nv.QkRope.D.offset and nv.QkRope.pos.offset + T._WHERE.size == nv.QkRope.naxes.offset
-    d = T._rope_desc(T.RopeAxes((16, 24), theta=7.0, style="half", shared=True, scale=(2.0, 3.0)), 64, torch.float16, "layer", 0.5, 11,
-                     torch.zeros(11, 2, dtype=torch.int64), torch.zeros(20, dtype=torch.float64), torch.device("cpu"), (3, 4), ((5, 6), (7, 8)),
-                     ((9, 10), (11, 12)), ((13, 14), (15, 16)), (17, 18), (19, 20), (21, 22), (23, 24), 25)
-    assert [list(getattr(d, f)) for f in ("x", "ldx", "dy", "lddy", "y", "ldy", "heads", "w", "b", "dw", "db")] == [
-        [5, 7], [6, 8], [9, 11], [10, 12], [13, 15], [14, 16], [3, 4], [17, 18], [19, 20], [21, 22], [23, 24]]
-    assert (d.workspace, d.rows, d.D, d.dtype, d.norm, d.eps, d.ldpos, d.pos_type, d.naxes, list(d.dims), list(d.scale), d.theta, d.shared, d.style) == \
-        (25, 11, 64, 1, 2, 0.5, 2, 1, 2, [16, 24, 0, 0], [2.0, 3.0, 0.0, 0.0], 7.0, 1, 1) and d.pos and d.freqs
+    d = T._AttnFlat()
+    for n, name in enumerate(("q", "k", "v", "o", "lse", "prefix", "kv_len", "q_docs", "kv_docs", "slopes", "bias", "d_o", "dq", "dk", "dv", "delta",
+                              "dbias", "workspace", "meta")):
+        setattr(d, name, 100 + n)
+    a = nv.AttnMod.from_buffer_copy(d)
+    got = [getattr(a, n).ptr if k is nv.AttnOperand else getattr(a, n) for n, k in nv.AttnMod._fields_]
+    assert [v for v in got if v and v >= 100] == list(range(100, 119))
+    d = T._RopeFlat()
+    for n, name in enumerate(("x", "ldx", "dy", "lddy", "y", "ldy", "heads", "w", "b", "dw", "db")):
+        setattr(d, name + "0", 10 + 2 * n)
+        setattr(d, name + "1", 11 + 2 * n)
+    a = nv.QkRope.from_buffer_copy(d)
+    assert [x for n in ("x", "ldx", "dy", "lddy", "y", "ldy", "heads", "w", "b", "dw", "db") for x in getattr(a, n)] == list(range(10, 32))
+
+
+def test_plans_hold_no_addresses():
+    """A plan is made from shapes, strides, types and flags; the pointers of the call it was made for are not in it."""
+    import t2v_amd.token_ops as T
+    from t2v_amd.functional import SeqLayout
+    nv = _nv()
+    sig = lambda *s: (torch.Size(s), (s[-1], 1) if len(s) == 2 else (1,), torch.bfloat16, torch.device("cuda", 0))  # noqa: E731
+    i32 = lambda *s: (torch.Size(s), (s[-1], 1) if len(s) == 2 else (1,), torch.int32, torch.device("cuda", 0))  # noqa: E731
+    lay = SeqLayout(2, 8, 8, 0, 1)
+    p = T._plan_of((sig(16, 128),) * 3 + (2, 2, lay, lay, 0.125, 1, 0.0, i32(2), i32(2), i32(2, 8), i32(2, 8), None, sig(2, 5)))
+    a = nv.AttnMod.from_buffer_copy(p.raw)
+    assert (a.nbatch, a.heads, a.Sq, a.D, a.causal, a.radius, a.q.sstride, a.o.sstride) == (2, 2, 8, 64, 1, 2, 128, 128)
+    assert not any((a.q.ptr, a.k.ptr, a.v.ptr, a.o.ptr, a.lse, a.workspace, a.meta)) and a.kv_docs == 1 and p.meta > 0
+    b = nv.AttnMod.from_buffer_copy(p.bwd(True)[0])
+    assert b.kv_share == 1 and b.dq.sstride == 128 and not b.dq.ptr and p.bwd(True)[1] > p.bwd(False)[1]
+    r = T._rope_plan((sig(16, 128), sig(16, 64)), (2, 1), T.RopeAxes((16, 24), style="half", shared=True, scale=(2.0, 3.0), theta=7.0), "layer", 0.5, i32(16, 2),
+                     None, (None,) * 4)
+    d = nv.QkRope.from_buffer_copy(r[0])
+    assert (list(d.heads), list(d.ldx), list(d.lddy), d.rows, d.D, d.norm, d.eps, d.ldpos, d.pos_type, d.naxes, list(d.dims), list(d.scale), d.theta, d.shared,
+            d.style) == ([2, 1], [128, 64], [128, 64], 16, 64, 2, 0.5, 2, 0, 2, [16, 24, 0, 0], [2.0, 3.0, 0.0, 0.0], 7.0, 1, 1)
+    assert not any(d.x) and not any(d.y) and not d.pos and r[-1] > 0

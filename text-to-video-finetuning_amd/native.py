@@ -177,13 +177,13 @@ SYMBOLS = {
     "t2v_rowgroup_splits": ([c_int, c_int, c_int], c_int),
     "t2v_attn_fwd": ([C.POINTER(Attn), c_void_p], c_int),
     "t2v_attn_bwd": ([C.POINTER(Attn), c_void_p], c_int),
-    "t2v_qk_rope_fwd": ([C.POINTER(QkRope), c_void_p], c_int),
-    "t2v_qk_rope_bwd_floats": ([C.POINTER(QkRope)], c_ll),
-    "t2v_qk_rope_bwd": ([C.POINTER(QkRope), c_void_p], c_int),
-    "t2v_attn_mod_workspace": ([C.POINTER(AttnMod), c_int], c_ll),
-    "t2v_attn_mod_meta_bytes": ([C.POINTER(AttnMod)], c_ll),
-    "t2v_attn_mod_fwd": ([C.POINTER(AttnMod), c_void_p], c_int),
-    "t2v_attn_mod_bwd": ([C.POINTER(AttnMod), c_void_p], c_int),
+    "t2v_qk_rope_fwd": ([c_void_p, c_void_p], c_int),
+    "t2v_qk_rope_bwd_floats": ([c_void_p], c_ll),
+    "t2v_qk_rope_bwd": ([c_void_p, c_void_p], c_int),
+    "t2v_attn_mod_workspace": ([c_void_p, c_int], c_ll),
+    "t2v_attn_mod_meta_bytes": ([c_void_p], c_ll),
+    "t2v_attn_mod_fwd": ([c_void_p, c_void_p], c_int),
+    "t2v_attn_mod_bwd": ([c_void_p, c_void_p], c_int),
     "t2v_softmax_rows": ([c_void_p, c_ll, c_void_p, c_ll, c_ll, c_int, c_void_p], c_int),
     "t2v_dropout_mask": ([c_void_p, c_ll, c_void_p, c_ll, c_ll, c_int, c_float, c_ull, c_void_p], c_int),
     "t2v_lowrank_update": ([c_void_p, c_ll, c_void_p, c_ll, c_void_p, c_ll, c_ll, c_int, c_int, c_float, c_void_p], c_int),

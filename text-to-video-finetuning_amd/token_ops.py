@@ -4,11 +4,14 @@ and keys with the rotation in the same pass, and attention with capped scores, d
 They work on the token matrices of `functional` ([rows, heads * dim], unit inner stride, any row stride that keeps rows 16-byte
 aligned) and are re-exported there.  Every one launches hand-written HIP kernels (csrc/rope.hip, csrc/attn_mod.hip) on the current
 stream of its operands' device, forward and backward; nothing falls back to torch math, and a call the kernels do not take raises.
+
+Host side: what a call's arguments look like (shapes, strides, types, flags: never addresses or contents) is checked once and kept as
+a plan, the descriptor's bytes with the pointers left open and the sizes of its buffers; a call fills in the pointers.  Small
+calls are as long as their host code.
 """
 import ctypes as C
 import functools
 import math
-import struct
 from dataclasses import dataclass
 
 import torch
@@ -25,36 +28,49 @@ def _fail(text):
     raise RuntimeError("t2v_amd: " + text)
 
 
-def _tokens(t, name, types=(torch.bfloat16, torch.float16, torch.float32)):
-    if t.dim() != 2 or t.dtype not in types or (t.shape[1] > 1 and t.stride(1) != 1):
-        _fail(f"{name} must be a 2-D token matrix with unit inner stride in {[str(x)[6:] for x in types]}, got {tuple(t.shape)} {t.dtype} "
-              f"strides {t.stride()}")
-    if not t.is_cuda:
-        nv.require_cuda(t)
-    return t
+def _check_tokens(shape, stride, dtype, dev, name, types):
+    if len(shape) != 2 or dtype not in types or (shape[1] > 1 and stride[1] != 1):
+        _fail(f"{name} must be a 2-D token matrix with unit inner stride in {[str(x)[6:] for x in types]}, got {tuple(shape)} {dtype} "
+              f"strides {stride}")
+    if dev.type != "cuda":
+        nv.require_cuda(torch.empty(0, device=dev))
 
 
-def _ld(t):
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+def _ld(shape, stride):
+    return stride[0] if shape[0] > 1 else shape[1]
 
 
 def _upstream(dy):
     """A gradient as autograd hands it over (it may be expanded, transposed or a narrow view): rows the kernels can read."""
-    if dy.stride(1) != 1 or dy.data_ptr() % 16 or (_ld(dy) * dy.element_size()) % 16 or _ld(dy) < dy.shape[1]:
+    if dy.is_contiguous():
+        return dy if dy.data_ptr() % 16 == 0 else dy.clone()
+    ld = _ld(dy.shape, dy.stride())
+    if dy.stride(1) != 1 or dy.data_ptr() % 16 or (ld * dy.element_size()) % 16 or ld < dy.shape[1]:
         return dy.contiguous()
     return dy
 
 
-def _vector(t, n, dev, name):
-    """fp32 copy / view of a per-column parameter."""
-    if t is None:
-        return None
-    if tuple(t.shape) != (n,) or t.device != dev or not t.is_floating_point():
-        _fail(f"{name} must be a floating vector of {n} elements on {dev}, got {tuple(t.shape)} {t.dtype} on {t.device}")
-    t = t.detach()
-    return t if t.dtype == torch.float32 and t.is_contiguous() else t.float().contiguous()
+def _sig(t):
+    """What a plan needs to know of an optional operand."""
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
 
 
+def _flat(cls):
+    """A structure laid out like `cls` whose pointers are plain fields: operands become name (the pointer) and name_rest, pairs name0 and name1."""
+    fields = []
+    for name, kind in cls._fields_:
+        if kind is nv.AttnOperand:
+            fields += [(name, C.c_void_p), (name + "_rest", C.c_char * (C.sizeof(kind) - 8))]
+        elif isinstance(kind, type) and issubclass(kind, C.Array) and kind._length_ == 2:
+            fields += [(name + "0", kind._type_), (name + "1", kind._type_)]
+        else:
+            fields.append((name, kind))
+    flat = type(cls.__name__ + "Flat", (C.Structure,), {"_fields_": fields})
+    assert C.sizeof(flat) == C.sizeof(cls)
+    return flat
+
+
+_RopeFlat, _AttnFlat = _flat(nv.QkRope), _flat(nv.AttnMod)
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
 
 
@@ -68,6 +84,13 @@ def _launch(name, desc, dev):
             rc = getattr(nv.lib(), name)(C.byref(desc), _raw_stream(index))
     if rc:
         nv.check(rc, name)
+
+
+def _size(name, *args):
+    n = getattr(nv.lib(), name)(*args)
+    if n < 0:
+        nv.check(int(n), name)
+    return int(n)
 
 
 # --------------------------------------------------------------------------- rotary positions
@@ -86,164 +109,169 @@ class RopeAxes:
     shared: bool = False
     scale: tuple = None
 
+    def __post_init__(self):
+        object.__setattr__(self, "dims", tuple(int(n) for n in self.dims))
+        if self.scale is not None:
+            object.__setattr__(self, "scale", tuple(float(s) for s in self.scale))
 
-# T2VQkRope in three pieces, packed in one go (a ctypes structure filled field by field costs several microseconds of a call that takes ten)
-_SIDES = struct.Struct("@12Q2i8QQq")        # x, ldx, dy, lddy, y, ldy (both sides each); heads; w, b, dw, db; workspace; rows
-_WHERE = struct.Struct("@Qqi")              # pos, ldpos, pos_type
+
+_SOMEWHERE = 1 << 20            # an aligned address that is never read: sizes are asked for with it
 
 
-@functools.lru_cache(maxsize=256)
-def _rope_fixed(axes, D, dtype, norm, eps):
-    """(number of axes, bytes in front of the positions, bytes behind them but for `freqs`): fixed by values, nothing of a call's tensors."""
-    d = nv.QkRope()
-    d.D, d.dtype, d.norm, d.eps = D, _TYPE[dtype], _NORM[norm] if norm else 0, eps
+def _vector(t):
+    """fp32, dense form of a per-column parameter (checked by the plan)."""
+    if t is None or (t.dtype == torch.float32 and t.is_contiguous()):
+        return t
+    return t.detach().float().contiguous()
+
+
+def _addr(t):
+    return 0 if t is None else t.data_ptr()
+
+
+@functools.lru_cache(maxsize=512)
+def _rope_plan(xs, heads, axes, norm, eps, pos, freqs, params):
+    """xs: one or two operand signatures; params: signatures of (q_weight, k_weight, q_bias, k_bias).  Returns (forward bytes, backward bytes,
+    rows, columns of the sides, dtype, device, D, floats of the backward workspace for parameter gradients)."""
+    shape, stride, dtype, dev = xs[0]
+    for (sh, st, dt, dv), name in zip(xs, ("x",) if len(xs) == 1 else ("q", "k")):
+        _check_tokens(sh, st, dt, dv, name, tuple(_TYPE))
+    if heads[0] <= 0 or shape[1] % heads[0]:
+        _fail(f"{shape[1]} columns are not a multiple of {heads[0]} heads")
+    rows, D = shape[0], shape[1] // heads[0]
+    if len(xs) == 2:
+        sh, st, dt, dv = xs[1]
+        if dt != dtype or dv != dev or sh[0] != rows or heads[1] <= 0 or sh[1] != heads[1] * D:
+            _fail(f"q {tuple(shape)} {dtype} with {heads[0]} heads and k {tuple(sh)} {dt} with {heads[1]} must have the same rows, type, device and "
+                  f"head dim")
+    d = _RopeFlat()
+    d.heads0, d.heads1, d.rows, d.D, d.dtype, d.eps = heads[0], heads[1], rows, D, _TYPE[dtype], eps
+    if norm is not None:
+        if norm not in _NORM:
+            _fail(f"norm {norm!r}: 'rms' or 'layer'")
+        d.norm = _NORM[norm]
+    for t, name in zip(params or (), ("q_weight", "k_weight", "q_bias", "k_bias")):
+        if t is not None and (tuple(t[0]) != (D,) or t[3] != dev or not t[2].is_floating_point):
+            _fail(f"{name} must be a floating vector of {D} elements on {dev}, got {tuple(t[0])} {t[2]} on {t[3]}")
     if axes is not None:
-        dims = tuple(int(n) for n in axes.dims)
+        dims = axes.dims
         if not 1 <= len(dims) <= 4 or any(n <= 0 or n % 2 for n in dims) or sum(dims) % 8 or sum(dims) > D:
             _fail(f"RopeAxes.dims {axes.dims}: one to four even numbers whose sum is a multiple of 8 and at most the head dim {D}")
         if axes.style not in ("interleaved", "half"):
             _fail(f"RopeAxes.style {axes.style!r}: 'interleaved' or 'half'")
         if not (axes.theta > 0 and math.isfinite(axes.theta)):
             _fail(f"RopeAxes.theta {axes.theta}: a positive number is wanted")
-        scale = (1.0,) * len(dims) if axes.scale is None else tuple(float(s) for s in axes.scale)
+        scale = (1.0,) * len(dims) if axes.scale is None else axes.scale
         if len(scale) != len(dims) or not all(math.isfinite(s) for s in scale):
             _fail(f"RopeAxes.scale {axes.scale}: one finite number per axis")
         d.naxes, d.theta, d.shared, d.style = len(dims), axes.theta, int(axes.shared), int(axes.style == "half")
         for n, (k, s) in enumerate(zip(dims, scale)):
             d.dims[n], d.scale[n] = k, s
-    raw, q = bytes(d), nv.QkRope
-    return d.naxes, raw[q.D.offset:q.pos.offset], raw[q.naxes.offset:q.freqs.offset]
-
-
-def _rope_desc(axes, D, dtype, norm, eps, rows, pos, freqs, dev, heads, x, dy, y, w, b, dw, db, work):
-    """x, dy, y: two (pointer, row stride); w, b, dw, db: two pointers; 0: not there."""
-    naxes, mid, tail = _rope_fixed(axes, D, dtype, norm, eps)
-    fr = 0
-    where = (0, 0, 0)
-    if axes is not None:
-        if pos is None or pos.dim() != 2 or pos.shape[0] != rows or pos.shape[1] < naxes or pos.dtype not in _POS or pos.device != dev:
-            _fail(f"pos must be an int32, int64 or fp32 [{rows}, {naxes}] tensor on {dev}, got "
-                  f"{None if pos is None else (tuple(pos.shape), pos.dtype, pos.device)}")
-        ld = pos.stride(0) if rows > 1 else pos.shape[1]
-        if (pos.shape[1] > 1 and pos.stride(1) != 1) or ld < naxes:
-            _fail(f"pos must have unit inner stride and rows that do not overlap, got strides {pos.stride()}")
-        where = (pos.data_ptr(), ld, _POS[pos.dtype])
-        if freqs is not None:
-            rot = sum(axes.dims)
-            if tuple(freqs.shape) != (rot // 2,) or freqs.dtype != torch.float64 or freqs.device != dev or not freqs.is_contiguous():
-                _fail(f"freqs must be a contiguous fp64 tensor of {rot // 2} frequencies on {dev}")
-            fr = freqs.data_ptr()
+        if pos is None or len(pos[0]) != 2 or pos[0][0] != rows or pos[0][1] < len(dims) or pos[2] not in _POS or pos[3] != dev:
+            _fail(f"pos must be an int32, int64 or fp32 [{rows}, {len(dims)}] tensor on {dev}, got {None if pos is None else (tuple(pos[0]), *pos[2:])}")
+        ld = _ld(pos[0], pos[1])
+        if (pos[0][1] > 1 and pos[1][1] != 1) or ld < len(dims):
+            _fail(f"pos must have unit inner stride and rows that do not overlap, got strides {pos[1]}")
+        d.ldpos, d.pos_type = ld, _POS[pos[2]]
+        if freqs is not None and (tuple(freqs[0]) != (sum(dims) // 2,) or freqs[2] != torch.float64 or freqs[3] != dev or
+                                  (freqs[0][0] > 1 and freqs[1] != (1,))):
+            _fail(f"freqs must be a contiguous fp64 tensor of {sum(dims) // 2} frequencies on {dev}")
     elif pos is not None or freqs is not None:
         _fail("positions need RopeAxes that say what they turn")
-    (x0, lx0), (x1, lx1) = x
-    (g0, lg0), (g1, lg1) = dy
-    (y0, ly0), (y1, ly1) = y
-    sides = _SIDES.pack(x0, x1, lx0, lx1, g0, g1, lg0, lg1, y0, y1, ly0, ly1, *heads, *w, *b, *dw, *db, work, rows)
-    return nv.QkRope.from_buffer_copy(sides + mid + _WHERE.pack(*where) + tail + fr.to_bytes(8, "little"))
+    widths = tuple(sh[1] for sh, _, _, _ in xs)
+    d.ldx0, d.ldy0, d.lddy0 = _ld(shape, stride), widths[0], widths[0]
+    if len(xs) == 2:
+        d.ldx1, d.ldy1, d.lddy1 = _ld(xs[1][0], xs[1][1]), widths[1], widths[1]
+    floats = 0
+    if norm is not None and rows:
+        e = _RopeFlat.from_buffer_copy(d)
+        for n in ("x0", "x1", "dy0", "dy1", "y0", "y1", "dw0", "pos"):
+            setattr(e, n, _SOMEWHERE)
+        floats = _size("t2v_qk_rope_bwd_floats", C.byref(e))
+    return bytes(d), rows, widths, dtype, dev, D, floats
 
 
-_NO = ((0, 0), (0, 0))
-_ZZ = (0, 0)
-
-
-def _head_dim(x, heads, name):
-    if heads <= 0 or x.shape[1] % heads:
-        _fail(f"{name} has {x.shape[1]} columns: not a multiple of {heads} heads")
-    return x.shape[1] // heads
-
-
-def _ptrs(ts):
-    """(pointer, row stride) of one or two matrices."""
-    a = (ts[0].data_ptr(), _ld(ts[0]))
-    return (a, (ts[1].data_ptr(), _ld(ts[1]))) if len(ts) > 1 else (a, (0, 0))
-
-
-def _vptrs(ts):
-    return tuple(0 if t is None else t.data_ptr() for t in ts) if ts is not None else _ZZ
-
-
-def _rope_fwd(xs, heads, pos, axes, freqs, norm, eps, ws, bs):
-    x0 = xs[0]
-    dev, rows = x0.device, x0.shape[0]
-    ys = tuple([torch.empty(x.shape, dtype=x.dtype, device=dev) for x in xs])
-    d = _rope_desc(axes, _head_dim(x0, heads[0], "q"), x0.dtype, norm, eps, rows, pos, freqs, dev, heads, _ptrs(xs), _NO, _ptrs(ys),
-                   _vptrs(ws), _vptrs(bs), _ZZ, _ZZ, 0)
+def _rope_fwd(plan, xs, pos, freqs, ws, bs):
+    raw, rows, widths, dtype, dev = plan[:5]
+    d = _RopeFlat.from_buffer_copy(raw)
+    y = torch.empty((rows, widths[0]), dtype=dtype, device=dev)
+    d.x0, d.y0, d.pos, d.freqs = xs[0].data_ptr(), y.data_ptr(), _addr(pos), _addr(freqs)
+    ys = (y,)
+    if len(xs) == 2:
+        y = torch.empty((rows, widths[1]), dtype=dtype, device=dev)
+        d.x1, d.y1, d.w0, d.w1, d.b0, d.b1 = xs[1].data_ptr(), y.data_ptr(), _addr(ws[0]), _addr(ws[1]), _addr(bs[0]), _addr(bs[1])
+        ys += (y,)
     if rows:
         _launch("t2v_qk_rope_fwd", d, dev)
     return ys
 
 
-def _rope_bwd(xs, dys, heads, pos, axes, freqs, norm, eps, ws, want):
-    """want: per side (dw, db) wanted.  Returns dxs and the parameter gradients (fp32)."""
-    dy0 = dys[0]
-    dev, rows, D = dy0.device, dy0.shape[0], _head_dim(dy0, heads[0], "dy")
-    dxs = [torch.empty(dy.shape, dtype=dy.dtype, device=dev) for dy in dys]
-    dws, dbs = [None, None], [None, None]
-    if norm:
-        new = torch.empty if rows else torch.zeros
-        for i in range(2):
-            if want[i][0]:
-                dws[i] = new(D, dtype=torch.float32, device=dev)
-            if want[i][1]:
-                dbs[i] = new(D, dtype=torch.float32, device=dev)
-    d = _rope_desc(axes, D, dy0.dtype, norm, eps, rows, pos, freqs, dev, heads, _ptrs(xs) if norm else _NO, _ptrs(dys), _ptrs(dxs),
-                   _vptrs(ws), _ZZ, _vptrs(dws), _vptrs(dbs), 0)
+def _rope_bwd(plan, xs, dys, pos, freqs, ws, want):
+    """want: (dw0, dw1, db0, db1) wanted, or None.  Returns dxs and the four parameter gradients (fp32 or None)."""
+    raw, rows, widths, dtype, dev, D, floats = plan
+    d = _RopeFlat.from_buffer_copy(raw)
+    dx = torch.empty((rows, widths[0]), dtype=dtype, device=dev)
+    d.dy0, d.y0, d.pos, d.freqs = dys[0].data_ptr(), dx.data_ptr(), _addr(pos), _addr(freqs)
+    if not dys[0].is_contiguous():
+        d.lddy0 = _ld(dys[0].shape, dys[0].stride())
+    dxs, grads = (dx,), [None] * 4
+    if len(dys) == 2:
+        dx = torch.empty((rows, widths[1]), dtype=dtype, device=dev)
+        d.dy1, d.y1 = dys[1].data_ptr(), dx.data_ptr()
+        if not dys[1].is_contiguous():
+            d.lddy1 = _ld(dys[1].shape, dys[1].stride())
+        d.x0, d.x1, d.w0, d.w1 = xs[0].data_ptr(), xs[1].data_ptr(), _addr(ws[0]), _addr(ws[1])
+        dxs += (dx,)
+        if any(want):
+            new = torch.empty if rows else torch.zeros
+            grads = [new(D, dtype=torch.float32, device=dev) if w else None for w in want]
+            work = torch.empty(floats, dtype=torch.float32, device=dev)
+            d.dw0, d.dw1, d.db0, d.db1, d.workspace = _addr(grads[0]), _addr(grads[1]), _addr(grads[2]), _addr(grads[3]), work.data_ptr()
     if rows:
-        if norm and (want[0][0] or want[0][1] or want[1][0] or want[1][1]):
-            n = nv.lib().t2v_qk_rope_bwd_floats(C.byref(d))
-            if n < 0:
-                nv.check(int(n), "t2v_qk_rope_bwd_floats")
-            work = torch.empty(int(n), dtype=torch.float32, device=dev)
-            d.workspace = work.data_ptr()
         _launch("t2v_qk_rope_bwd", d, dev)
-    return dxs, dws, dbs
+    return dxs, grads
 
 
 # (The differentiable tensors are the Functions' arguments, the rest travels in one tuple: apply() spends about a microsecond per argument.)
 class _Rope(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, rest):
-        heads, pos, axes, freqs = rest
-        ctx.heads, ctx.axes = heads, axes
+        ctx.plan, pos, freqs = rest
         ctx.save_for_backward(pos, freqs)
-        return _rope_fwd((x,), (heads, 0), pos, axes, freqs, None, 0.0, None, None)[0]
+        return _rope_fwd(ctx.plan, (x,), pos, freqs, None, None)[0]
 
     @staticmethod
     def backward(ctx, dy):
         pos, freqs = ctx.saved_tensors
-        return _rope_bwd(None, (_upstream(dy),), (ctx.heads, 0), pos, ctx.axes, freqs, None, 0.0, None, None)[0][0], None
+        return _rope_bwd(ctx.plan, None, (_upstream(dy),), pos, freqs, None, None)[0][0], None
 
 
 def rope(x, heads, pos, axes, freqs=None):
     """Rotary positions: x [rows, heads * dim] (bf16, fp16 or fp32) with the columns `axes` (RopeAxes) names turned by pos [rows, number
     of axes] (int32, int64 or fp32).  Angles are formed in 64 bits.  freqs: fp64 [sum(dims) / 2] radians per unit of position, in the place of the
     ladder theta gives.  Returns a dense matrix of x's shape; differentiable in x."""
-    x = _tokens(x, "x")
-    heads = int(heads)
+    plan = _rope_plan((_sig(x),), (int(heads), 0), axes, None, 0.0, _sig(pos), _sig(freqs), None)
     if torch.is_grad_enabled() and x.requires_grad:
-        return _Rope.apply(x, (heads, pos, axes, freqs))
-    return _rope_fwd((x,), (heads, 0), pos, axes, freqs, None, 0.0, None, None)[0]
+        return _Rope.apply(x, (plan, pos, freqs))
+    return _rope_fwd(plan, (x,), pos, freqs, None, None)[0]
 
 
 class _QkNormRope(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, qw, kw, qb, kb, rest):
-        heads, pos, axes, freqs, norm, eps, ws, bs = rest
-        ctx.meta = (heads, axes, norm, eps)
+        ctx.plan, ctx.key, pos, freqs = rest
         ctx.types = [None if t is None else t.dtype for t in (qw, kw, qb, kb)]
         ctx.save_for_backward(q, k, qw, kw, pos, freqs)
-        return _rope_fwd((q, k), heads, pos, axes, freqs, norm, eps, ws, bs)
+        return _rope_fwd(ctx.plan, (q, k), pos, freqs, (_vector(qw), _vector(kw)), (_vector(qb), _vector(kb)))
 
     @staticmethod
     def backward(ctx, dq, dk):
         q, k, qw, kw, pos, freqs = ctx.saved_tensors
-        heads, axes, norm, eps = ctx.meta
-        D, dev, need = q.shape[1] // heads[0], q.device, ctx.needs_input_grad
-        ws = (_vector(qw, D, dev, "q_weight"), _vector(kw, D, dev, "k_weight"))
-        dxs, dws, dbs = _rope_bwd((q, k), (_upstream(dq), _upstream(dk)), heads, pos, axes, freqs, norm, eps, ws,
-                                  ((need[2], need[4]), (need[3], need[5])))
-        g = [None if t is None else t.to(y) for t, y in zip(dws + dbs, ctx.types)]
-        return (dxs[0], dxs[1], *g, None)
+        plan, sigs = ctx.plan, (_sig(q), _sig(k))
+        if sigs != ctx.key[0]:                      # (a saved tensor may come back with other strides)
+            plan = _rope_plan(sigs, *ctx.key[1:])
+        dxs, grads = _rope_bwd(plan, (q, k), (_upstream(dq), _upstream(dk)), pos, freqs, (_vector(qw), _vector(kw)), ctx.needs_input_grad[2:6])
+        return (*dxs, *[g if g is None or g.dtype == t else g.to(t) for g, t in zip(grads, ctx.types)], None)
 
 
 def qk_norm_rope(q, k, heads, kv_heads, pos, axes, q_weight=None, k_weight=None, q_bias=None, k_bias=None, eps=1e-6, norm="rms",
@@ -253,19 +281,15 @@ def qk_norm_rope(q, k, heads, kv_heads, pos, axes, q_weight=None, k_weight=None,
     norm: "rms" (x * rsqrt(mean x^2 + eps)) or "layer" (centred first); q_weight, k_weight, q_bias, k_bias: [dim] vectors shared by the
     heads, or None.  pos, axes, freqs: as in `rope`; both None: the norm alone.  Differentiable in q, k and the four vectors; the
     statistics are recomputed in the backward pass from the saved inputs."""
-    q, k = _tokens(q, "q"), _tokens(k, "k")
-    heads, kv_heads = int(heads), int(kv_heads)
-    if norm not in _NORM:
-        _fail(f"norm {norm!r}: 'rms' or 'layer'")
-    if k.dtype != q.dtype or k.device != q.device or k.shape[0] != q.shape[0] or _head_dim(q, heads, "q") != _head_dim(k, kv_heads, "k"):
-        _fail(f"q {tuple(q.shape)} {q.dtype} and k {tuple(k.shape)} {k.dtype} must have the same rows, type, device and head dim")
-    D, dev = q.shape[1] // heads, q.device
-    params = (q_weight, k_weight, q_bias, k_bias)
-    ws = (_vector(q_weight, D, dev, "q_weight"), _vector(k_weight, D, dev, "k_weight"))
-    bs = (_vector(q_bias, D, dev, "q_bias"), _vector(k_bias, D, dev, "k_bias"))
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or any([t is not None and t.requires_grad for t in params])):
-        return _QkNormRope.apply(q, k, *params, ((heads, kv_heads), pos, axes, freqs, norm, float(eps), ws, bs))
-    return _rope_fwd((q, k), (heads, kv_heads), pos, axes, freqs, norm, float(eps), ws, bs)
+    if norm is None:
+        _fail("norm None: 'rms' or 'layer' (`rope` turns without a norm)")
+    key = ((_sig(q), _sig(k)), (int(heads), int(kv_heads)), axes, norm, float(eps), _sig(pos), _sig(freqs),
+           (_sig(q_weight), _sig(k_weight), _sig(q_bias), _sig(k_bias)))
+    plan = _rope_plan(*key)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or
+                                    any([t is not None and t.requires_grad for t in (q_weight, k_weight, q_bias, k_bias)])):
+        return _QkNormRope.apply(q, k, q_weight, k_weight, q_bias, k_bias, (plan, key, pos, freqs))
+    return _rope_fwd(plan, (q, k), pos, freqs, (_vector(q_weight), _vector(k_weight)), (_vector(q_bias), _vector(k_bias)))
 
 
 # --------------------------------------------------------------------------- attention with modified scores
@@ -285,108 +309,201 @@ def _layout_facts(lay, rows):
     return last < rows, own, own and lay.nbatch * lay.S == rows
 
 
-def _op(t, lay):
-    """The five fields of a T2VAttnOperand."""
-    ld = _ld(t)
-    return t.data_ptr(), lay.hi * ld, lay.lo * ld, lay.ss * ld, lay.bdiv
+def _operand(ld, lay):
+    """A T2VAttnOperand without its pointer."""
+    return nv.AttnOperand(0, lay.hi * ld, lay.lo * ld, lay.ss * ld, lay.bdiv)
 
 
-def _ints(t, shapes, dev, name):
-    if t is None:
-        return None
-    if t.dtype != torch.int32 or tuple(t.shape) not in shapes or t.device != dev or not t.is_contiguous():
-        _fail(f"{name} must be a contiguous int32 tensor of shape {' or '.join(map(str, shapes))} on {dev}, got {tuple(t.shape)} {t.dtype} on {t.device}")
-    return t.data_ptr()
+def _check_ints(t, shapes, dev, name):
+    if t is not None and (t[2] != torch.int32 or tuple(t[0]) not in shapes or t[3] != dev or not _dense(t)):
+        _fail(f"{name} must be a contiguous int32 tensor of shape {' or '.join(map(str, shapes))} on {dev}, got {tuple(t[0])} {t[2]} on {t[3]}")
 
 
-# T2VAttnMod field by field, packed in one go (see _SIDES); _FWD ends where the fields of the backward pass begin
-_OP = "Qqqqi4x"
-_FWD = struct.Struct("@8i2f" + 4 * _OP + "QQi4xQQQQQii")
-_BWD = struct.Struct("@" + 4 * _OP + "QQi4xQqQqi4x")
-_NO_BWD = bytes(_BWD.size)
+def _dense(t):
+    expect = 1
+    for n, s in zip(reversed(t[0]), reversed(t[1])):
+        if n != 1 and s != expect:
+            return False
+        expect *= n
+    return True
 
 
-def _attn_desc(q, k, v, o, meta, lse, prefix, kv_len, q_docs, kv_docs, slopes, bias, bwd=None):
-    heads, kv_heads, qlay, klay, scale, causal, softcap = meta
-    ptr = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
-    fwd = _FWD.pack(qlay.nbatch, heads, kv_heads, qlay.S, klay.S, q.shape[1] // heads, _TYPE[q.dtype], causal, scale, softcap,
-                    *_op(q, qlay), *_op(k, klay), *_op(v, klay), *_op(o, qlay), ptr(lse), ptr(prefix), 0 if prefix is None else prefix.dim() - 1,
-                    ptr(kv_len), ptr(q_docs), ptr(kv_docs), ptr(slopes), ptr(bias), 0 if bias is None else bias.dtype == torch.float32,
-                    0 if bias is None else bias.shape[1] // 2)
-    return nv.AttnMod.from_buffer_copy(fwd + (_NO_BWD if bwd is None else _BWD.pack(*bwd, 0, 0, 0, 0, 0)))
+class _AttnPlan:
+    """raw: descriptor of the forward; work, meta: bytes of its buffers; bwd: (descriptor, workspace bytes, with dense gradients), made on first use."""
+    __slots__ = ("key", "raw", "work", "meta", "empty", "covered", "kv_covered", "share", "rows", "dtype", "dev", "lse", "shared_ok", "_bwd", "lays")
+
+    def bwd(self, with_bias):
+        if self._bwd.get(with_bias) is None:
+            qlay, klay, width, kwidth = self.lays
+            d = nv.AttnMod.from_buffer_copy(self.raw)
+            d.d_o, d.dq, d.dk, d.dv = _operand(width, qlay), _operand(width, qlay), _operand(kwidth, klay), _operand(kwidth, klay)
+            d.kv_share = self.share
+            e = nv.AttnMod.from_buffer_copy(d)
+            for n in ("q", "k", "v", "o"):
+                getattr(e, n).ptr = _SOMEWHERE
+            e.dbias = _SOMEWHERE if with_bias else None
+            _somewhere(e)
+            self._bwd[with_bias] = (bytes(d), _size("t2v_attn_mod_workspace", C.byref(e), 1))
+        return self._bwd[with_bias]
 
 
-def _workspace(a, backward, dev):
-    n = nv.lib().t2v_attn_mod_workspace(C.byref(a), backward)
-    if n < 0:
-        nv.check(int(n), "t2v_attn_mod_workspace")
-    if n == 0:
-        return None
-    w = torch.empty(int(n), dtype=torch.uint8, device=dev)      # (the caching allocator's blocks are 512-byte aligned)
-    a.workspace, a.workspace_bytes = w.data_ptr(), int(n)
-    return w
+def _somewhere(e):
+    """Pointers that only have to be there: which masks and biases a call has is part of its plan (flagged in the open pointers by 1)."""
+    for n in ("prefix", "kv_len", "q_docs", "kv_docs", "slopes", "bias"):
+        if getattr(e, n):
+            setattr(e, n, _SOMEWHERE)
 
 
-def _meta(a, dev):
-    """The buffer for what a call derives from documents and prefixes per query, tile by tile (None where there are none)."""
-    if not a.q_docs and not (a.prefix and a.prefix_per_query):
-        return None
-    n = nv.lib().t2v_attn_mod_meta_bytes(C.byref(a))
-    if n < 0:
-        nv.check(int(n), "t2v_attn_mod_meta_bytes")
-    m = torch.empty(int(n), dtype=torch.uint8, device=dev)
-    a.meta, a.meta_bytes = m.data_ptr(), int(n)
-    return m
+@functools.lru_cache(maxsize=512)
+def _attn_plan(qs, ks, vs, heads, kv_heads, qlay, klay, scale, causal, softcap, prefix, kv_len, q_docs, kv_docs, slopes, bias):
+    types = (torch.bfloat16, torch.float16)
+    for (sh, st, dt, dv), name in ((qs, "q"), (ks, "k"), (vs, "v")):
+        _check_tokens(sh, st, dt, dv, name, types)
+    (qsh, qst, dtype, dev), (ksh, kst, _, _), (vsh, vst, _, _) = qs, ks, vs
+    if heads <= 0 or qsh[1] % heads:
+        _fail(f"q has {qsh[1]} columns: not a multiple of {heads} heads")
+    D = qsh[1] // heads
+    if kv_heads <= 0 or heads % kv_heads:
+        _fail(f"{heads} query heads cannot share {kv_heads} key / value heads evenly")
+    if ksh != vsh or ksh[1] != kv_heads * D or not dtype == ks[2] == vs[2] or not dev == ks[3] == vs[3]:
+        _fail(f"q {tuple(qsh)} {dtype}, k {tuple(ksh)} {ks[2]}, v {tuple(vsh)} {vs[2]}: one type, one device, {kv_heads} key / value heads of {D} "
+              f"columns are wanted")
+    if D % 8 or D > 128:
+        _fail(f"attention_mod takes head dims that are multiples of 8 up to 128, got {D}")
+    nb, Sq, Sk = qlay.nbatch, qlay.S, klay.S
+    qf, kf = _layout_facts(qlay, qsh[0]), _layout_facts(klay, ksh[0])
+    if nb != klay.nbatch or not qf[0] or not kf[0]:
+        _fail(f"layouts {qlay} over {qsh[0]} rows and {klay} over {ksh[0]} rows: as many batches on both sides, rows that exist")
+    if not qf[1]:
+        _fail(f"query layout {qlay} names a row twice")
+    if not 0.0 <= softcap < 1e30 or not math.isfinite(scale):
+        _fail(f"softcap {softcap}, scale {scale}: a finite scale and a cap of 0 (none) or more are wanted")
+    if prefix is not None and not causal:
+        _fail("prefix opens a causal mask: pass causal=True with it")
+    if (q_docs is None) != (kv_docs is None):
+        _fail("q_docs and kv_docs come together")
+    _check_ints(prefix, ((nb,), (nb, Sq)), dev, "prefix")
+    _check_ints(kv_len, ((nb,),), dev, "kv_len")
+    _check_ints(q_docs, ((nb, Sq),), dev, "q_docs")
+    _check_ints(kv_docs, ((nb, Sk),), dev, "kv_docs")
+    if slopes is not None and (slopes[2] != torch.float32 or tuple(slopes[0]) != (heads,) or slopes[3] != dev or not _dense(slopes)):
+        _fail(f"slopes must be a contiguous fp32 tensor of {heads} elements on {dev}")
+    if bias is not None and (bias[2] not in (dtype, torch.float32) or len(bias[0]) != 2 or bias[0][0] != heads or bias[0][1] % 2 == 0 or
+                             bias[0][1] > 2049 or bias[3] != dev or not _dense(bias)):
+        _fail(f"bias must be a contiguous [{heads}, 2R + 1] table with R <= 1024 in {dtype} or fp32 on {dev}, got {tuple(bias[0])} {bias[2]}")
+    p = _AttnPlan()
+    p.empty = nb * Sq == 0 or Sk == 0                   # nothing is asked, or there is nothing to see
+    p.rows, p.dtype, p.dev, p.lse = qsh[0], dtype, dev, nb * heads * Sq
+    p.covered = qf[2]
+    p.share = klay.bdiv if klay.bdiv > 1 and klay.lo == 0 else 1
+    p.kv_covered = kf[2] or (p.share > 1 and nb % p.share == 0 and nb // p.share * Sk == ksh[0] and klay.ss == 1 and klay.hi == Sk)
+    p.shared_ok = kf[1] or (p.share > 1 and klay.ss > 0 and klay.hi >= (Sk - 1) * klay.ss + 1)
+    p._bwd, p.lays, p.work, p.meta, p.raw = {}, (qlay, klay, heads * D, kv_heads * D), 0, 0, b""
+    if p.empty:
+        return p
+    a = nv.AttnMod()
+    a.nbatch, a.heads, a.kv_heads, a.Sq, a.Sk, a.D = nb, heads, kv_heads, Sq, Sk, D
+    a.dtype, a.causal, a.scale, a.softcap = _TYPE[dtype], causal, scale, softcap
+    a.q, a.k, a.v, a.o = _operand(_ld(qsh, qst), qlay), _operand(_ld(ksh, kst), klay), _operand(_ld(vsh, vst), klay), _operand(heads * D, qlay)
+    a.prefix_per_query = int(prefix is not None and len(prefix[0]) == 2)
+    if bias is not None:
+        a.bias_f32, a.radius = int(bias[2] == torch.float32), bias[0][1] // 2
+    for name, t in (("prefix", prefix), ("kv_len", kv_len), ("q_docs", q_docs), ("kv_docs", kv_docs), ("slopes", slopes), ("bias", bias)):
+        setattr(a, name, None if t is None else 1)      # (there: the address comes with the call)
+    p.raw = bytes(a)
+    for n in ("q", "k", "v", "o"):
+        getattr(a, n).ptr = _SOMEWHERE
+    _somewhere(a)
+    p.work, p.meta = _size("t2v_attn_mod_workspace", C.byref(a), 0), _size("t2v_attn_mod_meta_bytes", C.byref(a))
+    return p
 
 
-def _attn_fwd(q, k, v, meta, prefix, kv_len, q_docs, kv_docs, slopes, bias, keep):
-    heads, _, qlay, klay = meta[:4]
-    dev = q.device
-    if qlay.nbatch * qlay.S == 0 or klay.S == 0:        # nothing is asked, or there is nothing to see
-        o = torch.zeros(q.shape, dtype=q.dtype, device=dev)
-        return o, (torch.full((qlay.nbatch * heads * qlay.S,), math.inf, device=dev) if keep else None), None
-    covered = _layout_facts(qlay, q.shape[0])[2]
-    o = (torch.empty if covered else torch.zeros)(q.shape, dtype=q.dtype, device=dev)      # rows that no sequence owns: zeros
-    lse = torch.empty(qlay.nbatch * heads * qlay.S, dtype=torch.float32, device=dev) if keep else None
-    a = _attn_desc(q, k, v, o, meta, lse, prefix, kv_len, q_docs, kv_docs, slopes, bias)
-    tiles = _meta(a, dev)
-    work = _workspace(a, 0, dev)      # noqa: F841 (kept until the launch is issued)
-    _launch("t2v_attn_mod_fwd", a, dev)
+def _fill(d, q, k, v, o, prefix, kv_len, q_docs, kv_docs, slopes, bias):
+    d.q, d.k, d.v, d.o = q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr()
+    if prefix is not None:
+        d.prefix = prefix.data_ptr()
+    if kv_len is not None:
+        d.kv_len = kv_len.data_ptr()
+    if q_docs is not None:
+        d.q_docs, d.kv_docs = q_docs.data_ptr(), kv_docs.data_ptr()
+    if slopes is not None:
+        d.slopes = slopes.data_ptr()
+    if bias is not None:
+        d.bias = bias.data_ptr()
+
+
+def _bytes(n, dev):
+    return torch.empty(n, dtype=torch.uint8, device=dev)      # (the caching allocator's blocks are 512-byte aligned)
+
+
+def _attn_fwd(p, q, k, v, masks, bias, keep):
+    """o, and with `keep` what the backward pass wants: lse, and the tile data of the masks."""
+    dev = p.dev
+    if p.empty:
+        return torch.zeros(q.shape, dtype=p.dtype, device=dev), torch.full((p.lse,), math.inf, device=dev) if keep else None, None
+    o = (torch.empty if p.covered else torch.zeros)(q.shape, dtype=p.dtype, device=dev)      # rows that no sequence owns: zeros
+    d = _AttnFlat.from_buffer_copy(p.raw)
+    _fill(d, q, k, v, o, *masks, bias)
+    lse = tiles = None
+    if keep:
+        lse = torch.empty(p.lse, dtype=torch.float32, device=dev)
+        d.lse = lse.data_ptr()
+    if p.meta:
+        tiles = _bytes(p.meta, dev)
+        d.meta, d.meta_bytes = tiles.data_ptr(), p.meta
+    if p.work:
+        work = _bytes(p.work, dev)
+        d.workspace, d.workspace_bytes = work.data_ptr(), p.work
+    _launch("t2v_attn_mod_fwd", d, dev)
     return o, lse, tiles
 
 
 class _AttentionMod(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, bias, rest):
-        meta, prefix, kv_len, q_docs, kv_docs, slopes = rest
-        o, lse, tiles = _attn_fwd(q, k, v, meta, prefix, kv_len, q_docs, kv_docs, slopes, bias, True)
-        ctx.meta = meta
-        ctx.save_for_backward(q, k, v, bias, prefix, kv_len, q_docs, kv_docs, slopes, o, lse, tiles)
+        ctx.plan, masks = rest
+        o, lse, tiles = _attn_fwd(ctx.plan, q, k, v, masks, bias, True)
+        ctx.save_for_backward(q, k, v, bias, o, lse, tiles, *masks)
         return o
 
     @staticmethod
     def backward(ctx, do):
-        q, k, v, bias, prefix, kv_len, q_docs, kv_docs, slopes, o, lse, tiles = ctx.saved_tensors
-        qlay, klay = ctx.meta[2:4]
-        dev = q.device
+        q, k, v, bias, o, lse, tiles, *masks = ctx.saved_tensors
+        p = ctx.plan
+        dev, dtype = p.dev, p.dtype
+        with_bias = bias is not None and ctx.needs_input_grad[3]
+        if p.empty:
+            return (*[torch.zeros(t.shape, dtype=dtype, device=dev) for t in (q, k, v)], torch.zeros_like(bias) if with_bias else None, None)
+        if (_sig(q), _sig(k), _sig(v)) != p.key[:3]:            # (a saved tensor may come back with other strides)
+            p = _plan_of((_sig(q), _sig(k), _sig(v)) + p.key[3:])
+        raw, work_bytes = p.bwd(with_bias)
+        dq = (torch.empty if p.covered else torch.zeros)(q.shape, dtype=dtype, device=dev)
+        new = torch.empty if p.kv_covered else torch.zeros
+        dk, dv = new(k.shape, dtype=dtype, device=dev), new(v.shape, dtype=dtype, device=dev)
         do = _upstream(do)
-        empty = qlay.nbatch * qlay.S == 0 or klay.S == 0
-        share = klay.bdiv if klay.bdiv > 1 and klay.lo == 0 else 1
-        kfacts = _layout_facts(klay, k.shape[0])
-        kall = kfacts[2] or (share > 1 and klay.nbatch % share == 0 and klay.nbatch // share * klay.S == k.shape[0])
-        new = lambda t, full: (torch.empty if full and not empty else torch.zeros)(t.shape, dtype=t.dtype, device=dev)  # noqa: E731
-        dq, dk, dv = new(q, _layout_facts(qlay, q.shape[0])[2]), new(k, kall), new(v, kall)
-        dbias = new(bias, True) if bias is not None and ctx.needs_input_grad[3] else None
-        if not empty:
-            delta = torch.empty_like(lse)
-            a = _attn_desc(q, k, v, o, ctx.meta, lse, prefix, kv_len, q_docs, kv_docs, slopes, bias,
-                           (*_op(do, qlay), *_op(dq, qlay), *_op(dk, klay), *_op(dv, klay), delta.data_ptr(),
-                            0 if dbias is None else dbias.data_ptr(), share))
-            if tiles is not None:
-                a.meta, a.meta_bytes, a.meta_ready = tiles.data_ptr(), tiles.numel(), 1
-            work = _workspace(a, 1, dev)      # noqa: F841 (kept until the launches are issued)
-            _launch("t2v_attn_mod_bwd", a, dev)
+        delta = torch.empty(p.lse, dtype=torch.float32, device=dev)
+        d = _AttnFlat.from_buffer_copy(raw)
+        _fill(d, q, k, v, o.contiguous(), *masks, bias)
+        d.lse, d.delta, d.d_o, d.dq, d.dk, d.dv = lse.data_ptr(), delta.data_ptr(), do.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
+        if not do.is_contiguous():
+            d.d_o_rest = bytes(_operand(_ld(do.shape, do.stride()), p.lays[0]))[8:]
+        dbias = None
+        if with_bias:
+            dbias = torch.empty(bias.shape, dtype=bias.dtype, device=dev)
+            d.dbias = dbias.data_ptr()
+        if tiles is not None:
+            d.meta, d.meta_bytes, d.meta_ready = tiles.data_ptr(), tiles.numel(), 1
+        if work_bytes:
+            work = _bytes(work_bytes, dev)
+            d.workspace, d.workspace_bytes = work.data_ptr(), work_bytes
+        _launch("t2v_attn_mod_bwd", d, dev)
         return dq, dk, dv, dbias, None
+
+
+def _plan_of(key):
+    p = _attn_plan(*key)
+    p.key = key
+    return p
 
 
 def attention_mod(q, k, v, heads, qlay, klay, kv_heads=None, scale=None, causal=False, prefix=None, kv_len=None, q_docs=None, kv_docs=None,
@@ -409,47 +526,15 @@ def attention_mod(q, k, v, heads, qlay, klay, kv_heads=None, scale=None, causal=
     Few query rows over many keys (serving steps, chunks of new tokens) split the keys over workgroups and join them.
     Returns [rows_q, heads * dim]; rows that no sequence owns are zero.  Differentiable in q, k, v and bias; K / V shared by the bdiv batches
     of a layout with lo = 0 get the sum of their gradients.  The order of all sums is fixed: repeated runs are bit-equal."""
-    types = (torch.bfloat16, torch.float16)
-    q, k, v = _tokens(q, "q", types), _tokens(k, "k", types), _tokens(v, "v", types)
     heads = int(heads)
-    kv_heads = heads if kv_heads is None else int(kv_heads)
-    dev, D = q.device, _head_dim(q, heads, "q")
-    if kv_heads <= 0 or heads % kv_heads:
-        _fail(f"{heads} query heads cannot share {kv_heads} key / value heads evenly")
-    if k.shape != v.shape or k.shape[1] != kv_heads * D or not q.dtype == k.dtype == v.dtype or not dev == k.device == v.device:
-        _fail(f"q {tuple(q.shape)} {q.dtype}, k {tuple(k.shape)} {k.dtype}, v {tuple(v.shape)} {v.dtype}: one type, one device, {kv_heads} "
-              f"key / value heads of {D} columns are wanted")
-    if D % 8 or D > 128:
-        _fail(f"attention_mod takes head dims that are multiples of 8 up to 128, got {D}")
-    nb, Sq, Sk = qlay.nbatch, qlay.S, klay.S
-    qf, kf = _layout_facts(qlay, q.shape[0]), _layout_facts(klay, k.shape[0])
-    if nb != klay.nbatch or not qf[0] or not kf[0]:
-        _fail(f"layouts {qlay} over {q.shape[0]} rows and {klay} over {k.shape[0]} rows: as many batches on both sides, rows that exist")
-    if not qf[1]:
-        _fail(f"query layout {qlay} names a row twice")
-    softcap, scale = float(softcap), float(D ** -0.5 if scale is None else scale)
-    if not 0.0 <= softcap < 1e30 or not math.isfinite(scale):
-        _fail(f"softcap {softcap}, scale {scale}: a finite scale and a cap of 0 (none) or more are wanted")
-    if prefix is not None and not causal:
-        _fail("prefix opens a causal mask: pass causal=True with it")
-    if (q_docs is None) != (kv_docs is None):
-        _fail("q_docs and kv_docs come together")
-    _ints(prefix, ((nb,), (nb, Sq)), dev, "prefix")
-    _ints(kv_len, ((nb,),), dev, "kv_len")
-    _ints(q_docs, ((nb, Sq),), dev, "q_docs")
-    _ints(kv_docs, ((nb, Sk),), dev, "kv_docs")
-    if slopes is not None:
-        if slopes.dtype != torch.float32 or tuple(slopes.shape) != (heads,) or slopes.device != dev or not slopes.is_contiguous():
-            _fail(f"slopes must be a contiguous fp32 tensor of {heads} elements on {dev}")
-        if slopes.requires_grad:
-            _fail("slopes are not trained: pass slopes.detach(), or a bias table for a learned distance bias")
-    if bias is not None:
-        if bias.dtype not in (q.dtype, torch.float32) or bias.dim() != 2 or bias.shape[0] != heads or bias.shape[1] % 2 == 0 or \
-                bias.shape[1] > 2049 or bias.device != dev or not bias.is_contiguous():
-            _fail(f"bias must be a contiguous [{heads}, 2R + 1] table with R <= 1024 in {q.dtype} or fp32 on {dev}, got {tuple(bias.shape)} {bias.dtype}")
-    meta = (heads, kv_heads, qlay, klay, scale, int(bool(causal)), softcap)
+    p = _plan_of((_sig(q), _sig(k), _sig(v), heads, heads if kv_heads is None else int(kv_heads), qlay, klay,
+                  (q.shape[-1] // max(heads, 1)) ** -0.5 if scale is None else float(scale), int(bool(causal)), float(softcap), _sig(prefix), _sig(kv_len),
+                  _sig(q_docs), _sig(kv_docs), _sig(slopes), _sig(bias)))
+    if slopes is not None and slopes.requires_grad:
+        _fail("slopes are not trained: pass slopes.detach(), or a bias table for a learned distance bias")
+    masks = (prefix, kv_len, q_docs, kv_docs, slopes)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (bias is not None and bias.requires_grad)):
-        if not kf[1] and not (klay.bdiv > 1 and klay.lo == 0 and klay.hi >= (klay.S - 1) * klay.ss + 1 and klay.ss > 0):
+        if not p.shared_ok:
             _fail(f"key layout {klay} names a row twice: gradients are defined for rows of their own, or shared by the bdiv batches (lo = 0)")
-        return _AttentionMod.apply(q, k, v, bias, (meta, prefix, kv_len, q_docs, kv_docs, slopes))
-    return _attn_fwd(q, k, v, meta, prefix, kv_len, q_docs, kv_docs, slopes, bias, False)[0]
+        return _AttentionMod.apply(q, k, v, bias, (p, masks))
+    return _attn_fwd(p, q, k, v, masks, bias, False)[0]
