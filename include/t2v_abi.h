@@ -296,6 +296,9 @@ int t2v_attn_bwd(const T2VAttn* p, t2v_stream_t stream);
  * into any sum: they may hold anything.  Operands as in T2VAttn with head stride D: element (b, s, h, d) at
  *   ptr + (b / bdiv) * bstride_hi + (b % bdiv) * bstride_lo + s * sstride + h * D + d      (k, v, dk, dv: kv_heads)
  * lse: fp32 [nbatch, heads, Sq], base-2 log-sum-exp in an order of the library's own: kept for the backward call; NULL: not written.
+ * o_rest: NULL, or laid out and typed like o: what rounding o to its type left behind; the backward call's delta = rowsum(dO * O) is formed
+ * with it where it is given again (the error of delta, 2^-9 of bf16's O, is otherwise as large as that of the gradients' own rounding).
+ * scale: 1e-15 to 1e6; softcap: 0 or 1e-6 to 1e4 (the cap's tanh is good to 4e-7 cap: a larger one is no cap for any score that counts).
  * Backward: the descriptor of the forward with d_o, dq, dk, dv, delta (fp32 [nbatch, heads, Sq] scratch) and dbias (NULL or like
  * bias) filled in; every row of dq, dk, dv is written.  kv_share: batches b with the same b / kv_share have one K / V (and one
  * dk / dv, the sum); 1: each has its own.  workspace: t2v_attn_mod_workspace(p, backward) bytes, 256-byte aligned, no
@@ -306,7 +309,7 @@ typedef struct T2VAttnMod {
   int nbatch, heads, kv_heads, Sq, Sk, D, dtype, causal;
   float scale, softcap;
   T2VAttnOperand q, k, v, o;
-  float* lse;
+  float* lse; void* o_rest;
   const int* prefix; int prefix_per_query;
   const int* kv_len;
   const int* q_docs; const int* kv_docs;

@@ -467,6 +467,29 @@ def test_steps_over_a_growing_cache_match_the_whole_sequence():
             assert float((o[0].float() - whole[i].float()).norm() / whole[i].float().norm()) < 6e-3
 
 
+@pytest.mark.parametrize("dim,splits", [(64, False), (128, False), (128, True)])
+def test_delta_is_formed_from_more_of_o_than_its_type_holds(dim, splits):
+    """Values with a large common part: delta = dO . O is large and cancels against dP.  With q = 0 every P is 2^-6 (2^-12), exactly, so the
+    products' fp32 sums, o and its rest (2^-8 of 2^-8), and dS's one rounding are all that dq may be off."""
+    F = _f()
+    n, rows = (4096, 64) if splits else (64, 64)
+    g = torch.Generator().manual_seed(dim + n)
+    v, k = 8 + 0.3 * torch.randn(n, dim, generator=g), 1 + torch.randn(n, dim, generator=g)
+    do = torch.randn(rows, dim, generator=g)
+    k, v, do = (t.to(BF) for t in (k, v, do))
+    q = torch.zeros(rows, dim, dtype=BF, device="cuda", requires_grad=True)
+    kd, vd = k.cuda(), v.cuda()
+    F.attention_mod(q, kd, vd, 1, F.SeqLayout(1, rows, rows, 0, 1), F.SeqLayout(1, n, n, 0, 1)).backward(do.cuda())
+    K, V, G = (t.to(F64) for t in (k, v, do))
+    dP = G @ V.T
+    dS = (dP - dP.mean(1, keepdim=True)) / n
+    want = dS @ K * dim ** -0.5
+    size = (G.abs() @ V.abs().amax(0).unsqueeze(1))                      # >= sum_d |dO||V|, |dO||O|
+    e = 2.0 ** -16 * size + (3 * dim + n // 64) * 2.0 ** -23 * size      # o and its rest; fp32 sums of dP, delta and (over tiles and splits) o
+    bound = ((2.0 ** -8 * dS.abs() + (1 + 2.0 ** -8) * e / n) @ K.abs() + n * 2.0 ** -23 * dS.abs() @ K.abs()) * dim ** -0.5 * (1 + 2.0 ** -8)
+    _within("dq", q.grad, want, bound + 2.0 ** -8 * want.abs())
+
+
 def test_captured_steps_replay_with_new_lengths_and_positions():
     F = _f()
     g = torch.Generator().manual_seed(13)
@@ -615,6 +638,11 @@ def test_refusals():
         lambda: F.attention_mod(x, x.clone().requires_grad_(), x, 2, F.SeqLayout(2, 8, 8, 0, 1), F.SeqLayout(2, 8, 0, 0, 1)),
         lambda: F.attention_mod(x, x, x, 2, lay, lay, softcap=-1.0),
         lambda: F.attention_mod(x, x, x, 2, lay, lay, scale=math.nan),
+        lambda: F.attention_mod(x, x, x, 2, lay, lay, scale=0.0),
+        lambda: F.attention_mod(x, x, x, 2, lay, lay, softcap=1e9),
+        lambda: F.attention_mod(x[:, :0], x[:, :0], x[:, :0], 2, lay, lay),
+        lambda: F.attention_mod(x[:, :1], x[:, :1], x[:, :1], 2, lay, lay),
+        lambda: F.rope(x[:, :0], 2, pos, F.RopeAxes((64,))),
         lambda: F.attention_mod(x, x, x, 2, lay, lay, prefix=i32(1)),
         lambda: F.attention_mod(x, x, x, 2, lay, lay, causal=True, prefix=i32(2)),
         lambda: F.attention_mod(x, x, x, 2, lay, lay, kv_len=i32(1).long()),

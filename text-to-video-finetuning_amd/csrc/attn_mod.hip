@@ -14,7 +14,9 @@
 // Grouped heads: the gp query heads that share a K/V head are packed into the row index (row r = query r / gp, head r % gp), so K and V
 // are read once for all of them; with a table each head is a unit of its own (gp = 1: the table of one head lives in LDS).
 // Statistics, the running maximum and sum, lse, delta and all accumulators are fp32; P and dS are rounded to the input type for the
-// matrix cores (one rounding of a factor in [0, 1], and of a gradient, the same size as the output's own rounding).
+// matrix cores (one rounding of a factor in [0, 1], and of a gradient, the same size as the output's own rounding).  delta_i = dO_i . O_i
+// wants more of O than its type holds: an error of delta stands in every dS of the row and does not average out.  A forward pass that is
+// to be differentiated stores what O's rounding left behind too (o_rest), in the same type.
 #include <type_traits>
 
 #include "common.h"
@@ -26,6 +28,7 @@ constexpr float LOG2E = 1.44269504088896341f;
 constexpr float LOWEST = -1.0e30f;              // running maximum before the first visible key: finite, below every score
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
+typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2_t;
 typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
 
 __device__ __attribute__((aligned(16))) const unsigned zero_chunk[4] = {0, 0, 0, 0};
@@ -38,6 +41,9 @@ struct El<bf16_t> {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
   static __device__ __forceinline__ unsigned pack2(float a, float b) { return pack2bf(a, b); }
+  static __device__ __forceinline__ float add2(unsigned ab, float c) {    // a + b + c in fp32, one instruction
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, ab), __builtin_bit_cast(bf16x2_t, 0x3f803f80u), c, false);
+  }
   static __device__ __forceinline__ float up(short v) { return bf2f((unsigned short)v); }
 };
 template <>
@@ -48,6 +54,9 @@ struct El<_Float16> {
   static __device__ __forceinline__ unsigned pack2(float a, float b) {
     const t2v_f32x2 v = {a, b};
     return __builtin_bit_cast(unsigned, __builtin_convertvector(v, f16x2));
+  }
+  static __device__ __forceinline__ float add2(unsigned ab, float c) {
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, ab), __builtin_bit_cast(f16x2, 0x3c003c00u), c, false);
   }
   static __device__ __forceinline__ float up(short v) { return (float)__builtin_bit_cast(_Float16, v); }
 };
@@ -271,18 +280,31 @@ __device__ __forceinline__ bf16x8 trfrag(const bf16_t* s, int blk, int fm, int k
 }
 
 // 32 FM columns of the lane's row from the accumulators, times mul, 16 bytes per store: the halves of a wave hold columns 4 hi .. 4 hi + 3 of
-// every eight and exchange them first (v_permlane32_swap), so that the lower half stores eight columns and the upper the next eight
+// every eight and exchange them first (v_permlane32_swap), so that the lower half stores eight columns and the upper the next eight.
+// To `rest`, where there is one, goes what the rounding to T left behind
 template <typename T, int FM>
-__device__ __forceinline__ void store_row(bf16_t* row, const f32x16 (&v)[FM], float mul, int hi, int D, bool ok) {
+__device__ __forceinline__ void store_row(bf16_t* row, const f32x16 (&v)[FM], float mul, int hi, int D, bool ok, bf16_t* rest = nullptr) {
+  const auto store = [&](bf16_t* to, const unsigned (&w)[4], int f, int h) {
+    const auto x = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);
+    const auto y = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
+    const int col = 32 * f + 16 * h + 8 * hi;
+    if (ok && col < D) *(u32x4*)(to + col) = u32x4{x[0], y[0], x[1], y[1]};
+  };
 #pragma unroll
   for (int f = 0; f < FM; ++f)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int r = 8 * h;
-      const auto x = __builtin_amdgcn_permlane32_swap(El<T>::pack2(v[f][r] * mul, v[f][r + 1] * mul), El<T>::pack2(v[f][r + 4] * mul, v[f][r + 5] * mul), false, false);
-      const auto y = __builtin_amdgcn_permlane32_swap(El<T>::pack2(v[f][r + 2] * mul, v[f][r + 3] * mul), El<T>::pack2(v[f][r + 6] * mul, v[f][r + 7] * mul), false, false);
-      const int col = 32 * f + 16 * h + 8 * hi;
-      if (ok && col < D) *(u32x4*)(row + col) = u32x4{x[0], y[0], x[1], y[1]};
+      unsigned w[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = El<T>::pack2(v[f][8 * h + 2 * e] * mul, v[f][8 * h + 2 * e + 1] * mul);
+      store(row, w, f, h);
+      if (rest) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          w[e] = El<T>::pack2(fmaf(v[f][8 * h + 2 * e], mul, -El<T>::up((short)(w[e] & 0xffffu))),
+                              fmaf(v[f][8 * h + 2 * e + 1], mul, -El<T>::up((short)(w[e] >> 16))));
+        store(rest, w, f, h);
+      }
     }
 }
 // the accumulators as they are, a wave's registers one after the other (1 KB per instruction): partial sums of the splits
@@ -374,40 +396,35 @@ __device__ __forceinline__ int wave_max_i(int v) {
   return __builtin_amdgcn_readfirstlane(v);
 }
 
-// What a wave knows about the 32 QB query rows of its lanes (lane & 31 = row of the block)
-template <int QB>
+// What a wave knows about the 32 query rows of its lanes (lane & 31 = row of the block)
 struct Rows {
-  int r[QB], i[QB], h[QB];          // row in the unit, query, head
-  bool ok[QB];                      // the row exists
-  int bound[QB], pos[QB], doc[QB];  // bound 0: sees nothing
-  float slope[QB];                  // in base-2 units
+  int r, i, h;                      // row in the unit, query, head
+  bool ok;                          // the row exists
+  int bound, pos, doc;              // bound 0: sees nothing
+  float slope;                      // in base-2 units
   int bmin, bmax, dmin, dmax, pmin; // over the wave
   bool neg;
 };
-template <int QB>
-__device__ __forceinline__ void load_rows(Rows<QB>& R, const Args& a, const Unit& u, const Seq& sq, const Part& part, int r0, int lane) {
+__device__ __forceinline__ void load_rows(Rows& R, const Args& a, const Unit& u, const Seq& sq, const Part& part, int r0, int lane) {
   int lo = 0x7fffffff, hi = 0, dlo = 0x7fffffff, dhi = -1, ng = 0;
-#pragma unroll
-  for (int q = 0; q < QB; ++q) {
-    R.r[q] = r0 + 32 * q + (lane & 31);
-    R.ok[q] = R.r[q] < a.M;
-    const int rc = min(R.r[q], a.M - 1);
-    R.i[q] = div_gp(a, rc);
-    R.h[q] = u.h0 + rc - R.i[q] * a.gp;
-    R.doc[q] = a.p.q_docs ? a.p.q_docs[(long long)u.b * a.p.Sq + R.i[q]] : 0;
-    R.ok[q] = R.ok[q] && part.owns(R.doc[q]);
-    R.bound[q] = R.ok[q] ? row_bound(sq, R.i[q]) : 0;
-    R.pos[q] = R.i[q] + sq.off;
-    if (R.doc[q] < 0) R.bound[q] = 0;
-    R.slope[q] = a.p.slopes ? a.p.slopes[R.h[q]] * LOG2E : 0.f;
-    if (R.ok[q]) lo = min(lo, R.bound[q]);
-    hi = max(hi, R.bound[q]);
-    if (R.bound[q] > 0) {
-      dlo = min(dlo, R.doc[q]);
-      dhi = max(dhi, R.doc[q]);
-    } else if (R.ok[q]) {
-      ng = 1;
-    }
+  R.r = r0 + (lane & 31);
+  R.ok = R.r < a.M;
+  const int rc = min(R.r, a.M - 1);
+  R.i = div_gp(a, rc);
+  R.h = u.h0 + rc - R.i * a.gp;
+  R.doc = a.p.q_docs ? a.p.q_docs[(long long)u.b * a.p.Sq + R.i] : 0;
+  R.ok = R.ok && part.owns(R.doc);
+  R.bound = R.ok ? row_bound(sq, R.i) : 0;
+  R.pos = R.i + sq.off;
+  if (R.doc < 0) R.bound = 0;
+  R.slope = a.p.slopes ? a.p.slopes[R.h] * LOG2E : 0.f;
+  if (R.ok) lo = min(lo, R.bound);
+  hi = max(hi, R.bound);
+  if (R.bound > 0) {
+    dlo = min(dlo, R.doc);
+    dhi = max(dhi, R.doc);
+  } else if (R.ok) {
+    ng = 1;
   }
   R.bmin = wave_min_i(lo);
   R.pmin = __builtin_amdgcn_readfirstlane(div_gp(a, min(r0, a.M - 1)) + sq.off);      // rows are in the queries' order
@@ -419,8 +436,8 @@ __device__ __forceinline__ void load_rows(Rows<QB>& R, const Args& a, const Unit
 
 // ------------------------------------------------------------------------------------------------ forward
 // MOD: bit 0 cap, bit 1 distance bias (slopes / table), compile-time so that a tile is straight-line code
-template <typename T, int DP, int QB, int MOD>
-__global__ __launch_bounds__(256, DP == 64 && MOD < 2 ? 3 : DP * QB <= 128 ? 2 : 1) void attn_mod_fwd_kernel(const Args a) {
+template <typename T, int DP, int MOD>
+__global__ __launch_bounds__(256, DP == 64 && MOD < 2 ? 3 : 2) void attn_mod_fwd_kernel(const Args a) {
   warm_kernargs<(int)sizeof(Args)>();
   constexpr int NT = 256, KD = DP / 16, FM = DP / 32;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -442,15 +459,12 @@ __global__ __launch_bounds__(256, DP == 64 && MOD < 2 ? 3 : DP * QB <= 128 ? 2 :
   const int* kdoc = docs ? a.p.kv_docs + (long long)u.b * Sk : nullptr;
   const Mod mod = make_mod(a);
 
-  Rows<QB> R;
-  load_rows(R, a, u, seq, part, (tile * 4 + wave) * 32 * QB, lane);
-  bf16x8 qf[QB][KD];
+  Rows R;
+  load_rows(R, a, u, seq, part, (tile * 4 + wave) * 32, lane);
+  bf16x8 qf[KD];
+  const bf16_t* qp = Q + (long long)R.i * a.p.q.sstride + (long long)R.h * D;
 #pragma unroll
-  for (int q = 0; q < QB; ++q) {
-    const bf16_t* qp = Q + (long long)R.i[q] * a.p.q.sstride + (long long)R.h[q] * D;
-#pragma unroll
-    for (int kd = 0; kd < KD; ++kd) qf[q][kd] = *chunk_ptr(qp + 16 * kd + 8 * hi, R.bound[q] > 0 && 16 * kd + 8 * hi < D);
-  }
+  for (int kd = 0; kd < KD; ++kd) qf[kd] = *chunk_ptr(qp + 16 * kd + 8 * hi, R.bound > 0 && 16 * kd + 8 * hi < D);
   if ((MOD & 2) && mod.table) load_table<T>(a, u.h0, tab, tid, NT);
   if (lane == 0) {
     swg[wave * 4] = R.bmax;
@@ -500,29 +514,22 @@ __global__ __launch_bounds__(256, DP == 64 && MOD < 2 ? 3 : DP * QB <= 128 ? 2 :
     }
   };
 
-  float m[QB], l[QB];
-  f32x16 o[QB][FM], s[QB][2];
+  const float defer = a.p.o_rest ? 0.f : 6.f;
+  float m = LOWEST, l = 0.f;
+  f32x16 o[FM], s[2];
 #pragma unroll
-  for (int q = 0; q < QB; ++q) {
-    m[q] = LOWEST;
-    l[q] = 0.f;
+  for (int f = 0; f < FM; ++f)
 #pragma unroll
-    for (int f = 0; f < FM; ++f)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) o[q][f][r] = 0.f;
-  }
-  auto scores = [&](f32x16 (&x)[QB][2], const bf16_t* sk) {             // K Q^T of a tile
+    for (int r = 0; r < 16; ++r) o[f][r] = 0.f;
+  auto scores = [&](f32x16 (&x)[2], const bf16_t* sk) {                 // K Q^T of a tile
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
 #pragma unroll
-      for (int q = 0; q < QB; ++q)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) x[q][kb][r] = 0.f;
+      for (int r = 0; r < 16; ++r) x[kb][r] = 0.f;
 #pragma unroll
       for (int kd = 0; kd < KD; ++kd) {
         const bf16x8 kf = rowfrag<DP>(sk + lrow, kb, kd);
-#pragma unroll
-        for (int q = 0; q < QB; ++q) x[q][kb] = El<T>::mfma(kf, qf[q][kd], x[q][kb]);
+        x[kb] = El<T>::mfma(kf, qf[kd], x[kb]);
       }
     }
   };
@@ -551,118 +558,117 @@ __global__ __launch_bounds__(256, DP == 64 && MOD < 2 ? 3 : DP * QB <= 128 ? 2 :
       if (docs) some |= (kn.neg != 0) | (kn.dmin != kn.dmax) | (R.dmin != R.dmax) | R.neg | (kn.dmin != R.dmin);
       const bool partial = __builtin_amdgcn_readfirstlane(some);
       const bf16_t* sv = st[cur].b;
-      f32x16 n[QB][2];
+      f32x16 n[2];
       const float c = MOD ? 1.f : mod.c;
-      float off[QB][2];                                                 // score = s + off[kb]
+      float off[2];                                                     // score = s + off[kb]
       if (MOD & 1) {                                                    // the cap's exponentials run beside the next tile's scores
         scores(n, st[cur ^ 1].a);
 #pragma unroll
-        for (int q = 0; q < QB; ++q)
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            float w;
+            s[kb][r] = capped(mod, s[kb][r], w);
+          }
+      }
+      off[0] = off[1] = 0.f;
+      if (MOD & 2) {
+        const int d0 = k0 + 4 * hi - R.pos;
+        const float cc = (MOD & 1) ? 1.f : mod.c;
+        if (mod.slope) {
+          if (k0 + TILE - 1 <= R.pmin) {                              // every key at or before every query: |d| = -d, linear in the row
+            const float sl = R.slope;
+            off[0] = sl * (float)d0;
+            off[1] = sl * (float)(d0 + 32);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const float b = sl * (float)crow(r, 0);
+              s[0][r] = fmaf(s[0][r], cc, b);
+              s[1][r] = fmaf(s[1][r], cc, b);
+            }
+          } else {
+            const float f0 = (float)d0;
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+              for (int r = 0; r < 16; ++r)
+                s[kb][r] = fmaf(-R.slope, fabsf(f0 + (32 * kb + crow(r, 0))), s[kb][r] * cc);
+          }
+        } else if (!(MOD & 1)) {
 #pragma unroll
           for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-              float w;
-              s[q][kb][r] = capped(mod, s[q][kb][r], w);
-            }
+            for (int r = 0; r < 16; ++r) s[kb][r] *= cc;
+        }
+        if (mod.table) {
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[kb][r] += tab[max(-mod.R, min(mod.R, d0 + 32 * kb + crow(r, 0))) + mod.R];
+        }
       }
+      if (partial) {
 #pragma unroll
-      for (int q = 0; q < QB; ++q) {
-        off[q][0] = off[q][1] = 0.f;
-        if (MOD & 2) {
-          const int d0 = k0 + 4 * hi - R.pos[q];
-          const float cc = (MOD & 1) ? 1.f : mod.c;
-          if (mod.slope) {
-            if (k0 + TILE - 1 <= R.pmin) {                              // every key at or before every query: |d| = -d, linear in the row
-              const float sl = R.slope[q];
-              off[q][0] = sl * (float)d0;
-              off[q][1] = sl * (float)(d0 + 32);
+        for (int kb = 0; kb < 2; ++kb) {
+          const int lim = R.bound - k0 - 32 * kb - 4 * hi;
 #pragma unroll
-              for (int r = 0; r < 16; ++r) {
-                const float b = sl * (float)crow(r, 0);
-                s[q][0][r] = fmaf(s[q][0][r], cc, b);
-                s[q][1][r] = fmaf(s[q][1][r], cc, b);
-              }
-            } else {
-              const float f0 = (float)d0;
+          for (int r = 0; r < 16; ++r) s[kb][r] = crow(r, 0) < lim ? s[kb][r] : -INFINITY;
+          if (docs) {
 #pragma unroll
-              for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                  s[q][kb][r] = fmaf(-R.slope[q], fabsf(f0 + (32 * kb + crow(r, 0))), s[q][kb][r] * cc);
-            }
-          } else if (!(MOD & 1)) {
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-              for (int r = 0; r < 16; ++r) s[q][kb][r] *= cc;
-          }
-          if (mod.table) {
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-              for (int r = 0; r < 16; ++r) s[q][kb][r] += tab[max(-mod.R, min(mod.R, d0 + 32 * kb + crow(r, 0))) + mod.R];
-          }
-        }
-        if (partial) {
-#pragma unroll
-          for (int kb = 0; kb < 2; ++kb) {
-            const int lim = R.bound[q] - k0 - 32 * kb - 4 * hi;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[q][kb][r] = crow(r, 0) < lim ? s[q][kb][r] : -INFINITY;
-            if (docs) {
-#pragma unroll
-              for (int g = 0; g < 4; ++g) {
-                const int4 dv = *(const int4*)(sdoc + cur * TILE + 32 * kb + 8 * g + 4 * hi);
-                s[q][kb][4 * g] = dv.x == R.doc[q] ? s[q][kb][4 * g] : -INFINITY;
-                s[q][kb][4 * g + 1] = dv.y == R.doc[q] ? s[q][kb][4 * g + 1] : -INFINITY;
-                s[q][kb][4 * g + 2] = dv.z == R.doc[q] ? s[q][kb][4 * g + 2] : -INFINITY;
-                s[q][kb][4 * g + 3] = dv.w == R.doc[q] ? s[q][kb][4 * g + 3] : -INFINITY;
-              }
+            for (int g = 0; g < 4; ++g) {
+              const int4 dv = *(const int4*)(sdoc + cur * TILE + 32 * kb + 8 * g + 4 * hi);
+              s[kb][4 * g] = dv.x == R.doc ? s[kb][4 * g] : -INFINITY;
+              s[kb][4 * g + 1] = dv.y == R.doc ? s[kb][4 * g + 1] : -INFINITY;
+              s[kb][4 * g + 2] = dv.z == R.doc ? s[kb][4 * g + 2] : -INFINITY;
+              s[kb][4 * g + 3] = dv.w == R.doc ? s[kb][4 * g + 3] : -INFINITY;
             }
           }
         }
-        float mx0 = s[q][0][0], mx1 = s[q][1][0];
+      }
+      float mx0 = s[0][0], mx1 = s[1][0];
 #pragma unroll
-        for (int r = 1; r < 16; ++r) {
-          mx0 = fmaxf(mx0, s[q][0][r]);
-          mx1 = fmaxf(mx1, s[q][1][r]);
-        }
-        const float mx = half_max(fmaxf(mx0 + off[q][0], mx1 + off[q][1]));
-        // the running maximum is raised only when some row of the wave grew by more than DEFER exponent units: p <= 2^DEFER instead of
-        // <= 1, the same relative precision, and the common tile skips the rescale of O
-        constexpr float DEFER = 6.f;
-        if (!__all((mx - m[q]) * c <= DEFER)) {
-          const float mn = fmaxf(m[q], mx);
-          const float alpha = __builtin_amdgcn_exp2f((m[q] - mn) * c);
-          m[q] = mn;
-          l[q] *= alpha;
+      for (int r = 1; r < 16; ++r) {
+        mx0 = fmaxf(mx0, s[0][r]);
+        mx1 = fmaxf(mx1, s[1][r]);
+      }
+      const float mx = half_max(fmaxf(mx0 + off[0], mx1 + off[1]));
+      // The running maximum is raised only when some row of the wave grew by more than `defer` exponent units: p <= 2^defer instead of
+      // <= 1, and the common tile skips the rescale of O (8192 x 8192, 16 heads: 678 us, with defer = 0 702).  A pass that is to be differentiated
+      // raises it at once: the weight of a key that dominates its row is then 1, which P's type holds exactly, and delta comes out closer
+      // (dQ 0.0025 -> 0.0024 of its norm off where scores have a deviation of 4; dS's and the result's own rounding are 0.0023).
+      if (!__all((mx - m) * c <= defer)) {
+        const float mn = fmaxf(m, mx);
+        const float alpha = __builtin_amdgcn_exp2f((m - mn) * c);
+        m = mn;
+        l *= alpha;
 #pragma unroll
-          for (int f = 0; f < FM; ++f)
+        for (int f = 0; f < FM; ++f)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) o[q][f][r] *= alpha;
-        }
+          for (int r = 0; r < 16; ++r) o[f][r] *= alpha;
       }
       // one straight block: the next tile's scores, this tile's exponentials, P V  (behind the last tile the scores are of stale rows, unused)
       if (!(MOD & 1)) scores(n, st[cur ^ 1].a);
-      bf16x8 pb[QB][4];
+      bf16x8 pb[4];
+      float rs[2] = {0.f, 0.f};
 #pragma unroll
-      for (int q = 0; q < QB; ++q) {
-        float rs[2] = {0.f, 0.f};
+      for (int kb = 0; kb < 2; ++kb) {
+        const float mc = MOD ? m - off[kb] : m * c;
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-          const float mc = MOD ? m[q] - off[q][kb] : m[q] * c;
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const float pv = __builtin_amdgcn_exp2f(MOD ? s[q][kb][r] - mc : fmaf(s[q][kb][r], c, -mc));
-            s[q][kb][r] = pv;
-            rs[r & 1] += pv;
-          }
-          pb[q][2 * kb] = pack8<T>(s[q][kb], 0);
-          pb[q][2 * kb + 1] = pack8<T>(s[q][kb], 1);
+        for (int r = 0; r < 16; ++r) {
+          const float pv = __builtin_amdgcn_exp2f(MOD ? s[kb][r] - mc : fmaf(s[kb][r], c, -mc));
+          s[kb][r] = pv;
         }
-        l[q] += rs[0] + rs[1];
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+          pb[2 * kb + kk] = pack8<T>(s[kb], kk);
+          // The sum is of the rounded weights, those that multiply V: O is a mean of V with slightly other weights, never off by a factor.  Two
+          // weights are added by one instruction (D = 64, 8192 x 8192, 16 heads: 400 -> 370 us)
+          const u32x4 w = __builtin_bit_cast(u32x4, pb[2 * kb + kk]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) rs[e & 1] = El<T>::add2(w[e], rs[e & 1]);
+        }
       }
+      l += rs[0] + rs[1];
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
@@ -670,14 +676,10 @@ __global__ __launch_bounds__(256, DP == 64 && MOD < 2 ? 3 : DP * QB <= 128 ? 2 :
 #pragma unroll
           for (int f = 0; f < FM; ++f) {
             const bf16x8 vf = trfrag<DP>(sv + ltr, kb, f, kk);
-#pragma unroll
-            for (int q = 0; q < QB; ++q) o[q][f] = El<T>::mfma(vf, pb[q][2 * kb + kk], o[q][f]);
+            o[f] = El<T>::mfma(vf, pb[2 * kb + kk], o[f]);
           }
-#pragma unroll
-      for (int q = 0; q < QB; ++q) {
-        s[q][0] = n[q][0];
-        s[q][1] = n[q][1];
-      }
+      s[0] = n[0];
+      s[1] = n[1];
     }
     if (t1 < tend) landed(t1, cur ^ 1, docs ? k1.neg : 0);
     cur ^= 1;
@@ -685,21 +687,18 @@ __global__ __launch_bounds__(256, DP == 64 && MOD < 2 ? 3 : DP * QB <= 128 ? 2 :
     t1 = t2;
     kn = k1;
   }
-#pragma unroll
-  for (int q = 0; q < QB; ++q) {
-    const float lt = half_sum(l[q]);
-    const float m2 = MOD ? m[q] : m[q] * mod.c;
-    if (a.splits > 1) {
-      const long long block = (((long long)sp * NU + u.x) * a.ntile + tile) * 4 * QB + wave * QB + q;       // of 32 rows
-      store_part<FM>(a.part + block * (32 * DP), o[q], lane, R.ok[q]);
-      if (R.ok[q] && hi == 0) *(float2*)(a.part_ml + (block * 32 + lane) * 2) = float2{m2, lt};
-    } else {
-      bf16_t* op = (bf16_t*)a.p.o.ptr + op_base(a.p.o, u.b) + (long long)R.i[q] * a.p.o.sstride + (long long)R.h[q] * D;
-      store_row<T, FM>(op, o[q], lt > 0.f ? 1.f / lt : 0.f, hi, D, R.ok[q]);
-      // base-2 log-sum-exp; +inf marks a row that saw nothing: every exp2(t - lse) of the backward pass is then 0
-      if (R.ok[q] && hi == 0 && a.p.lse)
-        a.p.lse[((long long)u.b * a.p.heads + u.h0) * a.p.Sq + R.r[q]] = lt > 0.f ? m2 + __builtin_amdgcn_logf(lt) : INFINITY;
-    }
+  const float lt = half_sum(l);
+  const float m2 = MOD ? m : m * mod.c;
+  if (a.splits > 1) {
+    const long long block = (((long long)sp * NU + u.x) * a.ntile + tile) * 4 + wave;       // of 32 rows
+    store_part<FM>(a.part + block * (32 * DP), o, lane, R.ok);
+    if (R.ok && hi == 0) *(float2*)(a.part_ml + (block * 32 + lane) * 2) = float2{m2, lt};
+  } else {
+    const long long at = op_base(a.p.o, u.b) + (long long)R.i * a.p.o.sstride + (long long)R.h * D;
+    store_row<T, FM>((bf16_t*)a.p.o.ptr + at, o, lt > 0.f ? 1.f / lt : 0.f, hi, D, R.ok, a.p.o_rest ? (bf16_t*)a.p.o_rest + at : nullptr);
+    // base-2 log-sum-exp; +inf marks a row that saw nothing: every exp2(t - lse) of the backward pass is then 0
+    if (R.ok && hi == 0 && a.p.lse)
+      a.p.lse[((long long)u.b * a.p.heads + u.h0) * a.p.Sq + R.r] = lt > 0.f ? m2 + __builtin_amdgcn_logf(lt) : INFINITY;
   }
 }
 
@@ -755,8 +754,8 @@ __global__ __launch_bounds__(64) void attn_mod_join_kernel(const Args a) {
   }
   const Unit u = unit_of(a, x);
   const int i = div_gp(a, min(r, a.M - 1)), h = u.h0 + min(r, a.M - 1) - i * a.gp;
-  bf16_t* op = (bf16_t*)a.p.o.ptr + op_base(a.p.o, u.b) + (long long)i * a.p.o.sstride + (long long)h * D + 32 * f;
-  store_row<T, 1>(op, acc, l > 0.f ? 1.f / l : 0.f, hi, D - 32 * f, ok);
+  const long long col = op_base(a.p.o, u.b) + (long long)i * a.p.o.sstride + (long long)h * D + 32 * f;
+  store_row<T, 1>((bf16_t*)a.p.o.ptr + col, acc, l > 0.f ? 1.f / l : 0.f, hi, D - 32 * f, ok, a.p.o_rest ? (bf16_t*)a.p.o_rest + col : nullptr);
   if (ok && f == 0 && hi == 0 && a.p.lse) a.p.lse[((long long)u.b * a.p.heads + u.h0) * a.p.Sq + r] = l > 0.f ? m + __builtin_amdgcn_logf(l) : INFINITY;
 }
 
@@ -836,8 +835,8 @@ __global__ __launch_bounds__(1024) void attn_mod_order_kernel(const Args a, int*
 }
 
 // ------------------------------------------------------------------------------------------------ backward: dQ, delta, table gradient
-template <typename T, int DP, int QB, int MOD>
-__global__ __launch_bounds__(256, (DP * QB <= 128) ? 2 : 1) void attn_mod_dq_kernel(const Args a) {
+template <typename T, int DP, int MOD>
+__global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(const Args a) {
   warm_kernargs<(int)sizeof(Args)>();
   constexpr int NT = 256, KD = DP / 16, FM = DP / 32;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -865,31 +864,25 @@ __global__ __launch_bounds__(256, (DP * QB <= 128) ? 2 : 1) void attn_mod_dq_ker
   float* sums = tab + ntab + wave * ntab;
   const bool dtab = (MOD & 2) && mod.table && a.p.dbias != nullptr;
 
-  Rows<QB> R;
-  load_rows(R, a, u, seq, part, (tile * 4 + wave) * 32 * QB, lane);
-  bf16x8 qf[QB][KD], gf[QB][KD];
-  float lse[QB], dl[QB];
+  Rows R;
+  load_rows(R, a, u, seq, part, (tile * 4 + wave) * 32, lane);
+  bf16x8 qf[KD], gf[KD];
+  const bf16_t* qp = (const bf16_t*)a.p.q.ptr + op_base(a.p.q, u.b) + (long long)R.i * a.p.q.sstride + (long long)R.h * D;
+  const bf16_t* gp = (const bf16_t*)a.p.d_o.ptr + op_base(a.p.d_o, u.b) + (long long)R.i * a.p.d_o.sstride + (long long)R.h * D;
+  const bf16_t* op = (const bf16_t*)a.p.o.ptr + op_base(a.p.o, u.b) + (long long)R.i * a.p.o.sstride + (long long)R.h * D;
+  const bool rest = a.p.o_rest != nullptr;
+  const bf16_t* orest = rest ? (const bf16_t*)a.p.o_rest + (op - (const bf16_t*)a.p.o.ptr) : op;
+  bf16x8 of[KD], og[KD];
 #pragma unroll
-  for (int q = 0; q < QB; ++q) {
-    const bf16_t* qp = (const bf16_t*)a.p.q.ptr + op_base(a.p.q, u.b) + (long long)R.i[q] * a.p.q.sstride + (long long)R.h[q] * D;
-    const bf16_t* gp = (const bf16_t*)a.p.d_o.ptr + op_base(a.p.d_o, u.b) + (long long)R.i[q] * a.p.d_o.sstride + (long long)R.h[q] * D;
-    const bf16_t* op = (const bf16_t*)a.p.o.ptr + op_base(a.p.o, u.b) + (long long)R.i[q] * a.p.o.sstride + (long long)R.h[q] * D;
-    float d = 0.f;
-#pragma unroll
-    for (int kd = 0; kd < KD; ++kd) {
-      const bool ok = R.bound[q] > 0 && 16 * kd + 8 * hi < D;
-      qf[q][kd] = *chunk_ptr(qp + 16 * kd + 8 * hi, ok);
-      gf[q][kd] = *chunk_ptr(gp + 16 * kd + 8 * hi, ok);
-      const bf16x8 of = *chunk_ptr(op + 16 * kd + 8 * hi, ok);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) d = fmaf(El<T>::up(of[e]), El<T>::up(gf[q][kd][e]), d);
-    }
-    d = half_sum(d);
-    dl[q] = d;
-    const long long sidx = ((long long)u.b * a.p.heads + u.h0) * a.p.Sq + min(R.r[q], a.M - 1);
-    lse[q] = R.ok[q] ? a.p.lse[sidx] : INFINITY;
-    if (R.ok[q] && hi == 0) a.p.delta[sidx] = d;
+  for (int kd = 0; kd < KD; ++kd) {
+    const bool ok = R.bound > 0 && 16 * kd + 8 * hi < D;
+    qf[kd] = *chunk_ptr(qp + 16 * kd + 8 * hi, ok);
+    gf[kd] = *chunk_ptr(gp + 16 * kd + 8 * hi, ok);
+    of[kd] = *chunk_ptr(op + 16 * kd + 8 * hi, ok);
+    og[kd] = *chunk_ptr(orest + 16 * kd + 8 * hi, ok && rest);
   }
+  const long long sidx = ((long long)u.b * a.p.heads + u.h0) * a.p.Sq + min(R.r, a.M - 1);
+  const float lse = R.ok ? a.p.lse[sidx] : INFINITY;
   if ((MOD & 2) && mod.table) load_table<T>(a, u.h0, tab, tid, NT);
   if (dtab)
     for (int i = lane; i < ntab; i += 64) sums[i] = 0.f;
@@ -935,120 +928,116 @@ __global__ __launch_bounds__(256, (DP * QB <= 128) ? 2 : 1) void attn_mod_dq_ker
       __syncthreads();
     }
   };
-  f32x16 acc[QB][FM];
+  f32x16 acc[FM];
 #pragma unroll
-  for (int q = 0; q < QB; ++q)
+  for (int f = 0; f < FM; ++f)
 #pragma unroll
-    for (int f = 0; f < FM; ++f)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc[q][f][r] = 0.f;
+    for (int r = 0; r < 16; ++r) acc[f][r] = 0.f;
   float below = 0.f, above = 0.f;                                       // gradient of the table's two ends, per lane
   int t = tile_next(it, active), cur = 0;
   KMeta kn = {0, 0, 0};                                                 // of the tile at hand (documents)
   if (t < tend) {
     if (docs) kn = tile_entry(km, t);
     fetch(t, 0);
-    landed(t, 0, kn.neg);
   }
+  float dl = 0.f;                                                       // delta, while the first tile is on its way
+#pragma unroll
+  for (int kd = 0; kd < KD; ++kd)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) dl = fmaf(El<T>::up(of[kd][e]) + El<T>::up(og[kd][e]), El<T>::up(gf[kd][e]), dl);
+  dl = half_sum(dl);
+  if (R.ok && hi == 0) a.p.delta[sidx] = dl;
+  if (t < tend) landed(t, 0, kn.neg);
   auto math = [&](bool partial, int t) {
     const int k0 = t * TILE;
     const bf16_t* sk = st[cur].a;
     const bf16_t* sv = st[cur].b;
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
-      f32x16 s[QB], dp[QB];
+      f32x16 s, dp;
 #pragma unroll
-      for (int q = 0; q < QB; ++q)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[q][r] = dp[q][r] = 0.f;
+      for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.f;
 #pragma unroll
       for (int kd = 0; kd < KD; ++kd) {
         const bf16x8 kf = rowfrag<DP>(sk + lrow, kb, kd), vf = rowfrag<DP>(sv + lrow, kb, kd);
-#pragma unroll
-        for (int q = 0; q < QB; ++q) {
-          s[q] = El<T>::mfma(kf, qf[q][kd], s[q]);
-          dp[q] = El<T>::mfma(vf, gf[q][kd], dp[q]);
-        }
+        s = El<T>::mfma(kf, qf[kd], s);
+        dp = El<T>::mfma(vf, gf[kd], dp);
       }
-      bf16x8 db[QB][2];
-#pragma unroll
-      for (int q = 0; q < QB; ++q) {
-        const int d0 = k0 + 32 * kb + 4 * hi - R.pos[q];
-        f32x16 w;                                                       // derivative of the cap
-        if (MOD & 1) {
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            float y;
-            s[q][r] = capped(mod, s[q][r], y);
-            w[r] = 4.f * y * (1.f - y);
-          }
-        } else if (MOD & 2) {
-#pragma unroll
-          for (int r = 0; r < 16; ++r) s[q][r] *= mod.c;
-        }
-        if (MOD & 2) {
-          if (mod.slope) {
-            const float f0 = (float)d0;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[q][r] = fmaf(-R.slope[q], fabsf(f0 + crow(r, 0)), s[q][r]);
-          }
-          if (mod.table) {
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[q][r] += tab[max(-mod.R, min(mod.R, d0 + crow(r, 0))) + mod.R];
-          }
-        }
+      bf16x8 db[2];
+      const int d0 = k0 + 32 * kb + 4 * hi - R.pos;
+      f32x16 w;                                                         // derivative of the cap
+      if (MOD & 1) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const float pv = __builtin_amdgcn_exp2f(MOD ? s[q][r] - lse[q] : fmaf(s[q][r], mod.c, -lse[q]));
-          s[q][r] = pv * (dp[q][r] - dl[q]);
+          float y;
+          s[r] = capped(mod, s[r], y);
+          w[r] = 4.f * y * (1.f - y);
         }
-        if (partial) {
-          const int lim = R.bound[q] - k0 - 32 * kb - 4 * hi;
+      } else if (MOD & 2) {
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s[q][r] = crow(r, 0) < lim ? s[q][r] : 0.f;
-          if (docs) {
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-              const int4 dv = *(const int4*)(sdoc + cur * TILE + 32 * kb + 8 * g + 4 * hi);
-              s[q][4 * g] = dv.x == R.doc[q] ? s[q][4 * g] : 0.f;
-              s[q][4 * g + 1] = dv.y == R.doc[q] ? s[q][4 * g + 1] : 0.f;
-              s[q][4 * g + 2] = dv.z == R.doc[q] ? s[q][4 * g + 2] : 0.f;
-              s[q][4 * g + 3] = dv.w == R.doc[q] ? s[q][4 * g + 3] : 0.f;
-            }
-          }
-        }
-        if ((MOD & 2) && dtab) {
-          // sums over diagonals, in the wave's own table, by LDS additions that complete in program order: a register's 32 lanes of one
-          // half hold 32 different distances, so one half at a time meets no address twice and the order of the additions is fixed
-          // (the wave barriers keep the compiler from joining the two halves); the clipped ends are summed per lane
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int d = d0 + crow(r, 0);
-            const float v = s[q][r];
-            const bool in = d > -mod.R && d < mod.R;
-            below += d <= -mod.R ? v : 0.f;
-            above += (d >= mod.R && d > -mod.R) ? v : 0.f;
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              if (in && hi == half) __builtin_amdgcn_ds_atomic_fadd_f32((__attribute__((address_space(3))) float*)(sums + d + mod.R), v);
-              __builtin_amdgcn_wave_barrier();
-            }
-          }
-        }
-        if (MOD & 1) {
-#pragma unroll
-          for (int r = 0; r < 16; ++r) s[q][r] *= w[r];
-        }
-        db[q][0] = pack8<T>(s[q], 0);
-        db[q][1] = pack8<T>(s[q], 1);
+        for (int r = 0; r < 16; ++r) s[r] *= mod.c;
       }
+      if (MOD & 2) {
+        if (mod.slope) {
+          const float f0 = (float)d0;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[r] = fmaf(-R.slope, fabsf(f0 + crow(r, 0)), s[r]);
+        }
+        if (mod.table) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[r] += tab[max(-mod.R, min(mod.R, d0 + crow(r, 0))) + mod.R];
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float pv = __builtin_amdgcn_exp2f(MOD ? s[r] - lse : fmaf(s[r], mod.c, -lse));
+        s[r] = pv * (dp[r] - dl);
+      }
+      if (partial) {
+        const int lim = R.bound - k0 - 32 * kb - 4 * hi;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = crow(r, 0) < lim ? s[r] : 0.f;
+        if (docs) {
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const int4 dv = *(const int4*)(sdoc + cur * TILE + 32 * kb + 8 * g + 4 * hi);
+            s[4 * g] = dv.x == R.doc ? s[4 * g] : 0.f;
+            s[4 * g + 1] = dv.y == R.doc ? s[4 * g + 1] : 0.f;
+            s[4 * g + 2] = dv.z == R.doc ? s[4 * g + 2] : 0.f;
+            s[4 * g + 3] = dv.w == R.doc ? s[4 * g + 3] : 0.f;
+          }
+        }
+      }
+      if ((MOD & 2) && dtab) {
+        // sums over diagonals, in the wave's own table, by LDS additions that complete in program order: a register's 32 lanes of one
+        // half hold 32 different distances, so one half at a time meets no address twice and the order of the additions is fixed
+        // (the wave barriers keep the compiler from joining the two halves); the clipped ends are summed per lane
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int d = d0 + crow(r, 0);
+          const float v = s[r];
+          const bool in = d > -mod.R && d < mod.R;
+          below += d <= -mod.R ? v : 0.f;
+          above += (d >= mod.R && d > -mod.R) ? v : 0.f;
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            if (in && hi == half) __builtin_amdgcn_ds_atomic_fadd_f32((__attribute__((address_space(3))) float*)(sums + d + mod.R), v);
+            __builtin_amdgcn_wave_barrier();
+          }
+        }
+      }
+      if (MOD & 1) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] *= w[r];
+      }
+      db[0] = pack8<T>(s, 0);
+      db[1] = pack8<T>(s, 1);
 #pragma unroll
       for (int kk = 0; kk < 2; ++kk)
 #pragma unroll
         for (int f = 0; f < FM; ++f) {
           const bf16x8 kT = trfrag<DP>(sk + ltr, kb, f, kk);
-#pragma unroll
-          for (int q = 0; q < QB; ++q) acc[q][f] = El<T>::mfma(kT, db[q][kk], acc[q][f]);
+          acc[f] = El<T>::mfma(kT, db[kk], acc[f]);
         }
     }
   };
@@ -1069,11 +1058,8 @@ __global__ __launch_bounds__(256, (DP * QB <= 128) ? 2 : 1) void attn_mod_dq_ker
     cur ^= 1;
     t = tn;
   }
-#pragma unroll
-  for (int q = 0; q < QB; ++q) {
-    bf16_t* op = (bf16_t*)a.p.dq.ptr + op_base(a.p.dq, u.b) + (long long)R.i[q] * a.p.dq.sstride + (long long)R.h[q] * D;
-    store_row<T, FM>(op, acc[q], a.p.scale, hi, D, R.ok[q]);
-  }
+  bf16_t* dqp = (bf16_t*)a.p.dq.ptr + op_base(a.p.dq, u.b) + (long long)R.i * a.p.dq.sstride + (long long)R.h * D;
+  store_row<T, FM>(dqp, acc, a.p.scale, hi, D, R.ok);
   if (dtab) {
     below = wave_sum(below);
     above = wave_sum(above);
@@ -1427,11 +1413,14 @@ int check_mod(const char* fn, const T2VAttnMod* p, bool bwd) {
   T2V_CHECK_ARG(p->heads % p->kv_heads == 0, "%s: %d heads cannot share %d key / value heads evenly", fn, p->heads, p->kv_heads);
   T2V_CHECK_ARG(p->D >= 8 && p->D <= 128 && p->D % 8 == 0, "%s: the head dim must be a multiple of 8 up to 128 (got %d)", fn, p->D);
   T2V_CHECK_ARG(p->dtype == 0 || p->dtype == 1, "%s: bf16 (0) or fp16 (1) operands are wanted", fn);
-  T2V_CHECK_ARG(p->softcap >= 0.f && p->softcap < 1e30f && p->scale == p->scale, "%s: bad softcap / scale", fn);
+  T2V_CHECK_ARG(p->scale >= 1e-15f && p->scale <= 1e6f && (p->softcap == 0.f || (p->softcap >= 1e-6f && p->softcap <= 1e4f)),
+                "%s: the scale must lie in [1e-15, 1e6], the cap be 0 or lie in [1e-6, 1e4]", fn);
   T2V_CHECK_ARG((p->q_docs == nullptr) == (p->kv_docs == nullptr), "%s: documents of queries and keys come together", fn);
   T2V_CHECK_ARG(!p->prefix || p->causal, "%s: a prefix opens a causal mask: set causal", fn);
   T2V_CHECK_ARG(!p->bias || (p->radius >= 0 && p->radius <= 1024), "%s: the table's radius must be 0..1024 (got %d)", fn, p->radius);
   T2V_CHECK_ARG((long long)p->Sq * p->heads < (1ll << 26) && p->Sk < (1 << 26), "%s: too many rows (Sq * heads and Sk below 2^26)", fn);
+  T2V_CHECK_ARG((long long)p->Sq * (p->heads / p->kv_heads) * (p->heads / p->kv_heads) < (1ll << 32),
+                "%s: too many query heads of one key / value head (Sq * (heads / kv_heads)^2 below 2^32)", fn);      // (Args::magic is exact below it)
   T2V_CHECK_ARG((long long)p->nbatch * p->heads < (1 << 20), "%s: nbatch * heads below 2^20 is wanted", fn);
   const T2VAttnOperand* ops[] = {&p->q, &p->k, &p->v, &p->o, &p->d_o, &p->dq, &p->dk, &p->dv};
   const char* names[] = {"q", "k", "v", "o", "d_o", "dq", "dk", "dv"};
@@ -1441,6 +1430,7 @@ int check_mod(const char* fn, const T2VAttnMod* p, bool bwd) {
                       o.sstride >= 0 && o.sstride < (1ll << 31),
                   "%s: operand %s: 16-byte aligned rows, less than 2^31 elements apart, are wanted (ptr %p, row stride %lld)", fn, names[i], o.ptr, o.sstride);
   }
+  T2V_CHECK_ARG(((uintptr_t)p->o_rest & 15) == 0, "%s: o_rest must be 16-byte aligned", fn);
   T2V_CHECK_ARG(!bwd || (p->lse && p->delta), "%s: lse and delta are required", fn);
   T2V_CHECK_ARG(!bwd || p->kv_share >= 1, "%s: kv_share is the number of batches that share a K / V (1: none do)", fn);
   return T2V_OK;
@@ -1591,8 +1581,8 @@ int run_fwd(Layout& L, hipStream_t st) {
   const size_t sm = smem_bytes(L, 1, false);
   const int which = L.fwd_splits > 1 ? 1 : 3;
   const int mb = mod_bits(&a.p);
-  const int e = mb == 0 ? launch(which, attn_mod_fwd_kernel<T, DP, 1, 0>, grid, sm, st, a) : mb == 1 ? launch(which, attn_mod_fwd_kernel<T, DP, 1, 1>, grid, sm, st, a) :
-                mb == 2 ? launch(which, attn_mod_fwd_kernel<T, DP, 1, 2>, grid, sm, st, a) : launch(which, attn_mod_fwd_kernel<T, DP, 1, 3>, grid, sm, st, a);
+  const int e = mb == 0 ? launch(which, attn_mod_fwd_kernel<T, DP, 0>, grid, sm, st, a) : mb == 1 ? launch(which, attn_mod_fwd_kernel<T, DP, 1>, grid, sm, st, a) :
+                mb == 2 ? launch(which, attn_mod_fwd_kernel<T, DP, 2>, grid, sm, st, a) : launch(which, attn_mod_fwd_kernel<T, DP, 3>, grid, sm, st, a);
   if (e) return e;
   T2V_CHECK_LAUNCH();
   if (L.fwd_splits > 1) {
@@ -1611,8 +1601,8 @@ int run_bwd(Layout& L, hipStream_t st) {
   a.fold = fold(L, L.dq_tiles);
   const size_t sm = smem_bytes(L, a.p.dbias ? 5 : 1, false);
   const long long gq = (long long)a.p.nbatch * a.nunit * L.dq_tiles * (a.qorder ? 2 : 1);
-  int e = mb == 0 ? launch(1, attn_mod_dq_kernel<T, DP, 1, 0>, gq, sm, st, a) : mb == 1 ? launch(1, attn_mod_dq_kernel<T, DP, 1, 1>, gq, sm, st, a) :
-          mb == 2 ? launch(1, attn_mod_dq_kernel<T, DP, 1, 2>, gq, sm, st, a) : launch(1, attn_mod_dq_kernel<T, DP, 1, 3>, gq, sm, st, a);
+  int e = mb == 0 ? launch(1, attn_mod_dq_kernel<T, DP, 0>, gq, sm, st, a) : mb == 1 ? launch(1, attn_mod_dq_kernel<T, DP, 1>, gq, sm, st, a) :
+          mb == 2 ? launch(1, attn_mod_dq_kernel<T, DP, 2>, gq, sm, st, a) : launch(1, attn_mod_dq_kernel<T, DP, 3>, gq, sm, st, a);
   if (e) return e;
   T2V_CHECK_LAUNCH();
   if (a.p.dbias) {

@@ -125,7 +125,7 @@ class AttnMod(C.Structure):
         ("nbatch", c_int), ("heads", c_int), ("kv_heads", c_int), ("Sq", c_int), ("Sk", c_int), ("D", c_int), ("dtype", c_int),
         ("causal", c_int), ("scale", c_float), ("softcap", c_float),
         ("q", AttnOperand), ("k", AttnOperand), ("v", AttnOperand), ("o", AttnOperand),
-        ("lse", c_void_p), ("prefix", c_void_p), ("prefix_per_query", c_int), ("kv_len", c_void_p),
+        ("lse", c_void_p), ("o_rest", c_void_p), ("prefix", c_void_p), ("prefix_per_query", c_int), ("kv_len", c_void_p),
         ("q_docs", c_void_p), ("kv_docs", c_void_p), ("slopes", c_void_p), ("bias", c_void_p), ("bias_f32", c_int),
         ("radius", c_int), ("d_o", AttnOperand), ("dq", AttnOperand), ("dk", AttnOperand), ("dv", AttnOperand),
         ("delta", c_void_p), ("dbias", c_void_p), ("kv_share", c_int), ("workspace", c_void_p), ("workspace_bytes", c_ll),

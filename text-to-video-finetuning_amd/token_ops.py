@@ -368,16 +368,17 @@ def _attn_plan(qs, ks, vs, heads, kv_heads, qlay, klay, scale, causal, softcap, 
     if ksh != vsh or ksh[1] != kv_heads * D or not dtype == ks[2] == vs[2] or not dev == ks[3] == vs[3]:
         _fail(f"q {tuple(qsh)} {dtype}, k {tuple(ksh)} {ks[2]}, v {tuple(vsh)} {vs[2]}: one type, one device, {kv_heads} key / value heads of {D} "
               f"columns are wanted")
-    if D % 8 or D > 128:
+    if D % 8 or not 8 <= D <= 128:
         _fail(f"attention_mod takes head dims that are multiples of 8 up to 128, got {D}")
+    scale = D ** -0.5 if scale is None else scale
     nb, Sq, Sk = qlay.nbatch, qlay.S, klay.S
     qf, kf = _layout_facts(qlay, qsh[0]), _layout_facts(klay, ksh[0])
     if nb != klay.nbatch or not qf[0] or not kf[0]:
         _fail(f"layouts {qlay} over {qsh[0]} rows and {klay} over {ksh[0]} rows: as many batches on both sides, rows that exist")
     if not qf[1]:
         _fail(f"query layout {qlay} names a row twice")
-    if not 0.0 <= softcap < 1e30 or not math.isfinite(scale):
-        _fail(f"softcap {softcap}, scale {scale}: a finite scale and a cap of 0 (none) or more are wanted")
+    if not 1e-15 <= scale <= 1e6 or not (softcap == 0.0 or 1e-6 <= softcap <= 1e4):
+        _fail(f"softcap {softcap}, scale {scale}: a scale between 1e-15 and 1e6 and a cap of 0 (none) or between 1e-6 and 1e4 are wanted")
     if prefix is not None and not causal:
         _fail("prefix opens a causal mask: pass causal=True with it")
     if (q_docs is None) != (kv_docs is None):
@@ -437,17 +438,18 @@ def _bytes(n, dev):
 
 
 def _attn_fwd(p, q, k, v, masks, bias, keep):
-    """o, and with `keep` what the backward pass wants: lse, and the tile data of the masks."""
+    """o, and with `keep` what the backward pass wants: lse, what o's rounding left behind, and the tile data of the masks."""
     dev = p.dev
     if p.empty:
-        return torch.zeros(q.shape, dtype=p.dtype, device=dev), torch.full((p.lse,), math.inf, device=dev) if keep else None, None
+        return torch.zeros(q.shape, dtype=p.dtype, device=dev), None, None, None
     o = (torch.empty if p.covered else torch.zeros)(q.shape, dtype=p.dtype, device=dev)      # rows that no sequence owns: zeros
     d = _AttnFlat.from_buffer_copy(p.raw)
     _fill(d, q, k, v, o, *masks, bias)
-    lse = tiles = None
+    lse = rest = tiles = None
     if keep:
         lse = torch.empty(p.lse, dtype=torch.float32, device=dev)
-        d.lse = lse.data_ptr()
+        rest = torch.empty_like(o)
+        d.lse, d.o_rest = lse.data_ptr(), rest.data_ptr()
     if p.meta:
         tiles = _bytes(p.meta, dev)
         d.meta, d.meta_bytes = tiles.data_ptr(), p.meta
@@ -455,20 +457,20 @@ def _attn_fwd(p, q, k, v, masks, bias, keep):
         work = _bytes(p.work, dev)
         d.workspace, d.workspace_bytes = work.data_ptr(), p.work
     _launch("t2v_attn_mod_fwd", d, dev)
-    return o, lse, tiles
+    return o, lse, rest, tiles
 
 
 class _AttentionMod(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, bias, rest):
         ctx.plan, masks = rest
-        o, lse, tiles = _attn_fwd(ctx.plan, q, k, v, masks, bias, True)
-        ctx.save_for_backward(q, k, v, bias, o, lse, tiles, *masks)
+        o, lse, rest, tiles = _attn_fwd(ctx.plan, q, k, v, masks, bias, True)
+        ctx.save_for_backward(q, k, v, bias, o, lse, rest, tiles, *masks)
         return o
 
     @staticmethod
     def backward(ctx, do):
-        q, k, v, bias, o, lse, tiles, *masks = ctx.saved_tensors
+        q, k, v, bias, o, lse, rest, tiles, *masks = ctx.saved_tensors
         p = ctx.plan
         dev, dtype = p.dev, p.dtype
         with_bias = bias is not None and ctx.needs_input_grad[3]
@@ -480,11 +482,11 @@ class _AttentionMod(torch.autograd.Function):
         dq = (torch.empty if p.covered else torch.zeros)(q.shape, dtype=dtype, device=dev)
         new = torch.empty if p.kv_covered else torch.zeros
         dk, dv = new(k.shape, dtype=dtype, device=dev), new(v.shape, dtype=dtype, device=dev)
-        do = _upstream(do)
+        do, o, rest, lse = _upstream(do), o.contiguous(), rest.contiguous(), lse.contiguous()
         delta = torch.empty(p.lse, dtype=torch.float32, device=dev)
         d = _AttnFlat.from_buffer_copy(raw)
-        _fill(d, q, k, v, o.contiguous(), *masks, bias)
-        d.lse, d.delta, d.d_o, d.dq, d.dk, d.dv = lse.data_ptr(), delta.data_ptr(), do.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
+        _fill(d, q, k, v, o, *masks, bias)
+        d.lse, d.o_rest, d.delta, d.d_o, d.dq, d.dk, d.dv = lse.data_ptr(), rest.data_ptr(), delta.data_ptr(), do.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
         if not do.is_contiguous():
             d.d_o_rest = bytes(_operand(_ld(do.shape, do.stride()), p.lays[0]))[8:]
         dbias = None
@@ -513,7 +515,7 @@ def attention_mod(q, k, v, heads, qlay, klay, kv_heads=None, scale=None, causal=
     q: [rows_q, heads * dim]; k, v: [rows_kv, kv_heads * dim] token matrices in bf16 or fp16 (dim a multiple of 8 up to 128; heads a
     multiple of kv_heads, which defaults to heads); qlay, klay: SeqLayout of the sequences.  With t = scale * q.k (scale defaults to
     dim^-0.5):
-      softcap > 0    t <- softcap * tanh(t / softcap)
+      softcap > 0    t <- softcap * tanh(t / softcap)                                             (1e-6 to 1e4; scale: 1e-15 to 1e6)
       slopes         fp32 [heads]: t <- t - slopes[h] * |j - i'|                                  (not trained)
       bias           [heads, 2R + 1] (R <= 1024, the operands' type or fp32): t <- t + bias[h, clip(j - i', -R, R) + R]; trained when it
                      requires a gradient; an entry at or below its type's lowest finite value hides its distance
@@ -528,7 +530,7 @@ def attention_mod(q, k, v, heads, qlay, klay, kv_heads=None, scale=None, causal=
     of a layout with lo = 0 get the sum of their gradients.  The order of all sums is fixed: repeated runs are bit-equal."""
     heads = int(heads)
     p = _plan_of((_sig(q), _sig(k), _sig(v), heads, heads if kv_heads is None else int(kv_heads), qlay, klay,
-                  (q.shape[-1] // max(heads, 1)) ** -0.5 if scale is None else float(scale), int(bool(causal)), float(softcap), _sig(prefix), _sig(kv_len),
+                  None if scale is None else float(scale), int(bool(causal)), float(softcap), _sig(prefix), _sig(kv_len),
                   _sig(q_docs), _sig(kv_docs), _sig(slopes), _sig(bias)))
     if slopes is not None and slopes.requires_grad:
         _fail("slopes are not trained: pass slopes.detach(), or a bias table for a learned distance bias")
