@@ -37,7 +37,7 @@ def _mod(**kw):
 @pytest.mark.parametrize("bad", [dict(nbatch=0), dict(heads=3), dict(kv_heads=0), dict(D=60), dict(D=136), dict(dtype=2), dict(softcap=-1.0),
                                  dict(q_docs=256), dict(prefix=256), dict(bias=256, radius=1025), dict(Sq=1 << 26), dict(scale=float("nan")),
                                  dict(scale=0.0), dict(scale=-1.0), dict(softcap=1e5),
-                                 dict(o_rest=264), dict(heads=1 << 16, kv_heads=1, Sq=4)])
+                                 dict(o_rest=264), dict(nbatch=1 << 18, Sq=1 << 16), dict(heads=1 << 16, kv_heads=1, Sq=4)])
 def test_attention_descriptors_that_are_refused(bad):
     nv = _nv()
     l = nv.lib()

@@ -364,6 +364,45 @@ def test_attention_mod_shared_keys_get_the_sum_of_their_gradients(dt):
         _within(n, t.grad, *(w.view(2, 3, 21, 2, 64).sum(1) for w in want[n]))
 
 
+@pytest.mark.parametrize("mask", ["lengths", "documents", "prefix per query", "documents, long"])
+def test_attention_mod_keys_shared_by_uneven_groups_under_masks(mask):
+    """Five batches, three to a K / V: the second group has two.  Each batch has masks of its own over the shared keys."""
+    F = _f()
+    g = torch.Generator().manual_seed(len(mask))
+    B, Sq, Sk, H, KV, D = 5, 50, 90, 2, 1, 72
+    if mask.endswith("long"):
+        Sq, Sk, H = 700, 333, 4
+    r = lambda *s: torch.randn(*s, generator=g).to(BF)  # noqa: E731
+    q, do, k, v = r(B, Sq, H, D), r(B, Sq, H, D), r(2, Sk, KV, D), r(2, Sk, KV, D)
+    kw = dict(causal=True)
+    if mask == "lengths":
+        kw["kv_len"] = torch.tensor([90, 0, 17, 64, 65], dtype=torch.int32)
+    elif mask == "prefix per query":
+        kw["prefix"] = torch.randint(0, Sk + 20, (B, Sq), generator=g).int()
+    else:
+        kw["q_docs"], kw["kv_docs"] = (torch.randint(-1, 3, (B, n), generator=g).int() for n in (Sq, Sk))
+    at = torch.tensor([0, 0, 0, 1, 1])
+    want = ref.attention(q, k[at], v[at], D ** -0.5, BF, do=do, **kw)
+    flat = [t.reshape(t.shape[0] * t.shape[1], -1).cuda().requires_grad_() for t in (q, k, v)]
+    o = F.attention_mod(*flat, H, F.SeqLayout(B, Sq, Sq, 0, 1), F.SeqLayout(B, Sk, Sk, 0, 1, 3), kv_heads=KV, **{n: _dev(t) for n, t in kw.items()})
+    o.backward(do.reshape(B * Sq, -1).cuda())
+    _within("o", o, *want["o"])
+    _within("dq", flat[0].grad, *want["dq"])
+    for n, t in zip(("dk", "dv"), flat[1:]):
+        _within(n, t.grad, *(torch.stack([w[at == i].sum(0) for i in (0, 1)]) for w in want[n]))
+
+
+def test_gradients_of_gradients_are_refused():
+    F = _f()
+    x = torch.randn(16, 64, device="cuda").to(BF).requires_grad_()
+    lay, pos = F.SeqLayout(1, 16, 16, 0, 1), torch.arange(16, dtype=torch.int32, device="cuda")[:, None]
+    for y in (F.rope(x, 1, pos, F.RopeAxes((64,))), F.qk_norm_rope(x, x, 1, 1, pos, F.RopeAxes((64,)))[0], F.attention_mod(x, x, x, 1, lay, lay)):
+        up = torch.ones_like(y, requires_grad=True)
+        gx, = torch.autograd.grad(y, x, up, create_graph=True)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            gx.float().sum().backward()
+
+
 def test_attention_mod_of_nothing():
     F = _f()
     e, k = torch.empty(0, 128, dtype=BF, device="cuda"), torch.randn(8, 128, device="cuda").to(BF)
@@ -620,6 +659,8 @@ def test_refusals():
         lambda: F.rope(x, 2, pos, F.RopeAxes((64,)), freqs=torch.zeros(31, dtype=F64, device="cuda")),
         lambda: F.rope(x[:, 4:68], 1, pos, F.RopeAxes((64,))),                                  # rows not 16-byte aligned
         lambda: F.rope(torch.zeros(16, 12, dtype=BF, device="cuda"), 1, pos, F.RopeAxes((8,))),   # head dim 12
+        lambda: F.rope(x, 2, pos.float().requires_grad_(), F.RopeAxes((64,))),
+        lambda: F.rope(x, 2, pos, F.RopeAxes((64,)), freqs=torch.ones(32, dtype=F64, device="cuda", requires_grad=True)),
         lambda: F.qk_norm_rope(x, x.half(), 2, 2, pos, F.RopeAxes((64,))),
         lambda: F.qk_norm_rope(x, x[:8], 2, 2, pos, F.RopeAxes((64,))),
         lambda: F.qk_norm_rope(x, x, 2, 4, pos, F.RopeAxes((64,))),

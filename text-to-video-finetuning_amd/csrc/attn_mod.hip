@@ -1562,8 +1562,8 @@ int launch(int which, K kern, long long grid, size_t smem, hipStream_t st, const
   t2v_launch_timed(which, kern, dim3((unsigned)grid), dim3(threads), (unsigned)smem, st, a);
   return T2V_OK;
 }
-// bit 0 cap, bit 1 distance bias; a scale that is not positive takes the form that does not fold it into the running maximum
-int mod_bits(const T2VAttnMod* p) { return (p->softcap > 0.f ? 1 : 0) | (p->slopes || p->bias || !(p->scale > 0.f) ? 2 : 0); }
+// bit 0 cap, bit 1 distance bias
+int mod_bits(const T2VAttnMod* p) { return (p->softcap > 0.f ? 1 : 0) | (p->slopes || p->bias ? 2 : 0); }
 
 // all workgroups resident, two on some CUs
 int fold(const Layout& L, long long tiles) {
@@ -1626,13 +1626,19 @@ int run_bwd(Layout& L, hipStream_t st) {
   }
   return T2V_OK;
 }
+int check_grids(const char* fn, const Layout& L, bool bwd) {
+  // the largest launches, in threads: rows (256 a tile, two entries a tile with a work list), the joins (64 per 32 x 32 block), dK / dV (512 or 256)
+  const long long row_wgs = (long long)L.a.p.nbatch * L.a.nunit * L.fwd_tiles * L.fwd_splits, join = 4 * (L.dp / 32) * 64ll;
+  const long long kv_wgs = bwd ? (long long)L.a.p.nbatch * L.a.p.kv_heads * L.a.wgs * (L.dp == 64 ? 1 : 2) : 0;
+  T2V_CHECK_ARG(row_wgs * (join > 512 ? join : 512) < (1ll << 32) && kv_wgs * (2 * join) < (1ll << 32), "%s: too many workgroups (%lld, %lld)", fn, row_wgs, kv_wgs);
+  return T2V_OK;
+}
 int run(const char* fn, const T2VAttnMod* p, bool bwd, hipStream_t st) {
   if (int e = check_mod(fn, p, bwd)) return e;
   Layout L = make_layout(p, bwd);
   T2V_CHECK_ARG(L.bytes == 0 || (p->workspace && ((uintptr_t)p->workspace & 255) == 0 && p->workspace_bytes >= L.bytes),
                 "%s: a 256-byte aligned workspace of %lld bytes is wanted (got %p, %lld)", fn, L.bytes, p->workspace, p->workspace_bytes);
-  const long long worst = (long long)p->nbatch * p->heads * ((long long)L.fwd_tiles * L.fwd_splits * 4 * (L.dp / 32) + (bwd ? (long long)L.a.wgs * 64 : 0));
-  T2V_CHECK_ARG(worst < (1ll << 31), "%s: too many workgroups", fn);
+  if (int e = check_grids(fn, L, bwd)) return e;
   T2V_CHECK_ARG(!L.meta || (p->meta && ((uintptr_t)p->meta & 255) == 0 && p->meta_bytes >= L.meta_bytes),
                 "%s: documents and prefixes per query want a 256-byte aligned meta buffer of %lld bytes (got %p, %lld)", fn, L.meta_bytes, p->meta,
                 p->meta_bytes);
@@ -1660,7 +1666,8 @@ int run(const char* fn, const T2VAttnMod* p, bool bwd, hipStream_t st) {
 
 extern "C" long long t2v_attn_mod_workspace(const T2VAttnMod* p, int backward) {
   if (check_mod("t2v_attn_mod_workspace", p, false)) return -1;
-  return make_layout(p, backward != 0).bytes;
+  const Layout L = make_layout(p, backward != 0);
+  return check_grids("t2v_attn_mod_workspace", L, backward != 0) ? -1 : L.bytes;
 }
 extern "C" long long t2v_attn_mod_meta_bytes(const T2VAttnMod* p) {
   if (check_mod("t2v_attn_mod_meta_bytes", p, false)) return -1;

@@ -15,6 +15,7 @@ import math
 from dataclasses import dataclass
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import native as nv
 
@@ -123,6 +124,11 @@ def _vector(t):
     if t is None or (t.dtype == torch.float32 and t.is_contiguous()):
         return t
     return t.detach().float().contiguous()
+
+
+def _fixed(pos, freqs):
+    if (pos is not None and pos.requires_grad) or (freqs is not None and freqs.requires_grad):
+        _fail("positions and frequencies are not trained: pass them detached")
 
 
 def _addr(t):
@@ -241,6 +247,7 @@ class _Rope(torch.autograd.Function):
         return _rope_fwd(ctx.plan, (x,), pos, freqs, None, None)[0]
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         pos, freqs = ctx.saved_tensors
         return _rope_bwd(ctx.plan, None, (_upstream(dy),), pos, freqs, None, None)[0][0], None
@@ -250,6 +257,7 @@ def rope(x, heads, pos, axes, freqs=None):
     """Rotary positions: x [rows, heads * dim] (bf16, fp16 or fp32) with the columns `axes` (RopeAxes) names turned by pos [rows, number
     of axes] (int32, int64 or fp32).  Angles are formed in 64 bits.  freqs: fp64 [sum(dims) / 2] radians per unit of position, in the place of the
     ladder theta gives.  Returns a dense matrix of x's shape; differentiable in x."""
+    _fixed(pos, freqs)
     plan = _rope_plan((_sig(x),), (int(heads), 0), axes, None, 0.0, _sig(pos), _sig(freqs), None)
     if torch.is_grad_enabled() and x.requires_grad:
         return _Rope.apply(x, (plan, pos, freqs))
@@ -265,6 +273,7 @@ class _QkNormRope(torch.autograd.Function):
         return _rope_fwd(ctx.plan, (q, k), pos, freqs, (_vector(qw), _vector(kw)), (_vector(qb), _vector(kb)))
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dq, dk):
         q, k, qw, kw, pos, freqs = ctx.saved_tensors
         plan, sigs = ctx.plan, (_sig(q), _sig(k))
@@ -283,6 +292,7 @@ def qk_norm_rope(q, k, heads, kv_heads, pos, axes, q_weight=None, k_weight=None,
     statistics are recomputed in the backward pass from the saved inputs."""
     if norm is None:
         _fail("norm None: 'rms' or 'layer' (`rope` turns without a norm)")
+    _fixed(pos, freqs)
     key = ((_sig(q), _sig(k)), (int(heads), int(kv_heads)), axes, norm, float(eps), _sig(pos), _sig(freqs),
            (_sig(q_weight), _sig(k_weight), _sig(q_bias), _sig(k_bias)))
     plan = _rope_plan(*key)
@@ -469,6 +479,7 @@ class _AttentionMod(torch.autograd.Function):
         return o
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, do):
         q, k, v, bias, o, lse, rest, tiles, *masks = ctx.saved_tensors
         p = ctx.plan
