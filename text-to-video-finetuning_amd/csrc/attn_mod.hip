@@ -435,7 +435,14 @@ __device__ __forceinline__ void load_rows(Rows& R, const Args& a, const Unit& u,
 }
 
 // ------------------------------------------------------------------------------------------------ forward
-// MOD: bit 0 cap, bit 1 distance bias (slopes / table), compile-time so that a tile is straight-line code
+// MOD: bit 0 cap, bit 1 distance bias (slopes / table), compile-time so that a tile is straight-line code.
+// A workgroup is 128 rows (four waves of 32) and walks the key tiles its rows may see.  64 rows a wave instead (K and V fragments read once for
+// both halves) leave one wave per SIMD: 656 -> 801 us at head dim 128, no change at 64.
+// Measured, bf16, 8192 x 8192, 16 heads: head dim 128 653 us, 842 TFLOP/s where a library product of 8192^3 reaches 1243 (causal 298 us, capped
+// 709 us); head dim 64 404 us, 680 TFLOP/s.  At 64 the vector unit bounds it: the exponential, maximum, sum and conversion of a score take longer
+// than its 64 columns in the two products.  At 128 it is the chain inside a wave (score, maximum, exponential, product); without the tile
+// copies it would be 10 % faster at most.
+// One new token for 8 sequences of up to 16384 keys (165 MB of them), 16 / 4 heads of 128: 37 us, 4.4 TB/s, and 7 us for the join.
 template <typename T, int DP, int MOD>
 __global__ __launch_bounds__(256, DP == 64 && MOD < 2 ? 3 : 2) void attn_mod_fwd_kernel(const Args a) {
   warm_kernargs<(int)sizeof(Args)>();
@@ -759,7 +766,8 @@ __global__ __launch_bounds__(64) void attn_mod_join_kernel(const Args a) {
   if (ok && f == 0 && hi == 0 && a.p.lse) a.p.lse[((long long)u.b * a.p.heads + u.h0) * a.p.Sq + r] = l > 0.f ? m + __builtin_amdgcn_logf(l) : INFINITY;
 }
 
-// bounds and documents of every 64 rows / keys (launched where a mask has documents or one prefix per query): one wave per tile
+// bounds and documents of every 64 rows / keys (launched where a mask has documents or one prefix per query): one wave per tile (5 us at 8200
+// rows and keys: a launch and a chain of three loads)
 __global__ __launch_bounds__(64) void attn_mod_meta_kernel(const Args a, QMeta* qm, KMeta* km, int nq, int nk) {
   const int lane = threadIdx.x, b = blockIdx.y, t = blockIdx.x;
   const Seq seq = load_seq(a, b);
@@ -794,7 +802,8 @@ __global__ __launch_bounds__(64) void attn_mod_meta_kernel(const Args a, QMeta* 
 // for the rows of its first document (and those of none), one for the others.  Entries (batch, tile, part) are sorted by the tiles they
 // will visit, the longest first; equal ones stay in order, and second parts of tiles with one document come last and end at once.
 // Block 0: row tiles of 128; block 1: key tiles.  One thread counts an entry and its rank among the others.
-// (Nine clips of 273 .. 1804 tokens: see the table of the operators; the two short launches are paid once per mask.)
+// (Nine clips, 8200 tokens, 10 heads of 64: forward 93 -> 54 us, dQ 102 -> 64 us, dK / dV 149 -> 105 us for the 9 us of this launch, once per
+// mask and step.)
 constexpr int ORDER_MAX = 1024, ORDER_TILES = 4096;
 __global__ __launch_bounds__(1024) void attn_mod_order_kernel(const Args a, int* qorder, int* korder, int nq, int nk, int keys) {
   __shared__ unsigned long long key[ORDER_MAX];
@@ -802,25 +811,26 @@ __global__ __launch_bounds__(1024) void attn_mod_order_kernel(const Args a, int*
   const int tid = threadIdx.x, side = blockIdx.x;
   const int ntile = side ? nk : nq, n = 2 * a.p.nbatch * ntile, per = side ? keys / TILE : 2;
   const int nqt = (a.M + TILE - 1) / TILE, nkt = (a.p.Sk + TILE - 1) / TILE, nown = side ? nkt : nqt, nother = side ? nqt : nkt;
+  const int e = min(tid, n - 1), part = e & 1, b = (e >> 1) / ntile, t = (e >> 1) - b * ntile;
+  int lo = 0x7fffffff, hi = -1, bmax = 0;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {                                         // (all loads in flight; one that is met twice changes nothing)
+    const long long at = (long long)b * nown + min(t * per + min(k, per - 1), nown - 1);
+    lo = min(lo, side ? a.kmeta[at].dmin : a.qmeta[at].dmin);
+    hi = max(hi, side ? a.kmeta[at].dmax : a.qmeta[at].dmax);
+    if (!side) bmax = max(bmax, a.qmeta[at].bmax);
+  }
   for (int i = tid; i < a.p.nbatch * nother; i += 1024) {
     slo[i] = side ? a.qmeta[i].dmin : a.kmeta[i].dmin;
     shi[i] = side ? a.qmeta[i].dmax : a.kmeta[i].dmax;
     sbound[i] = side ? a.qmeta[i].bmax : 0x7fffffff;
   }
-  const int e = min(tid, n - 1), part = e & 1, b = (e >> 1) / ntile, t = (e >> 1) - b * ntile;
-  int lo = 0x7fffffff, hi = -1, bmax = 0;
-  for (int i = t * per; i < min((t + 1) * per, nown); ++i) {
-    const long long at = (long long)b * nown + i;
-    lo = min(lo, side ? a.kmeta[at].dmin : a.qmeta[at].dmin);
-    hi = max(hi, side ? a.kmeta[at].dmax : a.qmeta[at].dmax);
-    if (!side) bmax = max(bmax, a.qmeta[at].bmax);
-  }
   if (part) lo = lo == 0x7fffffff ? lo : lo + 1;
   else hi = min(lo, hi);
-  const int end = lo > hi ? 0 : side ? nqt : (bmax + TILE - 1) / TILE, floor = side ? t * keys : 0;
+  const int end = lo > hi || tid >= n ? 0 : side ? nqt : (bmax + TILE - 1) / TILE, floor = side ? t * keys : 0;
   __syncthreads();
   int count = 0;
-#pragma unroll 4
+#pragma unroll 8
   for (int c = 0; c < end; ++c) {
     const int i = b * nother + c;
     count += (sbound[i] > floor) & (shi[i] >= lo) & (slo[i] <= hi);
@@ -828,13 +838,15 @@ __global__ __launch_bounds__(1024) void attn_mod_order_kernel(const Args a, int*
   const unsigned long long mine = ((unsigned long long)(2 * count + 2 - part) << 32) | (unsigned)(~e);
   if (tid < n) key[tid] = mine;
   __syncthreads();
+  if (tid >= n) return;
   int rank = 0;
 #pragma unroll 8
   for (int k = 0; k < n; ++k) rank += key[k] > mine;
-  if (tid < n) (side ? korder : qorder)[rank] = tid;
+  (side ? korder : qorder)[rank] = tid;
 }
 
 // ------------------------------------------------------------------------------------------------ backward: dQ, delta, table gradient
+// Three products per score, Q, dO and dQ of the wave's 32 rows in registers.  8192 x 8192, 16 heads of 128, bf16: 814 us, 1013 TFLOP/s.
 template <typename T, int DP, int MOD>
 __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(const Args a) {
   warm_kernargs<(int)sizeof(Args)>();
@@ -1075,7 +1087,7 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(const Args a) {
   }
 }
 
-// dtable[h][d] = sum over (batch, row tile), in order; entries that hide their distance get 0 by construction (P = 0 there)
+// dtable[h][d] = sum over (batch, row tile), in order (4 us, a launch); entries that hide their distance get 0 by construction (P = 0 there)
 template <typename T>
 __global__ __launch_bounds__(256) void attn_mod_dbias_kernel(const Args a) {
   const long long n = (long long)a.p.heads * (2 * a.p.radius + 1), i = (long long)blockIdx.x * 256 + threadIdx.x;
@@ -1094,8 +1106,9 @@ struct RowInfo {                    // of one query row, as loaded
 };
 // A wave owns 32 keys and streams the rows that see them.  K, V, dK and dV of 32 keys of 128 columns are 192 registers: with the score and
 // gradient tiles a wave would need more than half of a SIMD's file, and one wave per SIMD has nothing to run under its exponentials
-// (measured 301 us at 2 x 2011 rows, 16 / 4 heads; this form: see the table).  So at DP = 128 the workgroup is eight waves, its V rows
-// stay in LDS (read once per block: LDS then delivers 156 bytes per clock at full matrix rate, against its 128), and two waves share a SIMD.
+// (301 us at 2 x 2011 rows, 16 / 4 heads; this form 144 us).  So at DP = 128 the workgroup is eight waves, its V rows stay in LDS, and two
+// waves share a SIMD.  LDS bounds it then: at full matrix rate it would deliver 156 bytes per clock, against its 128.  8192 x 8192, 16 heads of 128:
+// 1.42 ms, 775 TFLOP/s.
 template <typename T, int DP, int MOD>
 __global__ __launch_bounds__(DP == 128 ? 512 : 256, 2) void attn_mod_dkdv_kernel(const Args a) {
   warm_kernargs<(int)sizeof(Args)>();
@@ -1365,6 +1378,7 @@ __global__ __launch_bounds__(DP == 128 ? 512 : 256, 2) void attn_mod_dkdv_kernel
 }
 
 // dK, dV = sum of the partial sums of the splits and of the batches that share a K / V head, in order: one wave per 32 keys, 32 columns and side
+// (67 MB of partial sums in 13.6 us, 4.9 TB/s)
 template <typename T, int DP>
 __global__ __launch_bounds__(64) void attn_mod_dkdv_join_kernel(const Args a) {
   constexpr int FM = DP / 32, NW = DP == 128 ? 8 : 4, KEYS = 32 * NW;

@@ -11,6 +11,8 @@
 // recomputed in the backward pass, which saves their round trip.  Parameter gradients: per-lane fp32 sums over the rows a group
 // visits, one fixed-order sum over the groups of a workgroup in LDS, one partial row per workgroup, one fixed-order reduction
 // kernel: no atomics, repeated runs are bit-equal.
+// Measured, bf16, norm + rotation of 69120 rows, 2 x 20 heads of 64: forward 161 us (4.4 TB/s; a large copy reaches 4.9), forward and backward
+// 400 us (1.77 GB: 4.4 TB/s with the gaps between launches).  Few rows are launch-bound: 3.6 us of kernel at 8 rows.
 #include "common.h"
 
 namespace {
@@ -278,7 +280,7 @@ __global__ __launch_bounds__(256) void rope_kernel(const RopeArgs p) {
   }
 }
 
-// out[side][which][col] = sum over the side's partial rows, in order within a slice and over the slices
+// out[side][which][col] = sum over the side's partial rows, in order within a slice and over the slices (4 us, a launch)
 __global__ __launch_bounds__(1024) void rope_param_reduce_kernel(const float* __restrict__ partial, int D, int n0, int n1, float* dw0,
                                                                  float* db0, float* dw1, float* db1) {
   __shared__ float s[32][33];
