@@ -78,7 +78,7 @@ _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_get
 def _launch(name, desc, dev):
     """The entry point `name` on the current stream of the operands' device (made the current device where it is not)."""
     index = dev.index
-    if index == torch.cuda.current_device():
+    if index == torch._C._cuda_getDevice():
         rc = getattr(nv.lib(), name)(C.byref(desc), _raw_stream(index))
     else:
         with torch.cuda.device(dev):
@@ -340,7 +340,7 @@ def _dense(t):
 
 class _AttnPlan:
     """raw: descriptor of the forward; work, meta: bytes of its buffers; bwd: (descriptor, workspace bytes, with dense gradients), made on first use."""
-    __slots__ = ("key", "raw", "work", "meta", "empty", "covered", "kv_covered", "share", "rows", "dtype", "dev", "lse", "shared_ok", "_bwd", "lays")
+    __slots__ = ("key", "raw", "work", "meta", "empty", "covered", "kv_covered", "share", "dtype", "dev", "lse", "rest", "shared_ok", "_bwd", "lays")
 
     def bwd(self, with_bias):
         if self._bwd.get(with_bias) is None:
@@ -404,7 +404,7 @@ def _attn_plan(qs, ks, vs, heads, kv_heads, qlay, klay, scale, causal, softcap, 
         _fail(f"bias must be a contiguous [{heads}, 2R + 1] table with R <= 1024 in {dtype} or fp32 on {dev}, got {tuple(bias[0])} {bias[2]}")
     p = _AttnPlan()
     p.empty = nb * Sq == 0 or Sk == 0                   # nothing is asked, or there is nothing to see
-    p.rows, p.dtype, p.dev, p.lse = qsh[0], dtype, dev, nb * heads * Sq
+    p.dtype, p.dev, p.lse, p.rest = dtype, dev, nb * heads * Sq, qsh[0] * heads * D * 2      # elements of lse, bytes of o's rest (a multiple of 16)
     p.covered = qf[2]
     p.share = klay.bdiv if klay.bdiv > 1 and klay.lo == 0 else 1
     p.kv_covered = kf[2] or (p.share > 1 and nb % p.share == 0 and nb // p.share * Sk == ksh[0] and klay.ss == 1 and klay.hi == Sk)
@@ -448,18 +448,18 @@ def _bytes(n, dev):
 
 
 def _attn_fwd(p, q, k, v, masks, bias, keep):
-    """o, and with `keep` what the backward pass wants: lse, what o's rounding left behind, and the tile data of the masks."""
+    """o, and with `keep` what the backward pass wants: what o's rounding left behind with lse behind it, and the tile data of the masks."""
     dev = p.dev
     if p.empty:
-        return torch.zeros(q.shape, dtype=p.dtype, device=dev), None, None, None
+        return torch.zeros(q.shape, dtype=p.dtype, device=dev), None, None
     o = (torch.empty if p.covered else torch.zeros)(q.shape, dtype=p.dtype, device=dev)      # rows that no sequence owns: zeros
     d = _AttnFlat.from_buffer_copy(p.raw)
     _fill(d, q, k, v, o, *masks, bias)
-    lse = rest = tiles = None
+    kept = tiles = None
     if keep:
-        lse = torch.empty(p.lse, dtype=torch.float32, device=dev)
-        rest = torch.empty_like(o)
-        d.lse, d.o_rest = lse.data_ptr(), rest.data_ptr()
+        kept = _bytes(p.rest + 4 * p.lse, dev)
+        d.o_rest = at = kept.data_ptr()
+        d.lse = at + p.rest
     if p.meta:
         tiles = _bytes(p.meta, dev)
         d.meta, d.meta_bytes = tiles.data_ptr(), p.meta
@@ -467,21 +467,21 @@ def _attn_fwd(p, q, k, v, masks, bias, keep):
         work = _bytes(p.work, dev)
         d.workspace, d.workspace_bytes = work.data_ptr(), p.work
     _launch("t2v_attn_mod_fwd", d, dev)
-    return o, lse, rest, tiles
+    return o, kept, tiles
 
 
 class _AttentionMod(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, bias, rest):
         ctx.plan, masks = rest
-        o, lse, rest, tiles = _attn_fwd(ctx.plan, q, k, v, masks, bias, True)
-        ctx.save_for_backward(q, k, v, bias, o, lse, rest, tiles, *masks)
+        o, kept, tiles = _attn_fwd(ctx.plan, q, k, v, masks, bias, True)
+        ctx.save_for_backward(q, k, v, bias, o, kept, tiles, *masks)
         return o
 
     @staticmethod
     @once_differentiable
     def backward(ctx, do):
-        q, k, v, bias, o, lse, rest, tiles, *masks = ctx.saved_tensors
+        q, k, v, bias, o, kept, tiles, *masks = ctx.saved_tensors
         p = ctx.plan
         dev, dtype = p.dev, p.dtype
         with_bias = bias is not None and ctx.needs_input_grad[3]
@@ -493,11 +493,15 @@ class _AttentionMod(torch.autograd.Function):
         dq = (torch.empty if p.covered else torch.zeros)(q.shape, dtype=dtype, device=dev)
         new = torch.empty if p.kv_covered else torch.zeros
         dk, dv = new(k.shape, dtype=dtype, device=dev), new(v.shape, dtype=dtype, device=dev)
-        do, o, rest, lse = _upstream(do), o.contiguous(), rest.contiguous(), lse.contiguous()
-        delta = torch.empty(p.lse, dtype=torch.float32, device=dev)
+        do, o = _upstream(do), o.contiguous()
+        work = _bytes(work_bytes + 4 * p.lse, dev)              # and delta behind it
         d = _AttnFlat.from_buffer_copy(raw)
         _fill(d, q, k, v, o, *masks, bias)
-        d.lse, d.o_rest, d.delta, d.d_o, d.dq, d.dk, d.dv = lse.data_ptr(), rest.data_ptr(), delta.data_ptr(), do.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
+        d.o_rest = at = kept.data_ptr()
+        d.lse = at + p.rest
+        d.workspace = at = work.data_ptr()
+        d.workspace_bytes, d.delta = work_bytes, at + work_bytes
+        d.d_o, d.dq, d.dk, d.dv = do.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
         if not do.is_contiguous():
             d.d_o_rest = bytes(_operand(_ld(do.shape, do.stride()), p.lays[0]))[8:]
         dbias = None
@@ -506,9 +510,6 @@ class _AttentionMod(torch.autograd.Function):
             d.dbias = dbias.data_ptr()
         if tiles is not None:
             d.meta, d.meta_bytes, d.meta_ready = tiles.data_ptr(), tiles.numel(), 1
-        if work_bytes:
-            work = _bytes(work_bytes, dev)
-            d.workspace, d.workspace_bytes = work.data_ptr(), work_bytes
         _launch("t2v_attn_mod_bwd", d, dev)
         return dq, dk, dv, dbias, None
 
