@@ -709,33 +709,43 @@ __global__ __launch_bounds__(256, DP == 64 && MOD < 2 ? 3 : 2) void attn_mod_fwd
   }
 }
 
-// joins the splits: one wave per 32 rows and 32 columns, laid out like the accumulators
-template <typename T, int DP>
-__global__ __launch_bounds__(64) void attn_mod_join_kernel(const Args a) {
-  constexpr int FM = DP / 32;
-  const int lane = threadIdx.x, hi = lane >> 5, D = a.p.D;
+// joins the splits: a workgroup per 32 rows and 32 columns, laid out like the accumulators.  It is as long as its chain of loads, so more
+// than eight splits are dealt out to W = 8 waves, each has four in flight, and the eight results meet in LDS, in order; up to eight are all in
+// flight in one wave.  One row, 32 / 8 heads of 128 over 32768 keys (64 splits): 48 -> 31 us with the forward kernel; 16 rows of 8 heads of 64 over 4096
+// keys (4 splits): 28 us by one wave, 31 by eight.
+template <typename T, int DP, int W>
+__global__ __launch_bounds__(64 * W) void attn_mod_join_kernel(const Args a) {
+  constexpr int FM = DP / 32, AT = W == 1 ? 8 : 4, ROW = 16 + 4;        // (16-byte aligned rows, 80 bytes apart)
+  __shared__ __attribute__((aligned(16))) float meet[W > 1 ? W : 1][W > 1 ? 64 : 1][ROW];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hi = lane >> 5, D = a.p.D;
   const int f = blockIdx.x % FM;
   const long long block = blockIdx.x / FM;                              // over (unit x, tile, 32 rows)
   const int NU = a.p.nbatch * a.nunit, per = a.ntile * 4, x = (int)(block / per);
   const int r = (int)(block - (long long)x * per) * 32 + (lane & 31);
   const bool ok = r < a.M;
   const long long stride = (long long)NU * per;                         // blocks of a split
-  if (__all(!ok)) return;
+  if (r - (lane & 31) >= a.M) return;                                   // workgroup-uniform
   const long long at = block * 32 + (lane & 31);
-  // Eight splits at a time, all their loads in flight: the launch is as long as its chain of loads (6.5 -> 4.5 us at 16 splits of few rows).
   // (Lanes behind the last row read their part of the padded buffer, whatever it holds, and store nothing: a branch around the loads would
   // put a wait behind each.)
-  constexpr int AT = 8;
   float m = LOWEST * 4.f, l = 0.f;
   f32x16 acc[1];
 #pragma unroll
   for (int e = 0; e < 16; ++e) acc[0][e] = 0.f;
-  for (int s0 = 0; s0 < a.splits; s0 += AT) {
+  const auto add = [&](float ms, float ls, const f32x4 (&v)[4]) {       // one more partial result; m is not below ms
+    const float w = __builtin_amdgcn_exp2f(ms - m);
+    l = fmaf(w, ls, l);
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[0][4 * g + e] = fmaf(w, v[g][e], acc[0][4 * g + e]);
+  };
+  for (int s0 = wave; s0 < a.splits; s0 += AT * W) {
     float2 ml[AT];
     f32x4 v[AT][4];
 #pragma unroll
     for (int k = 0; k < AT; ++k) {
-      const long long s = min(s0 + k, a.splits - 1);
+      const long long s = min(s0 + k * W, a.splits - 1);
       ml[k] = *(const float2*)(a.part_ml + (s * stride * 32 + at) * 2);
 #pragma unroll
       for (int g = 0; g < 4; ++g) v[k][g] = *(const f32x4*)(a.part + (s * stride + block) * (32 * DP) + (f * 256 + lane) * 4 + g * 256);
@@ -750,13 +760,36 @@ __global__ __launch_bounds__(64) void attn_mod_join_kernel(const Args a) {
     for (int e = 0; e < 16; ++e) acc[0][e] *= alpha;
 #pragma unroll
     for (int k = 0; k < AT; ++k) {
-      if (s0 + k >= a.splits) break;                                    // launch-uniform
-      const float w = __builtin_amdgcn_exp2f(ml[k].x - m);
-      l = fmaf(w, ml[k].y, l);
+      if (s0 + k * W >= a.splits) break;                       // wave-uniform
+      add(ml[k].x, ml[k].y, v[k]);
+    }
+  }
+  if constexpr (W > 1) {
+    float* mine = meet[wave][lane];
 #pragma unroll
-      for (int g = 0; g < 4; ++g)
+    for (int g = 0; g < 4; ++g) *(f32x4*)(mine + 4 * g) = f32x4{acc[0][4 * g], acc[0][4 * g + 1], acc[0][4 * g + 2], acc[0][4 * g + 3]};
+    *(float2*)(mine + 16) = float2{m, l};
+    __syncthreads();
+    if (wave) return;
+    float ms[W], ls[W], mn = m;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[0][4 * g + e] = fmaf(w, v[k][g][e], acc[0][4 * g + e]);
+    for (int k = 0; k < W; ++k) {
+      const float2 ml = *(const float2*)(meet[k][lane] + 16);
+      ms[k] = ml.x;
+      ls[k] = ml.y;
+      mn = fmaxf(mn, ml.x);
+    }
+    const float own = __builtin_amdgcn_exp2f(m - mn);
+    m = mn;
+    l *= own;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[0][e] *= own;
+#pragma unroll
+    for (int k = 1; k < W; ++k) {
+      f32x4 v[4];
+#pragma unroll
+      for (int g = 0; g < 4; ++g) v[g] = *(const f32x4*)(meet[k][lane] + 4 * g);
+      add(ms[k], ls[k], v);
     }
   }
   const Unit u = unit_of(a, x);
@@ -1472,7 +1505,6 @@ Layout make_layout(const T2VAttnMod* p, bool bwd) {
     if (wgs < 256) {
       int s = (int)(512 / wgs);
       s = s < kt / 4 ? s : kt / 4;
-      s = s > 64 ? 64 : s;
       L.fwd_splits = s > 1 ? s : 1;
     }
   }
@@ -1601,7 +1633,8 @@ int run_fwd(Layout& L, hipStream_t st) {
   T2V_CHECK_LAUNCH();
   if (L.fwd_splits > 1) {
     const long long blocks = (long long)a.p.nbatch * a.nunit * a.ntile * 4 * (DP / 32);
-    T2V_LAUNCH_LAST((attn_mod_join_kernel<T, DP>), dim3((unsigned)blocks), dim3(64), 0, st, a);
+    if (a.splits > 8) T2V_LAUNCH_LAST((attn_mod_join_kernel<T, DP, 8>), dim3((unsigned)blocks), dim3(512), 0, st, a);
+    else T2V_LAUNCH_LAST((attn_mod_join_kernel<T, DP, 1>), dim3((unsigned)blocks), dim3(64), 0, st, a);
     T2V_CHECK_LAUNCH();
   }
   return T2V_OK;
@@ -1641,8 +1674,8 @@ int run_bwd(Layout& L, hipStream_t st) {
   return T2V_OK;
 }
 int check_grids(const char* fn, const Layout& L, bool bwd) {
-  // the largest launches, in threads: rows (256 a tile, two entries a tile with a work list), the joins (64 per 32 x 32 block), dK / dV (512 or 256)
-  const long long row_wgs = (long long)L.a.p.nbatch * L.a.nunit * L.fwd_tiles * L.fwd_splits, join = 4 * (L.dp / 32) * 64ll;
+  // the largest launches, in threads: rows (256 a tile, two entries a tile with a work list), the joins (512 or 64 per 32 x 32 block), dK / dV (512 or 256)
+  const long long row_wgs = (long long)L.a.p.nbatch * L.a.nunit * L.fwd_tiles * L.fwd_splits, join = 4 * (L.dp / 32) * 512ll;
   const long long kv_wgs = bwd ? (long long)L.a.p.nbatch * L.a.p.kv_heads * L.a.wgs * (L.dp == 64 ? 1 : 2) : 0;
   T2V_CHECK_ARG(row_wgs * (join > 512 ? join : 512) < (1ll << 32) && kv_wgs * (2 * join) < (1ll << 32), "%s: too many workgroups (%lld, %lld)", fn, row_wgs, kv_wgs);
   return T2V_OK;
