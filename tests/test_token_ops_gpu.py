@@ -214,6 +214,7 @@ ATTN = {  # B, Sq, Sk, H, KV, D, dtype, options
     "many documents shuffled": (2, 1100, 1100, 16, 16, 8, BF, dict(docs="shuffled")),
     "long": (1, 1100, 1100, 2, 1, 64, BF, dict(causal=True, softcap=15.0)),
     "long keys": (1, 5, 4000, 4, 2, 128, BF, dict(causal=True, slopes=True)),
+    "rows for a little more than one workgroup per CU": (1, 2100, 2110, 16, 16, 16, HF, dict(causal=True, prefix=[100], softcap=9.0)),
     "very long keys": (1, 3, 40000, 2, 1, 64, HF, dict(causal=True, slopes=True)),
     "steps of long and short keys": (2, 1, 20000, 8, 2, 128, BF, dict(causal=True, softcap=12.0, kv_len=[20000, 777])),
     "few keys, many rows": (1, 1500, 30, 2, 2, 64, BF, {}),

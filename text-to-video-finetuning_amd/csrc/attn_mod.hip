@@ -102,7 +102,7 @@ struct Args {
   unsigned magic;                   // r / gp = r * magic >> 32 (gp > 1)
   int ntile, splits;                // row (or key) tiles of a unit, splits of the other axis
   int chunk, wgs;                   // dK / dV: row tiles a split is meant to take, workgroups of a K / V head (see kv_runs)
-  int fold;                         // order of the row tiles (see row_tile)
+  int fold;                         // where the order of the row tiles turns (see row_tile)
   const int* qorder;                // [nbatch * row tiles], [nbatch * key tiles]: (batch, tile) pairs by falling work, or NULL
   const int* korder;
   int to_part;                      // dK / dV go to `part` as fp32 (several splits, or several batches that share K / V)
@@ -154,11 +154,10 @@ __host__ __device__ __forceinline__ int kv_runs(const Args& a, int k, int keys, 
   return run > a.chunk ? (run + a.chunk - 1) / a.chunk : 1;
 }
 // forward, dQ: the row tile of rank r.  Under a causal mask the last tiles are the longest: they come first (they then end first come, first
-// served), or (fold) the long half falls and the short half rises, where all workgroups are resident at once, two per CU: the second
-// workgroup of a CU is then short where the first is long.
+// served).  Where all workgroups are resident at once, two on some CUs, the order turns at rank `fold`, behind the first workgroup of every CU:
+// the second of a CU is then short where the first is long (264 workgroups over 2112 keys: 56 us where it turned in the middle, 53 at fold).
 __device__ __forceinline__ int row_tile(const Args& a, int r) {
-  const int half = (a.ntile + 1) / 2;
-  return a.fold && r >= half ? r - half : a.ntile - 1 - r;
+  return r >= a.fold ? r - a.fold : a.ntile - 1 - r;
 }
 
 // workgroup id -> (batch, unit): workgroups go round-robin over the eight XCDs, so units that share a K/V head are placed a multiple of
@@ -1499,13 +1498,18 @@ Layout make_layout(const T2VAttnMod* p, bool bwd) {
   L.fwd_tiles = (a.M + rows - 1) / rows;
   L.fwd_splits = 1;
   if (!bwd) {
-    // few workgroups and a long key axis: split the keys until ~512 workgroups exist, at least four 64-key tiles each
+    // Few workgroups and a long key axis: the keys are split until ~512 workgroups exist, at least four 64-key tiles each (8 steps over up to 16384
+    // keys, 16 / 4 heads of 128: 45 us; with 256 or 1024 workgroups 61 and 58).  A little more than one workgroup per CU leaves most CUs with one
+    // and a few with two: three splits fill both places about twice (264 workgroups, 6731 keys: 214 -> 173 us, 320: 214 -> 201, 264 causal ones of 2112
+    // keys: 53 -> 50; at 400 they lose, 228 -> 246, and below 32 tiles of keys their join takes what they gain).
     const long long wgs = NU * L.fwd_tiles;
     const int kt = (p->Sk + TILE - 1) / TILE;
     if (wgs < 256) {
-      int s = (int)(512 / wgs);
-      s = s < kt / 4 ? s : kt / 4;
-      L.fwd_splits = s > 1 ? s : 1;
+      const int s = (int)(512 / wgs);
+      L.fwd_splits = s < kt / 4 ? s : kt / 4;
+      if (L.fwd_splits < 1) L.fwd_splits = 1;
+    } else if (wgs <= 1024 / 3 && kt >= 32 && !p->q_docs) {
+      L.fwd_splits = 3;
     }
   }
   L.dq_tiles = (a.M + 127) / 128;
@@ -1611,10 +1615,10 @@ int launch(int which, K kern, long long grid, size_t smem, hipStream_t st, const
 // bit 0 cap, bit 1 distance bias
 int mod_bits(const T2VAttnMod* p) { return (p->softcap > 0.f ? 1 : 0) | (p->slopes || p->bias ? 2 : 0); }
 
-// all workgroups resident, two on some CUs
+// the rank at which the order turns: where all workgroups are resident, two on some CUs, the 256 longest come first
 int fold(const Layout& L, long long tiles) {
-  const long long wgs = (long long)L.a.p.nbatch * L.a.nunit * tiles;
-  return L.a.p.causal && wgs > 256 && wgs <= 512;
+  const long long NU = (long long)L.a.p.nbatch * L.a.nunit, wgs = NU * tiles;
+  return L.a.p.causal && wgs > 256 && wgs <= 512 ? (int)((256 + NU - 1) / NU) : 1 << 30;
 }
 
 template <typename T, int DP>
