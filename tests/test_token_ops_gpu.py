@@ -668,6 +668,7 @@ def test_refusals():
         lambda: F.qk_norm_rope(x, x[:8], 2, 2, pos, F.RopeAxes((64,))),
         lambda: F.qk_norm_rope(x, x, 2, 4, pos, F.RopeAxes((64,))),
         lambda: F.qk_norm_rope(x, x, 2, 2, pos, F.RopeAxes((64,)), norm="batch"),
+        lambda: F.qk_norm_rope(x, x, 2, 2, pos, F.RopeAxes((64,)), eps=-1.0),
         lambda: F.qk_norm_rope(x, x, 2, 2, pos, F.RopeAxes((64,)), torch.ones(128, device="cuda")),
         lambda: F.qk_norm_rope(x, x, 2, 2, pos, F.RopeAxes((64,)), torch.ones(64)),
         lambda: F.attention_mod(x.float(), x.float(), x.float(), 2, lay, lay),

@@ -8,6 +8,10 @@ stream of its operands' device, forward and backward; nothing falls back to torc
 Host side: what a call's arguments look like (shapes, strides, types, flags: never addresses or contents) is checked once and kept as
 a plan, the descriptor's bytes with the pointers left open and the sizes of its buffers; a call fills in the pointers.  Small
 calls are as long as their host code.
+
+Calls and their backward passes can be captured into a graph.  As with every autograd function, a captured backward() that accumulates
+into a leaf wants no other graph of that leaf alive from outside the capture (its accumulation belongs to the other stream): drop it first, or
+use autograd.grad.
 """
 import ctypes as C
 import functools
@@ -153,8 +157,8 @@ def _rope_plan(xs, heads, axes, norm, eps, pos, freqs, params):
     d = _RopeFlat()
     d.heads0, d.heads1, d.rows, d.D, d.dtype, d.eps = heads[0], heads[1], rows, D, _TYPE[dtype], eps
     if norm is not None:
-        if norm not in _NORM:
-            _fail(f"norm {norm!r}: 'rms' or 'layer'")
+        if norm not in _NORM or not (eps >= 0 and math.isfinite(eps)):
+            _fail(f"norm {norm!r}, eps {eps}: 'rms' or 'layer' and a number that is not negative are wanted")
         d.norm = _NORM[norm]
     for t, name in zip(params or (), ("q_weight", "k_weight", "q_bias", "k_bias")):
         if t is not None and (tuple(t[0]) != (D,) or t[3] != dev or not t[2].is_floating_point):
@@ -535,8 +539,8 @@ def attention_mod(q, k, v, heads, qlay, klay, kv_heads=None, scale=None, causal=
       causal         keys j <= i';  prefix (int32 [nbatch] or [nbatch, Sq], with causal): and all keys j < prefix
       q_docs, kv_docs  int32 [nbatch, Sq], [nbatch, Sk]: only keys of the query's document; numbers below 0 mark padding
     i' = i + kv_len - Sq is the query's place among the keys: the queries are the last positions.  A row that may see nothing is zero.
-    Keys and values that no query may see (behind kv_len, padding) may hold anything; a key or value that is visible to one query of a
-    sequence must be finite, since masked weights of its tile are exact zeros that multiply it.
+    Keys and values behind kv_len and of documents below 0 may hold anything; all others must be finite, also where the masks happen to
+    leave no query that sees them: masked weights of a tile are exact zeros that multiply its rows.
     Few query rows over many keys (serving steps, chunks of new tokens) split the keys over workgroups and join them.
     Returns [rows_q, heads * dim]; rows that no sequence owns are zero.  Differentiable in q, k, v and bias; K / V shared by the bdiv batches
     of a layout with lo = 0 get the sum of their gradients.  The order of all sums is fixed: repeated runs are bit-equal."""
