@@ -215,6 +215,8 @@ ATTN = {  # B, Sq, Sk, H, KV, D, dtype, options
     "long": (1, 1100, 1100, 2, 1, 64, BF, dict(causal=True, softcap=15.0)),
     "long keys": (1, 5, 4000, 4, 2, 128, BF, dict(causal=True, slopes=True)),
     "rows for a little more than one workgroup per CU": (1, 2100, 2110, 16, 16, 16, HF, dict(causal=True, prefix=[100], softcap=9.0)),
+    "documents in splits": (1, 1100, 1100, 2, 2, 64, BF, dict(docs=((200, 333, 5, 400), 162), causal=True, bias=20)),
+    "documents shuffled in splits": (2, 700, 5000, 2, 1, 40, HF, dict(docs="shuffled", softcap=7.0)),
     "very long keys": (1, 3, 40000, 2, 1, 64, HF, dict(causal=True, slopes=True)),
     "steps of long and short keys": (2, 1, 20000, 8, 2, 128, BF, dict(causal=True, softcap=12.0, kv_len=[20000, 777])),
     "few keys, many rows": (1, 1500, 30, 2, 2, 64, BF, {}),
@@ -602,6 +604,39 @@ def test_captured_training_step_replays_bit_equal():
         torch.cuda.synchronize()
         want = step()
         assert all(torch.equal(a, b) for a, b in zip(got, want)), n
+
+
+def test_a_captured_backward_pass_is_refused_while_an_eager_graph_holds_its_leaves():
+    """The leaf's accumulation belongs to the eager graph's stream: refused before it is reached.  Once that graph is gone the same pass is captured."""
+    F = _f()
+    x = torch.randn(64, 128, device="cuda").to(BF).requires_grad_()
+    w = torch.ones(64, device="cuda", requires_grad=True)
+    up, lay = torch.randn(64, 128, device="cuda").to(BF), F.SeqLayout(1, 64, 64, 0, 1)
+    pos = torch.arange(64, dtype=torch.int32, device="cuda").view(64, 1)
+    calls = {
+        "rope": (lambda: F.rope(x, 2, pos, F.RopeAxes((64,))), (x,)),
+        "norm": (lambda: F.qk_norm_rope(x, x, 2, 2, pos, F.RopeAxes((64,)), w, w)[0], (x, w)),
+        "attention": (lambda: F.attention_mod(x, x, x, 2, lay, lay, causal=True), (x,)),
+    }
+    for name, (f, leaves) in calls.items():
+        eager = f()
+        want = [t.clone() for t in torch.autograd.grad(eager, leaves, up, retain_graph=True)]
+        torch.cuda.synchronize()
+        with pytest.raises(RuntimeError, match="holds one of its leaves"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                torch.autograd.grad(f(), leaves, up)
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            f()                                                          # without a backward pass there is nothing to refuse
+        del eager
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            first = f()                                                  # (a graph of the capture's own that holds the leaves is no hindrance)
+            got = torch.autograd.grad(f(), leaves, up)
+        for _ in range(2):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(got, want)), name
+        del first
 
 
 def test_another_stream_than_the_operands_own():

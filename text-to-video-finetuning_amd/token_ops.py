@@ -9,9 +9,8 @@ Host side: what a call's arguments look like (shapes, strides, types, flags: nev
 a plan, the descriptor's bytes with the pointers left open and the sizes of its buffers; a call fills in the pointers.  Small
 calls are as long as their host code.
 
-Calls and their backward passes can be captured into a graph.  As with every autograd function, a captured backward() that accumulates
-into a leaf wants no other graph of that leaf alive from outside the capture (its accumulation belongs to the other stream): drop it first, or
-use autograd.grad.
+Calls and their backward passes can be captured into a graph; a captured backward pass whose leaves a graph from outside the capture still
+holds is refused (see _foreign_leaves).
 """
 import ctypes as C
 import functools
@@ -76,6 +75,7 @@ def _flat(cls):
 
 
 _RopeFlat, _AttnFlat = _flat(nv.QkRope), _flat(nv.AttnMod)
+_capturing = torch.cuda.is_current_stream_capturing
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
 
 
@@ -89,6 +89,38 @@ def _launch(name, desc, dev):
             rc = getattr(nv.lib(), name)(C.byref(desc), _raw_stream(index))
     if rc:
         nv.check(rc, name)
+
+
+def _foreign_leaves(tensors, dev):
+    """During a capture: (whether a graph from outside of it holds one of the leaves among `tensors`, what keeps the answer true until the call).
+
+    A leaf's accumulation node belongs to the stream on which the first living graph made it.  A captured backward pass that meets such a node of
+    another stream would join that stream to the capture, which ends the process.  Whether somebody holds the node shows by a mark that
+    outlives our own reference to it; nodes that a captured call has made carry the capture's stream."""
+    stream, kept, foreign = _raw_stream(dev.index), [], False
+    for t in tensors:
+        if t is None or not t.requires_grad or not t.is_leaf:
+            continue
+        node = torch.autograd.graph.get_gradient_edge(t).node
+        mark = node.metadata.get("t2v_stream")
+        if mark is None:
+            node.metadata["t2v_stream"] = "?"
+            del node
+            node = torch.autograd.graph.get_gradient_edge(t).node
+            if node.metadata.pop("t2v_stream", None) == "?":
+                foreign = True
+                continue
+            node.metadata["t2v_stream"] = stream
+        elif mark != stream:
+            foreign = True
+        kept.append(node)
+    return foreign, kept
+
+
+def _no_foreign_leaves(foreign):
+    if foreign and _capturing():
+        _fail("a backward pass cannot be captured while a graph from outside of the capture holds one of its leaves (the gradient would go "
+              "through that graph's stream): drop that graph, its outputs and losses, first")
 
 
 def _size(name, *args):
@@ -246,13 +278,14 @@ def _rope_bwd(plan, xs, dys, pos, freqs, ws, want):
 class _Rope(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, rest):
-        ctx.plan, pos, freqs = rest
+        ctx.plan, pos, freqs, ctx.foreign = rest
         ctx.save_for_backward(pos, freqs)
         return _rope_fwd(ctx.plan, (x,), pos, freqs, None, None)[0]
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
+        _no_foreign_leaves(ctx.foreign)
         pos, freqs = ctx.saved_tensors
         return _rope_bwd(ctx.plan, None, (_upstream(dy),), pos, freqs, None, None)[0][0], None
 
@@ -264,14 +297,15 @@ def rope(x, heads, pos, axes, freqs=None):
     _fixed(pos, freqs)
     plan = _rope_plan((_sig(x),), (int(heads), 0), axes, None, 0.0, _sig(pos), _sig(freqs), None)
     if torch.is_grad_enabled() and x.requires_grad:
-        return _Rope.apply(x, (plan, pos, freqs))
+        foreign, _kept = _foreign_leaves((x,), x.device) if _capturing() else (False, None)
+        return _Rope.apply(x, (plan, pos, freqs, foreign))
     return _rope_fwd(plan, (x,), pos, freqs, None, None)[0]
 
 
 class _QkNormRope(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, qw, kw, qb, kb, rest):
-        ctx.plan, ctx.key, pos, freqs = rest
+        ctx.plan, ctx.key, pos, freqs, ctx.foreign = rest
         ctx.types = [None if t is None else t.dtype for t in (qw, kw, qb, kb)]
         ctx.save_for_backward(q, k, qw, kw, pos, freqs)
         return _rope_fwd(ctx.plan, (q, k), pos, freqs, (_vector(qw), _vector(kw)), (_vector(qb), _vector(kb)))
@@ -279,6 +313,7 @@ class _QkNormRope(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dq, dk):
+        _no_foreign_leaves(ctx.foreign)
         q, k, qw, kw, pos, freqs = ctx.saved_tensors
         plan, sigs = ctx.plan, (_sig(q), _sig(k))
         if sigs != ctx.key[0]:                      # (a saved tensor may come back with other strides)
@@ -302,7 +337,8 @@ def qk_norm_rope(q, k, heads, kv_heads, pos, axes, q_weight=None, k_weight=None,
     plan = _rope_plan(*key)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or
                                     any([t is not None and t.requires_grad for t in (q_weight, k_weight, q_bias, k_bias)])):
-        return _QkNormRope.apply(q, k, q_weight, k_weight, q_bias, k_bias, (plan, key, pos, freqs))
+        foreign, _kept = _foreign_leaves((q, k, q_weight, k_weight, q_bias, k_bias), q.device) if _capturing() else (False, None)
+        return _QkNormRope.apply(q, k, q_weight, k_weight, q_bias, k_bias, (plan, key, pos, freqs, foreign))
     return _rope_fwd(plan, (q, k), pos, freqs, (_vector(q_weight), _vector(k_weight)), (_vector(q_bias), _vector(k_bias)))
 
 
@@ -477,7 +513,7 @@ def _attn_fwd(p, q, k, v, masks, bias, keep):
 class _AttentionMod(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, bias, rest):
-        ctx.plan, masks = rest
+        ctx.plan, masks, ctx.foreign = rest
         o, kept, tiles = _attn_fwd(ctx.plan, q, k, v, masks, bias, True)
         ctx.save_for_backward(q, k, v, bias, o, kept, tiles, *masks)
         return o
@@ -485,6 +521,7 @@ class _AttentionMod(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, do):
+        _no_foreign_leaves(ctx.foreign)
         q, k, v, bias, o, kept, tiles, *masks = ctx.saved_tensors
         p = ctx.plan
         dev, dtype = p.dev, p.dtype
@@ -554,5 +591,6 @@ def attention_mod(q, k, v, heads, qlay, klay, kv_heads=None, scale=None, causal=
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (bias is not None and bias.requires_grad)):
         if not p.shared_ok:
             _fail(f"key layout {klay} names a row twice: gradients are defined for rows of their own, or shared by the bdiv batches (lo = 0)")
-        return _AttentionMod.apply(q, k, v, bias, (p, masks))
+        foreign, _kept = _foreign_leaves((q, k, v, bias), p.dev) if _capturing() else (False, None)
+        return _AttentionMod.apply(q, k, v, bias, (p, masks, foreign))
     return _attn_fwd(p, q, k, v, masks, bias, False)[0]
