@@ -383,6 +383,31 @@ __device__ __forceinline__ int tile_next(TileIter& it, F active) {
   return t;
 }
 
+// The tiles [tbeg, tend) of split sp of [0, nt): equal numbers of those that count.  (Equal ranges of packed documents are mostly empty: 1839 tokens in
+// seven documents, 8 heads of 80, four splits: 42 us, so 34, unsplit 31; but the one document of a step over 4000 keys: 69 us unsplit, 17 split.)
+template <typename F>
+__device__ __forceinline__ void split_tiles(int nt, int splits, int sp, bool filter, F active, int& tbeg, int& tend) {
+  if (!filter || splits == 1) {
+    const int per = (nt + splits - 1) / splits;
+    tbeg = min(nt, sp * per);
+    tend = min(nt, tbeg + per);
+    return;
+  }
+  const int lane = threadIdx.x & 63;
+  int total = 0, seen = 0;
+  for (int base = 0; base < nt; base += 64) total += __popcll(__ballot(base + lane < nt && active(min(base + lane, nt - 1))));
+  const int per = (total + splits - 1) / splits, first = min(total, sp * per), last = first + per;
+  tbeg = tend = nt;
+  for (int base = 0; base < nt; base += 64) {
+    const unsigned long long m = __ballot(base + lane < nt && active(min(base + lane, nt - 1)));
+    const int n = __popcll(m), number = seen + __popcll(m & ((1ull << lane) - 1));       // of the lane's tile among those that count
+    const unsigned long long b = __ballot((m >> lane & 1) && number == first), e = __ballot((m >> lane & 1) && number == last);
+    if (b) tbeg = base + __builtin_ctzll(b);
+    if (e) tend = base + __builtin_ctzll(e);
+    seen += n;
+  }
+}
+
 // minimum / maximum over the wave as a scalar
 __device__ __forceinline__ int wave_min_i(int v) {
 #pragma unroll
@@ -486,10 +511,10 @@ __global__ __launch_bounds__(256, DP == 64 && MOD < 2 ? 3 : 2) void attn_mod_fwd
     dmax = max(dmax, swg[w * 4 + 2]);
   }
   bmax = __builtin_amdgcn_readfirstlane(bmax);
-  const int nt = (bmax + TILE - 1) / TILE, per = (nt + a.splits - 1) / a.splits;
-  const int tbeg = min(nt, sp * per), tend = min(nt, tbeg + per);
   const KMeta* km = docs ? a.kmeta + (long long)u.b * ((Sk + TILE - 1) / TILE) : nullptr;
   auto active = [&](int c) { return km[c].dmax >= dmin && km[c].dmin <= dmax; };
+  int tbeg, tend;
+  split_tiles((bmax + TILE - 1) / TILE, a.splits, sp, docs, active, tbeg, tend);
   TileIter it = {0ull, tbeg, tend, docs};
   const Lane<DP, 4> ln(wave, lane, D);
   const int lrow = lane_row<DP>(lane), ltr = lane_tr<DP>(lane);
@@ -889,11 +914,13 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(const Args a) {
   int* swg = sdoc + 2 * TILE;
   float* tab = (float*)(swg + 16);                                      // [2R + 1], then [4 waves][2R + 1] sums
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5;
+  const int NU = a.p.nbatch * a.nunit, sp = blockIdx.x / NU % a.splits;
   int tile;
   Part part;
-  const Unit u = work_of(a, blockIdx.x, tile, part);
+  const Unit u = work_of(a, blockIdx.x / (NU * a.splits) * NU + blockIdx.x % NU, tile, part);
   float* dtable = a.part_bias;                                          // of this workgroup (its head's 2R + 1 sums)
-  if (a.p.dbias) dtable += ((((long long)u.b * a.ntile + tile) * (a.qorder ? 2 : 1) + max(part.part, 0)) * a.p.heads + u.h0) * (2 * a.p.radius + 1);
+  if (a.p.dbias)
+    dtable += ((((long long)u.b * a.ntile + tile) * (a.qorder ? 2 : a.splits) + max(part.part, 0) + sp) * a.p.heads + u.h0) * (2 * a.p.radius + 1);
   if (part.none) {                                                      // workgroup-uniform
     if (a.p.dbias)
       for (int i = threadIdx.x; i < 2 * a.p.radius + 1; i += 256) dtable[i] = 0.f;
@@ -944,10 +971,11 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(const Args a) {
     dmax = max(dmax, swg[w * 4 + 2]);
   }
   bmax = __builtin_amdgcn_readfirstlane(bmax);
-  const int tend = (bmax + TILE - 1) / TILE;
   const KMeta* km = docs ? a.kmeta + (long long)u.b * ((Sk + TILE - 1) / TILE) : nullptr;
   auto active = [&](int c) { return km[c].dmax >= dmin && km[c].dmin <= dmax; };
-  TileIter it = {0ull, 0, tend, docs};
+  int tbeg, tend;
+  split_tiles((bmax + TILE - 1) / TILE, a.splits, sp, docs, active, tbeg, tend);
+  TileIter it = {0ull, tbeg, tend, docs};
   const Lane<DP, 4> ln(wave, lane, D);
   const int lrow = lane_row<DP>(lane), ltr = lane_tr<DP>(lane);
   const bf16_t* kp = ln.ok ? (const bf16_t*)a.p.k.ptr + op_base(a.p.k, u.b) + (long long)u.kv * D + ln.ch * 8 : (const bf16_t*)zero_chunk;
@@ -990,7 +1018,7 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(const Args a) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) dl = fmaf(El<T>::up(of[kd][e]) + El<T>::up(og[kd][e]), El<T>::up(gf[kd][e]), dl);
   dl = half_sum(dl);
-  if (R.ok && hi == 0) a.p.delta[sidx] = dl;
+  if (R.ok && hi == 0 && sp == 0) a.p.delta[sidx] = dl;
   if (t < tend) landed(t, 0, kn.neg);
   auto math = [&](bool partial, int t) {
     const int k0 = t * TILE;
@@ -1102,8 +1130,13 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(const Args a) {
     cur ^= 1;
     t = tn;
   }
-  bf16_t* dqp = (bf16_t*)a.p.dq.ptr + op_base(a.p.dq, u.b) + (long long)R.i * a.p.dq.sstride + (long long)R.h * D;
-  store_row<T, FM>(dqp, acc, a.p.scale, hi, D, R.ok);
+  if (a.splits > 1) {
+    const long long block = (((long long)sp * NU + u.x) * a.ntile + tile) * 4 + wave;                          // of 32 rows
+    store_part<FM>(a.part + block * (32 * DP), acc, lane, R.ok);
+  } else {
+    bf16_t* dqp = (bf16_t*)a.p.dq.ptr + op_base(a.p.dq, u.b) + (long long)R.i * a.p.dq.sstride + (long long)R.h * D;
+    store_row<T, FM>(dqp, acc, a.p.scale, hi, D, R.ok);
+  }
   if (dtab) {
     below = wave_sum(below);
     above = wave_sum(above);
@@ -1119,14 +1152,43 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(const Args a) {
   }
 }
 
-// dtable[h][d] = sum over (batch, row tile), in order (4 us, a launch); entries that hide their distance get 0 by construction (P = 0 there)
+// dQ = sum of the splits' partial sums, in order: one wave per 32 rows and 32 columns (8 us at 15 row tiles of 8 heads of 128 in four splits)
+template <typename T, int DP>
+__global__ __launch_bounds__(64) void attn_mod_dq_join_kernel(const Args a) {
+  constexpr int FM = DP / 32;
+  const int lane = threadIdx.x, hi = lane >> 5, D = a.p.D;
+  const int f = blockIdx.x % FM;
+  const long long block = blockIdx.x / FM;                              // over (unit x, tile, 32 rows)
+  const int NU = a.p.nbatch * a.nunit, per = a.ntile * 4, x = (int)(block / per);
+  const int r0 = (int)(block - (long long)x * per) * 32, r = min(r0 + (lane & 31), a.M - 1);
+  if (r0 >= a.M) return;                                                // workgroup-uniform
+  f32x16 acc[1];
+#pragma unroll
+  for (int e = 0; e < 16; ++e) acc[0][e] = 0.f;
+#pragma unroll 4
+  for (int s = 0; s < a.splits; ++s) {
+    const float* p = a.part + ((long long)s * NU * per + block) * (32 * DP) + (f * 256 + lane) * 4;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const f32x4 v = *(const f32x4*)(p + g * 256);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[0][4 * g + e] += v[e];
+    }
+  }
+  const Unit u = unit_of(a, x);
+  const int i = div_gp(a, r), h = u.h0 + r - i * a.gp;
+  bf16_t* dqp = (bf16_t*)a.p.dq.ptr + op_base(a.p.dq, u.b) + (long long)i * a.p.dq.sstride + (long long)h * D + 32 * f;
+  store_row<T, 1>(dqp, acc, a.p.scale, hi, D - 32 * f, r0 + (lane & 31) < a.M);
+}
+
+// dtable[h][d] = sum over (batch, row tile, split), in order (4 us, a launch); entries that hide their distance get 0 by construction (P = 0 there)
 template <typename T>
 __global__ __launch_bounds__(256) void attn_mod_dbias_kernel(const Args a) {
   const long long n = (long long)a.p.heads * (2 * a.p.radius + 1), i = (long long)blockIdx.x * 256 + threadIdx.x;
   if (i >= n) return;
   float s = 0.f;
 #pragma unroll 4
-  for (int k = 0; k < a.p.nbatch * a.ntile * (a.qorder ? 2 : 1); ++k) s += a.part_bias[(long long)k * n + i];
+  for (int k = 0; k < a.p.nbatch * a.ntile * (a.qorder ? 2 : a.splits); ++k) s += a.part_bias[(long long)k * n + i];
   if (a.p.bias_f32) ((float*)a.p.dbias)[i] = s;
   else ((unsigned short*)a.p.dbias)[i] = (unsigned short)(El<T>::pack2(s, 0.f) & 0xffffu);
 }
@@ -1445,8 +1507,8 @@ __global__ __launch_bounds__(64) void attn_mod_dkdv_join_kernel(const Args a) {
 // ------------------------------------------------------------------------------------------------ host
 struct Layout {
   Args a;
-  int qb, dp;
-  int fwd_tiles, fwd_splits, dq_tiles, kv_tiles;
+  int dp;
+  int fwd_tiles, fwd_splits, dq_tiles, dq_splits, kv_tiles;
   bool kv_split, meta;
   long long o_qmeta, o_kmeta, o_qorder, o_korder, meta_bytes, o_part, o_ml, o_bias, bytes;
   bool order;
@@ -1493,9 +1555,7 @@ Layout make_layout(const T2VAttnMod* p, bool bwd) {
   a.magic = a.gp > 1 ? (unsigned)(((1ull << 32) + a.gp - 1) / a.gp) : 0;
   L.dp = p->D <= 64 ? 64 : 128;
   const long long NU = (long long)p->nbatch * a.nunit;
-  L.qb = 1;
-  const int rows = 128 * L.qb;
-  L.fwd_tiles = (a.M + rows - 1) / rows;
+  L.fwd_tiles = (a.M + 127) / 128;
   L.fwd_splits = 1;
   if (!bwd) {
     // Few workgroups and a long key axis: the keys are split until ~512 workgroups exist, at least four 64-key tiles each (8 steps over up to 16384
@@ -1572,13 +1632,26 @@ Layout make_layout(const T2VAttnMod* p, bool bwd) {
     L.o_ml = at;
     at = align256(at + 8ll * L.fwd_splits * NU * L.fwd_tiles * 128);
   }
-  if (bwd && (L.kv_split || p->kv_share > 1)) {
+  if (bwd) {
+    // dQ: as the forward pass where there are few workgroups (backward of 4096 tokens, 2 heads of 64: 129 -> 83 us, 2500 causal, 4 heads of 128: 128 -> 94,
+    // 1024 tokens, 10 heads of 64: 58 -> 54)
+    const long long wgs = NU * L.dq_tiles;
+    const int kt = (p->Sk + TILE - 1) / TILE;
+    L.dq_splits = 1;
+    if (wgs < 256 && !L.order) {
+      const int s = (int)(512 / wgs);
+      L.dq_splits = s < kt / 4 ? s : kt / 4;
+      if (L.dq_splits < 1) L.dq_splits = 1;
+    }
+    // (the partial sums of dQ are joined before those of dK / dV are written)
+    const long long q = L.dq_splits > 1 ? 4ll * L.dq_splits * wgs * 128 * L.dp : 0;
+    const long long kv = L.kv_split || p->kv_share > 1 ? 8ll * p->nbatch * p->kv_heads * a.wgs * keys * L.dp : 0;
     L.o_part = at;
-    at = align256(at + 8ll * p->nbatch * p->kv_heads * a.wgs * keys * L.dp);
-  }
-  if (bwd && p->dbias) {
-    L.o_bias = at;
-    at = align256(at + 4ll * p->nbatch * L.dq_tiles * (L.order ? 2 : 1) * p->heads * (2 * p->radius + 1));
+    at = align256(at + (q > kv ? q : kv));
+    if (p->dbias) {
+      L.o_bias = at;
+      at = align256(at + 4ll * p->nbatch * L.dq_tiles * (L.order ? 2 : L.dq_splits) * p->heads * (2 * p->radius + 1));
+    }
   }
   L.bytes = at;
   char* w = (char*)p->meta;
@@ -1616,9 +1689,9 @@ int launch(int which, K kern, long long grid, size_t smem, hipStream_t st, const
 int mod_bits(const T2VAttnMod* p) { return (p->softcap > 0.f ? 1 : 0) | (p->slopes || p->bias ? 2 : 0); }
 
 // the rank at which the order turns: where all workgroups are resident, two on some CUs, the 256 longest come first
-int fold(const Layout& L, long long tiles) {
-  const long long NU = (long long)L.a.p.nbatch * L.a.nunit, wgs = NU * tiles;
-  return L.a.p.causal && wgs > 256 && wgs <= 512 ? (int)((256 + NU - 1) / NU) : 1 << 30;
+int fold(const Layout& L, int tiles, int splits) {
+  const long long row = (long long)L.a.p.nbatch * L.a.nunit * splits, wgs = row * tiles;
+  return L.a.p.causal && wgs > 256 && wgs <= 512 ? (int)((256 + row - 1) / row) : 1 << 30;
 }
 
 template <typename T, int DP>
@@ -1626,7 +1699,7 @@ int run_fwd(Layout& L, hipStream_t st) {
   Args& a = L.a;
   a.ntile = L.fwd_tiles;
   a.splits = L.fwd_splits;
-  a.fold = fold(L, L.fwd_tiles * L.fwd_splits);
+  a.fold = fold(L, L.fwd_tiles, L.fwd_splits);
   const long long grid = (long long)a.p.nbatch * a.nunit * L.fwd_tiles * L.fwd_splits * (a.qorder ? 2 : 1);
   const size_t sm = smem_bytes(L, 1, false);
   const int which = L.fwd_splits > 1 ? 1 : 3;
@@ -1648,14 +1721,19 @@ int run_bwd(Layout& L, hipStream_t st) {
   Args& a = L.a;
   const int mb = mod_bits(&a.p);
   a.ntile = L.dq_tiles;
-  a.splits = 1;
-  a.fold = fold(L, L.dq_tiles);
+  a.splits = L.dq_splits;
+  a.fold = fold(L, L.dq_tiles, L.dq_splits);
   const size_t sm = smem_bytes(L, a.p.dbias ? 5 : 1, false);
-  const long long gq = (long long)a.p.nbatch * a.nunit * L.dq_tiles * (a.qorder ? 2 : 1);
+  const long long gq = (long long)a.p.nbatch * a.nunit * L.dq_tiles * L.dq_splits * (a.qorder ? 2 : 1);
   int e = mb == 0 ? launch(1, attn_mod_dq_kernel<T, DP, 0>, gq, sm, st, a) : mb == 1 ? launch(1, attn_mod_dq_kernel<T, DP, 1>, gq, sm, st, a) :
           mb == 2 ? launch(1, attn_mod_dq_kernel<T, DP, 2>, gq, sm, st, a) : launch(1, attn_mod_dq_kernel<T, DP, 3>, gq, sm, st, a);
   if (e) return e;
   T2V_CHECK_LAUNCH();
+  if (a.splits > 1) {
+    const long long blocks = (long long)a.p.nbatch * a.nunit * a.ntile * 4 * (DP / 32);
+    hipLaunchKernelGGL((attn_mod_dq_join_kernel<T, DP>), dim3((unsigned)blocks), dim3(64), 0, st, a);
+    T2V_CHECK_LAUNCH();
+  }
   if (a.p.dbias) {
     const long long n = (long long)a.p.heads * (2 * a.p.radius + 1);
     hipLaunchKernelGGL(attn_mod_dbias_kernel<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, a);
