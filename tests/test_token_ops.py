@@ -149,6 +149,10 @@ def test_flat_descriptors_have_the_pointers_where_the_header_has_them():
     a = nv.AttnMod.from_buffer_copy(d)
     got = [getattr(a, n).ptr if k is nv.AttnOperand else getattr(a, n) for n, k in nv.AttnMod._fields_]
     assert [v for v in got if v and v >= 100] == list(range(100, 119))
+    d = T._AttnFlat()
+    d.d_o, d.d_o_bstride_hi, d.d_o_bstride_lo, d.d_o_sstride, d.d_o_bdiv, d.dq = 1, 1 << 40, 256, 768, 3, 5
+    a = nv.AttnMod.from_buffer_copy(d)
+    assert (a.d_o.ptr, a.d_o.bstride_hi, a.d_o.bstride_lo, a.d_o.sstride, a.d_o.bdiv, a.dq.ptr) == (1, 1 << 40, 256, 768, 3, 5)
     d = T._RopeFlat()
     for n, name in enumerate(("x", "ldx", "dy", "lddy", "y", "ldy", "heads", "w", "b", "dw", "db")):
         setattr(d, name + "0", 10 + 2 * n)

@@ -4,6 +4,7 @@ import math
 
 import pytest
 import torch
+import torch.utils.checkpoint
 
 import token_ops_ref as ref
 
@@ -652,6 +653,76 @@ def test_another_stream_than_the_operands_own():
         both = F.rope(got, 2, torch.arange(300, device="cuda").view(300, 1), F.RopeAxes((64,)))
     torch.cuda.current_stream().wait_stream(s)
     assert torch.equal(got, want) and torch.equal(both, F.rope(want, 2, torch.arange(300, device="cuda").view(300, 1), F.RopeAxes((64,))))
+
+
+def _train_call(F, S=700, H=4, KV=2, D=72, seed=21):
+    """One pass with every kind of saved tensor, as a function of how its gradients are asked for."""
+    g = torch.Generator().manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=g).to(BF).cuda().requires_grad_()  # noqa: E731
+    q, k, v, bias = r(S, H * D), r(S, KV * D), r(S, KV * D), r(H, 41)
+    w = torch.ones(D, device="cuda", requires_grad=True)
+    docs = torch.randint(0, 3, (1, S), generator=g).int().cuda()
+    pos = torch.arange(S, dtype=torch.int32, device="cuda").view(S, 1)
+    lay = F.SeqLayout(1, S, S, 0, 1)
+
+    def f(q, k, v, bias, w):
+        a, b = F.qk_norm_rope(q, k, H, KV, pos, F.RopeAxes((64,), style="half"), w, w)
+        return F.attention_mod(F.rope(a, H, pos, F.RopeAxes((32,))), b, v, H, lay, lay, kv_heads=KV, causal=True, bias=bias, q_docs=docs, kv_docs=docs, softcap=9.0)
+
+    return f, (q, k, v, bias, w)
+
+
+def test_upstream_gradients_of_any_layout():
+    F = _f()
+    f, leaves = _train_call(F)
+    for up in (torch.ones(1, 288, device="cuda").to(BF).expand(700, 288), torch.randn(288, 700, device="cuda").to(BF).t(),
+               torch.randn(700, 300, device="cuda").to(BF)[:, 5:293], torch.randn(700, 320, device="cuda").to(BF)[:, 8:296]):
+        got = torch.autograd.grad(f(*leaves), leaves, up)
+        want = torch.autograd.grad(f(*leaves), leaves, up.contiguous().clone())
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_saved_tensors_may_travel_and_calls_may_be_recomputed():
+    """Saved tensors moved to the host and back, and a recomputed forward pass, give the bits of the plain pass."""
+    F = _f()
+    f, leaves = _train_call(F)
+    up = torch.randn(700, 288, device="cuda").to(BF)
+    want = torch.autograd.grad(f(*leaves), leaves, up)
+    with torch.autograd.graph.save_on_cpu():
+        o = f(*leaves)
+    got = torch.autograd.grad(o, leaves, up)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    again = torch.utils.checkpoint.checkpoint(f, *leaves, use_reentrant=False)
+    got = torch.autograd.grad(again, leaves, up)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_two_calls_at_once():
+    """Passes with workspaces of their own on two streams, interleaved."""
+    F = _f()
+    jobs = [_train_call(F, seed=n) for n in (31, 32)]
+    up = torch.randn(700, 288, device="cuda").to(BF)
+    want = [torch.autograd.grad(f(*leaves), leaves, up) for f, leaves in jobs]
+    streams = [torch.cuda.Stream() for _ in jobs]
+    torch.cuda.synchronize()
+    got = [None, None]
+    for _ in range(5):
+        for n, ((f, leaves), s) in enumerate(zip(jobs, streams)):
+            with torch.cuda.stream(s):
+                got[n] = torch.autograd.grad(f(*leaves), leaves, up)
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_keys_that_all_batches_read():
+    """A key layout that names the same rows for every batch is read, but has no gradients of its own."""
+    F = _f()
+    q, k = torch.randn(40, 128, device="cuda").to(BF), torch.randn(33, 128, device="cuda").to(BF)
+    lay = F.SeqLayout(4, 10, 10, 0, 1)
+    a = F.attention_mod(q, k, k, 2, lay, F.SeqLayout(4, 33, 0, 0, 1))
+    b = F.attention_mod(q, k.repeat(4, 1), k.repeat(4, 1), 2, lay, F.SeqLayout(4, 33, 33, 0, 1))
+    assert torch.equal(a, b)
 
 
 def test_offsets_beyond_32_bits():

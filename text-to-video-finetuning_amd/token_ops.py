@@ -60,11 +60,11 @@ def _sig(t):
 
 
 def _flat(cls):
-    """A structure laid out like `cls` whose pointers are plain fields: operands become name (the pointer) and name_rest, pairs name0 and name1."""
+    """A structure laid out like `cls` whose pointers are plain fields: operands become name (the pointer), name_sstride, .., pairs name0 and name1."""
     fields = []
     for name, kind in cls._fields_:
         if kind is nv.AttnOperand:
-            fields += [(name, C.c_void_p), (name + "_rest", C.c_char * (C.sizeof(kind) - 8))]
+            fields += [(name if n == "ptr" else f"{name}_{n}", k) for n, k in kind._fields_] + [(name + "_pad", C.c_int)]
         elif isinstance(kind, type) and issubclass(kind, C.Array) and kind._length_ == 2:
             fields += [(name + "0", kind._type_), (name + "1", kind._type_)]
         else:
@@ -544,7 +544,8 @@ class _AttentionMod(torch.autograd.Function):
         d.workspace_bytes, d.delta = work_bytes, at + work_bytes
         d.d_o, d.dq, d.dk, d.dv = do.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
         if not do.is_contiguous():
-            d.d_o_rest = bytes(_operand(_ld(do.shape, do.stride()), p.lays[0]))[8:]
+            ld, lay = _ld(do.shape, do.stride()), p.lays[0]
+            d.d_o_bstride_hi, d.d_o_bstride_lo, d.d_o_sstride = lay.hi * ld, lay.lo * ld, lay.ss * ld
         dbias = None
         if with_bias:
             dbias = torch.empty(bias.shape, dtype=bias.dtype, device=dev)
