@@ -680,6 +680,17 @@ def test_upstream_gradients_of_any_layout():
         got = torch.autograd.grad(f(*leaves), leaves, up)
         want = torch.autograd.grad(f(*leaves), leaves, up.contiguous().clone())
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+    # the rotary calls alone, one side's upstream gradient dense and the other's a slice
+    x, w = torch.randn(300, 256, device="cuda").to(BF).requires_grad_(), torch.rand(64, device="cuda").requires_grad_()
+    pos = torch.arange(300, dtype=torch.int32, device="cuda").view(300, 1)
+    wide, dense = torch.randn(300, 400, device="cuda").to(BF)[:, 16:144], torch.randn(300, 128, device="cuda").to(BF)
+    for ups in ((wide, dense), (dense, wide), (wide, wide)):
+        call = lambda: F.qk_norm_rope(x[:, :128], x[:, 128:], 2, 2, pos, F.RopeAxes((64,)), w, w)  # noqa: E731
+        got = torch.autograd.grad(call(), (x, w), ups)
+        want = torch.autograd.grad(call(), (x, w), [u.contiguous().clone() for u in ups])
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    got, want = (torch.autograd.grad(F.rope(x[:, 128:], 2, pos, F.RopeAxes((64,))), x, u)[0] for u in (wide, wide.contiguous().clone()))
+    assert torch.equal(got, want)
 
 
 def test_saved_tensors_may_travel_and_calls_may_be_recomputed():
@@ -695,6 +706,20 @@ def test_saved_tensors_may_travel_and_calls_may_be_recomputed():
     again = torch.utils.checkpoint.checkpoint(f, *leaves, use_reentrant=False)
     got = torch.autograd.grad(again, leaves, up)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+    # slices of one matrix come back with other strides
+    x = torch.randn(200, 640, device="cuda").to(BF).requires_grad_()
+    lay, pos = F.SeqLayout(2, 100, 100, 0, 1), torch.arange(200, dtype=torch.int32, device="cuda").view(200, 1)
+    up = torch.randn(200, 256, device="cuda").to(BF)
+
+    def g(x):
+        o = F.attention_mod(x[:, :256], x[:, 256:384], x[:, 384:512], 4, lay, lay, kv_heads=2, causal=True)
+        return o + F.qk_norm_rope(x[:, 256:512], x[:, 512:], 4, 2, pos, F.RopeAxes((64,)))[0]
+
+    want, = torch.autograd.grad(g(x), x, up)
+    with torch.autograd.graph.save_on_cpu():
+        o = g(x)
+    got, = torch.autograd.grad(o, x, up)
+    assert torch.equal(got, want)
 
 
 def test_two_calls_at_once():
