@@ -199,6 +199,8 @@ ATTN = {  # B, Sq, Sk, H, KV, D, dtype, options
     "table fp32 groups": (1, 90, 150, 4, 2, 128, BF, dict(bias=16, bias_f32=True, softcap=10.0)),
     "table of one entry": (1, 40, 40, 2, 2, 64, BF, dict(bias=0)),
     "table wide": (1, 130, 130, 2, 1, 64, HF, dict(bias=1024, slopes=True)),
+    "table wide of 128": (1, 150, 190, 2, 2, 128, BF, dict(bias=1024, slopes=True, softcap=11.0, causal=True)),
+    "many query heads of one key head": (2, 37, 130, 70, 1, 24, HF, dict(causal=True, kv_len=[130, 64])),
     "lengths": (4, 50, 150, 2, 2, 64, BF, dict(kv_len=[150, 1, 0, 77], causal=True)),
     "lengths two ways": (3, 40, 100, 2, 1, 128, BF, dict(kv_len=[100, 3, 64])),
     "prefix per query": (2, 90, 90, 2, 2, 64, BF, dict(causal=True, prefix="query")),
@@ -720,6 +722,53 @@ def test_saved_tensors_may_travel_and_calls_may_be_recomputed():
         o = g(x)
     got, = torch.autograd.grad(o, x, up)
     assert torch.equal(got, want)
+
+
+def test_parameters_of_other_types_and_gradients_of_some_inputs_only():
+    F = _f()
+    x = torch.randn(130, 256, device="cuda").to(BF).requires_grad_()
+    pos, axes = torch.arange(130, dtype=torch.int32, device="cuda").view(130, 1), F.RopeAxes((32,))
+    w32 = torch.rand(128, device="cuda").to(BF).float()
+    ups = [torch.randn(130, 128, device="cuda").to(BF) for _ in range(2)]
+
+    def grads(w, b, wrt):
+        return torch.autograd.grad(F.qk_norm_rope(x[:, :128], x[:, 128:], 2, 2, pos, axes, w, None, None, b, norm="layer"), wrt, ups)
+
+    w, b = w32[:64].clone().requires_grad_(), w32[64:].clone().requires_grad_()
+    want = grads(w, b, (x, w, b))
+    for dt in (BF, torch.float64):                                       # (values of bf16: fp32 holds them too)
+        v, c = w.detach().to(dt).requires_grad_(), b.detach().to(dt).requires_grad_()
+        got = grads(v, c, (x, v, c))
+        assert torch.equal(got[0], want[0]) and all(g.dtype == dt and torch.equal(g, u.to(dt)) for g, u in zip(got[1:], want[1:]))
+    two = torch.stack([w32[:64], w32[64:]], 1).requires_grad_()           # columns of a matrix
+    got = grads(two[:, 0], two[:, 1], (x, two))
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], torch.stack(want[1:], 1))
+    assert torch.equal(grads(w, b.detach(), (w,))[0], want[1]) and torch.equal(grads(w.detach(), b, (b,))[0], want[2])
+    f, leaves = _train_call(F, S=150)
+    up = torch.randn(150, 288, device="cuda").to(BF)
+    want = torch.autograd.grad(f(*leaves), leaves, up)
+    for n in range(5):
+        only = [t if i == n else t.detach() for i, t in enumerate(leaves)]
+        assert torch.equal(torch.autograd.grad(f(*only), only[n], up)[0], want[n]), n
+
+
+def test_sequences_across_the_rows():
+    """Temporal layouts: sequence b = (clip, pixel), its rows a frame apart; keys of every second frame only."""
+    F = _f()
+    C, T, P, H, D = 2, 7, 9, 2, 64
+    q, k, v = (torch.randn(C * T * P, H * D, device="cuda").to(BF).requires_grad_() for _ in range(3))
+    up = torch.randn(C * T * P, H * D, device="cuda").to(BF)
+    o = F.attention_mod(q, k, v, H, F.SeqLayout(C * P, T, T * P, 1, P, P), F.SeqLayout(C * P, 4, T * P, 1, 2 * P, P), causal=True, softcap=5.0)
+    got = torch.autograd.grad(o, (q, k, v), up)
+    turn = lambda t: t.detach().view(C, T, P, H * D).transpose(1, 2).reshape(C * P * T, H * D).contiguous()  # noqa: E731
+    qs, us = turn(q).requires_grad_(), turn(up)
+    ks, vs = (turn(t).view(C * P, T, H * D)[:, ::2].reshape(-1, H * D).contiguous().requires_grad_() for t in (k, v))
+    p = F.attention_mod(qs, ks, vs, H, F.SeqLayout(C * P, T, T, 0, 1), F.SeqLayout(C * P, 4, 4, 0, 1), causal=True, softcap=5.0)
+    want = torch.autograd.grad(p, (qs, ks, vs), us)
+    assert torch.equal(turn(o), p) and torch.equal(turn(got[0]), want[0])
+    for a, b in zip(got[1:], want[1:]):
+        a = turn(a).view(C * P, T, H * D)
+        assert torch.equal(a[:, ::2].reshape(-1, H * D), b) and (a[:, 1::2] == 0).all()
 
 
 def test_two_calls_at_once():
