@@ -1,0 +1,93 @@
+"""Calls of the transformer-block operators at the edges of what they document: rows that a sorted work list must not lose, extreme table entries,
+large caps, forward-mode derivatives, operands that need no gradient.  Plain 64-bit forms and derived bounds as in tests/token_ops_ref.py."""
+import contextlib
+import math
+
+import pytest
+import torch
+
+import token_ops_ref as ref
+
+pytestmark = pytest.mark.gpu
+BF, HF, F32, F64 = torch.bfloat16, torch.float16, torch.float32, torch.float64
+
+
+def _f():
+    import t2v_amd  # noqa: F401
+    import t2v_amd.functional as F
+    return F
+
+
+def _within(name, got, want, bound):
+    got = got.detach().cpu().to(F64).reshape(want.shape)
+    assert torch.isfinite(got).all(), f"{name}: {int((~torch.isfinite(got)).sum())} values are not finite"
+    at = ((got - want).abs() / bound).max()
+    assert ((got - want).abs() <= bound).all(), f"{name}: {float(at):.2f} times the bound"
+
+
+@contextlib.contextmanager
+def _empty_is_nan():
+    """New tensors start as NaN (bytes: 255), so that what a call leaves unwritten shows."""
+    before = torch.are_deterministic_algorithms_enabled(), torch.is_deterministic_algorithms_warn_only_enabled()
+    torch.use_deterministic_algorithms(True, warn_only=True)
+    try:
+        assert torch.empty(8, dtype=BF, device="cuda").isnan().all()
+        yield
+    finally:
+        torch.use_deterministic_algorithms(before[0], warn_only=before[1])
+
+
+# ------------------------------------------------------------------------------------------------ rows that see nothing, sorted documents
+def _falling(n, *runs):
+    """Documents of falling number, one run behind the other."""
+    return torch.cat([torch.full((c,), len(runs) - k, dtype=torch.int32) for k, c in enumerate(runs)])[None].expand(n, -1).contiguous()
+
+
+UNSEEN = {  # B, Sq, Sk, H, KV, D, dtype, masks.  Enough workgroups for the sorted work list (rows * heads above 32768)
+    "short keys, falling documents": (1, 400, 400, 96, 96, 64, BF, dict(kv_len=[350], q=(50, 350), k=(50, 350))),
+    "fewer keys than queries": (1, 400, 330, 96, 96, 72, HF, dict(q=(60, 230, 110), k=(20, 200, 110))),
+    "grouped heads, two lengths": (2, 300, 300, 64, 8, 40, BF, dict(kv_len=[300, 170], q=(130, 100, 70), k=(130, 100, 70))),
+    "a table": (1, 400, 400, 96, 48, 16, BF, dict(kv_len=[290], q=(100, 60, 240), k=(100, 60, 240), bias=9)),
+    "a prefix per query": (1, 512, 512, 80, 80, 24, BF, dict(kv_len=[250], q="rising", k="rising", prefix=True)),
+    "no keys": (2, 300, 300, 64, 64, 8, BF, dict(kv_len=[0, 300], q=(100, 200), k=(100, 200))),
+}
+
+
+@pytest.mark.parametrize("name", list(UNSEEN))
+def test_rows_that_see_nothing_are_written_under_the_sorted_work_list(name):
+    F = _f()
+    B, Sq, Sk, H, KV, D, dt, opt = UNSEEN[name]
+    assert Sq * H * B > 32768
+    g = torch.Generator().manual_seed(len(name))
+    r = lambda *s: torch.randn(*s, generator=g).to(dt)  # noqa: E731
+    q, k, v, do = r(B, Sq, H, D), r(B, Sk, KV, D), r(B, Sk, KV, D), r(B, Sq, H, D)
+    docs = [(torch.arange(n) // 64).int()[None].repeat(B, 1) if opt[s] == "rising" else _falling(B, *opt[s]) for s, n in (("q", Sq), ("k", Sk))]
+    kw = dict(causal=True, q_docs=docs[0], kv_docs=docs[1])
+    if "kv_len" in opt:
+        kw["kv_len"] = torch.tensor(opt["kv_len"], dtype=torch.int32)
+    if "bias" in opt:
+        kw["bias"] = r(H, 2 * opt["bias"] + 1)
+    if "prefix" in opt:
+        kw["prefix"] = (10 * (torch.arange(Sq) // 64 % 2 == 0)).int()[None].repeat(B, 1)
+    want = ref.attention(q, k, v, D ** -0.5, dt, do=do, **kw)
+    flat = [t.reshape(t.shape[0] * t.shape[1], -1).cuda().requires_grad_() for t in (q, k, v)]
+    dkw = {n: t.cuda() if torch.is_tensor(t) else t for n, t in kw.items()}
+    if "bias" in dkw:
+        dkw["bias"].requires_grad_()
+    lays = F.SeqLayout(B, Sq, Sq, 0, 1), F.SeqLayout(B, Sk, Sk, 0, 1)
+    with _empty_is_nan():
+        o = F.attention_mod(*flat, H, *lays, kv_heads=KV, **dkw)
+        o.backward(do.reshape(B * Sq, -1).cuda())
+        with torch.no_grad():
+            o2 = F.attention_mod(*flat, H, *lays, kv_heads=KV, **dkw)
+    none = torch.stack([~ref.visible(Sq, Sk, Sk if "kv_len" not in opt else opt["kv_len"][b], True, kw["prefix"][b] if "prefix" in kw else None,
+                                     docs[0][b], docs[1][b]).any(1) for b in range(B)]).view(-1)
+    assert none.any()
+    for t in (o, o2, flat[0].grad):
+        assert (t[none.cuda()] == 0).all()
+    _within("o", o, *want["o"])
+    _within("o (no grad)", o2, *want["o"])
+    for n, t in zip(("dq", "dk", "dv"), flat):
+        _within(n, t.grad, *want[n])
+    if "bias" in dkw:
+        _within("dbias", dkw["bias"].grad, *want["dbias"])

@@ -176,7 +176,7 @@ __device__ __forceinline__ Unit unit_of(const Args& a, int x) {
 }
 // Which rows (keys) of a tile are a workgroup's own: all of them, or those of its entry (see attn_mod_order_kernel)
 struct Part {
-  int first, part;                  // part 0: documents <= first (and none), 1: documents > first, -1: all
+  int first, part;                  // part 0: documents <= first, and rows that see nothing, 1: documents > first, -1: all
   bool none;                        // an entry without rows
   __device__ __forceinline__ bool owns(int doc) const { return part < 0 || (doc > first) == (part == 1); }
 };
@@ -437,10 +437,12 @@ __device__ __forceinline__ void load_rows(Rows& R, const Args& a, const Unit& u,
   R.i = div_gp(a, rc);
   R.h = u.h0 + rc - R.i * a.gp;
   R.doc = a.p.q_docs ? a.p.q_docs[(long long)u.b * a.p.Sq + R.i] : 0;
-  R.ok = R.ok && part.owns(R.doc);
-  R.bound = R.ok ? row_bound(sq, R.i) : 0;
+  R.bound = R.ok && R.doc >= 0 ? row_bound(sq, R.i) : 0;
+  // (The tiles' entries hold the documents of rows that see something, and by them a second part may be empty: a row that sees nothing is of
+  // the first part, whatever its document.)
+  R.ok = R.ok && part.owns(R.bound > 0 ? R.doc : -1);
+  if (!R.ok) R.bound = 0;
   R.pos = R.i + sq.off;
-  if (R.doc < 0) R.bound = 0;
   R.slope = a.p.slopes ? a.p.slopes[R.h] * LOG2E : 0.f;
   if (R.ok) lo = min(lo, R.bound);
   hi = max(hi, R.bound);
