@@ -27,7 +27,7 @@ typedef void* t2v_stream_t; /* hipStream_t */
 #define T2V_OK 0
 #define T2V_EINVAL (-1)
 #define T2V_ELAUNCH (-2)
-#define T2V_ABI_VERSION 10   /* bumped whenever a struct layout or a signature changes (native.py checks it) */
+#define T2V_ABI_VERSION 11   /* bumped whenever a struct layout or a signature changes (native.py checks it) */
 
 int t2v_abi_version(void);
 const char* t2v_last_error(void);
@@ -292,10 +292,12 @@ int t2v_attn_bwd(const T2VAttn* p, t2v_stream_t stream);
  * len = kv_len[b] (clamped to 0..Sk) or Sk; i' = i + len - Sq: the queries are the last Sq positions.  Query i sees key j iff
  * j < len, (not causal or j <= i' or j < prefix), and q_docs[b][i] == kv_docs[b][j] >= 0 (where documents are given).
  * prefix: [nbatch] or (prefix_per_query) [nbatch, Sq].  bias: [heads, 2 radius + 1], in the operands' type or (bias_f32) fp32; an entry
- * at or below its type's lowest finite value hides its distance.  Rows that no query may see (key >= len, document < 0) are not read
+ * at or below its type's lowest finite value hides its distance; finite entries beyond +-2e38 count as +-2e38.  Scores are held in fp32: beside an
+ * entry of 1e6 the rest of a score is rounded to 0.1.  Rows that no query may see (key >= len, document < 0) are not read
  * into any sum: they may hold anything.  Operands as in T2VAttn with head stride D: element (b, s, h, d) at
  *   ptr + (b / bdiv) * bstride_hi + (b % bdiv) * bstride_lo + s * sstride + h * D + d      (k, v, dk, dv: kv_heads)
- * lse: fp32 [nbatch, heads, Sq], base-2 log-sum-exp in an order of the library's own: kept for the backward call; NULL: not written.
+ * lse: fp32 [nbatch, heads, Sq], base-2 log-sum-exp in an order of the library's own, with slopes or a bias [2, nbatch, heads, Sq] (largest exponent,
+ * logarithm of the sum behind it): kept for the backward call; NULL: not written.
  * o_rest: NULL, or laid out and typed like o: what rounding o to its type left behind; the backward call's delta = rowsum(dO * O) is formed
  * with it where it is given again (the error of delta, 2^-9 of bf16's O, is otherwise as large as that of the gradients' own rounding).
  * scale: 1e-15 to 1e6; softcap: 0 or 1e-6 to 1e4 (the cap's tanh is good to 4e-7 cap: a larger one is no cap for any score that counts).

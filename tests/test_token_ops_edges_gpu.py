@@ -91,3 +91,70 @@ def test_rows_that_see_nothing_are_written_under_the_sorted_work_list(name):
         _within(n, t.grad, *want[n])
     if "bias" in dkw:
         _within("dbias", dkw["bias"].grad, *want["dbias"])
+
+
+# ------------------------------------------------------------------------------------------------ table entries far outside of the scores
+FAR = {  # B, Sq, Sk, H, KV, D, dtype, far entry, table's type, rest.  "away": the documents of rows below 60 and above 89 lie at the other end
+    "low, bf16": (1, 150, 150, 2, 2, 64, BF, -1e30, BF, dict(away=True)),
+    "low, fp32, groups": (2, 150, 150, 4, 2, 128, BF, -1e30, F32, dict(away=True, softcap=9.0)),
+    "low, with slopes": (1, 150, 150, 2, 1, 72, HF, -1e30, F32, dict(away=True, slopes=True)),
+    "lowest but one": (1, 150, 150, 2, 2, 64, BF, -3.3e38, F32, dict(away=True)),
+    "lowest but one, bf16": (1, 150, 150, 2, 2, 128, BF, -3.3e38, BF, dict(away=True)),
+    "high": (1, 150, 150, 2, 2, 64, BF, 1e30, F32, dict(away=True)),
+    "highest": (1, 150, 150, 2, 2, 128, BF, 3.3e38, BF, dict(away=True)),
+    "a mask of -1e9": (1, 150, 150, 2, 2, 64, BF, -1e9, F32, dict(away=True, zero=True)),
+    "a mask of -60000 in fp16": (2, 150, 150, 2, 2, 128, HF, -60000.0, HF, dict(away=True, zero=True)),
+    "one far score for all keys": (1, 70, 200, 2, 2, 64, BF, 1e9, F32, dict(all=True, zero=True)),
+    "splits": (1, 3, 4000, 4, 2, 64, BF, -1e30, F32, dict(hide=100)),
+    "splits, some near": (1, 3, 4000, 4, 2, 128, HF, -1e30, F32, dict(causal=True)),
+    "no table: large negative products": (1, 40, 300, 2, 1, 64, BF, None, None, dict(huge=True)),
+}
+
+
+@pytest.mark.parametrize("name", list(FAR))
+def test_entries_far_outside_of_the_scores_are_scores(name):
+    """Only an entry at or below its type's lowest value hides its distance.  A row whose keys all carry -1e30 (or +1e30) is their mean: at that size a
+    score of ordinary size is lost in 64 bits too.  Entries that leave ordinary scores in 64 bits but not in 32 are tested with queries of zero."""
+    F = _f()
+    B, Sq, Sk, H, KV, D, dt, far, tdt, opt = FAR[name]
+    g = torch.Generator().manual_seed(len(name) + D)
+    r = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    q, k, v, do = r(B, Sq, H, D).to(dt), r(B, Sk, KV, D).to(dt), r(B, Sk, KV, D).to(dt), r(B, Sq, H, D).to(dt)
+    kw = dict(causal=opt.get("causal", False), softcap=opt.get("softcap", 0.0))
+    if opt.get("zero"):
+        q.zero_()
+    if opt.get("slopes"):
+        kw["slopes"] = 0.1 + 0.2 * torch.rand(H, generator=g)
+    if tdt is not None:
+        bias = r(H, 9).to(tdt)
+        bias[:, 0] = bias[:, -1] = far
+        if opt.get("all"):
+            bias[:] = far
+        kw["bias"] = bias
+    if opt.get("away"):
+        i = torch.arange(150).int()
+        kw["q_docs"] = ((i >= 60).int() + (i >= 90).int())[None].repeat(B, 1)
+        kw["kv_docs"] = (2 - kw["q_docs"]).contiguous()
+    if "hide" in opt:
+        kw["q_docs"], kw["kv_docs"] = torch.zeros(B, Sq, dtype=torch.int32), torch.zeros(B, Sk, dtype=torch.int32)
+        kw["kv_docs"][:, -opt["hide"]:] = -1
+    if opt.get("huge"):       # every product is -64 * 2^100, below -1e30, exactly: the weights are equal, and scores' gradients times keys cancel to 0
+        q[:], k[:] = 2.0 ** 50, -2.0 ** 50
+    want = ref.attention(q, k, v, D ** -0.5, dt, do=do, **kw)
+    flat = [t.reshape(t.shape[0] * t.shape[1], -1).cuda().requires_grad_() for t in (q, k, v)]
+    dkw = {n: t.cuda() if torch.is_tensor(t) else t for n, t in kw.items()}
+    if tdt is not None:
+        dkw["bias"].requires_grad_()
+    lays = F.SeqLayout(B, Sq, Sq, 0, 1), F.SeqLayout(B, Sk, Sk, 0, 1)
+    o = F.attention_mod(*flat, H, *lays, kv_heads=KV, **dkw)
+    o.backward(do.reshape(B * Sq, -1).cuda())
+    with torch.no_grad():
+        o2 = F.attention_mod(*flat, H, *lays, kv_heads=KV, **dkw)
+    _within("o", o, *want["o"])
+    _within("o (no grad)", o2, *want["o"])
+    if opt.get("huge"):
+        return                # (the backward pass's fp32 log-sum-exp cannot hold the logarithm of the count beside 2^106: no claim there)
+    for n, t in zip(("dq", "dk", "dv"), flat):
+        _within(n, t.grad, *want[n])
+    if tdt is not None:
+        _within("dbias", dkw["bias"].grad, *want["dbias"])

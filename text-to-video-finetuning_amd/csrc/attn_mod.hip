@@ -25,7 +25,8 @@ namespace {
 
 constexpr int TILE = 64;                        // staged rows
 constexpr float LOG2E = 1.44269504088896341f;
-constexpr float LOWEST = -1.0e30f;              // running maximum before the first visible key: finite, below every score
+constexpr float LOWEST = -3.0e38f;              // running maximum before the first visible key: finite, below every score
+constexpr float FAREST = 2.9e38f;               // finite table entries in base-2 units are held inside +-FAREST, above LOWEST
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
 typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2_t;
@@ -108,6 +109,7 @@ struct Args {
   int to_part;                      // dK / dV go to `part` as fp32 (several splits, or several batches that share K / V)
   const QMeta* qmeta;               // [nbatch][ceil(M / 64)] or NULL
   const KMeta* kmeta;               // [nbatch][ceil(Sk / 64)] or NULL
+  float* lsum;                      // second plane of lse (slopes or a bias), or NULL
   float* part;                      // partial results of the splits
   float* part_ml;
   float* part_bias;                 // [nbatch * ntile (* parts)][heads][2R + 1]
@@ -348,15 +350,19 @@ __device__ __forceinline__ float capped(const Mod& m, float s, float& w) {
 template <typename T>
 __device__ __forceinline__ void load_table(const Args& a, int h, float* tab, int tid, int nt) {
   const int n = 2 * a.p.radius + 1;
+  const auto units = [](float v) {                                      // (NaN stays NaN)
+    const float w = v * LOG2E;
+    return w < -FAREST ? -FAREST : w > FAREST && v < INFINITY ? FAREST : w;
+  };
   for (int i = tid; i < n; i += nt) {
     const long long at = (long long)h * n + i;
     float v;
     if (a.p.bias_f32) {
       v = ((const float*)a.p.bias)[at];
-      v = v <= -3.4028234e38f ? -INFINITY : v * LOG2E;
+      v = v <= -3.4028234e38f ? -INFINITY : units(v);
     } else {
       v = El<T>::up(((const short*)a.p.bias)[at]);
-      v = v <= (std::is_same<T, bf16_t>::value ? -3.3895313e38f : -65504.f) ? -INFINITY : v * LOG2E;
+      v = v <= (std::is_same<T, bf16_t>::value ? -3.3895313e38f : -65504.f) ? -INFINITY : units(v);
     }
     tab[i] = v;
   }
@@ -418,6 +424,15 @@ __device__ __forceinline__ int wave_max_i(int v) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) v = max(v, __shfl_xor(v, o));
   return __builtin_amdgcn_readfirstlane(v);
+}
+
+// What the backward pass forms a row's weights from: the base-2 log-sum-exp; with a distance bias the exponent of the row's largest weight and, in
+// a second plane, the logarithm of the sum behind it.  Beside an entry of 1e9 that every key of a row carries, one fp32 number would lose the sum
+// (all gradients too large by the number of keys), and 2^(s - m) / l does not.  +inf marks a row that saw nothing: every weight is then 0.
+__device__ __forceinline__ void store_lse(const Args& a, long long at, float m2, float l) {
+  const float ll = __builtin_amdgcn_logf(l);
+  a.p.lse[at] = l > 0.f ? (a.lsum ? m2 : m2 + ll) : INFINITY;
+  if (a.lsum) a.lsum[at] = l > 0.f ? ll : 0.f;
 }
 
 // What a wave knows about the 32 query rows of its lanes (lane & 31 = row of the block)
@@ -685,7 +700,7 @@ __global__ __launch_bounds__(256, DP == 64 && MOD < 2 ? 3 : 2) void attn_mod_fwd
       float rs[2] = {0.f, 0.f};
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb) {
-        const float mc = MOD ? m - off[kb] : m * c;
+        const float mc = MOD ? m - off[kb] : fmaxf(m * c, LOWEST);
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const float pv = __builtin_amdgcn_exp2f(MOD ? s[kb][r] - mc : fmaf(s[kb][r], c, -mc));
@@ -721,7 +736,7 @@ __global__ __launch_bounds__(256, DP == 64 && MOD < 2 ? 3 : 2) void attn_mod_fwd
     kn = k1;
   }
   const float lt = half_sum(l);
-  const float m2 = MOD ? m : m * mod.c;
+  const float m2 = MOD ? m : fmaxf(m * mod.c, LOWEST);
   if (a.splits > 1) {
     const long long block = (((long long)sp * NU + u.x) * a.ntile + tile) * 4 + wave;       // of 32 rows
     store_part<FM>(a.part + block * (32 * DP), o, lane, R.ok);
@@ -729,9 +744,7 @@ __global__ __launch_bounds__(256, DP == 64 && MOD < 2 ? 3 : 2) void attn_mod_fwd
   } else {
     const long long at = op_base(a.p.o, u.b) + (long long)R.i * a.p.o.sstride + (long long)R.h * D;
     store_row<T, FM>((bf16_t*)a.p.o.ptr + at, o, lt > 0.f ? 1.f / lt : 0.f, hi, D, R.ok, a.p.o_rest ? (bf16_t*)a.p.o_rest + at : nullptr);
-    // base-2 log-sum-exp; +inf marks a row that saw nothing: every exp2(t - lse) of the backward pass is then 0
-    if (R.ok && hi == 0 && a.p.lse)
-      a.p.lse[((long long)u.b * a.p.heads + u.h0) * a.p.Sq + R.r] = lt > 0.f ? m2 + __builtin_amdgcn_logf(lt) : INFINITY;
+    if (R.ok && hi == 0 && a.p.lse) store_lse(a, ((long long)u.b * a.p.heads + u.h0) * a.p.Sq + R.r, m2, lt);
   }
 }
 
@@ -754,7 +767,7 @@ __global__ __launch_bounds__(64 * W) void attn_mod_join_kernel(const Args a) {
   const long long at = block * 32 + (lane & 31);
   // (Lanes behind the last row read their part of the padded buffer, whatever it holds, and store nothing: a branch around the loads would
   // put a wait behind each.)
-  float m = LOWEST * 4.f, l = 0.f;
+  float m = -INFINITY, l = 0.f;                                         // (every split's m is finite)
   f32x16 acc[1];
 #pragma unroll
   for (int e = 0; e < 16; ++e) acc[0][e] = 0.f;
@@ -822,7 +835,7 @@ __global__ __launch_bounds__(64 * W) void attn_mod_join_kernel(const Args a) {
   const int i = div_gp(a, min(r, a.M - 1)), h = u.h0 + min(r, a.M - 1) - i * a.gp;
   const long long col = op_base(a.p.o, u.b) + (long long)i * a.p.o.sstride + (long long)h * D + 32 * f;
   store_row<T, 1>((bf16_t*)a.p.o.ptr + col, acc, l > 0.f ? 1.f / l : 0.f, hi, D - 32 * f, ok, a.p.o_rest ? (bf16_t*)a.p.o_rest + col : nullptr);
-  if (ok && f == 0 && hi == 0 && a.p.lse) a.p.lse[((long long)u.b * a.p.heads + u.h0) * a.p.Sq + r] = l > 0.f ? m + __builtin_amdgcn_logf(l) : INFINITY;
+  if (ok && f == 0 && hi == 0 && a.p.lse) store_lse(a, ((long long)u.b * a.p.heads + u.h0) * a.p.Sq + r, m, l);
 }
 
 // bounds and documents of every 64 rows / keys (launched where a mask has documents or one prefix per query): one wave per tile (5 us at 8200
@@ -907,7 +920,7 @@ __global__ __launch_bounds__(1024) void attn_mod_order_kernel(const Args a, int*
 // ------------------------------------------------------------------------------------------------ backward: dQ, delta, table gradient
 // Three products per score, Q, dO and dQ of the wave's 32 rows in registers.  8192 x 8192, 16 heads of 128, bf16: 814 us, 1013 TFLOP/s.
 template <typename T, int DP, int MOD>
-__global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(const Args a) {
+__global__ __launch_bounds__(256, DP == 64 && MOD < 3 ? 3 : 2) void attn_mod_dq_kernel(const Args a) {
   warm_kernargs<(int)sizeof(Args)>();
   constexpr int NT = 256, KD = DP / 16, FM = DP / 32;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -956,6 +969,7 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(const Args a) {
   }
   const long long sidx = ((long long)u.b * a.p.heads + u.h0) * a.p.Sq + min(R.r, a.M - 1);
   const float lse = R.ok ? a.p.lse[sidx] : INFINITY;
+  const float lsum = (MOD & 2) && R.ok ? a.lsum[sidx] : 0.f;
   if ((MOD & 2) && mod.table) load_table<T>(a, u.h0, tab, tid, NT);
   if (dtab)
     for (int i = lane; i < ntab; i += 64) sums[i] = 0.f;
@@ -1064,7 +1078,7 @@ __global__ __launch_bounds__(256, 2) void attn_mod_dq_kernel(const Args a) {
       }
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const float pv = __builtin_amdgcn_exp2f(MOD ? s[r] - lse : fmaf(s[r], mod.c, -lse));
+        const float pv = __builtin_amdgcn_exp2f((MOD & 2) ? (s[r] - lse) - lsum : MOD ? s[r] - lse : fmaf(s[r], mod.c, -lse));
         s[r] = pv * (dp[r] - dl);
       }
       if (partial) {
@@ -1196,8 +1210,9 @@ __global__ __launch_bounds__(256) void attn_mod_dbias_kernel(const Args a) {
 }
 
 // ------------------------------------------------------------------------------------------------ backward: dK, dV
+constexpr int INFO = 7;             // numbers of a staged query row
 struct RowInfo {                    // of one query row, as loaded
-  float lse, delta, slope;
+  float lse, lsum, delta, slope;
   int doc, prefix;
 };
 // A wave owns 32 keys and streams the rows that see them.  K, V, dK and dV of 32 keys of 128 columns are 192 registers: with the score and
@@ -1213,8 +1228,8 @@ __global__ __launch_bounds__(DP == 128 ? 512 : 256, 2) void attn_mod_dkdv_kernel
   constexpr int HALF = TILE * DP / 512 * GROUP;                         // elements of 64 staged rows
   extern __shared__ __attribute__((aligned(16))) char smem[];
   Stage<DP>* st = (Stage<DP>*)smem;
-  float* sinfo = (float*)(smem + 2 * sizeof(Stage<DP>));                // [2][6][TILE]: lse, delta, slope, bound, pos, doc
-  float* tab = sinfo + 2 * 6 * TILE;
+  float* sinfo = (float*)(smem + 2 * sizeof(Stage<DP>));                // [2][INFO][TILE]: lse, delta, slope, bound, pos, doc, lsum
+  float* tab = sinfo + 2 * INFO * TILE;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5;
   const int NKV = a.p.nbatch * a.p.kv_heads, G = a.p.heads / a.p.kv_heads, GU = G / a.gp, ntr = (a.M + TILE - 1) / TILE;
   Part part = {0, -1, false};
@@ -1306,7 +1321,7 @@ __global__ __launch_bounds__(DP == 128 ? 512 : 256, 2) void attn_mod_dkdv_kernel
   const bf16_t* qp = ln.ok ? Q + ln.ch * 8 : (const bf16_t*)zero_chunk;
   const bf16_t* gp = ln.ok ? dO + ln.ch * 8 : (const bf16_t*)zero_chunk;
   const unsigned qs = ln.ok ? (unsigned)a.p.q.sstride : 0u, gs = ln.ok ? (unsigned)a.p.d_o.sstride : 0u, hs = ln.ok ? (unsigned)D : 0u;
-  RowInfo ni = {0.f, 0.f, 0.f, 0, 0};
+  RowInfo ni = {0.f, 0.f, 0.f, 0.f, 0, 0};
   auto fetch = [&](int c, int sidx) {                                   // rows behind the last repeat it (their weights are masked to 0)
     const int gu = c / run, t = first + c - gu * run, h0 = kv * G + gu * a.gp;
 #pragma unroll
@@ -1320,6 +1335,7 @@ __global__ __launch_bounds__(DP == 128 ? 512 : 256, 2) void attn_mod_dkdv_kernel
       const int rc = min(t * TILE + tid, a.M - 1), i = div_gp(a, rc);
       const long long at = ((long long)b * a.p.heads + h0) * a.p.Sq + rc;
       ni.lse = a.p.lse[at];
+      if (MOD & 2) ni.lsum = a.lsum[at];
       ni.delta = a.p.delta[at];
       if (docs) ni.doc = a.p.q_docs[(long long)b * a.p.Sq + i];
       if ((MOD & 2) && a.p.slopes) ni.slope = a.p.slopes[h0 + rc - i * a.gp];
@@ -1327,7 +1343,7 @@ __global__ __launch_bounds__(DP == 128 ? 512 : 256, 2) void attn_mod_dkdv_kernel
     }
   };
   auto landed = [&](int c, int sidx, bool dead) {
-    float* in = sinfo + sidx * 6 * TILE;
+    float* in = sinfo + sidx * INFO * TILE;
     if (tid < TILE) {
       const int r = (first + c % run) * TILE + tid, i = div_gp(a, min(r, a.M - 1));
       const int bound = (r < a.M && ni.doc >= 0) ? bound_of(seq, i, seq.per_query ? ni.prefix : seq.prefix) : 0;
@@ -1337,6 +1353,7 @@ __global__ __launch_bounds__(DP == 128 ? 512 : 256, 2) void attn_mod_dkdv_kernel
       in[3 * TILE + tid] = __int_as_float(bound);
       in[4 * TILE + tid] = __int_as_float(i + seq.off);
       in[5 * TILE + tid] = __int_as_float(ni.doc);
+      if (MOD & 2) in[6 * TILE + tid] = ni.lsum;
     }
     copies_done();
     __syncthreads();
@@ -1355,7 +1372,7 @@ __global__ __launch_bounds__(DP == 128 ? 512 : 256, 2) void attn_mod_dkdv_kernel
   auto math = [&](bool partial) {
     const bf16_t* sq = st[cur].a;
     const bf16_t* sg = st[cur].b;
-    const float* in = sinfo + cur * 6 * TILE;
+    const float* in = sinfo + cur * INFO * TILE;
 #pragma unroll
     for (int qb = 0; qb < 2; ++qb) {
       f32x16 s, dp, pr;
@@ -1372,7 +1389,8 @@ __global__ __launch_bounds__(DP == 128 ? 512 : 256, 2) void attn_mod_dkdv_kernel
         for (int g = 0; g < 4; ++g) {
           const int o = 32 * qb + 8 * g + 4 * hi;
           const f32x4 L = *(const f32x4*)(in + o), E = *(const f32x4*)(in + TILE + o);
-          f32x4 W = {1.f, 1.f, 1.f, 1.f};
+          f32x4 W = {1.f, 1.f, 1.f, 1.f}, Z = {0.f, 0.f, 0.f, 0.f};
+          if (MOD & 2) Z = *(const f32x4*)(in + 6 * TILE + o);
           if (MOD & 1) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -1399,7 +1417,7 @@ __global__ __launch_bounds__(DP == 128 ? 512 : 256, 2) void attn_mod_dkdv_kernel
           }
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            pr[4 * g + e] = __builtin_amdgcn_exp2f(MOD ? s[4 * g + e] - L[e] : fmaf(s[4 * g + e], mod.c, -L[e]));
+            pr[4 * g + e] = __builtin_amdgcn_exp2f((MOD & 2) ? (s[4 * g + e] - L[e]) - Z[e] : MOD ? s[4 * g + e] - L[e] : fmaf(s[4 * g + e], mod.c, -L[e]));
             const float d = pr[4 * g + e] * (dp[4 * g + e] - E[e]);
             s[4 * g + e] = (MOD & 1) ? d * W[e] : d;
           }
@@ -1661,6 +1679,7 @@ Layout make_layout(const T2VAttnMod* p, bool bwd) {
   a.kmeta = L.meta ? (const KMeta*)(w + L.o_kmeta) : nullptr;
   a.qorder = L.order ? (const int*)(w + L.o_qorder) : nullptr;
   a.korder = L.order && !L.kv_split && p->kv_share <= 1 ? (const int*)(w + L.o_korder) : nullptr;
+  a.lsum = p->lse && (p->slopes || p->bias) ? p->lse + (long long)p->nbatch * p->heads * p->Sq : nullptr;
   w = (char*)p->workspace;
   a.part = (float*)(w + L.o_part);
   a.part_ml = (float*)(w + L.o_ml);
@@ -1671,7 +1690,7 @@ Layout make_layout(const T2VAttnMod* p, bool bwd) {
 size_t smem_bytes(const Layout& L, int tables, bool kv) {
   if (kv) {
     const size_t tab = L.a.p.bias ? 4 * ((2 * (size_t)L.a.p.radius + 1 + 3) / 4 * 4) : 0;
-    return (L.dp == 64 ? 2 * sizeof(Stage<64>) : 2 * sizeof(Stage<128>) + 4 * sizeof(Stage<128>) / 2) + 2 * 6 * TILE * 4 + tab;
+    return (L.dp == 64 ? 2 * sizeof(Stage<64>) : 2 * sizeof(Stage<128>) + 4 * sizeof(Stage<128>) / 2) + 2 * INFO * TILE * 4 + tab;
   }
   return 2 * (L.dp == 64 ? sizeof(Stage<64>) : sizeof(Stage<128>)) + 2 * TILE * 4 + 64 + (L.a.p.bias ? tables * 4 * (2 * (size_t)L.a.p.radius + 1) : 0);
 }

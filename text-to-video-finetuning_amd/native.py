@@ -133,7 +133,7 @@ class AttnMod(C.Structure):
     ]
 
 
-ABI_VERSION = 10          # include/t2v_abi.h T2V_ABI_VERSION
+ABI_VERSION = 11          # include/t2v_abi.h T2V_ABI_VERSION
 A_DENSE, A_CONV = 0, 1
 OUT_BF16, OUT_F32, OUT_F32_ATOMIC = 0, 1, 2
 ACT_NONE, ACT_SILU = 0, 1

@@ -380,7 +380,7 @@ def _dense(t):
 
 class _AttnPlan:
     """raw: descriptor of the forward; work, meta: bytes of its buffers; bwd: (descriptor, workspace bytes, with dense gradients), made on first use."""
-    __slots__ = ("key", "raw", "work", "meta", "empty", "covered", "kv_covered", "share", "dtype", "dev", "lse", "rest", "shared_ok", "_bwd", "lays")
+    __slots__ = ("key", "raw", "work", "meta", "empty", "covered", "kv_covered", "share", "dtype", "dev", "lse", "delta", "rest", "shared_ok", "_bwd", "lays")
 
     def bwd(self, with_bias):
         if self._bwd.get(with_bias) is None:
@@ -444,7 +444,8 @@ def _attn_plan(qs, ks, vs, heads, kv_heads, qlay, klay, scale, causal, softcap, 
         _fail(f"bias must be a contiguous [{heads}, 2R + 1] table with R <= 1024 in {dtype} or fp32 on {dev}, got {tuple(bias[0])} {bias[2]}")
     p = _AttnPlan()
     p.empty = nb * Sq == 0 or Sk == 0                   # nothing is asked, or there is nothing to see
-    p.dtype, p.dev, p.lse, p.rest = dtype, dev, nb * heads * Sq, qsh[0] * heads * D * 2      # elements of lse, bytes of o's rest (a multiple of 16)
+    p.dtype, p.dev, p.delta, p.rest = dtype, dev, nb * heads * Sq, qsh[0] * heads * D * 2    # elements of delta, bytes of o's rest (a multiple of 16)
+    p.lse = p.delta * (1 if slopes is None and bias is None else 2)
     p.covered = qf[2]
     p.share = klay.bdiv if klay.bdiv > 1 and klay.lo == 0 else 1
     p.kv_covered = kf[2] or (p.share > 1 and nb % p.share == 0 and nb // p.share * Sk == ksh[0] and klay.ss == 1 and klay.hi == Sk)
@@ -535,7 +536,7 @@ class _AttentionMod(torch.autograd.Function):
         new = torch.empty if p.kv_covered else torch.zeros
         dk, dv = new(k.shape, dtype=dtype, device=dev), new(v.shape, dtype=dtype, device=dev)
         do, o = _upstream(do), o.contiguous()
-        work = _bytes(work_bytes + 4 * p.lse, dev)              # and delta behind it
+        work = _bytes(work_bytes + 4 * p.delta, dev)              # and delta behind it
         d = _AttnFlat.from_buffer_copy(raw)
         _fill(d, q, k, v, o, *masks, bias)
         d.o_rest = at = kept.data_ptr()
@@ -572,7 +573,8 @@ def attention_mod(q, k, v, heads, qlay, klay, kv_heads=None, scale=None, causal=
       softcap > 0    t <- softcap * tanh(t / softcap)                                             (1e-6 to 1e4; scale: 1e-15 to 1e6)
       slopes         fp32 [heads]: t <- t - slopes[h] * |j - i'|                                  (not trained)
       bias           [heads, 2R + 1] (R <= 1024, the operands' type or fp32): t <- t + bias[h, clip(j - i', -R, R) + R]; trained when it
-                     requires a gradient; an entry at or below its type's lowest finite value hides its distance
+                     requires a gradient; an entry at or below its type's lowest finite value hides its distance (finite ones beyond 2e38
+                     count as 2e38; scores are held in 32 bits: beside an entry of 1e6 the rest of a score is rounded to 0.1)
       kv_len         int32 [nbatch]: keys 0 .. kv_len - 1 exist (default: all)
       causal         keys j <= i';  prefix (int32 [nbatch] or [nbatch, Sq], with causal): and all keys j < prefix
       q_docs, kv_docs  int32 [nbatch, Sq], [nbatch, Sk]: only keys of the query's document; numbers below 0 mark padding
