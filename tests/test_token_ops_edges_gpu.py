@@ -158,3 +158,26 @@ def test_entries_far_outside_of_the_scores_are_scores(name):
         _within(n, t.grad, *want[n])
     if tdt is not None:
         _within("dbias", dkw["bias"].grad, *want["dbias"])
+
+
+# ------------------------------------------------------------------------------------------------ forward-mode derivatives
+def test_tangents_are_refused_forward_and_backward():
+    F = _f()
+    import torch.autograd.forward_ad as fwd
+    x = torch.randn(16, 64, device="cuda").to(BF)
+    leaf = x.clone().requires_grad_()
+    lay, pos = F.SeqLayout(1, 16, 16, 0, 1), torch.arange(16, dtype=torch.int32, device="cuda")[:, None]
+    calls = (lambda t: F.rope(t, 1, pos, F.RopeAxes((64,))), lambda t: F.qk_norm_rope(t, t, 1, 1, pos, F.RopeAxes((64,)))[0],
+             lambda t: F.attention_mod(t, t, t, 1, lay, lay))
+    for f in calls:
+        plain, y = f(x), f(leaf)
+        want, = torch.autograd.grad(y, leaf, x, retain_graph=True)
+        with fwd.dual_level():
+            for t in (x, leaf):
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    f(fwd.make_dual(t, torch.ones_like(t)))
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                torch.autograd.grad(y, leaf, fwd.make_dual(x, torch.ones_like(x)), retain_graph=True)
+            assert torch.equal(f(x), plain) and torch.equal(torch.autograd.grad(y, leaf, x)[0], want)
+        with pytest.raises(RuntimeError):
+            torch.func.jvp(f, (x,), (torch.ones_like(x),))

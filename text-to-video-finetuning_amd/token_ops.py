@@ -18,6 +18,7 @@ import math
 from dataclasses import dataclass
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import native as nv
@@ -52,6 +53,12 @@ def _upstream(dy):
     if dy.stride(1) != 1 or dy.data_ptr() % 16 or (ld * dy.element_size()) % 16 or ld < dy.shape[1]:
         return dy.contiguous()
     return dy
+
+
+def _no_tangents(*tensors):
+    """A dual tensor needs no gradient in the sense of the tape: its tangent would be dropped by the launch."""
+    if getattr(forward_ad, "_current_level", 0) >= 0 and any([t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors]):
+        _fail("no forward-mode derivative: pass tensors without a tangent")
 
 
 def _sig(t):
@@ -285,6 +292,7 @@ class _Rope(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
+        _no_tangents(dy)
         _no_foreign_leaves(ctx.foreign)
         pos, freqs = ctx.saved_tensors
         return _rope_bwd(ctx.plan, None, (_upstream(dy),), pos, freqs, None, None)[0][0], None
@@ -294,6 +302,7 @@ def rope(x, heads, pos, axes, freqs=None):
     """Rotary positions: x [rows, heads * dim] (bf16, fp16 or fp32) with the columns `axes` (RopeAxes) names turned by pos [rows, number
     of axes] (int32, int64 or fp32).  Angles are formed in 64 bits.  freqs: fp64 [sum(dims) / 2] radians per unit of position, in the place of the
     ladder theta gives.  Returns a dense matrix of x's shape; differentiable in x."""
+    _no_tangents(x, pos, freqs)
     _fixed(pos, freqs)
     plan = _rope_plan((_sig(x),), (int(heads), 0), axes, None, 0.0, _sig(pos), _sig(freqs), None)
     if torch.is_grad_enabled() and x.requires_grad:
@@ -313,6 +322,7 @@ class _QkNormRope(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dq, dk):
+        _no_tangents(dq, dk)
         _no_foreign_leaves(ctx.foreign)
         q, k, qw, kw, pos, freqs = ctx.saved_tensors
         plan, sigs = ctx.plan, (_sig(q), _sig(k))
@@ -331,6 +341,7 @@ def qk_norm_rope(q, k, heads, kv_heads, pos, axes, q_weight=None, k_weight=None,
     statistics are recomputed in the backward pass from the saved inputs."""
     if norm is None:
         _fail("norm None: 'rms' or 'layer' (`rope` turns without a norm)")
+    _no_tangents(q, k, pos, freqs, q_weight, k_weight, q_bias, k_bias)
     _fixed(pos, freqs)
     key = ((_sig(q), _sig(k)), (int(heads), int(kv_heads)), axes, norm, float(eps), _sig(pos), _sig(freqs),
            (_sig(q_weight), _sig(k_weight), _sig(q_bias), _sig(k_bias)))
@@ -522,6 +533,7 @@ class _AttentionMod(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, do):
+        _no_tangents(do)
         _no_foreign_leaves(ctx.foreign)
         q, k, v, bias, o, kept, tiles, *masks = ctx.saved_tensors
         p = ctx.plan
@@ -585,6 +597,7 @@ def attention_mod(q, k, v, heads, qlay, klay, kv_heads=None, scale=None, causal=
     Returns [rows_q, heads * dim]; rows that no sequence owns are zero.  Differentiable in q, k, v and bias; K / V shared by the bdiv batches
     of a layout with lo = 0 get the sum of their gradients.  The order of all sums is fixed: repeated runs are bit-equal."""
     heads = int(heads)
+    _no_tangents(q, k, v, slopes, bias)
     p = _plan_of((_sig(q), _sig(k), _sig(v), heads, heads if kv_heads is None else int(kv_heads), qlay, klay,
                   None if scale is None else float(scale), int(bool(causal)), float(softcap), _sig(prefix), _sig(kv_len),
                   _sig(q_docs), _sig(kv_docs), _sig(slopes), _sig(bias)))
