@@ -181,3 +181,23 @@ def test_tangents_are_refused_forward_and_backward():
             assert torch.equal(f(x), plain) and torch.equal(torch.autograd.grad(y, leaf, x)[0], want)
         with pytest.raises(RuntimeError):
             torch.func.jvp(f, (x,), (torch.ones_like(x),))
+
+
+# ------------------------------------------------------------------------------------------------ operands that need no gradient
+def test_parameters_as_slopes_positions_and_frequencies_without_gradients():
+    """They are not trained; where nothing is recorded that makes no difference."""
+    F = _f()
+    x = torch.randn(16, 128, device="cuda").to(BF)
+    lay = F.SeqLayout(1, 16, 16, 0, 1)
+    pos, fr = torch.arange(16.0, device="cuda")[:, None], torch.rand(32, dtype=F64, device="cuda")
+    slopes = torch.tensor([0.5, 0.25], device="cuda")
+    P = torch.nn.Parameter
+    calls = (lambda s, p, f: F.attention_mod(x, x, x, 2, lay, lay, slopes=s), lambda s, p, f: F.rope(x, 2, p, F.RopeAxes((64,)), freqs=f),
+             lambda s, p, f: F.qk_norm_rope(x, x, 2, 2, p, F.RopeAxes((64,)), freqs=f)[1])
+    for call in calls:
+        want = call(slopes, pos, fr)
+        for guard in (torch.no_grad, torch.inference_mode):
+            with guard():
+                assert torch.equal(call(P(slopes.clone()), P(pos.clone()), P(fr.clone())), want)
+        with pytest.raises(RuntimeError, match="not trained"):
+            call(P(slopes.clone()), P(pos.clone()), P(fr.clone()))

@@ -170,7 +170,7 @@ def _vector(t):
 
 
 def _fixed(pos, freqs):
-    if (pos is not None and pos.requires_grad) or (freqs is not None and freqs.requires_grad):
+    if torch.is_grad_enabled() and ((pos is not None and pos.requires_grad) or (freqs is not None and freqs.requires_grad)):
         _fail("positions and frequencies are not trained: pass them detached")
 
 
@@ -601,7 +601,7 @@ def attention_mod(q, k, v, heads, qlay, klay, kv_heads=None, scale=None, causal=
     p = _plan_of((_sig(q), _sig(k), _sig(v), heads, heads if kv_heads is None else int(kv_heads), qlay, klay,
                   None if scale is None else float(scale), int(bool(causal)), float(softcap), _sig(prefix), _sig(kv_len),
                   _sig(q_docs), _sig(kv_docs), _sig(slopes), _sig(bias)))
-    if slopes is not None and slopes.requires_grad:
+    if slopes is not None and slopes.requires_grad and torch.is_grad_enabled():
         _fail("slopes are not trained: pass slopes.detach(), or a bias table for a learned distance bias")
     masks = (prefix, kv_len, q_docs, kv_docs, slopes)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (bias is not None and bias.requires_grad)):
