@@ -29,3 +29,15 @@ def test_tensors_with_a_tangent_are_refused():
                 pytest.fail(f"call {n} was not refused")
         with pytest.raises(RuntimeError, match="ROCm device"):
             F.rope(x, 1, pos, axes)                       # (a level that is open does not matter by itself)
+
+
+def test_gradients_of_keys_and_values_are_named_together_or_not_at_all():
+    import ctypes as C
+
+    from test_token_ops import _mod, _nv
+    nv = _nv()
+    op = nv.AttnOperand(1 << 20, 128 * 64, 0, 128, 1)
+    bwd = nv.lib().t2v_attn_mod_bwd
+    for named, word in (((), b"lse and delta"), (("dk",), b"operand dv"), (("dv",), b"operand dk"), (("dk", "dv"), b"lse and delta")):
+        a = _mod(d_o=op, dq=op, **{n: op for n in named})
+        assert bwd(C.byref(a), None) == -1 and word in nv.lib().t2v_last_error(), named

@@ -201,3 +201,25 @@ def test_parameters_as_slopes_positions_and_frequencies_without_gradients():
                 assert torch.equal(call(P(slopes.clone()), P(pos.clone()), P(fr.clone())), want)
         with pytest.raises(RuntimeError, match="not trained"):
             call(P(slopes.clone()), P(pos.clone()), P(fr.clone()))
+
+
+def test_queries_alone_are_trained_over_keys_that_sequences_share():
+    """Key layouts that name a row for several sequences have no gradients of their own; queries and the table do."""
+    F = _f()
+    g = torch.Generator().manual_seed(3)
+    r = lambda *s: torch.randn(*s, generator=g).to(BF).cuda()  # noqa: E731
+    q, up, k, v, bias = r(4 * 70, 256), r(4 * 70, 256), r(48, 128), r(48, 128), r(4, 21)
+    lay = F.SeqLayout(4, 70, 70, 0, 1)
+    for step in (0, 5):                                                   # one set of keys for all, windows five rows apart
+        rows = torch.cat([torch.arange(33) + b * step for b in range(4)]).cuda()
+        for with_bias in (False, True):
+            def grads(klay, k, v):
+                leaves = [t.detach().clone().requires_grad_() for t in ((q, bias) if with_bias else (q,))]
+                o = F.attention_mod(leaves[0], k, v, 4, lay, klay, kv_heads=2, softcap=9.0, bias=leaves[1] if with_bias else None)
+                return [o] + list(torch.autograd.grad(o, leaves, up))
+            got = grads(F.SeqLayout(4, 33, step, 0, 1), k, v)
+            want = grads(F.SeqLayout(4, 33, 33, 0, 1), k[rows].contiguous(), v[rows].contiguous())
+            full = grads(F.SeqLayout(4, 33, 33, 0, 1), k[rows].contiguous().requires_grad_(), v[rows].contiguous())
+            assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(got, want, full))
+        with pytest.raises(RuntimeError, match="names a row twice"):
+            F.attention_mod(q, k, v.clone().requires_grad_(), 4, lay, F.SeqLayout(4, 33, step, 0, 1), kv_heads=2)

@@ -1554,6 +1554,7 @@ int check_mod(const char* fn, const T2VAttnMod* p, bool bwd) {
   const char* names[] = {"q", "k", "v", "o", "d_o", "dq", "dk", "dv"};
   for (int i = 0; i < (bwd ? 8 : 4); ++i) {
     const T2VAttnOperand& o = *ops[i];
+    if (i >= 6 && !p->dk.ptr && !p->dv.ptr) continue;                   // no gradient of keys and values is asked for
     T2V_CHECK_ARG(o.ptr && o.bdiv > 0 && ((uintptr_t)o.ptr & 15) == 0 && o.sstride % 8 == 0 && o.bstride_hi % 8 == 0 && o.bstride_lo % 8 == 0 &&
                       o.sstride >= 0 && o.sstride < (1ll << 31),
                   "%s: operand %s: 16-byte aligned rows, less than 2^31 elements apart, are wanted (ptr %p, row stride %lld)", fn, names[i], o.ptr, o.sstride);
@@ -1746,25 +1747,28 @@ int run_bwd(Layout& L, hipStream_t st) {
   a.fold = fold(L, L.dq_tiles, L.dq_splits);
   const size_t sm = smem_bytes(L, a.p.dbias ? 5 : 1, false);
   const long long gq = (long long)a.p.nbatch * a.nunit * L.dq_tiles * L.dq_splits * (a.qorder ? 2 : 1);
-  int e = mb == 0 ? launch(1, attn_mod_dq_kernel<T, DP, 0>, gq, sm, st, a) : mb == 1 ? launch(1, attn_mod_dq_kernel<T, DP, 1>, gq, sm, st, a) :
-          mb == 2 ? launch(1, attn_mod_dq_kernel<T, DP, 2>, gq, sm, st, a) : launch(1, attn_mod_dq_kernel<T, DP, 3>, gq, sm, st, a);
+  const bool kv = a.p.dk.ptr != nullptr;
+  int which = kv || a.splits > 1 || a.p.dbias ? 1 : 3;
+  int e = mb == 0 ? launch(which, attn_mod_dq_kernel<T, DP, 0>, gq, sm, st, a) : mb == 1 ? launch(which, attn_mod_dq_kernel<T, DP, 1>, gq, sm, st, a) :
+          mb == 2 ? launch(which, attn_mod_dq_kernel<T, DP, 2>, gq, sm, st, a) : launch(which, attn_mod_dq_kernel<T, DP, 3>, gq, sm, st, a);
   if (e) return e;
   T2V_CHECK_LAUNCH();
   if (a.splits > 1) {
     const long long blocks = (long long)a.p.nbatch * a.nunit * a.ntile * 4 * (DP / 32);
-    hipLaunchKernelGGL((attn_mod_dq_join_kernel<T, DP>), dim3((unsigned)blocks), dim3(64), 0, st, a);
+    t2v_launch_timed(kv || a.p.dbias ? 0 : 2, attn_mod_dq_join_kernel<T, DP>, dim3((unsigned)blocks), dim3(64), 0, st, a);
     T2V_CHECK_LAUNCH();
   }
   if (a.p.dbias) {
     const long long n = (long long)a.p.heads * (2 * a.p.radius + 1);
-    hipLaunchKernelGGL(attn_mod_dbias_kernel<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, a);
+    t2v_launch_timed(kv ? 0 : 2, attn_mod_dbias_kernel<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, a);
     T2V_CHECK_LAUNCH();
   }
+  if (!kv) return T2V_OK;
   a.ntile = L.kv_tiles;
   const long long gk = (long long)a.p.nbatch * a.p.kv_heads * a.wgs * (a.korder ? 2 : 1);
   const size_t smk = smem_bytes(L, 1, true);
   a.to_part = L.kv_split || a.p.kv_share > 1;
-  const int which = a.to_part ? 0 : 2;
+  which = a.to_part ? 0 : 2;
   e = mb == 0 ? launch(which, attn_mod_dkdv_kernel<T, DP, 0>, gk, smk, st, a, DP == 128 ? 512 : 256) : mb == 1 ? launch(which, attn_mod_dkdv_kernel<T, DP, 1>, gk, smk, st, a, DP == 128 ? 512 : 256) :
       mb == 2 ? launch(which, attn_mod_dkdv_kernel<T, DP, 2>, gk, smk, st, a, DP == 128 ? 512 : 256) : launch(which, attn_mod_dkdv_kernel<T, DP, 3>, gk, smk, st, a, DP == 128 ? 512 : 256);
   if (e) return e;

@@ -539,14 +539,17 @@ class _AttentionMod(torch.autograd.Function):
         p = ctx.plan
         dev, dtype = p.dev, p.dtype
         with_bias = bias is not None and ctx.needs_input_grad[3]
+        with_kv = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
         if p.empty:
             return (*[torch.zeros(t.shape, dtype=dtype, device=dev) for t in (q, k, v)], torch.zeros_like(bias) if with_bias else None, None)
         if (_sig(q), _sig(k), _sig(v)) != p.key[:3]:            # (a saved tensor may come back with other strides)
             p = _plan_of((_sig(q), _sig(k), _sig(v)) + p.key[3:])
         raw, work_bytes = p.bwd(with_bias)
         dq = (torch.empty if p.covered else torch.zeros)(q.shape, dtype=dtype, device=dev)
-        new = torch.empty if p.kv_covered else torch.zeros
-        dk, dv = new(k.shape, dtype=dtype, device=dev), new(v.shape, dtype=dtype, device=dev)
+        dk = dv = None
+        if with_kv:
+            new = torch.empty if p.kv_covered else torch.zeros
+            dk, dv = new(k.shape, dtype=dtype, device=dev), new(v.shape, dtype=dtype, device=dev)
         do, o = _upstream(do), o.contiguous()
         work = _bytes(work_bytes + 4 * p.delta, dev)              # and delta behind it
         d = _AttnFlat.from_buffer_copy(raw)
@@ -555,7 +558,7 @@ class _AttentionMod(torch.autograd.Function):
         d.lse = at + p.rest
         d.workspace = at = work.data_ptr()
         d.workspace_bytes, d.delta = work_bytes, at + work_bytes
-        d.d_o, d.dq, d.dk, d.dv = do.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
+        d.d_o, d.dq, d.dk, d.dv = do.data_ptr(), dq.data_ptr(), _addr(dk), _addr(dv)
         if not do.is_contiguous():
             ld, lay = _ld(do.shape, do.stride()), p.lays[0]
             d.d_o_bstride_hi, d.d_o_bstride_lo, d.d_o_sstride = lay.hi * ld, lay.lo * ld, lay.ss * ld
@@ -595,7 +598,7 @@ def attention_mod(q, k, v, heads, qlay, klay, kv_heads=None, scale=None, causal=
     leave no query that sees them: masked weights of a tile are exact zeros that multiply its rows.
     Few query rows over many keys (serving steps, chunks of new tokens) split the keys over workgroups and join them.
     Returns [rows_q, heads * dim]; rows that no sequence owns are zero.  Differentiable in q, k, v and bias; K / V shared by the bdiv batches
-    of a layout with lo = 0 get the sum of their gradients.  The order of all sums is fixed: repeated runs are bit-equal."""
+    of a layout with lo = 0 get the sum of their gradients; other layouts that name a key row twice train q and bias alone.  The order of all sums is fixed: repeated runs are bit-equal."""
     heads = int(heads)
     _no_tangents(q, k, v, slopes, bias)
     p = _plan_of((_sig(q), _sig(k), _sig(v), heads, heads if kv_heads is None else int(kv_heads), qlay, klay,
@@ -605,7 +608,7 @@ def attention_mod(q, k, v, heads, qlay, klay, kv_heads=None, scale=None, causal=
         _fail("slopes are not trained: pass slopes.detach(), or a bias table for a learned distance bias")
     masks = (prefix, kv_len, q_docs, kv_docs, slopes)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (bias is not None and bias.requires_grad)):
-        if not p.shared_ok:
+        if not p.shared_ok and (k.requires_grad or v.requires_grad):
             _fail(f"key layout {klay} names a row twice: gradients are defined for rows of their own, or shared by the bdiv batches (lo = 0)")
         foreign, _kept = _foreign_leaves((q, k, v, bias), p.dev) if _capturing() else (False, None)
         return _AttentionMod.apply(q, k, v, bias, (p, masks, foreign))
