@@ -300,7 +300,7 @@ int t2v_attn_bwd(const T2VAttn* p, t2v_stream_t stream);
  * logarithm of the sum behind it): kept for the backward call; NULL: not written.
  * o_rest: NULL, or laid out and typed like o: what rounding o to its type left behind; the backward call's delta = rowsum(dO * O) is formed
  * with it where it is given again (the error of delta, 2^-9 of bf16's O, is otherwise as large as that of the gradients' own rounding).
- * scale: 1e-15 to 1e6; softcap: 0 or 1e-6 to 1e4 (the cap's tanh is good to 4e-7 cap: a larger one is no cap for any score that counts).
+ * scale: 1e-15 to 1e6; softcap: 0 or 1e-6 to 1e4 (up to 100 the capped score is good to 4e-7 of the cap, above to 2e-6 of the score).
  * Backward: the descriptor of the forward with d_o, dq, dk, dv, delta (fp32 [nbatch, heads, Sq] scratch) and dbias (NULL or like
  * bias) filled in; every row of dq, dk, dv is written.  dk and dv both NULL: not computed.  kv_share: batches b with the same b / kv_share have one K / V (and one
  * dk / dv, the sum); 1: each has its own.  workspace: t2v_attn_mod_workspace(p, backward) bytes, 256-byte aligned, no

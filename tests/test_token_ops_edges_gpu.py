@@ -21,8 +21,8 @@ def _f():
 def _within(name, got, want, bound):
     got = got.detach().cpu().to(F64).reshape(want.shape)
     assert torch.isfinite(got).all(), f"{name}: {int((~torch.isfinite(got)).sum())} values are not finite"
-    at = ((got - want).abs() / bound).max()
-    assert ((got - want).abs() <= bound).all(), f"{name}: {float(at):.2f} times the bound"
+    at, inside = float(((got - want).abs() / bound).max()), bool(((got - want).abs() <= bound).all())
+    assert inside, f"{name}: {at:.2f} times the bound"
 
 
 @contextlib.contextmanager
@@ -223,3 +223,60 @@ def test_queries_alone_are_trained_over_keys_that_sequences_share():
             assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(got, want, full))
         with pytest.raises(RuntimeError, match="names a row twice"):
             F.attention_mod(q, k, v.clone().requires_grad_(), 4, lay, F.SeqLayout(4, 33, step, 0, 1), kv_heads=2)
+
+
+# ------------------------------------------------------------------------------------------------ large caps
+@pytest.mark.parametrize("cap", [0.5, 30.0, 100.0, 101.0, 1000.0, 10000.0])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_capped_scores_lose_nothing_to_a_large_cap(cap, dim):
+    """One key, so a row's log-sum-exp is its score.  Up to a cap of 100 the exponential's form is good to 4e-7 of the cap; above, fp32 products
+    and a polynomial (six half steps of 2^-24, 4e-7) hold scores below a quarter of the cap, and the exponential's 4e-7 of the cap is 1.7e-6 of the others."""
+    F = _f()
+    a = torch.logspace(-3, math.log10(6e4), 3000, dtype=F64).to(HF)
+    a = torch.cat([-a.flip(0), torch.zeros(1, dtype=HF), a])
+    q, k = torch.zeros(len(a), dim, dtype=HF), torch.zeros(1, dim, dtype=HF)
+    q[:, 3], k[0, 3] = a, 1.0
+    qd = q.cuda().requires_grad_()
+    o = F.attention_mod(qd, k.cuda(), k.cuda(), 1, F.SeqLayout(1, len(a), len(a), 0, 1), F.SeqLayout(1, 1, 1, 0, 1), scale=1.0, softcap=cap)
+    kept, = [t for t in o.grad_fn.saved_tensors if t is not None and t.dtype == torch.uint8]
+    got = kept[o.grad_fn.plan.rest:].view(F32).cpu().to(F64) * math.log(2.0)
+    want = cap * torch.tanh(a.to(F64) / cap)
+    bound = 4e-7 * cap + 1e-12 if cap <= 100 else 2e-6 * want.abs() + 1e-12
+    at, inside = float(((got - want).abs() / bound).max()), bool(((got - want).abs() <= bound).all())
+    assert inside, f"{at:.1f} times the bound"
+
+
+WIDE = {  # B, Sq, Sk, H, KV, D, dtype, factor of the queries, options
+    "small scores": (2, 150, 150, 4, 2, 64, HF, 2.0, dict(softcap=10000.0, causal=True)),
+    "across the border": (1, 150, 200, 2, 2, 128, HF, 20.0, dict(softcap=101.0)),
+    "table": (1, 150, 150, 2, 2, 128, BF, 10.0, dict(softcap=120.0, bias=16, causal=True)),
+    "slopes": (1, 150, 150, 4, 2, 72, HF, 10.0, dict(softcap=500.0, slopes=True)),
+    "table, 64": (1, 150, 150, 2, 1, 64, BF, 10.0, dict(softcap=300.0, bias=5)),
+    "splits": (1, 4, 3000, 4, 2, 128, BF, 10.0, dict(softcap=150.0, causal=True)),
+}
+
+
+@pytest.mark.parametrize("name", list(WIDE))
+def test_large_caps_match_the_64_bit_form(name):
+    F = _f()
+    B, Sq, Sk, H, KV, D, dt, mul, opt = WIDE[name]
+    g = torch.Generator().manual_seed(len(name))
+    r = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    q, k, v, do = (r(B, Sq, H, D) * mul).to(dt), r(B, Sk, KV, D).to(dt), r(B, Sk, KV, D).to(dt), r(B, Sq, H, D).to(dt)
+    kw = dict(causal=opt.get("causal", False), softcap=opt["softcap"])
+    if "bias" in opt:
+        kw["bias"] = r(H, 2 * opt["bias"] + 1)
+    if opt.get("slopes"):
+        kw["slopes"] = 0.3 * torch.rand(H, generator=g)
+    want = ref.attention(q, k, v, D ** -0.5, dt, do=do, **kw)
+    flat = [t.reshape(t.shape[0] * t.shape[1], -1).cuda().requires_grad_() for t in (q, k, v)]
+    dkw = {n: t.cuda() if torch.is_tensor(t) else t for n, t in kw.items()}
+    if "bias" in dkw:
+        dkw["bias"].requires_grad_()
+    o = F.attention_mod(*flat, H, F.SeqLayout(B, Sq, Sq, 0, 1), F.SeqLayout(B, Sk, Sk, 0, 1), kv_heads=KV, **dkw)
+    o.backward(do.reshape(B * Sq, -1).cuda())
+    _within("o", o, *want["o"])
+    for n, t in zip(("dq", "dk", "dv"), flat):
+        _within(n, t.grad, *want[n])
+    if "bias" in dkw:
+        _within("dbias", dkw["bias"].grad, *want["dbias"])

@@ -323,27 +323,41 @@ __device__ __forceinline__ const bf16x8* chunk_ptr(const bf16_t* p, bool ok) { r
 // ------------------------------------------------------------------------------------------------ scores
 // t (in base-2 exponent units) of one lane's 16 scores.  `d0`: distance j - i' of accumulator row 0 (of the lane's half)
 struct Mod {
-  float c;            // scale * log2e (no cap)
+  float c;            // scale * log2e
   float k1, capl;     // cap: 2 log2e scale / cap, cap * log2e
-  bool cap, slope, table;
+  float k;            // cap: scale / cap
+  bool slope, table;
   int R;
 };
 __device__ __forceinline__ Mod make_mod(const Args& a) {
   Mod m;
-  m.cap = a.p.softcap > 0.f;
+  const bool cap = a.p.softcap > 0.f;
   m.slope = a.p.slopes != nullptr;
   m.table = a.p.bias != nullptr;
   m.c = a.p.scale * LOG2E;
-  m.k1 = m.cap ? 2.f * LOG2E * a.p.scale / a.p.softcap : 0.f;
+  m.k1 = cap ? 2.f * LOG2E * a.p.scale / a.p.softcap : 0.f;
+  m.k = cap ? a.p.scale / a.p.softcap : 0.f;
   m.capl = a.p.softcap * LOG2E;
   m.R = a.p.radius;
   return m;
 }
 // cap * tanh(x / cap) = cap (1 - 2 / (1 + e^(2 x / cap))): one exp, one reciprocal; exact at +-inf.  Returns it in base-2 units and
 // leaves w = 1 / (1 + e^(..)): the derivative is 4 w (1 - w).
+// The difference cancels: it is good to 4e-7 of the cap, 4e-5 at a cap of 100, where it costs nothing beside the weights' own rounding.  A larger cap
+// (WIDE, kernels of their own: nothing is added to those of ordinary caps) takes the odd series x (1 - y^2 / 3 + 2 y^4 / 15 - ..), y = x / cap, where
+// |y| < 1/4; its first term left out is 9e-9 there, and the exponential's error is 2e-6 of the score above.  (2 x 2011 rows, forward and backward: 16 / 4
+// heads of 128 303 -> 355 us, 16 heads of 64 299 -> 406 us.)
+constexpr float WIDE_CAP = 100.f;
+template <bool WIDE>
 __device__ __forceinline__ float capped(const Mod& m, float s, float& w) {
   w = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s * m.k1));
-  return fmaf(w, -2.f * m.capl, m.capl);
+  float t = fmaf(w, -2.f * m.capl, m.capl);
+  if (WIDE) {
+    const float y = s * m.k, z = y * y;
+    const float p = fmaf(z, fmaf(z, fmaf(z, fmaf(z, 62.f / 2835, -17.f / 315), 2.f / 15), -1.f / 3), 1.f);
+    t = z < 0.0625f ? s * m.c * p : t;
+  }
+  return t;
 }
 
 // table of head h in base-2 units in LDS; an entry at or below the type's lowest finite value hides its distance (-inf)
@@ -476,7 +490,7 @@ __device__ __forceinline__ void load_rows(Rows& R, const Args& a, const Unit& u,
 }
 
 // ------------------------------------------------------------------------------------------------ forward
-// MOD: bit 0 cap, bit 1 distance bias (slopes / table), compile-time so that a tile is straight-line code.
+// MOD: bit 0 cap, bit 1 distance bias (slopes / table), bit 2 a cap above WIDE_CAP, compile-time so that a tile is straight-line code.
 // A workgroup is 128 rows (four waves of 32) and walks the key tiles its rows may see.  64 rows a wave instead (K and V fragments read once for
 // both halves) leave one wave per SIMD: 656 -> 801 us at head dim 128, no change at 64.
 // Measured, bf16, 8192 x 8192, 16 heads: head dim 128 653 us, 842 TFLOP/s where a library product of 8192^3 reaches 1243 (causal 298 us, capped
@@ -616,7 +630,7 @@ __global__ __launch_bounds__(256, DP == 64 && MOD < 2 ? 3 : 2) void attn_mod_fwd
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             float w;
-            s[kb][r] = capped(mod, s[kb][r], w);
+            s[kb][r] = capped<(MOD & 4) != 0>(mod, s[kb][r], w);
           }
       }
       off[0] = off[1] = 0.f;
@@ -1058,7 +1072,7 @@ __global__ __launch_bounds__(256, DP == 64 && MOD < 3 ? 3 : 2) void attn_mod_dq_
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           float y;
-          s[r] = capped(mod, s[r], y);
+          s[r] = capped<(MOD & 4) != 0>(mod, s[r], y);
           w[r] = 4.f * y * (1.f - y);
         }
       } else if (MOD & 2) {
@@ -1395,7 +1409,7 @@ __global__ __launch_bounds__(DP == 128 ? 512 : 256, 2) void attn_mod_dkdv_kernel
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               float w;
-              s[4 * g + e] = capped(mod, s[4 * g + e], w);
+              s[4 * g + e] = capped<(MOD & 4) != 0>(mod, s[4 * g + e], w);
               W[e] = 4.f * w * (1.f - w);
             }
           } else if (MOD & 2) {
@@ -1707,8 +1721,14 @@ int launch(int which, K kern, long long grid, size_t smem, hipStream_t st, const
   t2v_launch_timed(which, kern, dim3((unsigned)grid), dim3(threads), (unsigned)smem, st, a);
   return T2V_OK;
 }
-// bit 0 cap, bit 1 distance bias
-int mod_bits(const T2VAttnMod* p) { return (p->softcap > 0.f ? 1 : 0) | (p->slopes || p->bias ? 2 : 0); }
+// f(integral constant MOD)
+template <typename F>
+int with_mod(const T2VAttnMod& p, F f) {
+  const bool bias = p.slopes || p.bias;
+  if (p.softcap > WIDE_CAP) return bias ? f(std::integral_constant<int, 7>()) : f(std::integral_constant<int, 5>());
+  if (p.softcap > 0.f) return bias ? f(std::integral_constant<int, 3>()) : f(std::integral_constant<int, 1>());
+  return bias ? f(std::integral_constant<int, 2>()) : f(std::integral_constant<int, 0>());
+}
 
 // the rank at which the order turns: where all workgroups are resident, two on some CUs, the 256 longest come first
 int fold(const Layout& L, int tiles, int splits) {
@@ -1725,9 +1745,7 @@ int run_fwd(Layout& L, hipStream_t st) {
   const long long grid = (long long)a.p.nbatch * a.nunit * L.fwd_tiles * L.fwd_splits * (a.qorder ? 2 : 1);
   const size_t sm = smem_bytes(L, 1, false);
   const int which = L.fwd_splits > 1 ? 1 : 3;
-  const int mb = mod_bits(&a.p);
-  const int e = mb == 0 ? launch(which, attn_mod_fwd_kernel<T, DP, 0>, grid, sm, st, a) : mb == 1 ? launch(which, attn_mod_fwd_kernel<T, DP, 1>, grid, sm, st, a) :
-                mb == 2 ? launch(which, attn_mod_fwd_kernel<T, DP, 2>, grid, sm, st, a) : launch(which, attn_mod_fwd_kernel<T, DP, 3>, grid, sm, st, a);
+  const int e = with_mod(a.p, [&](auto mod) { return launch(which, attn_mod_fwd_kernel<T, DP, decltype(mod)::value>, grid, sm, st, a); });
   if (e) return e;
   T2V_CHECK_LAUNCH();
   if (L.fwd_splits > 1) {
@@ -1741,7 +1759,6 @@ int run_fwd(Layout& L, hipStream_t st) {
 template <typename T, int DP>
 int run_bwd(Layout& L, hipStream_t st) {
   Args& a = L.a;
-  const int mb = mod_bits(&a.p);
   a.ntile = L.dq_tiles;
   a.splits = L.dq_splits;
   a.fold = fold(L, L.dq_tiles, L.dq_splits);
@@ -1749,8 +1766,7 @@ int run_bwd(Layout& L, hipStream_t st) {
   const long long gq = (long long)a.p.nbatch * a.nunit * L.dq_tiles * L.dq_splits * (a.qorder ? 2 : 1);
   const bool kv = a.p.dk.ptr != nullptr;
   int which = kv || a.splits > 1 || a.p.dbias ? 1 : 3;
-  int e = mb == 0 ? launch(which, attn_mod_dq_kernel<T, DP, 0>, gq, sm, st, a) : mb == 1 ? launch(which, attn_mod_dq_kernel<T, DP, 1>, gq, sm, st, a) :
-          mb == 2 ? launch(which, attn_mod_dq_kernel<T, DP, 2>, gq, sm, st, a) : launch(which, attn_mod_dq_kernel<T, DP, 3>, gq, sm, st, a);
+  int e = with_mod(a.p, [&](auto mod) { return launch(which, attn_mod_dq_kernel<T, DP, decltype(mod)::value>, gq, sm, st, a); });
   if (e) return e;
   T2V_CHECK_LAUNCH();
   if (a.splits > 1) {
@@ -1769,8 +1785,7 @@ int run_bwd(Layout& L, hipStream_t st) {
   const size_t smk = smem_bytes(L, 1, true);
   a.to_part = L.kv_split || a.p.kv_share > 1;
   which = a.to_part ? 0 : 2;
-  e = mb == 0 ? launch(which, attn_mod_dkdv_kernel<T, DP, 0>, gk, smk, st, a, DP == 128 ? 512 : 256) : mb == 1 ? launch(which, attn_mod_dkdv_kernel<T, DP, 1>, gk, smk, st, a, DP == 128 ? 512 : 256) :
-      mb == 2 ? launch(which, attn_mod_dkdv_kernel<T, DP, 2>, gk, smk, st, a, DP == 128 ? 512 : 256) : launch(which, attn_mod_dkdv_kernel<T, DP, 3>, gk, smk, st, a, DP == 128 ? 512 : 256);
+  e = with_mod(a.p, [&](auto mod) { return launch(which, attn_mod_dkdv_kernel<T, DP, decltype(mod)::value>, gk, smk, st, a, DP == 128 ? 512 : 256); });
   if (e) return e;
   T2V_CHECK_LAUNCH();
   if (a.to_part) {
