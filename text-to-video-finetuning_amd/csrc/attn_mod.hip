@@ -493,11 +493,13 @@ __device__ __forceinline__ void load_rows(Rows& R, const Args& a, const Unit& u,
 // MOD: bit 0 cap, bit 1 distance bias (slopes / table), bit 2 a cap above WIDE_CAP, compile-time so that a tile is straight-line code.
 // A workgroup is 128 rows (four waves of 32) and walks the key tiles its rows may see.  64 rows a wave instead (K and V fragments read once for
 // both halves) leave one wave per SIMD: 656 -> 801 us at head dim 128, no change at 64.
-// Measured, bf16, 8192 x 8192, 16 heads: head dim 128 653 us, 842 TFLOP/s where a library product of 8192^3 reaches 1243 (causal 298 us, capped
-// 709 us); head dim 64 404 us, 680 TFLOP/s.  At 64 the vector unit bounds it: the exponential, maximum, sum and conversion of a score take longer
-// than its 64 columns in the two products.  At 128 it is the chain inside a wave (score, maximum, exponential, product); without the tile
-// copies it would be 10 % faster at most.
-// One new token for 8 sequences of up to 16384 keys (165 MB of them), 16 / 4 heads of 128: 37 us, 4.4 TB/s, and 7 us for the join.
+// Measured, bf16, 8192 x 8192, 16 heads, first launch to sustained load: head dim 128 580 to 700 us, 785 to 950 TFLOP/s where a library product of
+// 8192^3 reaches 1243 (causal 310 to 340, capped 790 to 890 us); head dim 64 362 to 423 us, 650 to 760 TFLOP/s.  At 128, causal with slopes, the matrix cores
+// are busy for 0.38 of the time and vector instructions for about 0.58 (four cycles each, sixteen for an exponential): together the whole launch, so
+// that what bounds it is that the two waves of a SIMD do both at the same times.  At 64 a score's exponential, maximum, sum and conversion take
+// longer than its columns in the two products.  Without the tile copies it would be 10 % faster at most.
+// One new token for 8 sequences of up to 16384 keys (165 MB of them), 16 / 4 heads of 128: 38 us, 4.4 TB/s, and 6 us for the join.
+// Registers: no vectors spill but 4 at <64, 0>, held to three waves per SIMD, 4 at <128, 3>, and 13 / 16 at <128, 5 / 7>.
 template <typename T, int DP, int MOD>
 __global__ __launch_bounds__(256, DP == 64 && MOD < 2 ? 3 : 2) void attn_mod_fwd_kernel(const Args a) {
   warm_kernargs<(int)sizeof(Args)>();
@@ -932,7 +934,9 @@ __global__ __launch_bounds__(1024) void attn_mod_order_kernel(const Args a, int*
 }
 
 // ------------------------------------------------------------------------------------------------ backward: dQ, delta, table gradient
-// Three products per score, Q, dO and dQ of the wave's 32 rows in registers.  8192 x 8192, 16 heads of 128, bf16: 814 us, 1013 TFLOP/s.
+// Three products per score, Q, dO and dQ of the wave's 32 rows in registers.  8192 x 8192, 16 heads of 128, bf16: 780 to 814 us,
+// 1013 to 1057 TFLOP/s.  Scalars spill to vector lanes where there is a distance bias (88 to 102 of them), vectors at <128, 7> alone (8).  At <64, 2> three
+// waves per SIMD are asked for: without that the allocator takes one register more than they leave.
 template <typename T, int DP, int MOD>
 __global__ __launch_bounds__(256, DP == 64 && MOD < 3 ? 3 : 2) void attn_mod_dq_kernel(const Args a) {
   warm_kernargs<(int)sizeof(Args)>();
@@ -1233,7 +1237,8 @@ struct RowInfo {                    // of one query row, as loaded
 // gradient tiles a wave would need more than half of a SIMD's file, and one wave per SIMD has nothing to run under its exponentials
 // (301 us at 2 x 2011 rows, 16 / 4 heads; this form 144 us).  So at DP = 128 the workgroup is eight waves, its V rows stay in LDS, and two
 // waves share a SIMD.  LDS bounds it then: at full matrix rate it would deliver 156 bytes per clock, against its 128.  8192 x 8192, 16 heads of 128:
-// 1.42 ms, 775 TFLOP/s.
+// 1.36 to 1.42 ms, 775 to 808 TFLOP/s.  It does not fit its 256 registers at DP = 128: 31 / 39 / 60 / 63 vectors spill for the four score forms
+// (44 / 68 with caps above WIDE_CAP; 88 to 172 bytes of scratch a lane), because the 48 registers of scores, weights and dP live through a whole row block.
 template <typename T, int DP, int MOD>
 __global__ __launch_bounds__(DP == 128 ? 512 : 256, 2) void attn_mod_dkdv_kernel(const Args a) {
   warm_kernargs<(int)sizeof(Args)>();

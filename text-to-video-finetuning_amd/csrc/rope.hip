@@ -12,7 +12,8 @@
 // visits, one fixed-order sum over the groups of a workgroup in LDS, one partial row per workgroup, one fixed-order reduction
 // kernel: no atomics, repeated runs are bit-equal.
 // Measured, bf16, norm + rotation of 69120 rows, 2 x 20 heads of 64: forward 161 us (4.4 TB/s; a large copy reaches 4.9), forward and backward
-// 400 us (1.77 GB: 4.4 TB/s with the gaps between launches).  Few rows are launch-bound: 3.6 us of kernel at 8 rows.
+// 400 us (1.77 GB: 4.4 TB/s with the gaps between launches).  Few rows are launch-bound: 8 rows of 16 heads of 128 take 3.9 us a launch in a captured chain,
+// 5.3 us traced singly.
 #include "common.h"
 
 namespace {
@@ -308,7 +309,8 @@ struct Plan {
 // Heads per block of work: as many as leave 1.5 workgroups per CU — a block shares the angles and the per-lane set-up (16384 rows, five heads of
 // 64: 7.8 us with all heads in a block, 13.1 us with one; 6669 rows of five fp32 heads: 8.7 against 17.0).  Workgroups are bounded and
 // visit several rows: 2048 forward (69120 rows, 2 x 20 heads of 64: 161 us, 172 unbounded; 2 x 8 heads of 128: 113 against 128 us), and 1024
-// where each leaves a partial row of parameter gradients (205 us; 308 at 512, where too few loads are in flight).
+// where each leaves a partial row of parameter gradients (249 us; 337 at 512, where too few loads are in flight, 247 at 2048, whose partial rows cost
+// the reduction 3 us more).
 Plan rope_plan(const T2VQkRope* p, bool partials) {
   Plan q;
   const int lanes = p->D / 8;
