@@ -554,7 +554,7 @@ class _AttentionMod(torch.autograd.Function):
             new = torch.empty if p.kv_covered else torch.zeros
             dk, dv = new(k.shape, dtype=dtype, device=dev), new(v.shape, dtype=dtype, device=dev)
         do, o = _upstream(do), o.contiguous()
-        work = _bytes(work_bytes + 4 * p.delta, dev)              # and delta behind it
+        work = _bytes(work_bytes + 4 * p.delta, dev)            # and delta behind it
         d = _AttnFlat.from_buffer_copy(raw)
         _fill(d, q, k, v, o, *masks, bias)
         d.o_rest = at = kept.data_ptr()
@@ -603,7 +603,8 @@ def attention_mod(q, k, v, heads, qlay, klay, kv_heads=None, scale=None, causal=
     (bits are lost below 6e-5, infinite above 65504), so a small loss wants scaling there.
     Few query rows over many keys (serving steps, chunks of new tokens) split the keys over workgroups and join them.
     Returns [rows_q, heads * dim]; rows that no sequence owns are zero.  Differentiable in q, k, v and bias; K / V shared by the bdiv batches
-    of a layout with lo = 0 get the sum of their gradients; other layouts that name a key row twice train q and bias alone.  The order of all sums is fixed: repeated runs are bit-equal."""
+    of a layout with lo = 0 get the sum of their gradients; other layouts that name a key row twice train q and bias alone.  The order of all sums is
+    fixed: repeated runs are bit-equal."""
     heads = int(heads)
     _no_tangents(q, k, v, slopes, bias)
     p = _plan_of((_sig(q), _sig(k), _sig(v), heads, heads if kv_heads is None else int(kv_heads), qlay, klay,
